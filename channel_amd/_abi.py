@@ -99,6 +99,11 @@ PROTOTYPES = {
     "chn_model_read_state": (c_int, [c_void_p, c_void_p, c_void_p]),
     "chn_model_read_logits": (c_int, [c_void_p, c_void_p]),
     "chn_model_replay": (c_int, [c_void_p, c_int, c_void_p, c_void_p]),
+    "chn_block_tables": (c_int, [c_void_p] * 3 + [c_u32, c_void_p, c_u32, c_void_p, c_u32, c_void_p]
+                         + [c_u32] * 4 + [c_void_p] * 6),
+    "chn_batch_qkv_rope_at": (c_int, [c_void_p] + [c_void_p] * 10 + [c_u32] * 6 + [c_int, c_f32, c_f32]),
+    "chn_prefix_decode_attn": (c_int, [c_void_p] * 5 + [c_u32] + [c_void_p] * 2 + [c_u32] * 8 + [c_f32, c_void_p]),
+    "chn_sample": (c_int, [c_void_p] * 2 + [c_u32] * 3 + [c_void_p] * 5 + [c_f32] + [c_void_p] * 2),
     "chn_synth_q4": (c_int, [c_void_p, c_void_p, c_u32, c_u32, c_u64, c_f32, c_f32]),
     "chn_synth_q8": (c_int, [c_void_p, c_void_p, c_u32, c_u32, c_u64, c_f32, c_f32]),
     "chn_synth_normal": (c_int, [c_void_p, c_void_p, c_size, c_u64, c_f32]),

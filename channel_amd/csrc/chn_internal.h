@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -60,6 +61,41 @@ int noalloc_scratch_init(chn_ctx *ctx);
     do {                                                     \
         if (!(cond)) return chn::set_err((ctx), CHN_E_INVALID, __VA_ARGS__); \
     } while (0)
+
+// Makes the context's device current for a scope (launches, allocations).
+struct DeviceGuard {
+    int before = -1;
+    explicit DeviceGuard(const chn_ctx *ctx) {
+        int now = -1;
+        if (hipGetDevice(&now) == hipSuccess && now != ctx->device && hipSetDevice(ctx->device) == hipSuccess)
+            before = now;
+    }
+    ~DeviceGuard() {
+        if (before >= 0) (void)hipSetDevice(before);
+    }
+    DeviceGuard(const DeviceGuard &) = delete;
+};
+
+// A span of 32-bit words, for checks that buffers lie apart.
+struct Span {
+    const void *p;
+    size_t words;
+};
+inline bool overlap(const Span &a, const Span &b) {
+    const uintptr_t x = (uintptr_t)a.p, y = (uintptr_t)b.p;
+    return x && y && a.words && b.words && x < y + b.words * 4 && y < x + a.words * 4;
+}
+
+// The geometry of a paged cache: slots and token positions fit 32 bits.
+inline int check_blocks(chn_ctx *ctx, uint32_t block_size, uint32_t n_blocks, uint32_t max_blocks) {
+    CHN_REQUIRE(ctx, block_size && block_size <= 1024 && !(block_size & (block_size - 1)),
+                "block_size %u must be a power of two, at most 1024", block_size);
+    CHN_REQUIRE(ctx, n_blocks && (uint64_t)n_blocks * block_size <= 0xFFFFFFFFull, "%u blocks of %u: 1 .. 2^32 - 1 slots",
+                n_blocks, block_size);
+    CHN_REQUIRE(ctx, max_blocks && (uint64_t)max_blocks * block_size < (1ull << 31), "tables of %u blocks of %u",
+                max_blocks, block_size);
+    return CHN_OK;
+}
 
 inline bool aligned(const void *p, uintptr_t a) { return ((uintptr_t)p % a) == 0; }
 

@@ -62,7 +62,8 @@ const char *chn_device_name(const chn_ctx *ctx);
 void chn_destroy(chn_ctx *ctx);
 
 /* Text of the last error on `ctx` ("" if none).  With ctx == NULL: the last
- * error of a failed chn_init on this thread. */
+ * error on this thread of a failed chn_init, or of a call that checks its
+ * arguments without a context. */
 const char *chn_last_error(const chn_ctx *ctx);
 
 /* GpuBuffer.init (src/gpu/buffer.zig:57-97): device allocation, 256-byte
@@ -519,6 +520,115 @@ int chn_model_read_logits(chn_model *m, float *logits_out);
  * so the results equal a chn_decode_step call with x = the device stream and
  * the same lists. */
 int chn_model_replay(chn_model *m, int with_logits, uint32_t *topk_ids, float *topk_vals);
+
+/* ======================================================================
+ * Several sequences over one paged KV cache: one decode (or admission) step
+ * of a batch of requests.  No reference counterpart: the reference decodes
+ * one sequence over its ring (src/ring_buffer.zig).  The caches are the ones
+ * the entries above read and write, [slot][kv_dim] fp32, here of n_blocks
+ * blocks of block_size consecutive slots (block b holds slots b * block_size
+ * .. ; block_size a power of two <= 1024, n_blocks * block_size < 2^32, the
+ * caches may hold more than 4 GiB).  Each request has a row of max_blocks
+ * block ids (its table), in the order of its tokens.  All requests may begin
+ * with the same prefix, a whole number of blocks that is held once.
+ *
+ * A step is chn_block_tables, then per layer chn_batch_qkv_rope_at and
+ * chn_prefix_decode_attn, then chn_sample on the rows of logits.  All four
+ * only enqueue on the context's stream, read their lengths, tables and
+ * settings from device memory, and can be recorded (chn_record_begin).
+ * Argument checks come first: called with ctx == NULL they report through
+ * chn_last_error(NULL).
+ * ==================================================================== */
+
+#define CHN_NO_SLOT 0xFFFFFFFFu     /* a token without a place in the cache */
+#define CHN_NO_TOKEN 0xFFFFFFFFu    /* a row of logits that allows no token */
+
+/* Block tables and slot maps.  Request r holds lens[r] tokens and gains
+ * n_new[r] (both device arrays of n_req <= 8192).  With P = n_prefix_blocks *
+ * block_size and begin = n_new[r] > 0 ? max(lens[r], P) : lens[r]:
+ *  - a request with n_new[r] > 0 and lens[r] < P is new: its table begins
+ *    with prefix_blocks[0 .. n_prefix_blocks) (device), its tokens behind P;
+ *  - every block that tokens begin .. begin + n_new[r] - 1 open is the next
+ *    of free_blocks[taken .. n_free) (device; taken: a device count, or NULL
+ *    for 0), handed out request by request, and is entered in the table;
+ *  - the new tokens are rows row_start[r] .. row_start[r + 1] - 1 of the
+ *    batch, row_start[r] = n_new[0] + .. + n_new[r - 1]: slots[row] is the
+ *    cache slot of the row's token (CHN_NO_SLOT where its block id is not
+ *    below n_blocks), clocks[row] its position in its sequence;
+ *  - lens_out[r] = begin + n_new[r].
+ * row_start has n_req + 1 entries, slots and clocks max_tokens.  status (3
+ * device words): CHN_TABLES_* flags, taken + the blocks handed out (the next
+ * call's `taken` may point at it), the number of rows.  With a flag set
+ * nothing else is written; rows behind the last one, and table entries that
+ * hold no token yet, are left as they were.  lens, n_new, taken, the prefix
+ * and the free list must not overlap what is written (a loop alternates
+ * between two sets of lens_out and status). */
+#define CHN_TABLES_NO_BLOCKS 1u     /* the free list has too few blocks     */
+#define CHN_TABLES_TOO_LONG 2u      /* a request outgrows max_blocks        */
+#define CHN_TABLES_TOO_MANY 4u      /* more rows than max_tokens            */
+int chn_block_tables(chn_ctx *ctx, const uint32_t *lens, const uint32_t *n_new, uint32_t n_req,
+                     const uint32_t *prefix_blocks, uint32_t n_prefix_blocks, const uint32_t *free_blocks,
+                     uint32_t n_free, const uint32_t *taken, uint32_t n_blocks, uint32_t block_size,
+                     uint32_t max_blocks, uint32_t max_tokens, uint32_t *tables, uint32_t *lens_out,
+                     uint32_t *row_start, uint32_t *slots, uint32_t *clocks, uint32_t *status);
+
+/* chn_batch_qkv_rope for tokens of different sequences: token t is at clock
+ * clocks[t] and its K/V go to slot slots[t] (device arrays, as
+ * chn_block_tables writes them).  A slot that is not below n_slots (the
+ * caches' slots; CHN_NO_SLOT) gets no K/V; q_out is written for every token.
+ * The angle clock * theta^(-2d / rotary_dim) is formed and reduced in 64
+ * bits, so far positions keep fp32 accuracy (chn_batch_qkv_rope forms it in
+ * fp32 as the reference does).  Two tokens with one slot: either's values,
+ * element by element. */
+int chn_batch_qkv_rope_at(chn_ctx *ctx, const float *q_in, const float *k_in, const float *v_in,
+                          const float *q_norm_w, const float *k_norm_w, float *q_out, float *k_cache,
+                          float *v_cache, const uint32_t *clocks, const uint32_t *slots, uint32_t n_tok,
+                          uint32_t n_slots, uint32_t num_q_heads, uint32_t num_kv_heads, uint32_t head_dim,
+                          uint32_t rotary_dim, int k_eq_v, float theta, float eps);
+
+/* Decode attention of one token per request: q and out [n_req][num_q_heads *
+ * head_dim]; request r attends over its first lens[r] tokens (device;
+ * min(lens[r], max_blocks * block_size)), of which the first n_prefix_blocks
+ * * block_size lie in prefix_blocks (device, shared by all requests and read
+ * once for them), the others in row r of tables ([n_req][max_blocks],
+ * device; its first n_prefix_blocks entries are not read).  Softmax of scale
+ * * q.k; a request without tokens gets zeros.  A block id that is not below
+ * n_blocks takes its tokens out of the softmax; slots that no token occupies
+ * are never used, whatever they hold.  Query head h reads KV head h /
+ * gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; n_prefix_blocks <=
+ * max_blocks, max_blocks * block_size < 2^31.  Workspace: it grows with
+ * n_req * num_q_heads * head_dim, not with the lengths. */
+int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
+                           const uint32_t *prefix_blocks, uint32_t n_prefix_blocks, const uint32_t *tables,
+                           const uint32_t *lens, uint32_t n_req, uint32_t max_blocks, uint32_t block_size,
+                           uint32_t n_blocks, uint32_t num_q_heads, uint32_t head_dim, uint32_t kv_dim,
+                           uint32_t gqa_ratio, float scale, float *out);
+
+/* The next token of each of n_rows rows of logits (row r at logits + r * ld,
+ * V of ld values, V <= 2^20), drawn with the given u[r] in [0, 1):
+ *  - values that are not above -FLT_MAX (-inf, the lowest value, NaN) are
+ *    barred: never drawn.  A row that bars everything gets CHN_NO_TOKEN;
+ *  - softcap > 0 takes softcap * tanh(l / softcap) for l (0: l itself);
+ *  - weights w = exp((l - l_max) / temperature[r]);
+ *  - top_k[r] > 0 keeps the top_k[r] largest logits, equal ones by lower
+ *    index (0, or >= V: all);
+ *  - top_p[r] < 1 keeps of those, largest first, every token with less than
+ *    top_p[r] of their mass before it (the first always);
+ *  - min_p[r] > 0 keeps of those the tokens with w >= min(min_p[r], 1);
+ *  - the token is the first, by index, whose running sum of the kept w
+ *    exceeds u[r] times their sum; probs[r] = its w / that sum.
+ * temperature[r] <= 0 or NaN takes the largest logit (the lowest such index),
+ * probability 1.  A NaN top_p or min_p switches its filter off; a u below 0
+ * or NaN counts as 0, one of 1 or more draws the last kept token.
+ * +inf without softcap: all +inf tokens are equally likely.  All settings are
+ * device arrays of n_rows; temperature NULL: 1; top_k, top_p, min_p NULL:
+ * off; probs may be NULL.  Weights and their sums are held in 43-bit fixed
+ * point relative to the largest weight and summed exactly: the result does
+ * not depend on the order of the sums, and tokens below 2^-44 of the largest
+ * weight are never drawn. */
+int chn_sample(chn_ctx *ctx, const float *logits, uint32_t n_rows, uint32_t V, uint32_t ld,
+               const float *temperature, const uint32_t *top_k, const float *top_p, const float *min_p,
+               const float *u, float softcap, uint32_t *tokens, float *probs);
 
 /* ======================================================================
  * Seeded synthetic inputs (no reference counterpart: benchmark and test
