@@ -44,9 +44,9 @@ struct PrefixAttn {
     uint32_t splits, split_keys, tiles, prefix_wgs;
     // own items: at most own_cap + n_req of them per KV head
     uint32_t own_cap;
-    // partial results: [splits][n_req][num_q] of the prefix, then [own item][num_q]; sums [..][D], then maxima and
-    // denominators; own_start[n_req + 1]: the first own item of each request
-    float *po, *pm, *pl, *oo, *om, *ol;
+    // partial results, [splits][n_req][num_q] of the prefix and then [own item][num_q]: sums of D values, references
+    // and denominators; own_start[n_req + 1]: the first own item of each request
+    float *o, *m, *l;
     uint32_t *own_start;
 };
 
@@ -65,7 +65,7 @@ __device__ __forceinline__ uint32_t own_per(const PrefixAttn &a, int lane) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += (uint64_t)__shfl_xor((unsigned long long)sum, o, 64);
     const uint64_t per = (sum + a.own_cap - 1) / a.own_cap;
-    return per > kOwnMinGroups ? (uint32_t)per : kOwnMinGroups;
+    return (uint32_t)min(max(per, (uint64_t)kOwnMinGroups), (uint64_t)1 << 27);   // 2^31 positions at most
 }
 
 __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v, int lane) {      // inclusive
@@ -77,337 +77,607 @@ __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v, int lane) {      /
     return v;
 }
 
-// RT tiles of 16 rows over keys [begin, end) of the positions that `blocks`
-// maps.  The rows' q lie in LDS (sq, row stride D + 4 floats); lim[rt] is how
-// many positions this lane's row c of tile rt may see.
-template <int D, int RT>
-struct Tile {
-    static constexpr int H = D / 256;
-    f4a o[RT][D / 64][4];
-    float m[RT], l[RT];        // this row's reference, and this lane's part of its denominator
-
-    __device__ __forceinline__ void run(const PrefixAttn &a, const float *sq, const uint32_t *blocks, uint32_t kvh,
-                                        uint32_t begin, uint32_t end, const uint32_t (&lim)[RT]) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15;
-        const uint32_t mask = (1u << a.shift) - 1;
-        // Rows that see none of these keys are dead: computed along, dropped at the end.  Up to `full` every other row
-        // sees every key; behind it (a request shorter than the prefix) rows see parts of the groups.
-        uint32_t least = end;
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            m[rt] = kNone;
-            l[rt] = 0.0f;
-            if (lim[rt] > begin) least = min(least, lim[rt]);
-#pragma unroll
-            for (int n = 0; n < D / 64; ++n)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) o[rt][n][j] = f4a{0, 0, 0, 0};
-        }
-#pragma unroll
-        for (int x = 8; x >= 1; x >>= 1) least = min(least, (uint32_t)__shfl_xor(least, x, 64));   // the 16 rows
-        least = __builtin_amdgcn_readfirstlane(least);
-        const uint32_t full = least >= end ? end : begin + (least - begin) / 16 * 16;
-
-        // key c of the group at kb; a key past the end, or of a bad block, has no slot
-        auto block_of = [&](uint32_t kb) { return blocks[min(kb + c, end - 1) >> a.shift]; };
-        auto slot_of = [&](uint32_t kb, uint32_t b) {
-            const uint32_t k = kb + c;
-            return k < end && b < a.n_blocks ? (b << a.shift) + (k & mask) : kBadSlot;
-        };
-        auto row_of = [&](const float *cache, uint32_t slot) {
-            return cache + (size_t)(slot == kBadSlot ? 0u : slot) * a.kv_dim + (size_t)kvh * D;
-        };
-        f4a A[16], B[16];
-        auto load_k = [&](f4a (&d)[16], uint32_t slot, int h) {
-            const float *k = row_of(a.kc, slot) + 256 * h + 4 * g;
-#pragma unroll
-            for (int s = 0; s < 16; ++s) d[s] = *(const f4a *)(k + 16 * s);
-        };
-        uint32_t vs[4];                            // keys 4 g + i of the group
-        auto load_v = [&](f4a (&d)[16], int h) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float *v = row_of(a.vc, vs[i]) + 256 * h + 4 * c;
-#pragma unroll
-                for (int n = 0; n < 4; ++n) d[4 * i + n] = *(const f4a *)(v + 64 * n);
-            }
-        };
-        f4a S[RT], part[RT][4];                    // a score's sum in four chains: shorter ones round less
-        auto scores = [&](const f4a (&d)[16], int h) {
-#pragma unroll
-            for (int s = 0; s < 16; ++s)
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const f4a q = *(const f4a *)(sq + (rt * 16 + c) * (D + 4) + 256 * h + 16 * s + 4 * g);
-#pragma unroll
-                    for (int j = 0; j < 4; ++j)
-                        part[rt][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(d[s][j], q[j], part[rt][j], 0, 0, 0);
-                }
-        };
-        auto clear = [&] {
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int j = 0; j < 4; ++j) part[rt][j] = f4a{0, 0, 0, 0};
-        };
-        // scores to weights; seen(rt, i): whether row c of tile rt sees key 4 g + i
-        auto softmax = [&](auto &&seen) {
-            bool up = false;
-            float mx[RT];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                S[rt] = (part[rt][0] + part[rt][1]) + (part[rt][2] + part[rt][3]);
-                float t[4];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) t[i] = seen(rt, i) ? S[rt][i] * a.exp_hi : kNone;
-                mx[rt] = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
-                up = up || mx[rt] > m[rt] + kSlack;
-            }
-            if (__any(up)) {
-#pragma unroll
-                for (int rt = 0; rt < RT; ++rt) {
-                    const float mn = fmaxf(m[rt], rows4_max(mx[rt]));
-                    const float f = mn == m[rt] ? 1.0f : __builtin_amdgcn_exp2f(m[rt] - mn);
-                    m[rt] = mn;
-                    l[rt] *= f;
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float fr = __shfl(f, 4 * g + i, 64);
-#pragma unroll
-                        for (int n = 0; n < D / 64; ++n)
-#pragma unroll
-                            for (int j = 0; j < 4; ++j) o[rt][n][j][i] *= fr;
-                    }
-                }
-            }
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt) {
-                const float ref = m[rt] == kNone ? 0.0f : m[rt];
-                // the exponent's rounding is that of its distance to the reference, not of the score
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float w = __builtin_amdgcn_exp2f(fmaf(S[rt][i], a.exp_lo, fmaf(S[rt][i], a.exp_hi, -ref)));
-                    S[rt][i] = seen(rt, i) ? w : 0.0f;
-                }
-                l[rt] += (S[rt][0] + S[rt][1]) + (S[rt][2] + S[rt][3]);
-            }
-        };
-        auto weigh_v = [&](const f4a (&d)[16], int h) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t vm = opaque_mask(vs[i] != kBadSlot);
-#pragma unroll
-                for (int n = 0; n < 4; ++n)
-#pragma unroll
-                    for (int j = 0; j < 4; ++j) {
-                        const float v = mask_f(d[4 * i + n][j], vm);
-#pragma unroll
-                        for (int rt = 0; rt < RT; ++rt)
-                            o[rt][4 * h + n][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(S[rt][i], v, o[rt][4 * h + n][j], 0, 0, 0);
-                    }
-            }
-        };
-        // Loads are issued ahead of the products they run beside, one buffer of 64 registers each way, and stay there.
-        auto fence = [] { __builtin_amdgcn_sched_barrier(0); };
-
-        uint32_t kb = begin + 16 * wave;
-        if (kb >= end) return;                     // a whole wave
-        uint32_t slot = slot_of(kb, block_of(kb)), nextb = block_of(kb + 64);
-        if (kb < full) {
-            load_k(A, slot, 0);
-            for (;;) {
-#pragma unroll
-                for (int i = 0; i < 4; ++i) vs[i] = __shfl(slot, 4 * g + i, 64);
-                const uint32_t next = slot_of(kb + 64, nextb);
-                nextb = block_of(kb + 128);
-                clear();
-                if constexpr (H == 1) {
-                    load_v(B, 0);
-                    fence();
-                    scores(A, 0);
-                } else {
-                    load_k(B, slot, 1);
-                    fence();
-                    scores(A, 0);
-                    fence();
-                    load_v(A, 0);
-                    fence();
-                    scores(B, 1);
-                    fence();
-                    load_v(B, 1);
-                    fence();
-                }
-                softmax([&](int, int i) { return vs[i] != kBadSlot; });
-                slot = next;
-                fence();
-                if constexpr (H == 1) {
-                    load_k(A, slot, 0);            // past the end: slot 0, not used
-                    fence();
-                    weigh_v(B, 0);
-                } else {
-                    weigh_v(A, 0);
-                    fence();
-                    load_k(A, slot, 0);
-                    fence();
-                    weigh_v(B, 1);
-                }
-                fence();
-                kb += 64;
-                if (kb >= full) break;
-            }
-        }
-        // Groups that some row sees a part of: the weighted sum key by key, as a weight of zero does not keep an
-        // infinity or NaN of an unseen V row out of a product.
-#pragma unroll 1
-        for (; kb < end; kb += 64) {
-            slot = slot_of(kb, block_of(kb));
-            clear();
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                load_k(A, slot, h);
-                scores(A, h);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) vs[i] = __shfl(slot, 4 * g + i, 64);
-            softmax([&](int rt, int i) { return vs[i] != kBadSlot && kb + 4 * g + i < lim[rt]; });
-            uint32_t rlim[RT][4];
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                for (int i = 0; i < 4; ++i) rlim[rt][i] = __shfl(lim[rt], 4 * g + i, 64);
-#pragma unroll 1
-            for (int kg = 0; kg < 4; ++kg)
-#pragma unroll
-                for (int ki = 0; ki < 4; ++ki) {
-                    const uint32_t key = kb + 4 * kg + ki, ks = __shfl(slot, 4 * kg + ki, 64);
-                    if (ks == kBadSlot) continue;  // the whole wave
-                    const float *v = row_of(a.vc, ks) + 4 * c;
-#pragma unroll
-                    for (int rt = 0; rt < RT; ++rt)
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            const float p = __shfl(S[rt][ki], 16 * kg + 4 * g + i, 64);
-                            if (key < rlim[rt][i])
-#pragma unroll
-                                for (int n = 0; n < D / 64; ++n) {
-                                    const f4a x = *(const f4a *)(v + 64 * n);
-#pragma unroll
-                                    for (int j = 0; j < 4; ++j) o[rt][n][j][i] = fmaf(p, x[j], o[rt][n][j][i]);
-                                }
-                        }
-                }
-        }
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt)
-            if (lim[rt] <= begin) {
-                m[rt] = kNone;
-                l[rt] = 0.0f;
-            }
+// Keys [begin, end) of a list of positions that `blocks` maps, in groups of
+// 16.  Key c of the group at kb has no slot if it lies past the end or its
+// block is bad.
+struct Keys {
+    const uint32_t *blocks;
+    uint32_t begin, end, kvh;
+    __device__ __forceinline__ uint32_t block(const PrefixAttn &a, uint32_t kb, int c) const {
+        return blocks[min(kb + c, end - 1) >> a.shift];
     }
+    __device__ __forceinline__ uint32_t slot(const PrefixAttn &a, uint32_t kb, int c, uint32_t b) const {
+        const uint32_t k = kb + c;
+        return k < end && b < a.n_blocks ? (b << a.shift) + (k & ((1u << a.shift) - 1)) : kBadSlot;
+    }
+};
+// What is read where a key has no slot.
+static __device__ __align__(16) const float zero_row[512] = {};
+// A slot's row of one KV head.
+template <int D>
+__device__ __forceinline__ const float *cache_row(const PrefixAttn &a, const float *cache, uint32_t slot, uint32_t kvh) {
+    return slot == kBadSlot ? zero_row : cache + (size_t)slot * a.kv_dim + (size_t)kvh * D;
+}
 
-    // The waves' states joined, tile by tile: row c's sum of D values,
-    // reference and denominator to where(row) (NULL: no such row).
-    template <typename F>
-    __device__ __forceinline__ void join(float *sh, F &&where) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, g = lane >> 4, c = lane & 15, tid = threadIdx.x;
-        float *so = sh, *sm = sh + 4 * 16 * D, *sl = sm + 4 * 16;
+// 16 query rows of a wave over 256 dims: the weighted sums (lane 16 g + c,
+// element i of o[n][j]: row 4 g + i, dim 64 n + 4 c + j), and row c's reference
+// and this lane's part of its denominator.  lim: how many positions row c may
+// see.
+struct Rows {
+    f4a o[4][4];
+    float m, l;
+    uint32_t lim, full;
+
+    // Rows that see no key of the range are dead: computed along, dropped in
+    // end().  Groups below `full` are seen whole by every other row; behind
+    // it (requests shorter than the prefix) rows see parts of them.
+    __device__ __forceinline__ void start(uint32_t limit, const Keys &k) {
+        m = kNone;
+        l = 0.0f;
+        lim = limit;
 #pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const float lt = rows4_sum(l[rt]);
-            __syncthreads();                       // q, or the tile before, has been read
-            if (g == 0) {
-                sm[wave * 16 + c] = m[rt];
-                sl[wave * 16 + c] = lt;
-            }
-            __syncthreads();
-            const float M = fmaxf(fmaxf(sm[c], sm[16 + c]), fmaxf(sm[32 + c], sm[48 + c]));
-            const float f = m[rt] == kNone ? 0.0f : __builtin_amdgcn_exp2f(m[rt] - M);
+        for (int n = 0; n < 4; ++n)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) o[n][j] = f4a{0, 0, 0, 0};
+        uint32_t least = lim > k.begin ? min(lim, k.end) : k.end;
+#pragma unroll
+        for (int x = 8; x >= 1; x >>= 1) least = min(least, (uint32_t)__shfl_xor(least, x, 64));
+        least = __builtin_amdgcn_readfirstlane(least);
+        full = least >= k.end ? k.end : k.begin + (least - k.begin) / 16 * 16;
+    }
+    __device__ __forceinline__ void end(const Keys &k) {
+        if (lim <= k.begin) {
+            m = kNone;
+            l = 0.0f;
+        }
+    }
+    // The scores of a group to weights: element i is key 4 g + i of row c;
+    // seen(i): whether the row sees it.
+    template <typename F>
+    __device__ __forceinline__ f4a softmax(const PrefixAttn &a, f4a s, F &&seen) {
+        const int g = (threadIdx.x & 63) >> 4;
+        float t[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) t[i] = seen(i) ? s[i] * a.exp_hi : kNone;
+        const float mx = fmaxf(fmaxf(t[0], t[1]), fmaxf(t[2], t[3]));
+        if (__any(mx > m + kSlack)) {
+            const float mn = fmaxf(m, rows4_max(mx));
+            const float f = mn == m ? 1.0f : __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 const float fr = __shfl(f, 4 * g + i, 64);
-                const bool none = __shfl(m[rt], 4 * g + i, 64) == kNone;
 #pragma unroll
-                for (int n = 0; n < D / 64; ++n)
-                    *(f4a *)(so + ((size_t)wave * 16 + 4 * g + i) * D + 64 * n + 4 * c) =
-                        none ? f4a{0, 0, 0, 0} : f4a{o[rt][n][0][i], o[rt][n][1][i], o[rt][n][2][i], o[rt][n][3][i]} * fr;
-            }
-            __syncthreads();
-            if (tid < 16) {
-                float L = 0.0f;
-                const float Mr = fmaxf(fmaxf(sm[tid], sm[16 + tid]), fmaxf(sm[32 + tid], sm[48 + tid]));
+                for (int n = 0; n < 4; ++n)
 #pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const float mw = sm[w * 16 + tid];
-                    L += mw == kNone ? 0.0f : sl[w * 16 + tid] * __builtin_amdgcn_exp2f(mw - Mr);
-                }
-                float *po, *pm, *pl;
-                if (where(rt * 16 + tid, po, pm, pl)) {
-                    *pm = Mr;
-                    *pl = L;
+                    for (int j = 0; j < 4; ++j) o[n][j][i] *= fr;
+            }
+        }
+        const float ref = m == kNone ? 0.0f : m;
+        // the exponent's rounding is that of its distance to the reference, not of the score
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float w = __builtin_amdgcn_exp2f(fmaf(s[i], a.exp_lo, fmaf(s[i], a.exp_hi, -ref)));
+            s[i] = seen(i) ? w : 0.0f;
+        }
+        l += (s[0] + s[1]) + (s[2] + s[3]);
+        return s;
+    }
+    // Weights times V of a group that some row sees a part of, key by key: a
+    // weight of zero does not keep an infinity or NaN of an unseen V row out
+    // of a product, so that row is left out.  v(k): key k's V row, or NULL
+    // (the same for the whole wave).
+    template <typename F>
+    __device__ __forceinline__ void weigh_part(const f4a &s, uint32_t kb, F &&v) {
+        const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+        uint32_t rl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) rl[i] = __shfl(lim, 4 * g + i, 64);
+#pragma unroll 1
+        for (int kg = 0; kg < 4; ++kg)
+#pragma unroll
+            for (int ki = 0; ki < 4; ++ki) {
+                const uint32_t key = kb + 4 * kg + ki;
+                const float *row = v(4 * kg + ki);
+                float p[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) p[i] = __shfl(s[ki], 16 * kg + 4 * g + i, 64);
+                if (!row) continue;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const f4a x = *(const f4a *)(row + 64 * n + 4 * c);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[n][j][i] = key < rl[i] ? fmaf(p[i], x[j], o[n][j][i]) : o[n][j][i];
                 }
             }
-            for (int e = tid; e < 16 * D / 4; e += 256) {
-                const int row = e / (D / 4), d = (e % (D / 4)) * 4;
-                float *po, *pm, *pl;
-                if (!where(rt * 16 + row, po, pm, pl)) continue;
-                const float *s = so + (size_t)row * D + d;
-                *(f4a *)(po + d) = (*(const f4a *)s + *(const f4a *)(s + 16 * D)) +
-                                   (*(const f4a *)(s + 32 * D) + *(const f4a *)(s + 48 * D));
+    }
+};
+
+// Nothing may move across: the loads before it are issued ahead of the
+// products behind it, which run while they are under way.
+__device__ __forceinline__ void issue_fence() { __builtin_amdgcn_sched_barrier(0); }
+
+// --- few rows (RQ quads of four): the four waves take a group of 16 keys each
+// in turn, on v_mfma_f32_4x4x1_16b_f32, whose 16 blocks multiply 4 x 1 by 1 x
+// 4.  Lane l = 4 b + r belongs to block b.
+// Scores: the blocks share out the dims (block b: 64 m + 4 b + j), A is K[key 4
+// kq + r], B is q[row r]; a transposed sum over the blocks leaves lane 4 b + r
+// with the score of key b and row r, one register for the whole group.
+// V: every block has dims of its own (4 l + j), A is one key's weights,
+// broadcast from the block that holds them, B the lane's V value.
+// So K is read 256 bytes and V a whole row at a time, straight into the
+// registers they are multiplied from (two buffers of 64), and four rows cost a
+// quarter of what a 16-row tile would.  The query rows come from LDS (stride D
+// + 16).
+template <int D, int RQ>
+struct Quads {
+    static constexpr int H = D / 256;
+    f4a o[RQ][H][4];               // element i of o[.][h][j]: row i, dim 256 h + 4 l + j
+    float m[RQ], l[RQ];            // row r's reference, and this lane's part of its denominator
+    uint32_t lim[RQ];              // how many positions row r may see
+
+    // limit(row): how many positions row `row` may see
+    template <typename F>
+    __device__ __forceinline__ void run(const PrefixAttn &a, const float *sq, const Keys &k, F &&limit) {
+        const int lane = threadIdx.x & 63, b = lane >> 2, r = lane & 3;
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        uint32_t least = k.end;
+#pragma unroll
+        for (int x = 0; x < RQ; ++x) {
+            m[x] = kNone;
+            l[x] = 0.0f;
+            lim[x] = limit(4 * x + r);
+            if (lim[x] > k.begin) least = min(least, lim[x]);
+#pragma unroll
+            for (int h = 0; h < H; ++h)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) o[x][h][j] = f4a{0, 0, 0, 0};
+        }
+        least = min(least, (uint32_t)__shfl_xor(least, 1, 64));
+        least = min(least, (uint32_t)__shfl_xor(least, 2, 64));
+        least = __builtin_amdgcn_readfirstlane(least);
+        // rows that see none of these keys are dead: computed along, dropped at the end.  Up to `full` every other row
+        // sees every key; behind it (requests shorter than the prefix) rows see parts of the groups
+        const uint32_t full = least >= k.end ? k.end : k.begin + (least - k.begin) / 16 * 16;
+
+        f4a A[16], B[16];
+        auto load_k = [&](f4a (&d)[16], uint32_t slot, int h) {
+#pragma unroll
+            for (int kq = 0; kq < 4; ++kq) {
+                const float *x = cache_row<D>(a, a.kc, __shfl(slot, 16 * kq + 4 * r, 64), k.kvh) + 256 * h + 4 * b;
+#pragma unroll
+                for (int n = 0; n < 4; ++n) d[4 * kq + n] = *(const f4a *)(x + 64 * n);
             }
+        };
+        auto load_v = [&](f4a (&d)[16], uint32_t slot, int h) {
+#pragma unroll
+            for (int y = 0; y < 16; ++y)
+                d[y] = *(const f4a *)(cache_row<D>(a, a.vc, __builtin_amdgcn_readlane(slot, 4 * y), k.kvh) + 256 * h + 4 * lane);
+        };
+        // the transposed sum: lane 4 b + r gets key b's score of row r
+        auto total = [&](const f4a (&c)[4]) {
+            float v[8], y[4], z[2];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) v[i] = swap_add32(c[i >> 2][i & 3], c[2 + (i >> 2)][i & 3]);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) y[i] = swap_add16(v[i], v[4 + i]);
+            const bool h8 = lane & 8, h4 = lane & 4;
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                const float keep = h8 ? y[2 + i] : y[i], send = h8 ? y[i] : y[2 + i];
+                z[i] = keep + __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, send), 0x128, 0xF,
+                                                                                 0xF, true));        // row_ror:8
+            }
+            const float keep = h4 ? z[1] : z[0], send = h4 ? z[0] : z[1];
+            return keep + __shfl_xor(send, 4, 64);
+        };
+        // adds a half's scores, quad by quad
+        auto scores = [&](float (&s)[RQ], const f4a (&d)[16], int h) {
+#pragma unroll
+            for (int x = 0; x < RQ; ++x) {
+                f4a part[4];
+#pragma unroll
+                for (int kq = 0; kq < 4; ++kq) part[kq] = f4a{0, 0, 0, 0};
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const f4a q = *(const f4a *)(sq + (4 * x + r) * (D + 16) + 256 * h + 64 * n + 4 * b);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int kq = 0; kq < 4; ++kq)
+                            part[kq] = __builtin_amdgcn_mfma_f32_4x4x1f32(d[4 * kq + n][j], q[j], part[kq], 0, 0, 0);
+                }
+                s[x] = h ? s[x] + total(part) : total(part);
+                if (RQ > 1) issue_fence();
+            }
+        };
+        // scores to weights, in place; seen(x): whether row r of quad x sees key b
+        auto softmax = [&](float (&s)[RQ], auto &&seen) {
+            float t[RQ];
+            bool up = false;
+#pragma unroll
+            for (int x = 0; x < RQ; ++x) {
+                t[x] = seen(x) ? s[x] * a.exp_hi : kNone;
+                up = up || t[x] > m[x] + kSlack;
+            }
+            if (__any(up)) {
+#pragma unroll
+                for (int x = 0; x < RQ; ++x) {
+                    float mn = fmaxf(m[x], t[x]);
+#pragma unroll
+                    for (int y = 4; y <= 32; y <<= 1) mn = fmaxf(mn, __shfl_xor(mn, y, 64));
+                    const float f = mn == m[x] ? 1.0f : __builtin_amdgcn_exp2f(m[x] - mn);
+                    m[x] = mn;
+                    l[x] *= f;
+                    const f4a fr = {lane_f(f, 0), lane_f(f, 1), lane_f(f, 2), lane_f(f, 3)};
+#pragma unroll
+                    for (int h = 0; h < H; ++h)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) o[x][h][j] *= fr;
+                }
+            }
+#pragma unroll
+            for (int x = 0; x < RQ; ++x) {
+                const float ref = m[x] == kNone ? 0.0f : m[x];
+                // the exponent's rounding is that of its distance to the reference, not of the score
+                const float w = __builtin_amdgcn_exp2f(fmaf(s[x], a.exp_lo, fmaf(s[x], a.exp_hi, -ref)));
+                s[x] = seen(x) ? w : 0.0f;
+                l[x] += s[x];
+            }
+        };
+        auto weigh = [&](const float (&s)[RQ], const f4a (&d)[16], int h) {
+            static_for<16>([&](auto key) {
+#pragma unroll
+                for (int x = 0; x < RQ; ++x)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        o[x][h][j] = __builtin_amdgcn_mfma_f32_4x4x1f32(s[x], d[key][j], o[x][h][j], 4, key, 0);
+            });
+        };
+
+        uint32_t kb = k.begin + 16 * wave;
+        if (kb < k.end) {
+            uint32_t slot = k.slot(a, kb, b, k.block(a, kb, b)), nextb = k.block(a, kb + 64, b);
+            float s[RQ];
+            if (kb < full) {
+                load_k(A, slot, 0);
+                for (;;) {
+                    const uint32_t next = k.slot(a, kb + 64, b, nextb);
+                    nextb = k.block(a, kb + 128, b);
+                    if constexpr (H == 1) {
+                        load_v(B, slot, 0);
+                        issue_fence();
+                        scores(s, A, 0);
+                    } else {
+                        load_k(B, slot, 1);
+                        issue_fence();
+                        scores(s, A, 0);
+                        issue_fence();
+                        load_v(A, slot, 0);
+                        issue_fence();
+                        scores(s, B, 1);
+                        issue_fence();
+                        load_v(B, slot, 1);
+                        issue_fence();
+                    }
+                    softmax(s, [&](int) { return slot != kBadSlot; });
+                    slot = next;
+                    issue_fence();
+                    if constexpr (H == 1) {
+                        load_k(A, slot, 0);        // past the end: the row of zeros, not used
+                        issue_fence();
+                        weigh(s, B, 0);
+                    } else {
+                        weigh(s, A, 0);
+                        issue_fence();
+                        load_k(A, slot, 0);
+                        issue_fence();
+                        weigh(s, B, 1);
+                    }
+                    issue_fence();
+                    kb += 64;
+                    if (kb >= full) break;
+                }
+            }
+            // Groups that some row sees a part of: the weighted sum key by key, as a weight of zero does not keep an
+            // infinity or NaN of an unseen V row out of a product.
+#pragma unroll 1
+            for (; kb < k.end; kb += 64) {
+                slot = k.slot(a, kb, b, k.block(a, kb, b));
+#pragma unroll
+                for (int h = 0; h < H; ++h) {
+                    load_k(A, slot, h);
+                    scores(s, A, h);
+                }
+                softmax(s, [&](int x) { return slot != kBadSlot && kb + b < lim[x]; });
+#pragma unroll 1
+                for (int key = 0; key < 16; ++key) {
+                    const float *v = cache_row<D>(a, a.vc, __builtin_amdgcn_readlane(slot, 4 * key), k.kvh) + 4 * lane;
+#pragma unroll
+                    for (int h = 0; h < H; ++h) {
+                        const f4a y = *(const f4a *)(v + 256 * h);
+#pragma unroll
+                        for (int x = 0; x < RQ; ++x)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) {
+                                const float w = lane_f(s[x], 4 * key + i);
+                                if (kb + key < (uint32_t)__builtin_amdgcn_readlane(lim[x], i))
+#pragma unroll
+                                    for (int j = 0; j < 4; ++j) o[x][h][j][i] = fmaf(w, y[j], o[x][h][j][i]);
+                            }
+                    }
+                }
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < RQ; ++x) {
+#pragma unroll
+            for (int y = 4; y <= 32; y <<= 1) l[x] += __shfl_xor(l[x], y, 64);
+            if (lim[x] <= k.begin) {
+                m[x] = kNone;
+                l[x] = 0.0f;
+            }
+        }
+    }
+
+    // The four waves' sums of the n first rows joined: a row's sum of D
+    // values, reference and denominator as the partial result where(row).
+    template <typename F>
+    __device__ __forceinline__ void join(const PrefixAttn &a, float *sh, uint32_t n, F &&where) {
+        const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 3;
+        constexpr int R = 4 * RQ;
+        float *so = sh, *sm = sh + 4 * R * D, *sl = sm + 4 * R;
+#pragma unroll
+        for (int x = 0; x < RQ; ++x)
+            if (lane < 4) {
+                sm[wave * R + 4 * x + r] = m[x];
+                sl[wave * R + 4 * x + r] = l[x];
+            }
+        __syncthreads();                           // and the query rows have been read
+#pragma unroll
+        for (int x = 0; x < RQ; ++x) {
+            const float *mr = sm + 4 * x + r;
+            const float M = fmaxf(fmaxf(mr[0], mr[R]), fmaxf(mr[2 * R], mr[3 * R]));
+            const float f = m[x] == kNone ? 0.0f : __builtin_amdgcn_exp2f(m[x] - M);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (4 * x + i >= (int)n) continue;
+                const float fr = lane_f(f, i);
+                const bool none = lane_f(m[x], i) == kNone;
+#pragma unroll
+                for (int h = 0; h < H; ++h)
+                    *(f4a *)(so + (wave * R + 4 * x + i) * D + 256 * h + 4 * lane) =
+                        none ? f4a{0, 0, 0, 0} : f4a{o[x][h][0][i], o[x][h][1][i], o[x][h][2][i], o[x][h][3][i]} * fr;
+            }
+        }
+        __syncthreads();
+        if (tid < (int)n) {
+            const float *mr = sm + tid;
+            const float M = fmaxf(fmaxf(mr[0], mr[R]), fmaxf(mr[2 * R], mr[3 * R]));
+            float L = 0.0f;
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+                L += mr[y * R] == kNone ? 0.0f : sl[y * R + tid] * __builtin_amdgcn_exp2f(mr[y * R] - M);
+            const size_t at = where(tid);
+            a.m[at] = M;
+            a.l[at] = L;
+        }
+        for (int e = tid; e < (int)n * D / 4; e += 256) {
+            const int row = e / (D / 4), d = (e % (D / 4)) * 4;
+            const float *s = so + row * D + d;
+            *(f4a *)(a.o + where(row) * D + d) = (*(const f4a *)s + *(const f4a *)(s + R * D)) +
+                                                 (*(const f4a *)(s + 2 * R * D) + *(const f4a *)(s + 3 * R * D));
         }
     }
 };
 
-// LDS floats of an item: the query rows, or the four waves' sums of a tile.
-template <int D, int RT>
-constexpr int lds_floats() {
-    const int q = RT * 16 * (D + 4), j = 4 * 16 * D + 2 * 4 * 16;
-    return q > j ? q : j;
+// --- many rows: a wave takes 16 rows and 256 dims (of heads of 512, two waves
+// the halves, whose scores they exchange) and all waves share the keys, whose K
+// and V rows go through LDS (two buffers of 16 keys: the next group is read
+// while one is multiplied, and stored behind it).  The query rows stay in
+// registers.  A K row's stride of D + 4 floats spreads the 16 rows that a read
+// takes over the banks.
+template <int D>
+struct Shared {
+    f4a k[2][16][D / 4 + 1], v[2][16][D / 4], s[D == 512 ? 4 : 1][64];
+    uint32_t slot[2][16], full;
+};
+constexpr uint32_t rows_wg(uint32_t D) { return 64 / (D / 256); }     // rows of a workgroup
+// q: row c of this wave's 16, its 256 dims; n: how many rows the workgroup has
+template <int D, typename F>
+__device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a (&q)[16], Shared<D> &sh, const Keys &k,
+                                         uint32_t n, F &&where) {
+    constexpr int H = D / 256, RG = 4 / H;
+    const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rows = wave % RG, half = wave / RG;
+    f4a sk[4][H], sv[4][H];                        // keys wave, wave + 4, ..: this lane's dims 4 lane + 256 h
+    auto load = [&](uint32_t slot) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            const uint32_t s = __builtin_amdgcn_readlane(slot, wave + 4 * x);
+            const float *kr = cache_row<D>(a, a.kc, s, k.kvh) + 4 * lane, *vr = cache_row<D>(a, a.vc, s, k.kvh) + 4 * lane;
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                sk[x][h] = *(const f4a *)(kr + 256 * h);
+                sv[x][h] = *(const f4a *)(vr + 256 * h);
+            }
+        }
+    };
+    auto store = [&](int b, uint32_t slot) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x)
+#pragma unroll
+            for (int h = 0; h < H; ++h) {
+                sh.k[b][wave + 4 * x][64 * h + lane] = sk[x][h];
+                sh.v[b][wave + 4 * x][64 * h + lane] = sv[x][h];
+            }
+        if (threadIdx.x < 16) sh.slot[b][threadIdx.x] = slot;
+    };
+    f4a x[2][4];                                   // four LDS reads ahead of the products, no more: the registers are full
+    auto scores = [&](int b) {
+        f4a part[4];                               // four chains: shorter sums round less
+        auto read = [&](int s) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) x[s & 1][y] = sh.k[b][c][64 * half + 16 * s + 4 * y + g];
+        };
+#pragma unroll
+        for (int j = 0; j < 4; ++j) part[j] = f4a{0, 0, 0, 0};
+        read(0);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+            if (s + 1 < 4) read(s + 1);
+            issue_fence();
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    part[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s & 1][y][j], q[4 * s + y][j], part[j], 0, 0, 0);
+            issue_fence();
+        }
+        return (part[0] + part[1]) + (part[2] + part[3]);
+    };
+    // the whole heads' scores: both waves of a pair add them in the same order
+    auto whole = [&](f4a s) {
+        if constexpr (H == 2) {
+            sh.s[wave][lane] = s;
+            __syncthreads();
+            const f4a o = sh.s[wave ^ RG][lane];
+            s = half ? o + s : s + o;
+        }
+        return s;
+    };
+    auto weigh = [&](const f4a &s, int b) {
+        auto read = [&](int e) {
+#pragma unroll
+            for (int y = 0; y < 4; ++y) x[e & 1][y] = sh.v[b][4 * g + e][64 * half + 16 * y + c];
+        };
+        read(0);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            if (e + 1 < 4) read(e + 1);
+            issue_fence();
+#pragma unroll
+            for (int y = 0; y < 4; ++y)
+#pragma unroll
+                for (int j = 0; j < 4; ++j)
+                    w.o[y][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[e], x[e & 1][y][j], w.o[y][j], 0, 0, 0);
+            issue_fence();
+        }
+    };
+    // the groups that every row of the workgroup sees whole, then the others
+    if (threadIdx.x == 0) sh.full = k.end;
+    __syncthreads();
+    if (lane == 0) atomicMin(&sh.full, w.full);
+    uint32_t slot = k.slot(a, k.begin, c, k.block(a, k.begin, c)), nextb = k.block(a, k.begin + 16, c);
+    load(slot);
+    store(0, slot);
+    __syncthreads();
+    const uint32_t full = __builtin_amdgcn_readfirstlane(sh.full);
+    uint32_t kb = k.begin;
+    int b = 0;
+#pragma unroll 1
+    for (; kb < full; kb += 16, b ^= 1) {
+        slot = k.slot(a, kb + 16, c, nextb);
+        nextb = k.block(a, kb + 32, c);
+        load(slot);                                // past the end: the row of zeros, not used
+        issue_fence();
+        f4a s = whole(scores(b));
+        uint32_t vs[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) vs[i] = sh.slot[b][4 * g + i];
+        s = w.softmax(a, s, [&](int i) { return vs[i] != kBadSlot; });
+        weigh(s, b);
+        issue_fence();
+        store(b ^ 1, slot);                        // last read before the barrier at the end of the round before
+        __syncthreads();
+    }
+#pragma unroll 1
+    for (; kb < k.end; kb += 16, b ^= 1) {
+        slot = k.slot(a, kb + 16, c, k.block(a, kb + 16, c));
+        f4a s = whole(scores(b));
+        s = w.softmax(a, s, [&](int i) { return sh.slot[b][4 * g + i] != kBadSlot && kb + 4 * g + i < w.lim; });
+        w.weigh_part(s, kb, [&](int key) { return (const float *)&sh.v[b][key][64 * half]; });
+        load(slot);
+        store(b ^ 1, slot);
+        __syncthreads();
+    }
+    w.end(k);
+    const float lt = rows4_sum(w.l);
+    if (half == 0 && g == 0 && rows * 16 + c < (int)n) {
+        const size_t at = where(rows * 16 + c);
+        a.m[at] = w.m;
+        a.l[at] = lt;
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const uint32_t row = rows * 16 + 4 * g + i;
+        if (row >= n) continue;
+        float *out = a.o + where(row) * D + 256 * half + 4 * c;
+#pragma unroll
+        for (int y = 0; y < 4; ++y) *(f4a *)(out + 64 * y) = f4a{w.o[y][0][i], w.o[y][1][i], w.o[y][2][i], w.o[y][3][i]};
+    }
 }
 
-template <int D, int RT>
-__global__ __launch_bounds__(256, RT == 1 && D == 256 ? 2 : 1) void k_prefix_attn(PrefixAttn a) {
-    extern __shared__ float sh[];
+// LDS bytes of an item: the waves' sums (the query rows take less), or the
+// keys that they share.
+template <int D, int RQ, bool ROWS>
+constexpr size_t lds_bytes() {
+    const size_t own = (4 * 4 * RQ * (D + 2)) * 4, prefix = ROWS ? sizeof(Shared<D>) : (4 * 16 * (D + 2)) * 4;
+    return own > prefix ? own : prefix;
+}
+
+// RQ: quads of rows of own items.  ROWS: whether prefix items hold rows_wg
+// rows, 16 a wave, or 16 that the waves share.
+template <int D, int RQ, bool ROWS>
+__global__ __launch_bounds__(256, D == 256 ? 2 : 1) void k_prefix_attn(PrefixAttn a) {
+    extern __shared__ f4a sh4[];
+    float *const sh = (float *)sh4;
     const int tid = threadIdx.x, lane = tid & 63;
     const uint32_t P = a.npb << a.shift;
-    // rows from..from + n of the (request, head-in-group) rows of a KV head into LDS, zeros behind them
+    // a KV head's row: (request, head in the group)
+    auto q_row = [&](uint32_t kvh, uint32_t row) {
+        const uint32_t r = row / a.gqa, h = row - r * a.gqa;
+        return a.q + ((size_t)r * a.num_q + kvh * a.gqa + h) * D;
+    };
+    // rows from `from` on into LDS, zeros behind the n that there are
     auto load_q = [&](uint32_t kvh, uint32_t from, uint32_t n, int rows) {
         for (int e = tid; e < rows * (D / 4); e += 256) {
             const uint32_t row = e / (D / 4), d = (e % (D / 4)) * 4;
-            f4a v = {0, 0, 0, 0};
-            if (row < n) {
-                const uint32_t r = (from + row) / a.gqa, h = (from + row) - r * a.gqa;
-                v = *(const f4a *)(a.q + ((size_t)r * a.num_q + kvh * a.gqa + h) * D + d);
-            }
-            *(f4a *)(sh + row * (D + 4) + d) = v;
+            *(f4a *)(sh + row * (D + 16) + d) = row < n ? *(const f4a *)(q_row(kvh, from + row) + d) : f4a{0, 0, 0, 0};
         }
         __syncthreads();
     };
     if (blockIdx.x < a.prefix_wgs) {
         // the row tiles of one unit run on one XCD (workgroup i runs on XCD i % 8) and share its keys there
+        constexpr uint32_t R = ROWS ? rows_wg(D) : 16;
         const uint32_t b = blockIdx.x, tile = (b >> 3) % a.tiles, u = (b >> 3) / a.tiles * 8 + (b & 7);
         if (u >= a.num_kv * a.splits) return;
-        const uint32_t kvh = u % a.num_kv, split = u / a.num_kv;
-        const uint32_t begin = split * a.split_keys, end = min(begin + a.split_keys, P);
-        const uint32_t M = a.n_req * a.gqa, row0 = tile * (RT * 16), n = min(M - row0, (uint32_t)RT * 16);
-        uint32_t lim[RT];
-#pragma unroll
-        for (int rt = 0; rt < RT; ++rt) {
-            const uint32_t row = rt * 16 + (lane & 15);
-            lim[rt] = row < n ? a.lens[(row0 + row) / a.gqa] : 0u;
-        }
-        load_q(kvh, row0, n, RT * 16);
-        Tile<D, RT> t;
-        t.run(a, sh, a.prefix, kvh, begin, end, lim);
-        t.join(sh, [&](uint32_t row, float *&po, float *&pm, float *&pl) {
-            if (row >= n) return false;
+        const uint32_t kvh = u % a.num_kv, split = u / a.num_kv, begin = split * a.split_keys;
+        const Keys k{a.prefix, begin, min(begin + a.split_keys, P), kvh};
+        const uint32_t row0 = tile * R, n = min(a.n_req * a.gqa - row0, R);
+        auto where = [&](uint32_t row) {
             const uint32_t r = (row0 + row) / a.gqa, h = (row0 + row) - r * a.gqa;
-            const size_t at = ((size_t)split * a.n_req + r) * a.num_q + kvh * a.gqa + h;
-            po = a.po + at * D;
-            pm = a.pm + at;
-            pl = a.pl + at;
-            return true;
-        });
+            return ((size_t)split * a.n_req + r) * a.num_q + kvh * a.gqa + h;
+        };
+        auto limit = [&](uint32_t row) { return row < n ? a.lens[(row0 + row) / a.gqa] : 0u; };
+        if constexpr (ROWS) {
+            const uint32_t mine = (tid >> 6) * 16 % R + (lane & 15);
+            Rows w;
+            w.start(limit(mine), k);
+            f4a q[16];
+            const float *x = q_row(kvh, row0 + (mine < n ? mine : 0u)) + (tid >> 6) * 16 / R * 256 + 4 * (lane >> 4);
+#pragma unroll
+            for (int s = 0; s < 16; ++s) q[s] = *(const f4a *)(x + 16 * s);
+            run_rows<D>(a, w, q, *(Shared<D> *)sh4, k, n, where);
+        } else {
+            load_q(kvh, row0, n, 16);
+            Quads<D, 4> w;
+            w.run(a, sh, k, limit);
+            w.join(a, sh, n, where);
+        }
         return;
     }
     // an own item
@@ -419,9 +689,9 @@ __global__ __launch_bounds__(256, RT == 1 && D == 256 ? 2 : 1) void k_prefix_att
         const uint32_t incl = start + wave_scan_u32(n, lane);
         const uint64_t mine = __ballot(n && item >= incl - n && item < incl);
         if (mine) {
-            const int w = __ffsll((unsigned long long)mine) - 1;
-            req = r0 + w;
-            first = item - __shfl(incl - n, w, 64);
+            const int x = __ffsll((unsigned long long)mine) - 1;
+            req = r0 + x;
+            first = item - __shfl(incl - n, x, 64);
         }
         if (b == 0 && tid < 64 && r < a.n_req) {       // for the launch that joins
             a.own_start[r] = incl - n;
@@ -430,73 +700,94 @@ __global__ __launch_bounds__(256, RT == 1 && D == 256 ? 2 : 1) void k_prefix_att
         start = __shfl(incl, 63, 64);
     }
     if (req == kBadSlot) return;
-    const uint32_t len = min(a.lens[req], a.max_blocks << a.shift);
-    const uint32_t begin = P + first * per * 16, end = (uint32_t)min((uint64_t)len, (uint64_t)begin + (uint64_t)per * 16);
-    const uint32_t lim[1] = {(uint32_t)(lane & 15) < a.gqa ? end : 0u};
-    load_q(kvh, req * a.gqa, a.gqa, 16);
-    Tile<D, 1> t;
-    t.run(a, sh, a.tables + (size_t)req * a.max_blocks, kvh, begin, end, lim);
-    t.join(sh, [&](uint32_t row, float *&po, float *&pm, float *&pl) {
-        if (row >= a.gqa) return false;
-        const size_t at = (size_t)item * a.num_q + kvh * a.gqa + row;
-        po = a.oo + at * D;
-        pm = a.om + at;
-        pl = a.ol + at;
-        return true;
+    const uint32_t len = min(a.lens[req], a.max_blocks << a.shift), begin = P + first * per * 16;
+    const Keys k{a.tables + (size_t)req * a.max_blocks, begin,
+                 (uint32_t)min((uint64_t)len, (uint64_t)begin + (uint64_t)per * 16), kvh};
+    load_q(kvh, req * a.gqa, a.gqa, 4 * RQ);
+    Quads<D, RQ> w;
+    w.run(a, sh, k, [&](uint32_t row) { return row < a.gqa ? k.end : 0u; });
+    w.join(a, sh, a.gqa, [&](uint32_t row) {
+        return ((size_t)a.splits * a.n_req + item) * a.num_q + kvh * a.gqa + row;
     });
 }
 
-// Joins a query row's partial results: a wave per row, four values per lane
-// and 256 dims.
+// Joins a query row's partial results: a workgroup per row, its waves take
+// every fourth part, a lane four values per 256 dims.  The parts' weights are
+// formed a lane each, 64 parts at a time, so the sums' loads wait for nothing
+// but one another's queue.
 template <int D>
 __global__ __launch_bounds__(256) void k_prefix_join(PrefixAttn a) {
-    const int lane = threadIdx.x & 63;
-    const uint32_t row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= a.n_req * a.num_q) return;
-    const uint32_t r = row / a.num_q, h = row - r * a.num_q, stride = a.n_req * a.num_q;
-    const bool own = a.own_start != nullptr;
-    const uint32_t o0 = own ? a.own_start[r] : 0u, no = own ? a.own_start[r + 1] - o0 : 0u;
-    const uint32_t parts = a.splits + no;
-    auto at = [&](uint32_t p, bool &prefix) {
-        prefix = p < a.splits;
-        return prefix ? (size_t)p * stride + row : (size_t)(o0 + p - a.splits) * a.num_q + h;
+    __shared__ f4a sh[4][D / 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t row = blockIdx.x, r = row / a.num_q, h = row - r * a.num_q, stride = a.n_req * a.num_q;
+    const uint32_t o0 = a.own_start ? a.own_start[r] : 0u, parts = a.splits + (a.own_start ? a.own_start[r + 1] - o0 : 0u);
+    // part p's place; the prefix's arrays lie before the own items'
+    auto at = [&](uint32_t p) {
+        return p < a.splits ? (size_t)p * stride + row : (size_t)a.splits * stride + (size_t)(o0 + p - a.splits) * a.num_q + h;
     };
     float M = kNone;
-    for (uint32_t p = lane; p < parts; p += 64) {
-        bool pre;
-        const size_t i = at(p, pre);
-        M = fmaxf(M, pre ? a.pm[i] : a.om[i]);
-    }
+    for (uint32_t p = lane; p < parts; p += 64) M = fmaxf(M, a.m[at(p)]);
     M = wave_max64(M);
     f4a acc[D / 256];
 #pragma unroll
     for (int k = 0; k < D / 256; ++k) acc[k] = f4a{0, 0, 0, 0};
     float L = 0.0f;
-    for (uint32_t p = 0; p < parts; ++p) {
-        bool pre;
-        const size_t i = at(p, pre);
-        const float m = pre ? a.pm[i] : a.om[i];
-        if (m == kNone) continue;
-        const float w = __builtin_amdgcn_exp2f(m - M);
-        const float *o = (pre ? a.po : a.oo) + i * D;
-        L += w * (pre ? a.pl[i] : a.ol[i]);
+    for (uint32_t p0 = 0; p0 < parts; p0 += 64) {
+        const uint32_t n = min(parts - p0, 64u);
+        float w = 0.0f, l = 0.0f;
+        if ((uint32_t)lane < n) {
+            const size_t i = at(p0 + lane);
+            const float m = a.m[i];
+            if (m != kNone) {
+                w = __builtin_amdgcn_exp2f(m - M);
+                l = w * a.l[i];
+            }
+        }
+        L += wave_sum64(l);
+        constexpr int U = 4;                                     // loads in flight
+        for (uint32_t p = wave; p < n; p += 4 * U) {
+            f4a v[U][D / 256];
 #pragma unroll
-        for (int k = 0; k < D / 256; ++k) acc[k] += w * *(const f4a *)(o + 256 * k + 4 * lane);
+            for (int u = 0; u < U; ++u) {
+                const float *o = a.o + at(p0 + min(p + 4 * u, n - 1)) * D + 4 * lane;
+#pragma unroll
+                for (int k = 0; k < D / 256; ++k) v[u][k] = *(const f4a *)(o + 256 * k);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const uint32_t q = min(p + 4 * u, n - 1);
+                const float wq = lane_f(w, q);
+                const bool some = p + 4 * u < n && lane_f(l, q) != 0.0f;     // a part without keys holds nothing
+#pragma unroll
+                for (int k = 0; k < D / 256; ++k) acc[k] += some ? wq * v[u][k] : f4a{0, 0, 0, 0};
+            }
+        }
     }
-    const float inv = parts && L != 0.0f ? 1.0f / L : 0.0f;      // no token: zeros
 #pragma unroll
-    for (int k = 0; k < D / 256; ++k) *(f4a *)(a.out + (size_t)row * D + 256 * k + 4 * lane) = acc[k] * inv;
+    for (int k = 0; k < D / 256; ++k) sh[wave][64 * k + lane] = acc[k];
+    __syncthreads();
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;               // no token: zeros
+    for (int e = tid; e < D / 4; e += 256)
+        *(f4a *)(a.out + (size_t)row * D + 4 * e) = ((sh[0][e] + sh[1][e]) + (sh[2][e] + sh[3][e])) * inv;
 }
 
-template <int D, int RT>
-static int launch_items(chn_ctx *ctx, const PrefixAttn &a, uint32_t grid) {
-    constexpr size_t lds = lds_floats<D, RT>() * sizeof(float);
+template <int D, int RQ, bool ROWS>
+static void launch_items(hipStream_t st, const PrefixAttn &a, uint32_t grid) {
+    constexpr size_t lds = lds_bytes<D, RQ, ROWS>();
     static_assert(lds <= 160 * 1024, "LDS per workgroup");
+    k_prefix_attn<D, RQ, ROWS><<<grid, 256, lds, st>>>(a);
+}
+
+template <int D>
+static int launch_prefix(chn_ctx *ctx, const PrefixAttn &a, uint32_t grid, bool rows) {
     if (grid) {
-        k_prefix_attn<D, RT><<<grid, 256, lds, ctx->stream>>>(a);
+        if (a.gqa <= 4 && rows) launch_items<D, 1, true>(ctx->stream, a, grid);
+        else if (a.gqa <= 4) launch_items<D, 1, false>(ctx->stream, a, grid);
+        else if (rows) launch_items<D, 4, true>(ctx->stream, a, grid);
+        else launch_items<D, 4, false>(ctx->stream, a, grid);
         CHN_LAUNCHED(ctx, "k_prefix_attn");
     }
-    k_prefix_join<D><<<(a.n_req * a.num_q + 3) / 4, 256, 0, ctx->stream>>>(a);
+    k_prefix_join<D><<<a.n_req * a.num_q, 256, 0, ctx->stream>>>(a);
     CHN_LAUNCHED(ctx, "k_prefix_join");
     return CHN_OK;
 }
@@ -549,12 +840,10 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
     a.exp_lo = std::isfinite(a.exp_hi) ? (float)(e - a.exp_hi) : 0.0f;
     a.out = out;
     const uint32_t P = n_prefix_blocks << a.shift, M = n_req * gqa_ratio;
-    const uint32_t rt_most = head_dim == 256 ? 2 : 1;
-    uint32_t rt = 1;
-    while (rt < rt_most && M > rt * 16) rt *= 2;
-    if (!P) rt = 1;
+    const bool by_rows = P && M > 32;
     if (P) {
-        a.tiles = (M + rt * 16 - 1) / (rt * 16);
+        const uint32_t R = !by_rows ? 16 : rows_wg(head_dim);
+        a.tiles = (M + R - 1) / R;
         // about one workgroup per CU, 64 keys (16 per wave) at least
         const uint32_t want = std::max(1u, 256 / std::max(1u, a.tiles * a.num_kv));
         a.split_keys = ((P + want - 1) / want + 63) / 64 * 64;
@@ -570,19 +859,13 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
         grid += items * a.num_kv;
     }
     if (grid > 0x7FFFFFFF) return set_err(ctx, CHN_E_UNSUPPORTED, "too many requests and heads for one call");
-    const size_t prow = (size_t)a.splits * n_req * num_q_heads, orow = (size_t)items * num_q_heads;
-    rc = ensure_workspace(ctx, (prow + orow) * (head_dim + 2) * 4 + ((size_t)n_req + 1) * 4);
+    const size_t rows = ((size_t)a.splits * n_req + (size_t)items) * num_q_heads;
+    rc = ensure_workspace(ctx, rows * (head_dim + 2) * 4 + ((size_t)n_req + 1) * 4);
     if (rc) return rc;
-    a.po = (float *)ctx->ws;
-    a.oo = a.po + prow * head_dim;
-    a.pm = a.oo + orow * head_dim;
-    a.pl = a.pm + prow;
-    a.om = a.pl + prow;
-    a.ol = a.om + orow;
-    a.own_start = items ? (uint32_t *)(a.ol + orow) : nullptr;
-    if (head_dim == 256) {
-        if (rt == 1) return launch_items<256, 1>(ctx, a, (uint32_t)grid);
-        return launch_items<256, 2>(ctx, a, (uint32_t)grid);
-    }
-    return launch_items<512, 1>(ctx, a, (uint32_t)grid);
+    a.o = (float *)ctx->ws;
+    a.m = a.o + rows * head_dim;
+    a.l = a.m + rows;
+    a.own_start = items ? (uint32_t *)(a.l + rows) : nullptr;
+    return head_dim == 256 ? launch_prefix<256>(ctx, a, (uint32_t)grid, by_rows)
+                           : launch_prefix<512>(ctx, a, (uint32_t)grid, by_rows);
 }
