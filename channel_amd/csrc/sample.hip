@@ -10,15 +10,38 @@
 // 43 bits: 2^20 weights of at most 2^43 fit 64, and the 2^-44 a rounding
 // costs is far below what 32-bit sums would lose (a flat row of 2^18 tokens
 // has its borders 2^-18 of the sum apart).
+//
+// Four launches; what a row needs of them depends on its settings, which only
+// the device knows:
+//  1 k_sample_max: the largest logit of every block of 64, and of every 2048;
+//  2 k_sample_mass (rows without top-k): with top-p a histogram of the weights
+//    over their distance from the largest, else the sums of 2048 at a time;
+//  3 k_sample_border (rows with top-p and without top-k): the bin that holds
+//    the border goes into a list, the weights above it are summed;
+//  4 k_sample_draw: a workgroup per row.  With top-k, the k-th largest block
+//    maximum bounds the k-th largest logit from below, and only blocks whose
+//    maximum reaches it can hold a kept token: the row is read once, and k
+//    blocks of it again.  Otherwise the border is found in the list, and the
+//    draw reads the one stretch of 2048 that it falls into.
+// Rows that fit none of this (top-k above kMaxK, a border among more equal or
+// near equal logits than the list holds) take k_sample_draw's walk over the
+// whole row, eight bits of the key at a time.
 #include "chn_internal.h"
 
 #include <cmath>
 
 namespace chn {
 
+typedef float f4u __attribute__((ext_vector_type(4), aligned(4)));
+
 constexpr uint32_t kSampleMaxV = 1u << 20;
 constexpr int kWeightBits = 43;
-constexpr uint32_t kRowThreads = 1024;
+constexpr uint32_t kStretch = 2048;         // values of a wave: one sum, 32 blocks
+constexpr uint32_t kBins = 2048;            // of 2^-6 powers of two each
+constexpr uint32_t kList = 4096;            // tokens of a row's list
+constexpr uint32_t kMaxK = 1024;            // top-k by block maxima
+constexpr uint32_t kDrawThreads = 1024;
+constexpr uint32_t kRowsAtOnce = 1024;      // rows that share the workspace
 
 struct Sample {
     const float *logits;
@@ -29,6 +52,12 @@ struct Sample {
     float softcap;
     uint32_t *tokens;
     float *probs;
+    // workspace, per row: block maxima and stretch maxima (orderable, 0: nothing allowed), sums of stretches, the
+    // histogram, the list and its length
+    uint32_t blocks, stretches;
+    uint32_t *bmax, *smax;
+    uint64_t *sums, *hist, *list;
+    uint32_t *listed;
 };
 
 __device__ __forceinline__ bool allowed(float v) { return v > -3.4028234663852886e38f; }   // not NaN either
@@ -36,204 +65,588 @@ __device__ __forceinline__ uint32_t orderable(float v) {
     const uint32_t u = __builtin_bit_cast(uint32_t, v + 0.0f);                             // -0 orders as +0
     return (u & 0x80000000u) ? ~u : (u | 0x80000000u);
 }
+__device__ __forceinline__ float value_of(uint32_t o) {
+    return __builtin_bit_cast(float, (o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
+}
 __device__ __forceinline__ uint64_t token_key(float v, uint32_t i) {
     return ((uint64_t)orderable(v) << 32) | (0xFFFFFFFFu - i);
 }
 
-// Weights of a row: cap * tanh(l / cap) relative to the row's largest.
-struct Weigh {
+// exp on half a power of two either way: x = n ln 2 + r, and (exp(r) - 1) by
+// its series (the 13th term is below 2^-52 of the first).
+struct Exp {
+    double em1, n;
+    __device__ __forceinline__ explicit Exp(double x) {
+        const double t = x * 1.4426950408889634074;
+        n = rint(t);
+        const double r = (t - n) * 0.69314718055994530942;
+        double p = 1.0 / 479001600.0;
+        p = fma(p, r, 1.0 / 39916800.0);
+        p = fma(p, r, 1.0 / 3628800.0);
+        p = fma(p, r, 1.0 / 362880.0);
+        p = fma(p, r, 1.0 / 40320.0);
+        p = fma(p, r, 1.0 / 5040.0);
+        p = fma(p, r, 1.0 / 720.0);
+        p = fma(p, r, 1.0 / 120.0);
+        p = fma(p, r, 1.0 / 24.0);
+        p = fma(p, r, 1.0 / 6.0);
+        p = fma(p, r, 0.5);
+        p = fma(p, r, 1.0);
+        em1 = p * r;
+    }
+};
+// exp(x) 2^bits
+__device__ __forceinline__ double exp_scaled(double x, int bits) {
+    const Exp e(x);
+    return ldexp(1.0 + e.em1, (int)e.n + bits);
+}
+// tanh(y) from exp(-2 |y|) - 1, which keeps its digits near 0
+__device__ __forceinline__ double tanh_of(double y) {
+    const Exp e(fmax(-2.0 * fabs(y), -64.0));
+    const double s = ldexp(1.0, (int)e.n), m = fma(s, e.em1, s - 1.0);
+    return copysign(-m / (2.0 + m), y);
+}
+
+// A row's settings and the weights of its tokens: cap * tanh(l / cap) (or l)
+// relative to the row's largest.
+struct Row {
     double cap, inv_cap, top, inv_t;
-    float raw_top;
-    __device__ __forceinline__ double capped(float l) const { return cap > 0.0 ? cap * tanh((double)l * inv_cap) : (double)l; }
+    float raw_top, bin_scale;
+    uint64_t least;                // min_p, as a weight
+    uint32_t k;                    // 0: no top-k
+    float p;                       // 1: no top-p
+    bool some, greedy;             // a token is allowed; the largest is taken
+
+    __device__ __forceinline__ Row(const Sample &a, uint32_t row, uint32_t largest) {
+        const float T = a.temperature ? a.temperature[row] : 1.0f;
+        some = largest != 0;
+        greedy = !(T > 0.0f);
+        raw_top = value_of(largest);
+        cap = a.softcap;
+        inv_cap = 1.0 / cap;
+        inv_t = 1.0 / (double)T;
+        top = capped(raw_top);
+        // 64 bins per power of two of the weight where the cap does not flatten it
+        bin_scale = fminf((float)(92.332482616893657 * inv_t), 1e30f);
+        const uint32_t kk = a.top_k ? a.top_k[row] : 0u;
+        k = kk < a.V ? kk : 0u;
+        const float pp = a.top_p ? a.top_p[row] : 1.0f, mm = a.min_p ? a.min_p[row] : 0.0f;
+        p = pp < 1.0f ? fmaxf(pp, 0.0f) : 1.0f;
+        least = mm > 0.0f ? (uint64_t)ceil(fmin((double)mm, 1.0) * (double)(1ull << kWeightBits)) : 0;
+    }
+    __device__ __forceinline__ double capped(float l) const {
+        return cap > 0.0 ? cap * tanh_of((double)l * inv_cap) : (double)l;
+    }
     __device__ __forceinline__ double weight(float l) const {                              // 2^kWeightBits exp(..)
         if (l == raw_top) return (double)(1ull << kWeightBits);
         const double x = (capped(l) - top) * inv_t;
-        return x > -64.0 ? exp(x) * (double)(1ull << kWeightBits) : 0.0;                  // below: rounds to zero anyway
+        return x > -64.0 ? exp_scaled(fmin(x, 0.0), kWeightBits) : 0.0;                   // below: rounds to zero
     }
-    __device__ __forceinline__ uint64_t units(float l) const { return (uint64_t)(weight(l) + 0.5); }
+    // 2^52 added leaves the rounded weight in the low bits
+    __device__ __forceinline__ uint64_t units(float l) const {
+        return __builtin_bit_cast(uint64_t, weight(l) + 4503599627370496.0) & ((1ull << 52) - 1);
+    }
+    __device__ __forceinline__ uint64_t kept(uint64_t w) const { return w >= least ? w : 0; }
+    // the bin of an allowed logit: larger logits never lie in a later one
+    __device__ __forceinline__ uint32_t bin(float l) const {
+        return l >= raw_top ? 0u : (uint32_t)fminf((raw_top - l) * bin_scale, (float)(kBins - 1));
+    }
+    // the running sum at which top-p ends, of a mass Z: kept while the mass before is below p Z, so the last one is
+    // the first whose running sum reaches ceil(p Z)
+    __device__ __forceinline__ uint64_t goal(uint64_t Z) const {
+        const double g = ceil((double)p * (double)Z);
+        const uint64_t n = g < 1.0 ? 1 : (uint64_t)g;
+        return n < Z ? n : Z;
+    }
+    __device__ __forceinline__ bool by_mass() const { return some && !greedy && k == 0; }
 };
 
+__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
+    return (uint64_t)__shfl_xor((unsigned long long)v, m, 64);
+}
 __device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += (uint64_t)__shfl_xor((unsigned long long)v, o, 64);
+    for (int o = 32; o >= 1; o >>= 1) v += shfl_xor64(v, o);
     return v;
 }
-__device__ __forceinline__ uint64_t wave_max_u64(uint64_t v) {
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, int lane) {                  // inclusive
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) {
-        const uint64_t w = (uint64_t)__shfl_xor((unsigned long long)v, o, 64);
-        v = w > v ? w : v;
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint64_t w = (uint64_t)__shfl_up((unsigned long long)v, o, 64);
+        if (lane >= o) v += w;
     }
     return v;
 }
+__device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = max(v, (uint32_t)__shfl_xor(v, o, 64));
+    return v;
+}
 
-// One workgroup per row.
-__global__ __launch_bounds__(kRowThreads) void k_sample_row(Sample a) {
-    constexpr int NW = kRowThreads / 64;
-    __shared__ uint64_t part[NW];
-    __shared__ uint64_t hist_w[256];
-    __shared__ uint32_t hist_n[256];
-    __shared__ uint64_t found[3];
+// f(index, value) for the wave's stretch of 2048 values, four per lane and
+// load (rows start at any 4-byte address); NaN behind the row's end.  g() after
+// each load's four.
+template <typename F, typename G>
+__device__ __forceinline__ void stretch(const Sample &a, const float *x, uint32_t s, F &&f, G &&g) {
+    const uint32_t i0 = s * kStretch + 4 * (threadIdx.x & 63);
+    f4u v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        const uint32_t i = i0 + 256 * j;
+        if (i + 4 <= a.V) v[j] = *(const f4u *)(x + i);
+        else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j][e] = i + e < a.V ? x[i + e] : __builtin_nanf("");
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) f(i0 + 256 * j + e, v[j][e]);
+        g(j);
+    }
+}
+
+// the row's largest logit, by every wave
+__device__ __forceinline__ uint32_t row_top(const Sample &a, uint32_t row) {
+    uint32_t m = 0;
+    for (uint32_t i = threadIdx.x & 63; i < a.stretches; i += 64) m = max(m, a.smax[(size_t)row * a.stretches + i]);
+    return wave_max_u32(m);
+}
+
+// A wave per stretch: maxima of 64 (16 lanes of a load) and of all.  The
+// row's first workgroup clears its histogram.
+__global__ __launch_bounds__(256) void k_sample_max(Sample a) {
+    const uint32_t row = blockIdx.y, s = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    if (blockIdx.x == 0) {
+        for (uint32_t i = threadIdx.x; i < kBins; i += 256) a.hist[(size_t)row * kBins + i] = 0;
+        if (threadIdx.x == 0) a.listed[row] = 0;
+    }
+    if (s >= a.stretches) return;
+    float m = -__builtin_inff(), most = m;
+    stretch(a, a.logits + (size_t)row * a.ld, s,
+            [&](uint32_t, float v) { m = fmaxf(m, allowed(v) ? v : -__builtin_inff()); },
+            [&](int j) {
+                m = row16_max(m);
+                const uint32_t b = s * 32 + 4 * j + (lane >> 4);
+                if ((lane & 15) == 0 && b < a.blocks) a.bmax[(size_t)row * a.blocks + b] = allowed(m) ? orderable(m) : 0u;
+                most = fmaxf(most, m);
+                m = -__builtin_inff();
+            });
+    most = wave_max64(most);
+    if (lane == 0) a.smax[(size_t)row * a.stretches + s] = allowed(most) ? orderable(most) : 0u;
+}
+
+// Rows without top-k: the histogram of the weights (with top-p), or the sums of
+// the stretches.
+__global__ void k_sample_mass(Sample a) {
+    __shared__ uint64_t hist[kBins];
+    const uint32_t row = blockIdx.y, s = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    const Row r(a, row, row_top(a, row));
+    if (!r.by_mass()) return;                                        // the whole workgroup
+    const float *x = a.logits + (size_t)row * a.ld;
+    if (r.p < 1.0f) {
+        for (uint32_t i = threadIdx.x; i < kBins; i += blockDim.x) hist[i] = 0;
+        __syncthreads();
+        if (s < a.stretches)
+            stretch(a, x, s,
+                    [&](uint32_t, float v) {
+                        const uint64_t w = allowed(v) ? r.units(v) : 0;
+                        if (w) atomicAdd((unsigned long long *)&hist[r.bin(v)], (unsigned long long)w);
+                    },
+                    [](int) {});
+        __syncthreads();
+        for (uint32_t i = threadIdx.x; i < kBins; i += blockDim.x)
+            if (hist[i]) atomicAdd((unsigned long long *)&a.hist[(size_t)row * kBins + i], (unsigned long long)hist[i]);
+    } else if (s < a.stretches) {
+        uint64_t sum = 0;
+        stretch(a, x, s, [&](uint32_t, float v) { sum += allowed(v) ? r.kept(r.units(v)) : 0; }, [](int) {});
+        sum = wave_sum_u64(sum);
+        if ((threadIdx.x & 63) == 0) a.sums[(size_t)row * a.stretches + s] = sum;
+    }
+}
+
+// The bin in which a row's running sum reaches its goal, and the goal's rest
+// there.  All threads; sh: 20 words.
+__device__ __forceinline__ uint32_t border_bin(const Sample &a, const Row &r, uint32_t row, uint64_t *sh, uint64_t &rest) {
+    const uint32_t tid = threadIdx.x, nt = blockDim.x, per = kBins / nt;       // 256 or 1024 threads: 8 or 2 bins
+    const int lane = tid & 63, wave = tid >> 6, nw = nt >> 6;
+    const uint64_t *h = a.hist + (size_t)row * kBins + tid * per;
+    uint64_t own = 0;
+    for (uint32_t i = 0; i < per; ++i) own += h[i];
+    const uint64_t incl = wave_scan_u64(own, lane);
+    if (lane == 63) sh[wave] = incl;
+    __syncthreads();
+    uint64_t before = incl - own, Z = 0;
+    for (int w = 0; w < nw; ++w) {
+        before += w < wave ? sh[w] : 0;
+        Z += sh[w];
+    }
+    const uint64_t g = r.goal(Z);
+    if (before < g && before + own >= g) {
+        uint32_t b = tid * per;
+        for (; before + *h < g; ++h, ++b) before += *h;
+        sh[18] = b;
+        sh[19] = g - before;
+    }
+    __syncthreads();
+    rest = sh[19];
+    return (uint32_t)sh[18];
+}
+
+// Rows with top-p and without top-k: the tokens of the border's bin into the
+// list, the kept weights above it summed by stretch.
+__global__ void k_sample_border(Sample a) {
+    __shared__ uint64_t sh[20];
+    const uint32_t row = blockIdx.y, s = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    const Row r(a, row, row_top(a, row));
+    if (!r.by_mass() || !(r.p < 1.0f)) return;
+    uint64_t rest;
+    const uint32_t border = border_bin(a, r, row, sh, rest);
+    if (s >= a.stretches) return;
+    uint64_t sum = 0;
+    stretch(a, a.logits + (size_t)row * a.ld, s,
+            [&](uint32_t i, float v) {
+                const uint32_t b = allowed(v) ? r.bin(v) : kBins;
+                if (b < border) sum += r.kept(r.units(v));
+                if (b == border) {
+                    const uint32_t at = atomicAdd(&a.listed[row], 1u);
+                    if (at < kList) a.list[(size_t)row * kList + at] = token_key(v, i);
+                }
+            },
+            [](int) {});
+    sum = wave_sum_u64(sum);
+    if ((threadIdx.x & 63) == 0) a.sums[(size_t)row * a.stretches + s] = sum;
+}
+
+// LDS of k_sample_draw.
+struct Draw {
+    uint64_t list[kList], hist_w[256], part[kDrawThreads / 64], found[3];
+    uint32_t hist_n[256], n, hit;
+};
+
+// A workgroup per row: the kept tokens' last key, then the draw.
+__global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
+    extern __shared__ uint64_t lds[];
+    constexpr int NW = kDrawThreads / 64;
+    Draw &sh = *(Draw *)lds;
+    uint32_t *spare = (uint32_t *)(lds + sizeof(Draw) / 8);          // block maxima, then blocks; or sums of stretches
     const uint32_t tid = threadIdx.x, row = blockIdx.x;
     const int lane = tid & 63, wave = tid >> 6;
     const float *x = a.logits + (size_t)row * a.ld;
+    const uint32_t *bmax = a.bmax + (size_t)row * a.blocks;
+    const Row r(a, row, row_top(a, row));
 
-    auto block_sum = [&](uint64_t v) {
-        v = wave_sum_u64(v);
-        __syncthreads();
-        if (lane == 0) part[wave] = v;
-        __syncthreads();
-        uint64_t t = 0;
-        for (int w = 0; w < NW; ++w) t += part[w];
-        return t;
+    auto finish = [&](uint32_t token, float prob) {
+        a.tokens[row] = token;
+        if (a.probs) a.probs[row] = prob;
     };
-
-    uint64_t top = 0;
-    for (uint32_t i = tid; i < a.V; i += kRowThreads) {
-        const float v = x[i];
-        const uint64_t k = allowed(v) ? token_key(v, i) : 0;
-        top = k > top ? k : top;
+    if (!r.some) {
+        if (tid == 0) finish(CHN_NO_TOKEN, 0.0f);
+        return;
     }
-    top = wave_max_u64(top);
-    if (lane == 0) part[wave] = top;
-    __syncthreads();
-    for (int w = 0; w < NW; ++w) top = part[w] > top ? part[w] : top;
-    const float T = a.temperature ? a.temperature[row] : 1.0f;
-    if (top == 0 || !(T > 0.0f)) {
-        if (tid == 0) {
-            a.tokens[row] = top ? 0xFFFFFFFFu - (uint32_t)top : CHN_NO_TOKEN;
-            if (a.probs) a.probs[row] = top ? 1.0f : 0.0f;
+    if (r.greedy) {
+        // the first block that holds the largest logit, and its first place there
+        if (tid == 0) sh.hit = 0xFFFFFFFFu;
+        __syncthreads();
+        const uint32_t want = orderable(r.raw_top);
+        for (uint32_t b = tid; b < a.blocks; b += kDrawThreads)
+            if (bmax[b] == want) {
+                atomicMin(&sh.hit, b);
+                break;
+            }
+        __syncthreads();
+        if (wave == 0) {
+            const uint32_t i = sh.hit * 64 + lane;
+            const uint64_t at = __ballot(i < a.V && x[i < a.V ? i : a.V - 1] == r.raw_top);
+            if (lane == 0) finish(sh.hit * 64 + __ffsll((unsigned long long)at) - 1, 1.0f);
         }
         return;
     }
-    Weigh wg;
-    wg.cap = a.softcap;
-    wg.inv_cap = 1.0 / (double)a.softcap;
-    wg.raw_top = x[0xFFFFFFFFu - (uint32_t)top];
-    wg.top = wg.capped(wg.raw_top);
-    wg.inv_t = 1.0 / (double)T;
-
-    // The key of the last token of the order, from the tokens at or above
-    // `above`, that the running count (or sum of weights) needs to reach
-    // `goal`: eight bits of the key at a time, until the bin is wanted whole.
-    auto last_key = [&](uint64_t above, bool by_weight, uint64_t goal) {
+    auto block_sum = [&](uint64_t v) {
+        v = wave_sum_u64(v);
+        __syncthreads();
+        if (lane == 0) sh.part[wave] = v;
+        __syncthreads();
+        uint64_t t = 0;
+        for (int w = 0; w < NW; ++w) t += sh.part[w];
+        return t;
+    };
+    auto block_min = [&](uint64_t v) {
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) v = min(v, shfl_xor64(v, o));
+        __syncthreads();
+        if (lane == 0) sh.part[wave] = v;
+        __syncthreads();
+        for (int w = 0; w < NW; ++w) v = min(v, sh.part[w]);
+        return v;
+    };
+    // inclusive running sum over the threads, and the whole sum
+    auto block_scan = [&](uint64_t v, uint64_t &total) {
+        v = wave_scan_u64(v, lane);
+        __syncthreads();
+        if (lane == 63) sh.part[wave] = v;
+        __syncthreads();
+        total = 0;
+        for (int w = 0; w < NW; ++w) {
+            v += w < wave ? sh.part[w] : 0;
+            total += sh.part[w];
+        }
+        return v;
+    };
+    // what the draw looks for: a running sum above this
+    auto target_of = [&](uint64_t Z) {
+        const float u = a.u[row];
+        const double want = (u > 0.0f ? (double)u : 0.0) * (double)Z;
+        const uint64_t t = want >= (double)Z ? Z - 1 : (uint64_t)want;
+        return t < Z ? t : Z - 1;
+    };
+    // every(f): f(key) for all tokens looked through.  The key of the last token of the order, from those at or above
+    // `above`, that the running count (or sum of weights) needs to reach `goal`: eight bits of the key at a time, until
+    // the bin is wanted whole.
+    auto last_key = [&](auto &&every, uint64_t above, bool by_weight, uint64_t goal) {
         uint64_t prefix = 0;
         for (int shift = 56;; shift -= 8) {
             __syncthreads();
             if (tid < 256) {
-                hist_n[tid] = 0;
-                hist_w[tid] = 0;
+                sh.hist_n[tid] = 0;
+                sh.hist_w[tid] = 0;
             }
             __syncthreads();
-            for (uint32_t i = tid; i < a.V; i += kRowThreads) {
-                const float v = x[i];
-                if (!allowed(v)) continue;
-                const uint64_t k = token_key(v, i);
-                if (k < above || (shift < 56 && (k >> (shift + 8)) != prefix)) continue;
-                const uint32_t bin = (uint32_t)(k >> shift) & 255u;
-                atomicAdd(&hist_n[bin], 1u);
-                if (by_weight) atomicAdd((unsigned long long *)&hist_w[bin], (unsigned long long)wg.units(v));
-            }
+            every([&](uint64_t key) {
+                if (key < above || (shift < 56 && (key >> (shift + 8)) != prefix)) return;
+                const uint32_t bin = (uint32_t)(key >> shift) & 255u;
+                atomicAdd(&sh.hist_n[bin], 1u);
+                if (by_weight)
+                    atomicAdd((unsigned long long *)&sh.hist_w[bin], (unsigned long long)r.units(value_of(key >> 32)));
+            });
             __syncthreads();
-            if (tid == 0) {
-                uint64_t sum = 0;
-                int bin = 255, last = -1;
-                for (; bin >= 0; --bin) {
-                    const uint64_t c = by_weight ? hist_w[bin] : hist_n[bin];
-                    if (hist_n[bin]) last = bin;
-                    if (sum + c >= goal) break;
-                    sum += c;
+            if (wave == 0) {
+                // lane 0 has the four largest bins
+                uint64_t c[4], own = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const int bin = 255 - 4 * lane - i;
+                    c[i] = by_weight ? sh.hist_w[bin] : sh.hist_n[bin];
+                    own += c[i];
                 }
-                if (bin < 0) bin = last;                       // fewer than wanted: the last token there is
-                found[0] = bin;
-                found[1] = sum;
-                found[2] = shift == 0 || hist_n[bin] == 1 || (!by_weight && sum + hist_n[bin] == goal);
+                uint64_t before = wave_scan_u64(own, lane) - own;
+                if (before < goal && before + own >= goal) {
+                    int i = 0;
+                    for (; before + c[i] < goal; ++i) before += c[i];
+                    const int bin = 255 - 4 * lane - i;
+                    sh.found[0] = bin;
+                    sh.found[1] = before;
+                    sh.found[2] = shift == 0 || sh.hist_n[bin] == 1 || (!by_weight && before + sh.hist_n[bin] == goal);
+                }
             }
             __syncthreads();
-            prefix = (prefix << 8) | found[0];
-            goal -= found[1] < goal ? found[1] : goal;
-            if (found[2]) {
-                const uint64_t key = prefix << shift;          // the bin's lower end: it may reach below `above`
+            prefix = (prefix << 8) | sh.found[0];
+            goal -= sh.found[1];
+            if (sh.found[2]) {
+                const uint64_t key = prefix << shift;              // the bin's lower end: it may reach below `above`
                 return key > above ? key : above;
             }
         }
     };
-    auto mass = [&](uint64_t above, uint64_t least) {
-        uint64_t s = 0;
-        for (uint32_t i = tid; i < a.V; i += kRowThreads) {
+    auto whole_row = [&](auto &&f) {
+        for (uint32_t i = tid; i < a.V; i += kDrawThreads) {
             const float v = x[i];
-            if (!allowed(v) || token_key(v, i) < above) continue;
-            const uint64_t w = wg.units(v);
-            s += w >= least ? w : 0;
+            if (allowed(v)) f(token_key(v, i));
         }
-        return block_sum(s);
+    };
+    // The draw from the kept tokens of a row given the sums of its stretches (n of them, in LDS).
+    auto draw_stretch = [&](uint64_t above, const uint64_t *sums) {
+        uint64_t Z, own = 0;
+        const uint32_t n = a.stretches;                               // at most kSampleMaxV / kStretch = 512
+        own = tid < n ? sums[tid] : 0;
+        const uint64_t incl = block_scan(own, Z), target = target_of(Z);
+        if (own && incl > target && incl - own <= target) {
+            sh.hit = tid;
+            sh.found[0] = target - (incl - own);
+        }
+        __syncthreads();
+        const uint32_t i = sh.hit * kStretch + 2 * tid;
+        const uint64_t rest = sh.found[0];
+        float v[2];
+        uint64_t w[2], total;
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            v[e] = i + e < a.V ? x[i + e] : __builtin_nanf("");
+            w[e] = allowed(v[e]) && token_key(v[e], i + e) >= above ? r.kept(r.units(v[e])) : 0;
+        }
+        uint64_t run = block_scan(w[0] + w[1], total) - w[0] - w[1];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+            if (w[e] && run <= rest && run + w[e] > rest) finish(i + e, (float)(r.weight(v[e]) / (double)Z));
+            run += w[e];
+        }
+    };
+    // The sums of the stretches, formed here.
+    auto draw_whole = [&](uint64_t above) {
+        uint64_t *sums = (uint64_t *)spare;
+        for (uint32_t s = wave; s < a.stretches; s += NW) {
+            uint64_t sum = 0;
+            stretch(a, x, s,
+                    [&](uint32_t i, float v) {
+                        if (allowed(v) && token_key(v, i) >= above) sum += r.kept(r.units(v));
+                    },
+                    [](int) {});
+            sum = wave_sum_u64(sum);
+            if (lane == 0) sums[s] = sum;
+        }
+        __syncthreads();
+        draw_stretch(above, sums);
+    };
+    auto walk = [&] {
+        uint64_t above = 1, Z = 0;
+        if (r.k) {
+            uint64_t n = 0;
+            whole_row([&](uint64_t) { ++n; });
+            if (block_sum(n) > r.k) above = last_key(whole_row, 1, false, r.k);
+        }
+        if (r.p < 1.0f) {
+            whole_row([&](uint64_t key) { Z += key >= above ? r.units(value_of(key >> 32)) : 0; });
+            Z = block_sum(Z);
+            above = last_key(whole_row, above, true, r.goal(Z));
+        }
+        draw_whole(above);
     };
 
-    uint64_t above = 1;
-    const uint32_t k = a.top_k ? a.top_k[row] : 0;
-    if (k && k < a.V) {
-        uint64_t n = 0;
-        for (uint32_t i = tid; i < a.V; i += kRowThreads) n += allowed(x[i]) ? 1 : 0;
-        if (block_sum(n) > k) above = last_key(1, false, k);
-    }
-    const float p = a.top_p ? a.top_p[row] : 1.0f;
-    if (p < 1.0f) {
-        const uint64_t Z = mass(above, 0);
-        // kept while the mass before is below p Z: the last one is the first whose running sum reaches ceil(p Z)
-        const double goal = ceil((p > 0.0f ? (double)p : 0.0) * (double)Z);
-        const uint64_t g = goal < 1.0 ? 1 : (uint64_t)goal;
-        above = last_key(above, true, g < Z ? g : Z);
-    }
-    const float m = a.min_p ? a.min_p[row] : 0.0f;
-    const uint64_t least = m > 0.0f ? (uint64_t)ceil(fmin((double)m, 1.0) * (double)(1ull << kWeightBits)) : 0;
-    const uint64_t Z = mass(above, least);
-    const float uf = a.u[row];
-    const double want = (uf > 0.0f ? (double)uf : 0.0) * (double)Z;
-    uint64_t target = want >= (double)Z ? Z - 1 : (uint64_t)want;
-    target = target < Z ? target : Z - 1;
-
-    // the first index whose running sum exceeds target: a range of indexes in
-    // as many parts as there are waves, then that part again, until a thread
-    // each is left
-    uint32_t lo = 0, n = a.V;
-    for (;;) {
-        const uint32_t len = (n + NW - 1) / NW;               // per wave
-        const uint32_t b = lo + wave * len, e = min(b + len, lo + n);
-        uint64_t s = 0, run = 0;
-        for (uint32_t i = b + lane; i < e; i += 64) {
-            const float v = x[i];
-            if (!allowed(v) || token_key(v, i) < above) continue;
-            const uint64_t w = wg.units(v);
-            s += w >= least ? w : 0;
-        }
-        run = s;
-        s = wave_sum_u64(s);
-        __syncthreads();
-        if (lane == 0) part[wave] = s;
-        __syncthreads();
-        uint64_t before = 0;
-        int at = 0;
-        for (; at < NW - 1 && before + part[at] <= target; ++at) before += part[at];
-        target -= before;
-        if (len <= 64) {
-            // one value per lane of wave `at`
-            if (wave == at) {
-                const uint64_t own = run;
-#pragma unroll
-                for (int o = 1; o < 64; o <<= 1) {
-                    const uint64_t w = (uint64_t)__shfl_up((unsigned long long)run, o, 64);
-                    if (lane >= o) run += w;
-                }
-                if (own && run > target && run - own <= target) {
-                    const uint32_t i = b + lane;
-                    a.tokens[row] = i;
-                    if (a.probs) a.probs[row] = (float)(wg.weight(x[i]) / (double)Z);
-                }
-            }
+    if (r.k == 0) {
+        uint64_t *sums = (uint64_t *)spare;
+        if (!(r.p < 1.0f)) {
+            draw_stretch(1, a.sums + (size_t)row * a.stretches);
             return;
         }
-        lo += at * len;
-        n = min(len, a.V - lo);
+        const uint32_t n = a.listed[row];
+        if (n > kList) {
+            walk();
+            return;
+        }
+        uint64_t rest;
+        border_bin(a, r, row, sh.list, rest);                         // sh.list is still free
+        __syncthreads();
+        for (uint32_t i = tid; i < a.stretches; i += kDrawThreads) sums[i] = a.sums[(size_t)row * a.stretches + i];
+        for (uint32_t i = tid; i < n; i += kDrawThreads) sh.list[i] = a.list[(size_t)row * kList + i];
+        __syncthreads();
+        auto listed = [&](auto &&f) {
+            for (uint32_t i = tid; i < n; i += kDrawThreads) f(sh.list[i]);
+        };
+        uint64_t above = last_key(listed, 1, true, rest), least = ~0ull;
+        // that may be the lower end of keys which reach past the list's bin: the smallest listed key from there on
+        listed([&](uint64_t key) { least = key >= above && key < least ? key : least; });
+        above = block_min(least);
+        for (uint32_t i = tid; i < n; i += kDrawThreads) {
+            const uint64_t key = sh.list[i];
+            const uint64_t w = key >= above ? r.kept(r.units(value_of(key >> 32))) : 0;
+            if (w) atomicAdd((unsigned long long *)&sums[(0xFFFFFFFFu - (uint32_t)key) / kStretch], (unsigned long long)w);
+        }
+        __syncthreads();
+        draw_stretch(above, sums);
+        return;
+    }
+    if (r.k > kMaxK || r.k > a.blocks) {
+        walk();
+        return;
+    }
+    // top-k.  The blocks whose maximum is at or above (the upper 16 bits of) the k-th largest one; k tokens or all are
+    // that large.
+    for (uint32_t b = tid; b < a.blocks; b += kDrawThreads) spare[b] = bmax[b];
+    uint32_t floor_key = 1, prefix = 0, goal = r.k;
+    for (int shift = 24; shift >= 16; shift -= 8) {
+        __syncthreads();
+        if (tid < 256) sh.hist_n[tid] = 0;
+        if (tid == 0) sh.found[2] = 0;
+        __syncthreads();
+        for (uint32_t b = tid; b < a.blocks; b += kDrawThreads) {
+            const uint32_t m = spare[b];
+            if (m && (shift == 24 || (m >> (shift + 8)) == prefix)) atomicAdd(&sh.hist_n[(m >> shift) & 255u], 1u);
+        }
+        __syncthreads();
+        if (wave == 0) {
+            uint32_t c[4], own = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) own += c[i] = sh.hist_n[255 - 4 * lane - i];
+            uint32_t before = (uint32_t)wave_scan_u64(own, lane) - own;
+            if (before < goal && before + own >= goal) {
+                int i = 0;
+                for (; before + c[i] < goal; ++i) before += c[i];
+                sh.found[0] = 255 - 4 * lane - i;
+                sh.found[1] = before;
+                sh.found[2] = 1;
+            }
+        }
+        __syncthreads();
+        if (!sh.found[2]) break;                                      // fewer blocks with anything allowed than k: all
+        prefix = (prefix << 8) | (uint32_t)sh.found[0];
+        goal -= (uint32_t)sh.found[1];
+        floor_key = shift == 16 ? prefix << 16 : floor_key;
+    }
+    __syncthreads();
+    const bool bounded = sh.found[2];
+    floor_key = bounded ? max(floor_key, 1u) : 1u;
+    if (tid == 0) sh.n = sh.hit = 0;
+    __syncthreads();
+    // those blocks' numbers, in place of the maxima: every round writes only where it and earlier ones have read
+    for (uint32_t b0 = 0; b0 < a.blocks; b0 += kDrawThreads) {
+        const uint32_t b = b0 + tid;
+        const bool in = b < a.blocks && spare[b] >= floor_key;
+        __syncthreads();
+        if (in) spare[atomicAdd(&sh.hit, 1u)] = b;
+        __syncthreads();
+    }
+    const uint32_t nb = sh.hit;
+    // their tokens at or above the bound
+    for (uint32_t q = wave; q < nb; q += 4 * NW) {
+        float v[4];
+        uint32_t i[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+            i[e] = spare[min(q + e * NW, nb - 1)] * 64 + lane;
+            v[e] = x[min(i[e], a.V - 1)];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (q + e * NW < nb && i[e] < a.V && allowed(v[e]) && orderable(v[e]) >= floor_key) {
+                const uint32_t at = atomicAdd(&sh.n, 1u);
+                if (at < kList) sh.list[at] = token_key(v[e], i[e]);
+            }
+    }
+    __syncthreads();
+    const uint32_t n = sh.n;
+    if (n > kList) {
+        walk();
+        return;
+    }
+    // the k largest, in order: a thread counts what is larger than its key
+    uint64_t *sorted = (uint64_t *)spare;                              // kMaxK
+    for (uint32_t i = tid; i < n; i += kDrawThreads) {
+        const uint64_t key = sh.list[i];
+        uint32_t rank = 0;
+        for (uint32_t j = 0; j < n; ++j) rank += sh.list[j] > key ? 1u : 0u;
+        if (rank < r.k) sorted[rank] = key;
+    }
+    __syncthreads();
+    const uint32_t k = min(n, r.k);
+    const uint64_t key = tid < k ? sorted[tid] : 0;
+    const uint64_t w = tid < k ? r.units(value_of(key >> 32)) : 0;
+    uint64_t Z, total;
+    const uint64_t incl = block_scan(w, Z);
+    bool in = tid < k;
+    if (r.p < 1.0f) in = in && incl - w < r.goal(Z);
+    const uint64_t kw = in ? r.kept(w) : 0;
+    (void)block_scan(kw, total);
+    const uint64_t target = target_of(total);
+    // the draw goes by index: a kept token sums the kept ones before it
+    sh.list[tid] = kw;
+    __syncthreads();
+    if (kw) {
+        uint64_t before = 0;
+        const uint32_t mine = (uint32_t)key;                           // ~index: larger for lower indexes
+        for (uint32_t j = 0; j < k; ++j) before += (uint32_t)sorted[j] > mine ? sh.list[j] : 0;
+        if (before <= target && before + kw > target)
+            finish(0xFFFFFFFFu - mine, (float)(r.weight(value_of(key >> 32)) / (double)total));
     }
 }
 
@@ -252,8 +665,43 @@ extern "C" int chn_sample(chn_ctx *ctx, const float *logits, uint32_t n_rows, ui
     CHN_REQUIRE(ctx, ctx, "ctx is NULL");
     if (!n_rows) return CHN_OK;
     DeviceGuard dev(ctx);
-    k_sample_row<<<n_rows, kRowThreads, 0, ctx->stream>>>(
-        Sample{logits, V, ld, temperature, top_k, top_p, min_p, u, softcap, tokens, probs});
-    CHN_LAUNCHED(ctx, "k_sample_row");
+    const uint32_t blocks = (V + 63) / 64, stretches = (V + kStretch - 1) / kStretch;
+    const size_t rows = std::min(n_rows, kRowsAtOnce);
+    const size_t row_bytes = (size_t)(stretches + kBins + kList) * 8 + (size_t)(blocks + stretches + 1) * 4;
+    int rc = ensure_workspace(ctx, rows * row_bytes);
+    if (rc) return rc;
+    Sample a{};
+    a.V = V;
+    a.ld = ld;
+    a.softcap = softcap;
+    a.blocks = blocks;
+    a.stretches = stretches;
+    a.sums = (uint64_t *)ctx->ws;
+    a.hist = a.sums + rows * stretches;
+    a.list = a.hist + rows * kBins;
+    a.bmax = (uint32_t *)(a.list + rows * kList);
+    a.smax = a.bmax + rows * blocks;
+    a.listed = a.smax + rows * stretches;
+    // k_sample_draw's spare LDS: block maxima, kMaxK sorted keys, or the stretches' sums
+    const size_t lds = sizeof(Draw) + std::max<size_t>({(size_t)blocks * 4, (size_t)kMaxK * 8, (size_t)stretches * 8});
+    for (uint32_t r0 = 0; r0 < n_rows; r0 += kRowsAtOnce) {
+        const uint32_t n = std::min(n_rows - r0, kRowsAtOnce);
+        a.logits = logits + (size_t)r0 * ld;
+        a.temperature = temperature ? temperature + r0 : nullptr;
+        a.top_k = top_k ? top_k + r0 : nullptr;
+        a.top_p = top_p ? top_p + r0 : nullptr;
+        a.min_p = min_p ? min_p + r0 : nullptr;
+        a.u = u + r0;
+        a.tokens = tokens + r0;
+        a.probs = probs ? probs + r0 : nullptr;
+        // few rows: small workgroups, so that a row spreads over the chip; many: large ones, whose histograms are merged
+        // less often
+        const uint32_t nt = (uint64_t)n * stretches >= 16 * 256 ? 1024 : 256, wgs = (stretches + nt / 64 - 1) / (nt / 64);
+        k_sample_max<<<dim3((stretches + 3) / 4, n), 256, 0, ctx->stream>>>(a);
+        k_sample_mass<<<dim3(wgs, n), nt, 0, ctx->stream>>>(a);
+        k_sample_border<<<dim3(wgs, n), nt, 0, ctx->stream>>>(a);
+        k_sample_draw<<<n, kDrawThreads, lds, ctx->stream>>>(a);
+        CHN_LAUNCHED(ctx, "k_sample");
+    }
     return CHN_OK;
 }
