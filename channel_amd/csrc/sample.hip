@@ -25,7 +25,7 @@
 //    draw reads the one stretch of 2048 that it falls into.
 // Rows that fit none of this (top-k above kMaxK, a border among more equal or
 // near equal logits than the list holds) take k_sample_draw's walk over the
-// whole row, eight bits of the key at a time.
+// whole row.
 #include "chn_internal.h"
 
 #include <cmath>
@@ -295,34 +295,70 @@ __device__ __forceinline__ uint32_t border_bin(const Sample &a, const Row &r, ui
 }
 
 // Rows with top-p and without top-k: the tokens of the border's bin into the
-// list, the kept weights above it summed by stretch.
+// list, the kept weights above it summed by stretch.  A tenth to a half of a
+// row's tokens lie above: they are queued, and their weights (64-bit
+// arithmetic) formed by full waves.
 __global__ void k_sample_border(Sample a) {
-    __shared__ uint64_t sh[20];
+    constexpr uint32_t kMine = 1024;                                     // the workgroup's share of the list
+    __shared__ uint64_t sh[20], found[kMine];
+    __shared__ float queue[16][128];
+    __shared__ uint32_t nfound, at0;
     const uint32_t row = blockIdx.y, s = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
     const Row r(a, row, row_top(a, row));
     if (!r.by_mass() || !(r.p < 1.0f)) return;
     uint64_t rest;
     const uint32_t border = border_bin(a, r, row, sh, rest);
-    if (s >= a.stretches) return;
+    if (threadIdx.x == 0) nfound = 0;
+    __syncthreads();
+    float *q = queue[threadIdx.x >> 6];
+    uint32_t n = 0;                                                      // queued, below 64 between steps
     uint64_t sum = 0;
-    stretch(a, a.logits + (size_t)row * a.ld, s,
+    const uint64_t below = ((uint64_t)1 << lane) - 1;
+    auto fence = [] {                                                    // the wave reads what it wrote
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    };
+    if (s < a.stretches) stretch(a, a.logits + (size_t)row * a.ld, s,
             [&](uint32_t i, float v) {
                 const uint32_t b = allowed(v) ? r.bin(v) : kBins;
-                if (b < border) sum += r.kept(r.units(v));
-                if (b == border) {
-                    const uint32_t at = atomicAdd(&a.listed[row], 1u);
-                    if (at < kList) a.list[(size_t)row * kList + at] = token_key(v, i);
+                const uint64_t over = __ballot(b < border), in = __ballot(b == border);
+                if (b < border) q[n + __popcll(over & below)] = v;
+                n += __popcll(over);
+                if (n >= 64) {
+                    fence();
+                    sum += r.kept(r.units(q[lane]));
+                    const float tail = q[64 + lane];
+                    fence();
+                    q[lane] = tail;
+                    n -= 64;
+                }
+                if (in) {                                                // one atomic for the wave's
+                    const int first = __ffsll((unsigned long long)in) - 1;
+                    uint32_t at = 0;
+                    if (lane == first) at = atomicAdd(&nfound, (uint32_t)__popcll(in));
+                    at = __shfl(at, first, 64) + (uint32_t)__popcll(in & below);
+                    if (b == border && at < kMine) found[at] = token_key(v, i);
                 }
             },
             [](int) {});
+    fence();
+    if (lane < (int)n) sum += r.kept(r.units(q[lane]));
     sum = wave_sum_u64(sum);
-    if ((threadIdx.x & 63) == 0) a.sums[(size_t)row * a.stretches + s] = sum;
+    if (lane == 0 && s < a.stretches) a.sums[(size_t)row * a.stretches + s] = sum;
+    __syncthreads();
+    // more than its share: the row's list counts as full
+    if (threadIdx.x == 0 && nfound) at0 = atomicAdd(&a.listed[row], nfound <= kMine ? nfound : kList + 1);
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < min(nfound, kMine); i += blockDim.x)
+        if (at0 + i < kList) a.list[(size_t)row * kList + at0 + i] = found[i];
 }
 
 // LDS of k_sample_draw.
+constexpr uint32_t kDigits = 2 * kDrawThreads;
 struct Draw {
-    uint64_t list[kList], hist_w[256], part[kDrawThreads / 64], found[3];
-    uint32_t hist_n[256], n, hit;
+    uint64_t list[kList], hist_w[kDigits], part[kDrawThreads / 64], found[4];
+    uint32_t hist_n[kDigits], n, hit;
 };
 
 // A workgroup per row: the kept tokens' last key, then the draw.
@@ -401,53 +437,48 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         const uint64_t t = want >= (double)Z ? Z - 1 : (uint64_t)want;
         return t < Z ? t : Z - 1;
     };
-    // every(f): f(key) for all tokens looked through.  The key of the last token of the order, from those at or above
-    // `above`, that the running count (or sum of weights) needs to reach `goal`: eight bits of the key at a time, until
-    // the bin is wanted whole.
-    auto last_key = [&](auto &&every, uint64_t above, bool by_weight, uint64_t goal) {
-        uint64_t prefix = 0;
-        for (int shift = 56;; shift -= 8) {
+    // every(f): f(key) for all tokens looked through.  The key of the last token of the order, from those in [lo, hi],
+    // that the running count (or sum of weights) needs to reach `goal`: the range in up to 2048 parts, then the part
+    // that holds it, until that is wanted whole.
+    auto last_key = [&](auto &&every, uint64_t lo, uint64_t hi, bool by_weight, uint64_t goal) {
+        // each round leaves at most 2^-10 of the range: six at most
+        for (int round = 0; round < 7; ++round) {
+            const int bits = 64 - __clzll((long long)(hi - lo)), shift = hi == lo ? 0 : max(bits - 11, 0);
             __syncthreads();
-            if (tid < 256) {
-                sh.hist_n[tid] = 0;
-                sh.hist_w[tid] = 0;
+            for (uint32_t i = tid; i < kDigits; i += kDrawThreads) {
+                sh.hist_n[i] = 0;
+                sh.hist_w[i] = 0;
             }
             __syncthreads();
             every([&](uint64_t key) {
-                if (key < above || (shift < 56 && (key >> (shift + 8)) != prefix)) return;
-                const uint32_t bin = (uint32_t)(key >> shift) & 255u;
-                atomicAdd(&sh.hist_n[bin], 1u);
+                if (key < lo || key > hi) return;
+                const uint32_t d = (uint32_t)((key - lo) >> shift);
+                atomicAdd(&sh.hist_n[d], 1u);
                 if (by_weight)
-                    atomicAdd((unsigned long long *)&sh.hist_w[bin], (unsigned long long)r.units(value_of(key >> 32)));
+                    atomicAdd((unsigned long long *)&sh.hist_w[d], (unsigned long long)r.units(value_of(key >> 32)));
             });
             __syncthreads();
-            if (wave == 0) {
-                // lane 0 has the four largest bins
-                uint64_t c[4], own = 0;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int bin = 255 - 4 * lane - i;
-                    c[i] = by_weight ? sh.hist_w[bin] : sh.hist_n[bin];
-                    own += c[i];
-                }
-                uint64_t before = wave_scan_u64(own, lane) - own;
-                if (before < goal && before + own >= goal) {
-                    int i = 0;
-                    for (; before + c[i] < goal; ++i) before += c[i];
-                    const int bin = 255 - 4 * lane - i;
-                    sh.found[0] = bin;
-                    sh.found[1] = before;
-                    sh.found[2] = shift == 0 || sh.hist_n[bin] == 1 || (!by_weight && before + sh.hist_n[bin] == goal);
-                }
+            // thread 0 has the two largest parts
+            const uint32_t d = kDigits - 1 - 2 * tid;
+            const uint64_t c0 = by_weight ? sh.hist_w[d] : sh.hist_n[d], c1 = by_weight ? sh.hist_w[d - 1] : sh.hist_n[d - 1];
+            uint64_t total;
+            uint64_t before = block_scan(c0 + c1, total) - c0 - c1;
+            if (before < goal && before + c0 + c1 >= goal) {
+                const bool second = before + c0 < goal;
+                before += second ? c0 : 0;
+                const uint32_t n = sh.hist_n[d - second];
+                sh.found[0] = d - second;
+                sh.found[1] = before;
+                sh.found[2] = shift == 0 || n == 1 || (!by_weight && before + n == goal);
             }
             __syncthreads();
-            prefix = (prefix << 8) | sh.found[0];
+            lo += sh.found[0] << shift;
+            // (one type on both sides: min of unsigned long and unsigned long long is the one for doubles)
+            hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
             goal -= sh.found[1];
-            if (sh.found[2]) {
-                const uint64_t key = prefix << shift;              // the bin's lower end: it may reach below `above`
-                return key > above ? key : above;
-            }
+            if (sh.found[2]) break;
         }
+        return lo;
     };
     auto whole_row = [&](auto &&f) {
         for (uint32_t i = tid; i < a.V; i += kDrawThreads) {
@@ -498,17 +529,24 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         __syncthreads();
         draw_stretch(above, sums);
     };
+    const uint64_t top_key = ((uint64_t)orderable(r.raw_top) << 32) | 0xFFFFFFFFu;
+    auto least_key = [&](uint64_t &n) {                              // the row's, and how many are allowed
+        uint64_t m = ~0ull;
+        n = 0;
+        whole_row([&](uint64_t key) {
+            m = min(m, key);
+            ++n;
+        });
+        n = block_sum(n);
+        return block_min(m);
+    };
     auto walk = [&] {
-        uint64_t above = 1, Z = 0;
-        if (r.k) {
-            uint64_t n = 0;
-            whole_row([&](uint64_t) { ++n; });
-            if (block_sum(n) > r.k) above = last_key(whole_row, 1, false, r.k);
-        }
+        uint64_t n, above = least_key(n), Z = 0;
+        if (r.k && n > r.k) above = last_key(whole_row, above, top_key, false, r.k);
         if (r.p < 1.0f) {
             whole_row([&](uint64_t key) { Z += key >= above ? r.units(value_of(key >> 32)) : 0; });
             Z = block_sum(Z);
-            above = last_key(whole_row, above, true, r.goal(Z));
+            above = last_key(whole_row, above, top_key, true, r.goal(Z));
         }
         draw_whole(above);
     };
@@ -525,100 +563,108 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
             return;
         }
         uint64_t rest;
-        border_bin(a, r, row, sh.list, rest);                         // sh.list is still free
+        border_bin(a, r, row, sh.hist_w, rest);
         __syncthreads();
         for (uint32_t i = tid; i < a.stretches; i += kDrawThreads) sums[i] = a.sums[(size_t)row * a.stretches + i];
-        for (uint32_t i = tid; i < n; i += kDrawThreads) sh.list[i] = a.list[(size_t)row * kList + i];
-        __syncthreads();
+        uint64_t lo = ~0ull, hi = 0;
+        for (uint32_t i = tid; i < n; i += kDrawThreads) {
+            const uint64_t key = a.list[(size_t)row * kList + i];
+            sh.list[i] = key;
+            lo = min(lo, key);
+            hi = max(hi, key);
+        }
+        lo = block_min(lo);
+        hi = ~block_min(~hi);
         auto listed = [&](auto &&f) {
             for (uint32_t i = tid; i < n; i += kDrawThreads) f(sh.list[i]);
         };
-        uint64_t above = last_key(listed, 1, true, rest), least = ~0ull;
-        // that may be the lower end of keys which reach past the list's bin: the smallest listed key from there on
-        listed([&](uint64_t key) { least = key >= above && key < least ? key : least; });
-        above = block_min(least);
-        for (uint32_t i = tid; i < n; i += kDrawThreads) {
-            const uint64_t key = sh.list[i];
+        // a key at or below the wanted token's and above the next listed one's; it is not below the list's smallest, so no
+        // token of a later bin reaches it
+        const uint64_t above = last_key(listed, lo, hi, true, rest);
+        listed([&](uint64_t key) {
             const uint64_t w = key >= above ? r.kept(r.units(value_of(key >> 32))) : 0;
             if (w) atomicAdd((unsigned long long *)&sums[(0xFFFFFFFFu - (uint32_t)key) / kStretch], (unsigned long long)w);
-        }
+        });
         __syncthreads();
         draw_stretch(above, sums);
         return;
     }
-    if (r.k > kMaxK || r.k > a.blocks) {
+    if (r.k > kMaxK) {
         walk();
         return;
     }
-    // top-k.  The blocks whose maximum is at or above (the upper 16 bits of) the k-th largest one; k tokens or all are
-    // that large.
-    for (uint32_t b = tid; b < a.blocks; b += kDrawThreads) spare[b] = bmax[b];
-    uint32_t floor_key = 1, prefix = 0, goal = r.k;
-    for (int shift = 24; shift >= 16; shift -= 8) {
-        __syncthreads();
-        if (tid < 256) sh.hist_n[tid] = 0;
-        if (tid == 0) sh.found[2] = 0;
-        __syncthreads();
-        for (uint32_t b = tid; b < a.blocks; b += kDrawThreads) {
-            const uint32_t m = spare[b];
-            if (m && (shift == 24 || (m >> (shift + 8)) == prefix)) atomicAdd(&sh.hist_n[(m >> shift) & 255u], 1u);
-        }
-        __syncthreads();
-        if (wave == 0) {
-            uint32_t c[4], own = 0;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) own += c[i] = sh.hist_n[255 - 4 * lane - i];
-            uint32_t before = (uint32_t)wave_scan_u64(own, lane) - own;
-            if (before < goal && before + own >= goal) {
-                int i = 0;
-                for (; before + c[i] < goal; ++i) before += c[i];
-                sh.found[0] = 255 - 4 * lane - i;
-                sh.found[1] = before;
-                sh.found[2] = 1;
-            }
-        }
-        __syncthreads();
-        if (!sh.found[2]) break;                                      // fewer blocks with anything allowed than k: all
-        prefix = (prefix << 8) | (uint32_t)sh.found[0];
-        goal -= (uint32_t)sh.found[1];
-        floor_key = shift == 16 ? prefix << 16 : floor_key;
-    }
-    __syncthreads();
-    const bool bounded = sh.found[2];
-    floor_key = bounded ? max(floor_key, 1u) : 1u;
+    // top-k: the tokens that can be among the k largest into the list.  The blocks' maxima in up to 2048 parts between the
+    // smallest and the largest: where the running count from the top reaches k, k tokens are that large.
     if (tid == 0) sh.n = sh.hit = 0;
-    __syncthreads();
-    // those blocks' numbers, in place of the maxima: every round writes only where it and earlier ones have read
-    for (uint32_t b0 = 0; b0 < a.blocks; b0 += kDrawThreads) {
-        const uint32_t b = b0 + tid;
-        const bool in = b < a.blocks && spare[b] >= floor_key;
-        __syncthreads();
-        if (in) spare[atomicAdd(&sh.hit, 1u)] = b;
-        __syncthreads();
-    }
-    const uint32_t nb = sh.hit;
-    // their tokens at or above the bound
-    for (uint32_t q = wave; q < nb; q += 4 * NW) {
-        float v[4];
-        uint32_t i[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            i[e] = spare[min(q + e * NW, nb - 1)] * 64 + lane;
-            v[e] = x[min(i[e], a.V - 1)];
+    bool bounded = r.k <= a.blocks;
+    uint32_t floor_key = 1;
+    if (bounded) {
+        uint32_t least = 0xFFFFFFFFu;
+        uint64_t some = 0;
+        for (uint32_t b = tid; b < a.blocks; b += kDrawThreads) {
+            const uint32_t m = bmax[b];
+            spare[b] = m;
+            least = m ? min(least, m) : least;
+            some += m ? 1 : 0;
         }
+        for (uint32_t i = tid; i < kDigits; i += kDrawThreads) sh.hist_n[i] = 0;
+        some = block_sum(some);
+        least = (uint32_t)block_min(least);
+        if (some >= r.k) {
+            const uint32_t range = orderable(r.raw_top) - least;
+            const int shift = max(32 - __clz(range) - 11, 0);                 // range 0: 0
+            for (uint32_t b = tid; b < a.blocks; b += kDrawThreads)
+                if (spare[b]) atomicAdd(&sh.hist_n[(spare[b] - least) >> shift], 1u);
+            __syncthreads();
+            const uint32_t d = kDigits - 1 - 2 * tid, c0 = sh.hist_n[d], c1 = sh.hist_n[d - 1];
+            uint64_t total;
+            const uint64_t before = block_scan(c0 + c1, total) - c0 - c1;
+            if (before < r.k && before + c0 + c1 >= r.k) sh.found[0] = d - (before + c0 < r.k);
+            __syncthreads();
+            floor_key = least + ((uint32_t)sh.found[0] << shift);
+        }
+        // those blocks' numbers, in place of the maxima: every round writes only where it and earlier ones have read
+        for (uint32_t b0 = 0; b0 < a.blocks; b0 += kDrawThreads) {
+            const uint32_t b = b0 + tid;
+            const bool in = b < a.blocks && spare[b] >= floor_key;
+            __syncthreads();
+            if (in) spare[atomicAdd(&sh.hit, 1u)] = b;
+            __syncthreads();
+        }
+        const uint32_t nb = sh.hit;
+        // their tokens at or above the bound
+        for (uint32_t q = wave; q < nb; q += 4 * NW) {
+            float v[4];
+            uint32_t i[4];
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-            if (q + e * NW < nb && i[e] < a.V && allowed(v[e]) && orderable(v[e]) >= floor_key) {
-                const uint32_t at = atomicAdd(&sh.n, 1u);
-                if (at < kList) sh.list[at] = token_key(v[e], i[e]);
+            for (int e = 0; e < 4; ++e) {
+                i[e] = spare[min(q + e * NW, nb - 1)] * 64 + lane;
+                v[e] = x[min(i[e], a.V - 1)];
             }
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+                if (q + e * NW < nb && i[e] < a.V && allowed(v[e]) && orderable(v[e]) >= floor_key) {
+                    const uint32_t at = atomicAdd(&sh.n, 1u);
+                    if (at < kList) sh.list[at] = token_key(v[e], i[e]);
+                }
+        }
+        __syncthreads();
+        bounded = sh.n <= kList;
     }
-    __syncthreads();
+    if (!bounded) {
+        // more tokens than the list holds, or fewer blocks than k: the exact bound
+        uint64_t m;
+        uint64_t above = least_key(m);
+        if (m > r.k) above = last_key(whole_row, above, top_key, false, r.k);
+        __syncthreads();
+        if (tid == 0) sh.n = 0;
+        __syncthreads();
+        whole_row([&](uint64_t key) {
+            if (key >= above) sh.list[atomicAdd(&sh.n, 1u)] = key;         // at most k
+        });
+        __syncthreads();
+    }
     const uint32_t n = sh.n;
-    if (n > kList) {
-        walk();
-        return;
-    }
     // the k largest, in order: a thread counts what is larger than its key
     uint64_t *sorted = (uint64_t *)spare;                              // kMaxK
     for (uint32_t i = tid; i < n; i += kDrawThreads) {
