@@ -354,23 +354,209 @@ __global__ void k_sample_border(Sample a) {
         if (at0 + i < kList) a.list[(size_t)row * kList + at0 + i] = found[i];
 }
 
-// LDS of k_sample_draw.
+// LDS and steps of a workgroup of kDrawThreads that looks for a row's border.
 constexpr uint32_t kDigits = 2 * kDrawThreads;
-struct Draw {
-    uint64_t list[kList], hist_w[kDigits], part[kDrawThreads / 64], found[4];
+struct Group {
+    static constexpr int NW = kDrawThreads / 64;
+    uint64_t hist_w[kDigits], part[NW], found[4];
     uint32_t hist_n[kDigits], n, hit;
+
+    __device__ __forceinline__ uint64_t sum(uint64_t v) {
+        v = wave_sum_u64(v);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        uint64_t t = 0;
+        for (int w = 0; w < NW; ++w) t += part[w];
+        return t;
+    }
+    __device__ __forceinline__ uint64_t least(uint64_t v) {
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) v = min(v, shfl_xor64(v, o));
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
+        __syncthreads();
+        for (int w = 0; w < NW; ++w) v = min(v, part[w]);
+        return v;
+    }
+    // inclusive running sum over the threads, and the whole sum
+    __device__ __forceinline__ uint64_t scan(uint64_t v, uint64_t &total) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+        v = wave_scan_u64(v, lane);
+        __syncthreads();
+        if (lane == 63) part[wave] = v;
+        __syncthreads();
+        total = 0;
+        for (int w = 0; w < NW; ++w) {
+            v += w < wave ? part[w] : 0;
+            total += part[w];
+        }
+        return v;
+    }
+    // every(f): f(key, weight()) for all tokens looked through.  The key of the last token of the order, from those in
+    // [lo, hi], that the running count (or sum of weights) needs to reach `goal`: the range in up to 2048 parts, then the
+    // part that holds it, until that is wanted whole.
+    template <typename F>
+    __device__ __forceinline__ uint64_t last_key(F &&every, uint64_t lo, uint64_t hi, bool by_weight, uint64_t goal) {
+        const uint32_t tid = threadIdx.x;
+        // each round leaves at most 2^-10 of the range: six at most
+        for (int round = 0; round < 7; ++round) {
+            const int bits = 64 - __clzll((long long)(hi - lo)), shift = hi == lo ? 0 : max(bits - 11, 0);
+            __syncthreads();
+            for (uint32_t i = tid; i < kDigits; i += kDrawThreads) {
+                hist_n[i] = 0;
+                hist_w[i] = 0;
+            }
+            __syncthreads();
+            every([&](uint64_t key, auto &&weight) {
+                if (key < lo || key > hi) return;
+                const uint32_t d = (uint32_t)((key - lo) >> shift);
+                atomicAdd(&hist_n[d], 1u);
+                if (by_weight) atomicAdd((unsigned long long *)&hist_w[d], (unsigned long long)weight());
+            });
+            __syncthreads();
+            // thread 0 has the two largest parts
+            const uint32_t d = kDigits - 1 - 2 * tid;
+            const uint64_t c0 = by_weight ? hist_w[d] : hist_n[d], c1 = by_weight ? hist_w[d - 1] : hist_n[d - 1];
+            uint64_t total;
+            uint64_t before = scan(c0 + c1, total) - c0 - c1;
+            if (before < goal && before + c0 + c1 >= goal) {
+                const bool second = before + c0 < goal;
+                before += second ? c0 : 0;
+                const uint32_t cnt = hist_n[d - second];
+                found[0] = d - second;
+                found[1] = before;
+                found[2] = shift == 0 || cnt == 1 || (!by_weight && before + cnt == goal);
+            }
+            __syncthreads();
+            lo += found[0] << shift;
+            // (one type on both sides: min of unsigned long and unsigned long long is the one for doubles)
+            hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
+            goal -= found[1];
+            if (found[2]) break;
+        }
+        return lo;
+    }
+};
+
+// What the draw looks for in a sum of Z: a running sum above this.
+__device__ __forceinline__ uint64_t target_of(float u, uint64_t Z) {
+    const double want = (u > 0.0f ? (double)u : 0.0) * (double)Z;
+    const uint64_t t = want >= (double)Z ? Z - 1 : (uint64_t)want;
+    return t < Z ? t : Z - 1;
+}
+
+// Rows of up to kSmallV: one launch, a workgroup per row, which holds the row in
+// registers (thread t: values t, t + 1024, ..).  With more than a launch per row
+// latency is what counts: 50 rows of 10007 took 73 us in the four launches.
+constexpr uint32_t kSmallV = 16 * kDrawThreads;
+template <int J>
+__global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
+    __shared__ Group sh;
+    __shared__ uint64_t by_wave[J][Group::NW];
+    const uint32_t tid = threadIdx.x, row = blockIdx.x;
+    const int lane = tid & 63, wave = tid >> 6;
+    const float *x = a.logits + (size_t)row * a.ld;
+    float v[J];
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const uint32_t i = tid + j * kDrawThreads;
+        v[j] = i < a.V ? x[i] : __builtin_nanf("");
+    }
+    const float u = a.u[row];
+    uint64_t hi = 0, lo = ~0ull, n = 0;
+    auto key_of = [&](int j) { return allowed(v[j]) ? token_key(v[j], tid + j * kDrawThreads) : 0; };
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const uint64_t key = key_of(j);
+        hi = max(hi, key);
+        lo = key ? min(lo, key) : lo;
+        n += key ? 1 : 0;
+    }
+    hi = ~sh.least(~hi);
+    const Row r(a, row, (uint32_t)(hi >> 32));
+    auto finish = [&](uint32_t token, float prob) {
+        a.tokens[row] = token;
+        if (a.probs) a.probs[row] = prob;
+    };
+    if (!r.some || r.greedy) {
+        if (tid == 0) finish(r.some ? 0xFFFFFFFFu - (uint32_t)hi : CHN_NO_TOKEN, r.some ? 1.0f : 0.0f);
+        return;
+    }
+    lo = sh.least(lo);
+    if (r.k) {
+        n = sh.sum(n);
+        if (n > r.k)
+            lo = sh.last_key(
+                [&](auto &&f) {
+#pragma unroll
+                    for (int j = 0; j < J; ++j) f(key_of(j), [] { return (uint64_t)1; });   // key 0 is below lo
+                },
+                lo, hi, false, r.k);
+    }
+    uint64_t w[J], Z = 0;
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        w[j] = 0;
+        if (key_of(j) >= lo) w[j] = r.units(v[j]);
+        Z += w[j];
+        __builtin_amdgcn_sched_barrier(0);                             // one at a time: the registers are full
+    }
+    if (r.p < 1.0f) {
+        Z = sh.sum(Z);
+        lo = sh.last_key(
+            [&](auto &&f) {
+#pragma unroll
+                for (int j = 0; j < J; ++j) f(key_of(j), [&] { return w[j]; });
+            },
+            lo, hi, true, r.goal(Z));
+    }
+    // sums of 64 consecutive indexes
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        w[j] = key_of(j) >= lo ? r.kept(w[j]) : 0;
+        const uint64_t s = wave_sum_u64(w[j]);
+        if (lane == 0) by_wave[j][wave] = s;
+    }
+    __syncthreads();
+    static_assert(J * Group::NW <= (int)kDrawThreads, "one thread per sum");
+    const uint64_t own = tid < J * Group::NW ? by_wave[tid / Group::NW][tid % Group::NW] : 0;
+    const uint64_t incl = sh.scan(own, Z), target = target_of(u, Z);
+    if (own && incl > target && incl - own <= target) {
+        sh.hit = tid;
+        sh.found[0] = target - (incl - own);
+    }
+    __syncthreads();
+    if (wave == (int)(sh.hit % Group::NW)) {
+        const uint64_t rest = sh.found[0];
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (j == (int)(sh.hit / Group::NW)) {
+                const uint64_t run = wave_scan_u64(w[j], lane);
+                if (w[j] && run > rest && run - w[j] <= rest)
+                    finish(tid + j * kDrawThreads, (float)(r.weight(v[j]) / (double)Z));
+            }
+    }
+}
+
+// LDS of k_sample_draw.
+struct Draw {
+    uint64_t list[kList];
+    Group g;
 };
 
 // A workgroup per row: the kept tokens' last key, then the draw.
 __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
     extern __shared__ uint64_t lds[];
-    constexpr int NW = kDrawThreads / 64;
-    Draw &sh = *(Draw *)lds;
+    constexpr int NW = Group::NW;
+    Draw &d = *(Draw *)lds;
+    Group &sh = d.g;
     uint32_t *spare = (uint32_t *)(lds + sizeof(Draw) / 8);          // block maxima, then blocks; or sums of stretches
     const uint32_t tid = threadIdx.x, row = blockIdx.x;
     const int lane = tid & 63, wave = tid >> 6;
     const float *x = a.logits + (size_t)row * a.ld;
     const uint32_t *bmax = a.bmax + (size_t)row * a.blocks;
+    const float u = a.u[row];
     const Row r(a, row, row_top(a, row));
 
     auto finish = [&](uint32_t token, float prob) {
@@ -399,91 +585,10 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         }
         return;
     }
-    auto block_sum = [&](uint64_t v) {
-        v = wave_sum_u64(v);
-        __syncthreads();
-        if (lane == 0) sh.part[wave] = v;
-        __syncthreads();
-        uint64_t t = 0;
-        for (int w = 0; w < NW; ++w) t += sh.part[w];
-        return t;
-    };
-    auto block_min = [&](uint64_t v) {
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) v = min(v, shfl_xor64(v, o));
-        __syncthreads();
-        if (lane == 0) sh.part[wave] = v;
-        __syncthreads();
-        for (int w = 0; w < NW; ++w) v = min(v, sh.part[w]);
-        return v;
-    };
-    // inclusive running sum over the threads, and the whole sum
-    auto block_scan = [&](uint64_t v, uint64_t &total) {
-        v = wave_scan_u64(v, lane);
-        __syncthreads();
-        if (lane == 63) sh.part[wave] = v;
-        __syncthreads();
-        total = 0;
-        for (int w = 0; w < NW; ++w) {
-            v += w < wave ? sh.part[w] : 0;
-            total += sh.part[w];
-        }
-        return v;
-    };
-    // what the draw looks for: a running sum above this
-    auto target_of = [&](uint64_t Z) {
-        const float u = a.u[row];
-        const double want = (u > 0.0f ? (double)u : 0.0) * (double)Z;
-        const uint64_t t = want >= (double)Z ? Z - 1 : (uint64_t)want;
-        return t < Z ? t : Z - 1;
-    };
-    // every(f): f(key) for all tokens looked through.  The key of the last token of the order, from those in [lo, hi],
-    // that the running count (or sum of weights) needs to reach `goal`: the range in up to 2048 parts, then the part
-    // that holds it, until that is wanted whole.
-    auto last_key = [&](auto &&every, uint64_t lo, uint64_t hi, bool by_weight, uint64_t goal) {
-        // each round leaves at most 2^-10 of the range: six at most
-        for (int round = 0; round < 7; ++round) {
-            const int bits = 64 - __clzll((long long)(hi - lo)), shift = hi == lo ? 0 : max(bits - 11, 0);
-            __syncthreads();
-            for (uint32_t i = tid; i < kDigits; i += kDrawThreads) {
-                sh.hist_n[i] = 0;
-                sh.hist_w[i] = 0;
-            }
-            __syncthreads();
-            every([&](uint64_t key) {
-                if (key < lo || key > hi) return;
-                const uint32_t d = (uint32_t)((key - lo) >> shift);
-                atomicAdd(&sh.hist_n[d], 1u);
-                if (by_weight)
-                    atomicAdd((unsigned long long *)&sh.hist_w[d], (unsigned long long)r.units(value_of(key >> 32)));
-            });
-            __syncthreads();
-            // thread 0 has the two largest parts
-            const uint32_t d = kDigits - 1 - 2 * tid;
-            const uint64_t c0 = by_weight ? sh.hist_w[d] : sh.hist_n[d], c1 = by_weight ? sh.hist_w[d - 1] : sh.hist_n[d - 1];
-            uint64_t total;
-            uint64_t before = block_scan(c0 + c1, total) - c0 - c1;
-            if (before < goal && before + c0 + c1 >= goal) {
-                const bool second = before + c0 < goal;
-                before += second ? c0 : 0;
-                const uint32_t n = sh.hist_n[d - second];
-                sh.found[0] = d - second;
-                sh.found[1] = before;
-                sh.found[2] = shift == 0 || n == 1 || (!by_weight && before + n == goal);
-            }
-            __syncthreads();
-            lo += sh.found[0] << shift;
-            // (one type on both sides: min of unsigned long and unsigned long long is the one for doubles)
-            hi = min(hi, lo + (((uint64_t)1 << shift) - 1));
-            goal -= sh.found[1];
-            if (sh.found[2]) break;
-        }
-        return lo;
-    };
     auto whole_row = [&](auto &&f) {
         for (uint32_t i = tid; i < a.V; i += kDrawThreads) {
             const float v = x[i];
-            if (allowed(v)) f(token_key(v, i));
+            if (allowed(v)) f(token_key(v, i), [&] { return r.units(v); });
         }
     };
     // The draw from the kept tokens of a row given the sums of its stretches (n of them, in LDS).
@@ -491,7 +596,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         uint64_t Z, own = 0;
         const uint32_t n = a.stretches;                               // at most kSampleMaxV / kStretch = 512
         own = tid < n ? sums[tid] : 0;
-        const uint64_t incl = block_scan(own, Z), target = target_of(Z);
+        const uint64_t incl = sh.scan(own, Z), target = target_of(u, Z);
         if (own && incl > target && incl - own <= target) {
             sh.hit = tid;
             sh.found[0] = target - (incl - own);
@@ -506,7 +611,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
             v[e] = i + e < a.V ? x[i + e] : __builtin_nanf("");
             w[e] = allowed(v[e]) && token_key(v[e], i + e) >= above ? r.kept(r.units(v[e])) : 0;
         }
-        uint64_t run = block_scan(w[0] + w[1], total) - w[0] - w[1];
+        uint64_t run = sh.scan(w[0] + w[1], total) - w[0] - w[1];
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
             if (w[e] && run <= rest && run + w[e] > rest) finish(i + e, (float)(r.weight(v[e]) / (double)Z));
@@ -533,20 +638,20 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
     auto least_key = [&](uint64_t &n) {                              // the row's, and how many are allowed
         uint64_t m = ~0ull;
         n = 0;
-        whole_row([&](uint64_t key) {
+        whole_row([&](uint64_t key, auto &&) {
             m = min(m, key);
             ++n;
         });
-        n = block_sum(n);
-        return block_min(m);
+        n = sh.sum(n);
+        return sh.least(m);
     };
     auto walk = [&] {
         uint64_t n, above = least_key(n), Z = 0;
-        if (r.k && n > r.k) above = last_key(whole_row, above, top_key, false, r.k);
+        if (r.k && n > r.k) above = sh.last_key(whole_row, above, top_key, false, r.k);
         if (r.p < 1.0f) {
-            whole_row([&](uint64_t key) { Z += key >= above ? r.units(value_of(key >> 32)) : 0; });
-            Z = block_sum(Z);
-            above = last_key(whole_row, above, top_key, true, r.goal(Z));
+            whole_row([&](uint64_t key, auto &&weight) { Z += key >= above ? weight() : 0; });
+            Z = sh.sum(Z);
+            above = sh.last_key(whole_row, above, top_key, true, r.goal(Z));
         }
         draw_whole(above);
     };
@@ -569,20 +674,23 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         uint64_t lo = ~0ull, hi = 0;
         for (uint32_t i = tid; i < n; i += kDrawThreads) {
             const uint64_t key = a.list[(size_t)row * kList + i];
-            sh.list[i] = key;
+            d.list[i] = key;
             lo = min(lo, key);
             hi = max(hi, key);
         }
-        lo = block_min(lo);
-        hi = ~block_min(~hi);
+        lo = sh.least(lo);
+        hi = ~sh.least(~hi);
         auto listed = [&](auto &&f) {
-            for (uint32_t i = tid; i < n; i += kDrawThreads) f(sh.list[i]);
+            for (uint32_t i = tid; i < n; i += kDrawThreads) {
+                const uint64_t key = d.list[i];
+                f(key, [&] { return r.units(value_of(key >> 32)); });
+            }
         };
         // a key at or below the wanted token's and above the next listed one's; it is not below the list's smallest, so no
         // token of a later bin reaches it
-        const uint64_t above = last_key(listed, lo, hi, true, rest);
-        listed([&](uint64_t key) {
-            const uint64_t w = key >= above ? r.kept(r.units(value_of(key >> 32))) : 0;
+        const uint64_t above = sh.last_key(listed, lo, hi, true, rest);
+        listed([&](uint64_t key, auto &&weight) {
+            const uint64_t w = key >= above ? r.kept(weight()) : 0;
             if (w) atomicAdd((unsigned long long *)&sums[(0xFFFFFFFFu - (uint32_t)key) / kStretch], (unsigned long long)w);
         });
         __syncthreads();
@@ -608,18 +716,18 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
             some += m ? 1 : 0;
         }
         for (uint32_t i = tid; i < kDigits; i += kDrawThreads) sh.hist_n[i] = 0;
-        some = block_sum(some);
-        least = (uint32_t)block_min(least);
+        some = sh.sum(some);
+        least = (uint32_t)sh.least(least);
         if (some >= r.k) {
             const uint32_t range = orderable(r.raw_top) - least;
             const int shift = max(32 - __clz(range) - 11, 0);                 // range 0: 0
             for (uint32_t b = tid; b < a.blocks; b += kDrawThreads)
                 if (spare[b]) atomicAdd(&sh.hist_n[(spare[b] - least) >> shift], 1u);
             __syncthreads();
-            const uint32_t d = kDigits - 1 - 2 * tid, c0 = sh.hist_n[d], c1 = sh.hist_n[d - 1];
+            const uint32_t e = kDigits - 1 - 2 * tid, c0 = sh.hist_n[e], c1 = sh.hist_n[e - 1];
             uint64_t total;
-            const uint64_t before = block_scan(c0 + c1, total) - c0 - c1;
-            if (before < r.k && before + c0 + c1 >= r.k) sh.found[0] = d - (before + c0 < r.k);
+            const uint64_t before = sh.scan(c0 + c1, total) - c0 - c1;
+            if (before < r.k && before + c0 + c1 >= r.k) sh.found[0] = e - (before + c0 < r.k);
             __syncthreads();
             floor_key = least + ((uint32_t)sh.found[0] << shift);
         }
@@ -645,7 +753,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
             for (int e = 0; e < 4; ++e)
                 if (q + e * NW < nb && i[e] < a.V && allowed(v[e]) && orderable(v[e]) >= floor_key) {
                     const uint32_t at = atomicAdd(&sh.n, 1u);
-                    if (at < kList) sh.list[at] = token_key(v[e], i[e]);
+                    if (at < kList) d.list[at] = token_key(v[e], i[e]);
                 }
         }
         __syncthreads();
@@ -655,12 +763,12 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         // more tokens than the list holds, or fewer blocks than k: the exact bound
         uint64_t m;
         uint64_t above = least_key(m);
-        if (m > r.k) above = last_key(whole_row, above, top_key, false, r.k);
+        if (m > r.k) above = sh.last_key(whole_row, above, top_key, false, r.k);
         __syncthreads();
         if (tid == 0) sh.n = 0;
         __syncthreads();
-        whole_row([&](uint64_t key) {
-            if (key >= above) sh.list[atomicAdd(&sh.n, 1u)] = key;         // at most k
+        whole_row([&](uint64_t key, auto &&) {
+            if (key >= above) d.list[atomicAdd(&sh.n, 1u)] = key;         // at most k
         });
         __syncthreads();
     }
@@ -668,9 +776,9 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
     // the k largest, in order: a thread counts what is larger than its key
     uint64_t *sorted = (uint64_t *)spare;                              // kMaxK
     for (uint32_t i = tid; i < n; i += kDrawThreads) {
-        const uint64_t key = sh.list[i];
+        const uint64_t key = d.list[i];
         uint32_t rank = 0;
-        for (uint32_t j = 0; j < n; ++j) rank += sh.list[j] > key ? 1u : 0u;
+        for (uint32_t j = 0; j < n; ++j) rank += d.list[j] > key ? 1u : 0u;
         if (rank < r.k) sorted[rank] = key;
     }
     __syncthreads();
@@ -678,19 +786,19 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
     const uint64_t key = tid < k ? sorted[tid] : 0;
     const uint64_t w = tid < k ? r.units(value_of(key >> 32)) : 0;
     uint64_t Z, total;
-    const uint64_t incl = block_scan(w, Z);
+    const uint64_t incl = sh.scan(w, Z);
     bool in = tid < k;
     if (r.p < 1.0f) in = in && incl - w < r.goal(Z);
     const uint64_t kw = in ? r.kept(w) : 0;
-    (void)block_scan(kw, total);
-    const uint64_t target = target_of(total);
+    (void)sh.scan(kw, total);
+    const uint64_t target = target_of(u, total);
     // the draw goes by index: a kept token sums the kept ones before it
-    sh.list[tid] = kw;
+    d.list[tid] = kw;
     __syncthreads();
     if (kw) {
         uint64_t before = 0;
         const uint32_t mine = (uint32_t)key;                           // ~index: larger for lower indexes
-        for (uint32_t j = 0; j < k; ++j) before += (uint32_t)sorted[j] > mine ? sh.list[j] : 0;
+        for (uint32_t j = 0; j < k; ++j) before += (uint32_t)sorted[j] > mine ? d.list[j] : 0;
         if (before <= target && before + kw > target)
             finish(0xFFFFFFFFu - mine, (float)(r.weight(value_of(key >> 32)) / (double)total));
     }
@@ -711,15 +819,32 @@ extern "C" int chn_sample(chn_ctx *ctx, const float *logits, uint32_t n_rows, ui
     CHN_REQUIRE(ctx, ctx, "ctx is NULL");
     if (!n_rows) return CHN_OK;
     DeviceGuard dev(ctx);
+    Sample a{};
+    a.V = V;
+    a.ld = ld;
+    a.softcap = softcap;
+    auto rows_from = [&](uint32_t r0) {
+        a.logits = logits + (size_t)r0 * ld;
+        a.temperature = temperature ? temperature + r0 : nullptr;
+        a.top_k = top_k ? top_k + r0 : nullptr;
+        a.top_p = top_p ? top_p + r0 : nullptr;
+        a.min_p = min_p ? min_p + r0 : nullptr;
+        a.u = u + r0;
+        a.tokens = tokens + r0;
+        a.probs = probs ? probs + r0 : nullptr;
+    };
+    if (V <= kSmallV) {
+        rows_from(0);
+        if (V <= 4 * kDrawThreads) k_sample_small<4><<<n_rows, kDrawThreads, 0, ctx->stream>>>(a);
+        else k_sample_small<16><<<n_rows, kDrawThreads, 0, ctx->stream>>>(a);
+        CHN_LAUNCHED(ctx, "k_sample_small");
+        return CHN_OK;
+    }
     const uint32_t blocks = (V + 63) / 64, stretches = (V + kStretch - 1) / kStretch;
     const size_t rows = std::min(n_rows, kRowsAtOnce);
     const size_t row_bytes = (size_t)(stretches + kBins + kList) * 8 + (size_t)(blocks + stretches + 1) * 4;
     int rc = ensure_workspace(ctx, rows * row_bytes);
     if (rc) return rc;
-    Sample a{};
-    a.V = V;
-    a.ld = ld;
-    a.softcap = softcap;
     a.blocks = blocks;
     a.stretches = stretches;
     a.sums = (uint64_t *)ctx->ws;
@@ -732,14 +857,7 @@ extern "C" int chn_sample(chn_ctx *ctx, const float *logits, uint32_t n_rows, ui
     const size_t lds = sizeof(Draw) + std::max<size_t>({(size_t)blocks * 4, (size_t)kMaxK * 8, (size_t)stretches * 8});
     for (uint32_t r0 = 0; r0 < n_rows; r0 += kRowsAtOnce) {
         const uint32_t n = std::min(n_rows - r0, kRowsAtOnce);
-        a.logits = logits + (size_t)r0 * ld;
-        a.temperature = temperature ? temperature + r0 : nullptr;
-        a.top_k = top_k ? top_k + r0 : nullptr;
-        a.top_p = top_p ? top_p + r0 : nullptr;
-        a.min_p = min_p ? min_p + r0 : nullptr;
-        a.u = u + r0;
-        a.tokens = tokens + r0;
-        a.probs = probs ? probs + r0 : nullptr;
+        rows_from(r0);
         // few rows: small workgroups, so that a row spreads over the chip; many: large ones, whose histograms are merged
         // less often
         const uint32_t nt = (uint64_t)n * stretches >= 16 * 256 ? 1024 : 256, wgs = (stretches + nt / 64 - 1) / (nt / 64);
