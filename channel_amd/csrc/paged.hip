@@ -222,6 +222,85 @@ __global__ __launch_bounds__(256) void k_rope_at(RopeAt a) {
     }
 }
 
+// The same for head_dim 256 * N, rows of 16-byte aligned values and rot a
+// multiple of 8: lane l holds dims 4 l + 256 j .. + 3, and the row's partner
+// values come as 16 bytes from the wave's own LDS row.  A workgroup takes 4 *
+// HPW rows of one token, a wave HPW of them with all their loads in flight, so
+// the angles are evaluated once per 4 * HPW rows, while those loads are under
+// way.
+typedef float f4p __attribute__((ext_vector_type(4)));
+template <int N, int HPW>
+__global__ __launch_bounds__(256) void k_rope_at4(RopeAt a) {
+    constexpr uint32_t D = 256 * N;
+    __shared__ float2 cs[D / 2];
+    __shared__ f4p buf[4][D / 4];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const uint32_t t = blockIdx.x / a.groups, row0 = ((blockIdx.x - t * a.groups) * 4 + wave) * HPW;
+    const uint32_t half = a.rot / 2, nrow = a.num_q + 2 * a.num_kv, nk = a.num_q + a.num_kv;
+    const uint32_t slot = a.slots[t], clock = a.clocks[t];
+    f4p v[HPW][N], wq[N], wk[N];
+#pragma unroll
+    for (int i = 0; i < HPW; ++i) {
+        const uint32_t row = min(row0 + i, nrow - 1);                // past the last: it again, left out below
+        const float *in = row < a.num_q ? a.q_in + ((size_t)t * a.num_q + row) * D
+                          : row < nk    ? a.k_in + ((size_t)t * a.num_kv + row - a.num_q) * D
+                                        : a.v_in + ((size_t)t * a.num_kv + row - nk) * D;
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[i][j] = *(const f4p *)(in + 256 * j + 4 * lane);
+    }
+#pragma unroll
+    for (int j = 0; j < N; ++j) {
+        wq[j] = *(const f4p *)(a.qw + 256 * j + 4 * lane);
+        wk[j] = *(const f4p *)(a.kw + 256 * j + 4 * lane);
+    }
+    if ((uint32_t)tid < half) cs[tid] = rope_angle(a, clock, tid);
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < HPW; ++i) {
+        const uint32_t row = row0 + i;
+        if (row >= nrow) return;                                     // a whole wave; no barrier follows
+        float ss = 0.0f;
+#pragma unroll
+        for (int j = 0; j < N; ++j) ss += (v[i][j].x * v[i][j].x + v[i][j].y * v[i][j].y) + (v[i][j].z * v[i][j].z + v[i][j].w * v[i][j].w);
+        const float inv = 1.0f / sqrtf(wave_sum64(ss) / (float)D + a.eps);
+        if (row >= a.num_q && slot >= a.n_slots) continue;
+        if (row >= nk) {
+            float *o = a.vc + ((size_t)slot * a.num_kv + row - nk) * D;
+#pragma unroll
+            for (int j = 0; j < N; ++j) *(f4p *)(o + 256 * j + 4 * lane) = v[i][j] * inv;
+            continue;
+        }
+        const bool q = row < a.num_q;
+        float *o = q ? a.q_out + ((size_t)t * a.num_q + row) * D : a.kc + ((size_t)slot * a.num_kv + row - a.num_q) * D;
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            v[i][j] = (v[i][j] * inv) * (q ? wq[j] : wk[j]);
+            buf[wave][64 * j + lane] = v[i][j];
+        }
+        // the wave reads only what it wrote itself
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t d = 256 * j + 4 * lane;
+            f4p r = v[i][j];
+            if (d < a.rot) {
+                const bool lo = d < half;
+                const uint32_t at = lo ? d : d - half;
+                const f4p p = buf[wave][(lo ? d + half : d - half) / 4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float2 x = cs[at + e];
+                    r[e] = lo ? r[e] * x.x - p[e] * x.y : p[e] * x.y + r[e] * x.x;
+                }
+            }
+            *(f4p *)(o + d) = r;
+        }
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();                             // before the next row overwrites buf
+    }
+}
+
 }  // namespace chn
 
 using namespace chn;
@@ -282,7 +361,21 @@ extern "C" int chn_batch_qkv_rope_at(chn_ctx *ctx, const float *q_in, const floa
     DeviceGuard dev(ctx);
     const RopeAt a{q_in, k_in, k_eq_v ? k_in : v_in, q_norm_w, k_norm_w, q_out, k_cache, v_cache, clocks, slots,
                    n_slots, num_q_heads, num_kv_heads, head_dim, rotary_dim, groups, std::log2((double)theta), eps};
-    if (head_dim > 256) k_rope_at<8><<<groups * n_tok, 256, 0, ctx->stream>>>(a);
+    bool wide = (head_dim == 256 || head_dim == 512) && rotary_dim % 8 == 0;
+    for (const void *p : {(const void *)q_in, (const void *)a.k_in, (const void *)a.v_in, (const void *)q_norm_w,
+                          (const void *)k_norm_w, (const void *)q_out, (const void *)k_cache, (const void *)v_cache})
+        wide = wide && aligned(p, 16);
+    if (wide) {
+        // four rows per wave once they leave a workgroup for every CU
+        const uint32_t rows = num_q_heads + 2 * num_kv_heads;
+        const bool many = (uint64_t)n_tok * rows >= 16 * 512;
+        RopeAt b = a;
+        b.groups = many ? (rows + 15) / 16 : groups;
+        if (head_dim == 256 && many) k_rope_at4<1, 4><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
+        else if (head_dim == 256) k_rope_at4<1, 1><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
+        else if (many) k_rope_at4<2, 4><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
+        else k_rope_at4<2, 1><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
+    } else if (head_dim > 256) k_rope_at<8><<<groups * n_tok, 256, 0, ctx->stream>>>(a);
     else k_rope_at<4><<<groups * n_tok, 256, 0, ctx->stream>>>(a);
     CHN_LAUNCHED(ctx, "k_rope_at");
     return CHN_OK;

@@ -860,7 +860,7 @@ extern "C" int chn_sample(chn_ctx *ctx, const float *logits, uint32_t n_rows, ui
         rows_from(r0);
         // few rows: small workgroups, so that a row spreads over the chip; many: large ones, whose histograms are merged
         // less often
-        const uint32_t nt = (uint64_t)n * stretches >= 16 * 256 ? 1024 : 256, wgs = (stretches + nt / 64 - 1) / (nt / 64);
+        const uint32_t nt = (uint64_t)n * stretches >= 16 * 512 ? 1024 : 256, wgs = (stretches + nt / 64 - 1) / (nt / 64);
         k_sample_max<<<dim3((stretches + 3) / 4, n), 256, 0, ctx->stream>>>(a);
         k_sample_mass<<<dim3(wgs, n), nt, 0, ctx->stream>>>(a);
         k_sample_border<<<dim3(wgs, n), nt, 0, ctx->stream>>>(a);
