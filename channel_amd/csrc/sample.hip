@@ -40,7 +40,7 @@ constexpr uint32_t kStretch = 2048;         // values of a wave: one sum, 32 blo
 constexpr uint32_t kBins = 2048;            // of 2^-6 powers of two each
 constexpr uint32_t kList = 4096;            // tokens of a row's list
 constexpr uint32_t kMaxK = 1024;            // top-k by block maxima
-constexpr uint32_t kDrawThreads = 1024;
+constexpr uint32_t kDrawThreads = 1024, kPassThreads = 512;
 constexpr uint32_t kRowsAtOnce = 1024;      // rows that share the workspace
 
 struct Sample {
@@ -72,6 +72,13 @@ __device__ __forceinline__ uint64_t token_key(float v, uint32_t i) {
     return ((uint64_t)orderable(v) << 32) | (0xFFFFFFFFu - i);
 }
 
+// a b + c, c in scalar registers (otherwise it is moved into vector registers
+// before every use)
+__device__ __forceinline__ double fma_s(double a, double b, double c) {
+    double d;
+    asm("v_fma_f64 %0, %1, %2, %3" : "=v"(d) : "v"(a), "v"(b), "s"(c));
+    return d;
+}
 // exp on half a power of two either way: x = n ln 2 + r, and (exp(r) - 1) by
 // its series (the 13th term is below 2^-52 of the first).
 struct Exp {
@@ -80,16 +87,15 @@ struct Exp {
         const double t = x * 1.4426950408889634074;
         n = rint(t);
         const double r = (t - n) * 0.69314718055994530942;
-        double p = 1.0 / 479001600.0;
-        p = fma(p, r, 1.0 / 39916800.0);
-        p = fma(p, r, 1.0 / 3628800.0);
-        p = fma(p, r, 1.0 / 362880.0);
-        p = fma(p, r, 1.0 / 40320.0);
-        p = fma(p, r, 1.0 / 5040.0);
-        p = fma(p, r, 1.0 / 720.0);
-        p = fma(p, r, 1.0 / 120.0);
-        p = fma(p, r, 1.0 / 24.0);
-        p = fma(p, r, 1.0 / 6.0);
+        double p = fma(1.0 / 479001600.0, r, 1.0 / 39916800.0);
+        p = fma_s(p, r, 1.0 / 3628800.0);
+        p = fma_s(p, r, 1.0 / 362880.0);
+        p = fma_s(p, r, 1.0 / 40320.0);
+        p = fma_s(p, r, 1.0 / 5040.0);
+        p = fma_s(p, r, 1.0 / 720.0);
+        p = fma_s(p, r, 1.0 / 120.0);
+        p = fma_s(p, r, 1.0 / 24.0);
+        p = fma_s(p, r, 1.0 / 6.0);
         p = fma(p, r, 0.5);
         p = fma(p, r, 1.0);
         em1 = p * r;
@@ -109,6 +115,7 @@ __device__ __forceinline__ double tanh_of(double y) {
 
 // A row's settings and the weights of its tokens: cap * tanh(l / cap) (or l)
 // relative to the row's largest.
+template <bool CAP>
 struct Row {
     double cap, inv_cap, top, inv_t;
     float raw_top, bin_scale;
@@ -135,12 +142,12 @@ struct Row {
         least = mm > 0.0f ? (uint64_t)ceil(fmin((double)mm, 1.0) * (double)(1ull << kWeightBits)) : 0;
     }
     __device__ __forceinline__ double capped(float l) const {
-        return cap > 0.0 ? cap * tanh_of((double)l * inv_cap) : (double)l;
+        return CAP ? cap * tanh_of((double)l * inv_cap) : (double)l;
     }
     __device__ __forceinline__ double weight(float l) const {                              // 2^kWeightBits exp(..)
-        if (l == raw_top) return (double)(1ull << kWeightBits);
-        const double x = (capped(l) - top) * inv_t;
-        return x > -64.0 ? exp_scaled(fmin(x, 0.0), kWeightBits) : 0.0;                   // below: rounds to zero
+        // no branch, so that several run side by side.  exp(-64) rounds to zero; a NaN (infinities) becomes -64
+        const double x = fmin(fmax((capped(l) - top) * inv_t, -64.0), 0.0);
+        return l == raw_top ? (double)(1ull << kWeightBits) : exp_scaled(x, kWeightBits);
     }
     // 2^52 added leaves the rounded weight in the low bits
     __device__ __forceinline__ uint64_t units(float l) const {
@@ -158,24 +165,39 @@ struct Row {
         const uint64_t n = g < 1.0 ? 1 : (uint64_t)g;
         return n < Z ? n : Z;
     }
-    __device__ __forceinline__ bool by_mass() const { return some && !greedy && k == 0; }
 };
 
-__device__ __forceinline__ uint64_t shfl_xor64(uint64_t v, int m) {
-    return (uint64_t)__shfl_xor((unsigned long long)v, m, 64);
+// 64-bit sums and minima over the lanes in registers (DPP): few instructions,
+// as a workgroup that runs a kernel once waits for its code as well.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t old, uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp((int)(old >> 32), (int)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (uint64_t)hi << 32 | lo;
 }
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += shfl_xor64(v, o);
-    return v;
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {                          // the same lane for all
+    const uint32_t lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (uint64_t)hi << 32 | lo;
 }
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, int lane) {                  // inclusive
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t w = (uint64_t)__shfl_up((unsigned long long)v, o, 64);
-        if (lane >= o) v += w;
-    }
-    return v;
+__device__ __forceinline__ uint64_t row16_scan_u64(uint64_t v) {                            // inclusive, of 16 lanes
+    v += dpp64<0x111, 0xF>(0, v);                                                          // row_shr:1, 2, 4, 8
+    v += dpp64<0x112, 0xF>(0, v);
+    v += dpp64<0x114, 0xF>(0, v);
+    return v + dpp64<0x118, 0xF>(0, v);
+}
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {                             // inclusive
+    v = row16_scan_u64(v);
+    v += dpp64<0x142, 0xA>(0, v);                                                          // row_bcast:15, 31
+    return v + dpp64<0x143, 0xC>(0, v);
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) { return lane64(wave_scan_u64(v), 63); }
+__device__ __forceinline__ uint64_t wave_min_u64(uint64_t v) {
+    v = min(v, dpp64<0x111, 0xF>(v, v));
+    v = min(v, dpp64<0x112, 0xF>(v, v));
+    v = min(v, dpp64<0x114, 0xF>(v, v));
+    v = min(v, dpp64<0x118, 0xF>(v, v));
+    v = min(v, dpp64<0x142, 0xA>(v, v));
+    return lane64(min(v, dpp64<0x143, 0xC>(v, v)), 63);
 }
 __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
 #pragma unroll
@@ -183,27 +205,41 @@ __device__ __forceinline__ uint32_t wave_max_u32(uint32_t v) {
     return v;
 }
 
-// f(index, value) for the wave's stretch of 2048 values, four per lane and
-// load (rows start at any 4-byte address); NaN behind the row's end.  g() after
-// each load's four.
-template <typename F, typename G>
-__device__ __forceinline__ void stretch(const Sample &a, const float *x, uint32_t s, F &&f, G &&g) {
-    const uint32_t i0 = s * kStretch + 4 * (threadIdx.x & 63);
-    f4u v[8];
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t i = i0 + 256 * j;
-        if (i + 4 <= a.V) v[j] = *(const f4u *)(x + i);
+// A wave's stretch of 2048 values, four per lane and load (rows start at any
+// 4-byte address), half of it in registers at a time; NaN behind the row's end.
+struct Stretch {
+    f4u v[4];
+
+    __device__ __forceinline__ void load(const Sample &a, const float *x, uint32_t s, int j, f4u &d) {
+        const uint32_t i = s * kStretch + 4 * (threadIdx.x & 63) + 256 * j;
+        if (i + 4 <= a.V) d = *(const f4u *)(x + i);
         else
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[j][e] = i + e < a.V ? x[i + e] : __builtin_nanf("");
+            for (int e = 0; e < 4; ++e) d[e] = i + e < a.V ? x[i + e] : __builtin_nanf("");
     }
+    __device__ __forceinline__ void start(const Sample &a, const float *x, uint32_t s) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-#pragma unroll
-        for (int e = 0; e < 4; ++e) f(i0 + 256 * j + e, v[j][e]);
-        g(j);
+        for (int j = 0; j < 4; ++j) load(a, x, s, j, v[j]);
     }
+    // f(index of the first, four values, number of the load) for stretch s, which has been started
+    template <typename F>
+    __device__ __forceinline__ void each(const Sample &a, const float *x, uint32_t s, F &&f) {
+#pragma unroll 1
+        for (int h = 0; h < 2; ++h) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                f(s * kStretch + 4 * (threadIdx.x & 63) + 256 * (4 * h + j), v[j], 4 * h + j);
+                if (h == 0) load(a, x, s, 4 + j, v[j]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
+        }
+    }
+};
+template <typename F>
+__device__ __forceinline__ void stretch(const Sample &a, const float *x, uint32_t s, F &&f) {
+    Stretch v;
+    v.start(a, x, s);
+    v.each(a, x, s, f);
 }
 
 // the row's largest logit, by every wave
@@ -211,6 +247,11 @@ __device__ __forceinline__ uint32_t row_top(const Sample &a, uint32_t row) {
     uint32_t m = 0;
     for (uint32_t i = threadIdx.x & 63; i < a.stretches; i += 64) m = max(m, a.smax[(size_t)row * a.stretches + i]);
     return wave_max_u32(m);
+}
+
+// Rows whose weights k_sample_mass sums: neither greedy nor with top-k.
+__device__ __forceinline__ bool by_mass(const Sample &a, uint32_t row) {
+    return (!a.temperature || a.temperature[row] > 0.0f) && (!a.top_k || a.top_k[row] == 0 || a.top_k[row] >= a.V);
 }
 
 // A wave per stretch: maxima of 64 (16 lanes of a load) and of all.  The
@@ -223,15 +264,16 @@ __global__ __launch_bounds__(256) void k_sample_max(Sample a) {
         if (threadIdx.x == 0) a.listed[row] = 0;
     }
     if (s >= a.stretches) return;
-    float m = -__builtin_inff(), most = m;
+    float most = -__builtin_inff();
     stretch(a, a.logits + (size_t)row * a.ld, s,
-            [&](uint32_t, float v) { m = fmaxf(m, allowed(v) ? v : -__builtin_inff()); },
-            [&](int j) {
+            [&](uint32_t, const f4u &v, int j) {
+                float m = -__builtin_inff();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) m = fmaxf(m, allowed(v[e]) ? v[e] : -__builtin_inff());
                 m = row16_max(m);
                 const uint32_t b = s * 32 + 4 * j + (lane >> 4);
                 if ((lane & 15) == 0 && b < a.blocks) a.bmax[(size_t)row * a.blocks + b] = allowed(m) ? orderable(m) : 0u;
                 most = fmaxf(most, m);
-                m = -__builtin_inff();
             });
     most = wave_max64(most);
     if (lane == 0) a.smax[(size_t)row * a.stretches + s] = allowed(most) ? orderable(most) : 0u;
@@ -239,28 +281,38 @@ __global__ __launch_bounds__(256) void k_sample_max(Sample a) {
 
 // Rows without top-k: the histogram of the weights (with top-p), or the sums of
 // the stretches.
-__global__ void k_sample_mass(Sample a) {
+template <bool CAP>
+__global__ __launch_bounds__(kPassThreads) void k_sample_mass(Sample a) {
     __shared__ uint64_t hist[kBins];
-    const uint32_t row = blockIdx.y, s = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
-    const Row r(a, row, row_top(a, row));
-    if (!r.by_mass()) return;                                        // the whole workgroup
+    const uint32_t row = blockIdx.y, s = blockIdx.x * (kPassThreads / 64) + (threadIdx.x >> 6);
+    if (!by_mass(a, row)) return;                                    // the whole workgroup
     const float *x = a.logits + (size_t)row * a.ld;
+    Stretch v;
+    if (s < a.stretches) v.start(a, x, s);                            // while the row's settings and bins are prepared
+    __builtin_amdgcn_sched_barrier(0);
+    const Row<CAP> r(a, row, row_top(a, row));
     if (r.p < 1.0f) {
         for (uint32_t i = threadIdx.x; i < kBins; i += blockDim.x) hist[i] = 0;
         __syncthreads();
         if (s < a.stretches)
-            stretch(a, x, s,
-                    [&](uint32_t, float v) {
-                        const uint64_t w = allowed(v) ? r.units(v) : 0;
-                        if (w) atomicAdd((unsigned long long *)&hist[r.bin(v)], (unsigned long long)w);
-                    },
-                    [](int) {});
+            v.each(a, x, s,
+                   [&](uint32_t, const f4u &l, int) {
+                       uint64_t w[4];
+#pragma unroll
+                       for (int e = 0; e < 4; ++e) w[e] = allowed(l[e]) ? r.units(l[e]) : 0;
+#pragma unroll
+                       for (int e = 0; e < 4; ++e)
+                           if (w[e]) atomicAdd((unsigned long long *)&hist[r.bin(l[e])], (unsigned long long)w[e]);
+                   });
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < kBins; i += blockDim.x)
             if (hist[i]) atomicAdd((unsigned long long *)&a.hist[(size_t)row * kBins + i], (unsigned long long)hist[i]);
     } else if (s < a.stretches) {
         uint64_t sum = 0;
-        stretch(a, x, s, [&](uint32_t, float v) { sum += allowed(v) ? r.kept(r.units(v)) : 0; }, [](int) {});
+        v.each(a, x, s, [&](uint32_t, const f4u &l, int) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += allowed(l[e]) ? r.kept(r.units(l[e])) : 0;
+        });
         sum = wave_sum_u64(sum);
         if ((threadIdx.x & 63) == 0) a.sums[(size_t)row * a.stretches + s] = sum;
     }
@@ -268,20 +320,18 @@ __global__ void k_sample_mass(Sample a) {
 
 // The bin in which a row's running sum reaches its goal, and the goal's rest
 // there.  All threads; sh: 20 words.
-__device__ __forceinline__ uint32_t border_bin(const Sample &a, const Row &r, uint32_t row, uint64_t *sh, uint64_t &rest) {
+template <bool CAP>
+__device__ __forceinline__ uint32_t border_bin(const Sample &a, const Row<CAP> &r, uint32_t row, uint64_t *sh, uint64_t &rest) {
     const uint32_t tid = threadIdx.x, nt = blockDim.x, per = kBins / nt;       // 256 or 1024 threads: 8 or 2 bins
-    const int lane = tid & 63, wave = tid >> 6, nw = nt >> 6;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = nt >> 6;
     const uint64_t *h = a.hist + (size_t)row * kBins + tid * per;
     uint64_t own = 0;
     for (uint32_t i = 0; i < per; ++i) own += h[i];
-    const uint64_t incl = wave_scan_u64(own, lane);
+    const uint64_t incl = wave_scan_u64(own);
     if (lane == 63) sh[wave] = incl;
     __syncthreads();
-    uint64_t before = incl - own, Z = 0;
-    for (int w = 0; w < nw; ++w) {
-        before += w < wave ? sh[w] : 0;
-        Z += sh[w];
-    }
+    const uint64_t waves = row16_scan_u64((lane & 15) < nw ? sh[lane & 15] : 0), Z = lane64(waves, 15);
+    uint64_t before = incl - own + (wave ? lane64(waves, wave - 1) : 0);
     const uint64_t g = r.goal(Z);
     if (before < g && before + own >= g) {
         uint32_t b = tid * per;
@@ -298,54 +348,67 @@ __device__ __forceinline__ uint32_t border_bin(const Sample &a, const Row &r, ui
 // list, the kept weights above it summed by stretch.  A tenth to a half of a
 // row's tokens lie above: they are queued, and their weights (64-bit
 // arithmetic) formed by full waves.
-__global__ void k_sample_border(Sample a) {
+template <bool CAP>
+__global__ __launch_bounds__(kPassThreads) void k_sample_border(Sample a) {
     constexpr uint32_t kMine = 1024;                                     // the workgroup's share of the list
     __shared__ uint64_t sh[20], found[kMine];
-    __shared__ float queue[16][128];
+    __shared__ float queue[kPassThreads / 64][512];
     __shared__ uint32_t nfound, at0;
-    const uint32_t row = blockIdx.y, s = blockIdx.x * (blockDim.x >> 6) + (threadIdx.x >> 6);
+    const uint32_t row = blockIdx.y, s = blockIdx.x * (kPassThreads / 64) + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    const Row r(a, row, row_top(a, row));
-    if (!r.by_mass() || !(r.p < 1.0f)) return;
+    if (!by_mass(a, row) || !a.top_p || !(a.top_p[row] < 1.0f)) return;
+    const float *x = a.logits + (size_t)row * a.ld;
+    Stretch v;
+    if (s < a.stretches) v.start(a, x, s);
+    __builtin_amdgcn_sched_barrier(0);
+    const Row<CAP> r(a, row, row_top(a, row));
+    if (!r.some) return;
     uint64_t rest;
     const uint32_t border = border_bin(a, r, row, sh, rest);
     if (threadIdx.x == 0) nfound = 0;
     __syncthreads();
     float *q = queue[threadIdx.x >> 6];
-    uint32_t n = 0;                                                      // queued, below 64 between steps
-    uint64_t sum = 0;
     const uint64_t below = ((uint64_t)1 << lane) - 1;
     auto fence = [] {                                                    // the wave reads what it wrote
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
-    if (s < a.stretches) stretch(a, a.logits + (size_t)row * a.ld, s,
-            [&](uint32_t i, float v) {
-                const uint32_t b = allowed(v) ? r.bin(v) : kBins;
+    if (s < a.stretches) {
+        uint32_t n = 0;                                                  // queued, below 64 between steps
+        uint64_t sum = 0;
+        v.each(a, x, s, [&](uint32_t i, const f4u &l, int) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t b = allowed(l[e]) ? r.bin(l[e]) : kBins;
                 const uint64_t over = __ballot(b < border), in = __ballot(b == border);
-                if (b < border) q[n + __popcll(over & below)] = v;
+                if (b < border) q[n + __popcll(over & below)] = l[e];
                 n += __popcll(over);
-                if (n >= 64) {
-                    fence();
-                    sum += r.kept(r.units(q[lane]));
-                    const float tail = q[64 + lane];
-                    fence();
-                    q[lane] = tail;
-                    n -= 64;
-                }
                 if (in) {                                                // one atomic for the wave's
                     const int first = __ffsll((unsigned long long)in) - 1;
                     uint32_t at = 0;
                     if (lane == first) at = atomicAdd(&nfound, (uint32_t)__popcll(in));
                     at = __shfl(at, first, 64) + (uint32_t)__popcll(in & below);
-                    if (b == border && at < kMine) found[at] = token_key(v, i);
+                    if (b == border && at < kMine) found[at] = token_key(l[e], i + e);
                 }
-            },
-            [](int) {});
-    fence();
-    if (lane < (int)n) sum += r.kept(r.units(q[lane]));
-    sum = wave_sum_u64(sum);
-    if (lane == 0 && s < a.stretches) a.sums[(size_t)row * a.stretches + s] = sum;
+            }
+            if (n >= 256) {                                              // four a lane, side by side
+                fence();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) sum += r.kept(r.units(q[64 * e + lane]));
+                n -= 256;
+                float tail[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) tail[e] = q[256 + 64 * e + lane];
+                fence();
+#pragma unroll
+                for (int e = 0; e < 4; ++e) q[64 * e + lane] = tail[e];
+            }
+        });
+        fence();
+        for (uint32_t e = lane; e < n; e += 64) sum += r.kept(r.units(q[e]));
+        sum = wave_sum_u64(sum);
+        if (lane == 0) a.sums[(size_t)row * a.stretches + s] = sum;
+    }
     __syncthreads();
     // more than its share: the row's list counts as full
     if (threadIdx.x == 0 && nfound) at0 = atomicAdd(&a.listed[row], nfound <= kMine ? nfound : kList + 1);
@@ -358,6 +421,7 @@ __global__ void k_sample_border(Sample a) {
 constexpr uint32_t kDigits = 2 * kDrawThreads;
 struct Group {
     static constexpr int NW = kDrawThreads / 64;
+    static_assert(NW == 16, "the waves' parts are a row of 16 lanes");
     uint64_t hist_w[kDigits], part[NW], found[4];
     uint32_t hist_n[kDigits], n, hit;
 
@@ -366,32 +430,25 @@ struct Group {
         __syncthreads();
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
-        uint64_t t = 0;
-        for (int w = 0; w < NW; ++w) t += part[w];
-        return t;
+        return lane64(row16_scan_u64(part[threadIdx.x & 15]), 15);
     }
     __device__ __forceinline__ uint64_t least(uint64_t v) {
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) v = min(v, shfl_xor64(v, o));
+        v = wave_min_u64(v);
         __syncthreads();
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
-        for (int w = 0; w < NW; ++w) v = min(v, part[w]);
-        return v;
+        return wave_min_u64(part[threadIdx.x & 15]);
     }
     // inclusive running sum over the threads, and the whole sum
     __device__ __forceinline__ uint64_t scan(uint64_t v, uint64_t &total) {
-        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-        v = wave_scan_u64(v, lane);
+        const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        v = wave_scan_u64(v);
         __syncthreads();
-        if (lane == 63) part[wave] = v;
+        if ((threadIdx.x & 63) == 63) part[wave] = v;
         __syncthreads();
-        total = 0;
-        for (int w = 0; w < NW; ++w) {
-            v += w < wave ? part[w] : 0;
-            total += part[w];
-        }
-        return v;
+        const uint64_t waves = row16_scan_u64(part[threadIdx.x & 15]);
+        total = lane64(waves, 15);
+        return v + (wave ? lane64(waves, wave - 1) : 0);
     }
     // every(f): f(key, weight()) for all tokens looked through.  The key of the last token of the order, from those in
     // [lo, hi], that the running count (or sum of weights) needs to reach `goal`: the range in up to 2048 parts, then the
@@ -450,7 +507,7 @@ __device__ __forceinline__ uint64_t target_of(float u, uint64_t Z) {
 // registers (thread t: values t, t + 1024, ..).  With more than a launch per row
 // latency is what counts: 50 rows of 10007 took 73 us in the four launches.
 constexpr uint32_t kSmallV = 16 * kDrawThreads;
-template <int J>
+template <int J, bool CAP>
 __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
     __shared__ Group sh;
     __shared__ uint64_t by_wave[J][Group::NW];
@@ -474,7 +531,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
         n += key ? 1 : 0;
     }
     hi = ~sh.least(~hi);
-    const Row r(a, row, (uint32_t)(hi >> 32));
+    const Row<CAP> r(a, row, (uint32_t)(hi >> 32));
     auto finish = [&](uint32_t token, float prob) {
         a.tokens[row] = token;
         if (a.probs) a.probs[row] = prob;
@@ -532,7 +589,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
 #pragma unroll
         for (int j = 0; j < J; ++j)
             if (j == (int)(sh.hit / Group::NW)) {
-                const uint64_t run = wave_scan_u64(w[j], lane);
+                const uint64_t run = wave_scan_u64(w[j]);
                 if (w[j] && run > rest && run - w[j] <= rest)
                     finish(tid + j * kDrawThreads, (float)(r.weight(v[j]) / (double)Z));
             }
@@ -546,6 +603,7 @@ struct Draw {
 };
 
 // A workgroup per row: the kept tokens' last key, then the draw.
+template <bool CAP>
 __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
     extern __shared__ uint64_t lds[];
     constexpr int NW = Group::NW;
@@ -557,7 +615,12 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
     const float *x = a.logits + (size_t)row * a.ld;
     const uint32_t *bmax = a.bmax + (size_t)row * a.blocks;
     const float u = a.u[row];
-    const Row r(a, row, row_top(a, row));
+    // the first block maxima, on their way while the settings are looked at
+    uint32_t first[4];
+#pragma unroll
+    for (uint32_t e = 0; e < 4; ++e) first[e] = bmax[min(tid + e * kDrawThreads, a.blocks - 1)];
+    __builtin_amdgcn_sched_barrier(0);
+    const Row<CAP> r(a, row, row_top(a, row));
 
     auto finish = [&](uint32_t token, float prob) {
         a.tokens[row] = token;
@@ -585,14 +648,14 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         }
         return;
     }
-    auto whole_row = [&](auto &&f) {
+    auto whole_row = [&](auto &&f) __attribute__((always_inline)) {
         for (uint32_t i = tid; i < a.V; i += kDrawThreads) {
             const float v = x[i];
             if (allowed(v)) f(token_key(v, i), [&] { return r.units(v); });
         }
     };
     // The draw from the kept tokens of a row given the sums of its stretches (n of them, in LDS).
-    auto draw_stretch = [&](uint64_t above, const uint64_t *sums) {
+    auto draw_stretch = [&](uint64_t above, const uint64_t *sums) __attribute__((always_inline)) {
         uint64_t Z, own = 0;
         const uint32_t n = a.stretches;                               // at most kSampleMaxV / kStretch = 512
         own = tid < n ? sums[tid] : 0;
@@ -619,15 +682,15 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         }
     };
     // The sums of the stretches, formed here.
-    auto draw_whole = [&](uint64_t above) {
+    auto draw_whole = [&](uint64_t above) __attribute__((always_inline)) {
         uint64_t *sums = (uint64_t *)spare;
         for (uint32_t s = wave; s < a.stretches; s += NW) {
             uint64_t sum = 0;
-            stretch(a, x, s,
-                    [&](uint32_t i, float v) {
-                        if (allowed(v) && token_key(v, i) >= above) sum += r.kept(r.units(v));
-                    },
-                    [](int) {});
+            stretch(a, x, s, [&](uint32_t i, const f4u &v, int) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                    if (allowed(v[e]) && token_key(v[e], i + e) >= above) sum += r.kept(r.units(v[e]));
+            });
             sum = wave_sum_u64(sum);
             if (lane == 0) sums[s] = sum;
         }
@@ -635,7 +698,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         draw_stretch(above, sums);
     };
     const uint64_t top_key = ((uint64_t)orderable(r.raw_top) << 32) | 0xFFFFFFFFu;
-    auto least_key = [&](uint64_t &n) {                              // the row's, and how many are allowed
+    auto least_key = [&](uint64_t &n) __attribute__((always_inline)) {                              // the row's, and how many are allowed
         uint64_t m = ~0ull;
         n = 0;
         whole_row([&](uint64_t key, auto &&) {
@@ -645,7 +708,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         n = sh.sum(n);
         return sh.least(m);
     };
-    auto walk = [&] {
+    auto walk = [&]() __attribute__((always_inline)) {
         uint64_t n, above = least_key(n), Z = 0;
         if (r.k && n > r.k) above = sh.last_key(whole_row, above, top_key, false, r.k);
         if (r.p < 1.0f) {
@@ -680,7 +743,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         }
         lo = sh.least(lo);
         hi = ~sh.least(~hi);
-        auto listed = [&](auto &&f) {
+        auto listed = [&](auto &&f) __attribute__((always_inline)) {
             for (uint32_t i = tid; i < n; i += kDrawThreads) {
                 const uint64_t key = d.list[i];
                 f(key, [&] { return r.units(value_of(key >> 32)); });
@@ -709,11 +772,19 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
     if (bounded) {
         uint32_t least = 0xFFFFFFFFu;
         uint64_t some = 0;
-        for (uint32_t b = tid; b < a.blocks; b += kDrawThreads) {
-            const uint32_t m = bmax[b];
-            spare[b] = m;
-            least = m ? min(least, m) : least;
-            some += m ? 1 : 0;
+        for (uint32_t b0 = tid; b0 < a.blocks; b0 += 4 * kDrawThreads) {
+            uint32_t m[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const uint32_t b = b0 + e * kDrawThreads;
+                m[e] = b >= a.blocks ? 0 : b0 == tid ? first[e] : bmax[b];
+            }
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                if (b0 + e * kDrawThreads < a.blocks) spare[b0 + e * kDrawThreads] = m[e];
+                least = m[e] ? min(least, m[e]) : least;
+                some += m[e] ? 1 : 0;
+            }
         }
         for (uint32_t i = tid; i < kDigits; i += kDrawThreads) sh.hist_n[i] = 0;
         some = sh.sum(some);
@@ -721,8 +792,14 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         if (some >= r.k) {
             const uint32_t range = orderable(r.raw_top) - least;
             const int shift = max(32 - __clz(range) - 11, 0);                 // range 0: 0
-            for (uint32_t b = tid; b < a.blocks; b += kDrawThreads)
-                if (spare[b]) atomicAdd(&sh.hist_n[(spare[b] - least) >> shift], 1u);
+            for (uint32_t b0 = tid; b0 < a.blocks; b0 += 4 * kDrawThreads) {
+                uint32_t m[4];
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e) m[e] = b0 + e * kDrawThreads < a.blocks ? spare[b0 + e * kDrawThreads] : 0;
+#pragma unroll
+                for (uint32_t e = 0; e < 4; ++e)
+                    if (m[e]) atomicAdd(&sh.hist_n[(m[e] - least) >> shift], 1u);
+            }
             __syncthreads();
             const uint32_t e = kDigits - 1 - 2 * tid, c0 = sh.hist_n[e], c1 = sh.hist_n[e - 1];
             uint64_t total;
@@ -732,11 +809,17 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
             floor_key = least + ((uint32_t)sh.found[0] << shift);
         }
         // those blocks' numbers, in place of the maxima: every round writes only where it and earlier ones have read
-        for (uint32_t b0 = 0; b0 < a.blocks; b0 += kDrawThreads) {
-            const uint32_t b = b0 + tid;
-            const bool in = b < a.blocks && spare[b] >= floor_key;
+        for (uint32_t b0 = 0; b0 < a.blocks; b0 += 4 * kDrawThreads) {
+            bool in[4];
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e) {
+                const uint32_t b = b0 + e * kDrawThreads + tid;
+                in[e] = b < a.blocks && spare[b] >= floor_key;
+            }
             __syncthreads();
-            if (in) spare[atomicAdd(&sh.hit, 1u)] = b;
+#pragma unroll
+            for (uint32_t e = 0; e < 4; ++e)
+                if (in[e]) spare[atomicAdd(&sh.hit, 1u)] = b0 + e * kDrawThreads + tid;
             __syncthreads();
         }
         const uint32_t nb = sh.hit;
@@ -778,6 +861,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
     for (uint32_t i = tid; i < n; i += kDrawThreads) {
         const uint64_t key = d.list[i];
         uint32_t rank = 0;
+#pragma unroll 8
         for (uint32_t j = 0; j < n; ++j) rank += d.list[j] > key ? 1u : 0u;
         if (rank < r.k) sorted[rank] = key;
     }
@@ -798,10 +882,31 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
     if (kw) {
         uint64_t before = 0;
         const uint32_t mine = (uint32_t)key;                           // ~index: larger for lower indexes
-        for (uint32_t j = 0; j < k; ++j) before += (uint32_t)sorted[j] > mine ? d.list[j] : 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < k; ++j) {
+            const uint64_t other = d.list[j];                          // read either way: no branch, so reads overlap
+            before += (uint32_t)sorted[j] > mine ? other : 0;
+        }
         if (before <= target && before + kw > target)
             finish(0xFFFFFFFFu - mine, (float)(r.weight(value_of(key >> 32)) / (double)total));
     }
+}
+
+template <bool CAP>
+static int launch_small(chn_ctx *ctx, const Sample &a, uint32_t n) {
+    if (a.V <= 4 * kDrawThreads) k_sample_small<4, CAP><<<n, kDrawThreads, 0, ctx->stream>>>(a);
+    else k_sample_small<16, CAP><<<n, kDrawThreads, 0, ctx->stream>>>(a);
+    CHN_LAUNCHED(ctx, "k_sample_small");
+    return CHN_OK;
+}
+
+template <bool CAP>
+static void launch_rows(chn_ctx *ctx, const Sample &a, uint32_t n, size_t lds) {
+    const dim3 wide((a.stretches + kPassThreads / 64 - 1) / (kPassThreads / 64), n);
+    k_sample_max<<<dim3((a.stretches + 3) / 4, n), 256, 0, ctx->stream>>>(a);
+    k_sample_mass<CAP><<<wide, kPassThreads, 0, ctx->stream>>>(a);
+    k_sample_border<CAP><<<wide, kPassThreads, 0, ctx->stream>>>(a);
+    k_sample_draw<CAP><<<n, kDrawThreads, lds, ctx->stream>>>(a);
 }
 
 }  // namespace chn
@@ -835,10 +940,7 @@ extern "C" int chn_sample(chn_ctx *ctx, const float *logits, uint32_t n_rows, ui
     };
     if (V <= kSmallV) {
         rows_from(0);
-        if (V <= 4 * kDrawThreads) k_sample_small<4><<<n_rows, kDrawThreads, 0, ctx->stream>>>(a);
-        else k_sample_small<16><<<n_rows, kDrawThreads, 0, ctx->stream>>>(a);
-        CHN_LAUNCHED(ctx, "k_sample_small");
-        return CHN_OK;
+        return softcap > 0.0f ? launch_small<true>(ctx, a, n_rows) : launch_small<false>(ctx, a, n_rows);
     }
     const uint32_t blocks = (V + 63) / 64, stretches = (V + kStretch - 1) / kStretch;
     const size_t rows = std::min(n_rows, kRowsAtOnce);
@@ -858,13 +960,7 @@ extern "C" int chn_sample(chn_ctx *ctx, const float *logits, uint32_t n_rows, ui
     for (uint32_t r0 = 0; r0 < n_rows; r0 += kRowsAtOnce) {
         const uint32_t n = std::min(n_rows - r0, kRowsAtOnce);
         rows_from(r0);
-        // few rows: small workgroups, so that a row spreads over the chip; many: large ones, whose histograms are merged
-        // less often
-        const uint32_t nt = (uint64_t)n * stretches >= 16 * 512 ? 1024 : 256, wgs = (stretches + nt / 64 - 1) / (nt / 64);
-        k_sample_max<<<dim3((stretches + 3) / 4, n), 256, 0, ctx->stream>>>(a);
-        k_sample_mass<<<dim3(wgs, n), nt, 0, ctx->stream>>>(a);
-        k_sample_border<<<dim3(wgs, n), nt, 0, ctx->stream>>>(a);
-        k_sample_draw<<<n, kDrawThreads, lds, ctx->stream>>>(a);
+        softcap > 0.0f ? launch_rows<true>(ctx, a, n, lds) : launch_rows<false>(ctx, a, n, lds);
         CHN_LAUNCHED(ctx, "k_sample");
     }
     return CHN_OK;
