@@ -101,11 +101,30 @@ struct Exp {
         em1 = p * r;
     }
 };
-// exp(x) 2^bits
-__device__ __forceinline__ double exp_scaled(double x, int bits) {
-    const Exp e(x);
-    return ldexp(1.0 + e.em1, (int)e.n + bits);
-}
+// 2^t for -1000 < t < 900 as part * scale, scale a power of two times
+// 2^kWeightBits: 2^f on half a power of two either way by its series, whose
+// 12th term is 2^-47 of the first: a sixteenth of a weight's unit.
+struct Pow2 {
+    double part, scale;
+    __device__ __forceinline__ explicit Pow2(double t) {
+        constexpr double L = 0.69314718055994530942, c2 = L * L / 2, c3 = c2 * L / 3, c4 = c3 * L / 4, c5 = c4 * L / 5,
+                         c6 = c5 * L / 6, c7 = c6 * L / 7, c8 = c7 * L / 8, c9 = c8 * L / 9, c10 = c9 * L / 10,
+                         c11 = c10 * L / 11;
+        const double n = rint(t), f = t - n;
+        double p = fma_s(f, c11, c10);
+        p = fma_s(p, f, c9);
+        p = fma_s(p, f, c8);
+        p = fma_s(p, f, c7);
+        p = fma_s(p, f, c6);
+        p = fma_s(p, f, c5);
+        p = fma_s(p, f, c4);
+        p = fma_s(p, f, c3);
+        p = fma_s(p, f, c2);
+        p = fma_s(p, f, L);
+        part = fma(p, f, 1.0);
+        scale = __builtin_bit_cast(double, (uint64_t)(uint32_t)(((int)n + kWeightBits + 1023) << 20) << 32);
+    }
+};
 // tanh(y) from exp(-2 |y|) - 1, which keeps its digits near 0
 __device__ __forceinline__ double tanh_of(double y) {
     const Exp e(fmax(-2.0 * fabs(y), -64.0));
@@ -117,7 +136,7 @@ __device__ __forceinline__ double tanh_of(double y) {
 // relative to the row's largest.
 template <bool CAP>
 struct Row {
-    double cap, inv_cap, top, inv_t;
+    double cap, inv_cap, top, powers;   // powers: log2(e) / T
     float raw_top, bin_scale;
     uint64_t least;                // min_p, as a weight
     uint32_t k;                    // 0: no top-k
@@ -131,10 +150,10 @@ struct Row {
         raw_top = value_of(largest);
         cap = a.softcap;
         inv_cap = 1.0 / cap;
-        inv_t = 1.0 / (double)T;
+        powers = 1.4426950408889634074 / (double)T;
         top = capped(raw_top);
         // 64 bins per power of two of the weight where the cap does not flatten it
-        bin_scale = fminf((float)(92.332482616893657 * inv_t), 1e30f);
+        bin_scale = fminf((float)(64.0 * powers), 1e30f);
         const uint32_t kk = a.top_k ? a.top_k[row] : 0u;
         k = kk < a.V ? kk : 0u;
         const float pp = a.top_p ? a.top_p[row] : 1.0f, mm = a.min_p ? a.min_p[row] : 0.0f;
@@ -144,19 +163,30 @@ struct Row {
     __device__ __forceinline__ double capped(float l) const {
         return CAP ? cap * tanh_of((double)l * inv_cap) : (double)l;
     }
+    // a token's weight: no branch, so that several run side by side.  Below 2^-90 it is zero units anyway; a NaN (of
+    // infinities) ends there too
+    __device__ __forceinline__ Pow2 power(float l) const {
+        double x = fmax((capped(l) - top) * powers, -90.0);
+        if (CAP) x = fmin(x, 0.0);                                     // tanh need not grow in its last bit
+        return Pow2(l == raw_top ? 0.0 : x);
+    }
     __device__ __forceinline__ double weight(float l) const {                              // 2^kWeightBits exp(..)
-        // no branch, so that several run side by side.  exp(-64) rounds to zero; a NaN (infinities) becomes -64
-        const double x = fmin(fmax((capped(l) - top) * inv_t, -64.0), 0.0);
-        return l == raw_top ? (double)(1ull << kWeightBits) : exp_scaled(x, kWeightBits);
+        const Pow2 w = power(l);
+        return w.part * w.scale;
     }
     // 2^52 added leaves the rounded weight in the low bits
     __device__ __forceinline__ uint64_t units(float l) const {
-        return __builtin_bit_cast(uint64_t, weight(l) + 4503599627370496.0) & ((1ull << 52) - 1);
+        const Pow2 w = power(l);
+        return __builtin_bit_cast(uint64_t, fma(w.part, w.scale, 4503599627370496.0)) & ((1ull << 52) - 1);
+    }
+    __device__ __forceinline__ uint64_t units_if_allowed(float l) const {
+        const uint64_t w = units(l);
+        return allowed(l) ? w : 0;
     }
     __device__ __forceinline__ uint64_t kept(uint64_t w) const { return w >= least ? w : 0; }
     // the bin of an allowed logit: larger logits never lie in a later one
     __device__ __forceinline__ uint32_t bin(float l) const {
-        return l >= raw_top ? 0u : (uint32_t)fminf((raw_top - l) * bin_scale, (float)(kBins - 1));
+        return (uint32_t)fminf((raw_top - l) * bin_scale, (float)(kBins - 1));     // all in the last, if the largest is infinite
     }
     // the running sum at which top-p ends, of a mass Z: kept while the mass before is below p Z, so the last one is
     // the first whose running sum reaches ceil(p Z)
@@ -299,10 +329,10 @@ __global__ __launch_bounds__(kPassThreads) void k_sample_mass(Sample a) {
                    [&](uint32_t, const f4u &l, int) {
                        uint64_t w[4];
 #pragma unroll
-                       for (int e = 0; e < 4; ++e) w[e] = allowed(l[e]) ? r.units(l[e]) : 0;
+                       for (int e = 0; e < 4; ++e) w[e] = r.units(l[e]);
 #pragma unroll
                        for (int e = 0; e < 4; ++e)
-                           if (w[e]) atomicAdd((unsigned long long *)&hist[r.bin(l[e])], (unsigned long long)w[e]);
+                           if (w[e] && allowed(l[e])) atomicAdd((unsigned long long *)&hist[r.bin(l[e])], (unsigned long long)w[e]);
                    });
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < kBins; i += blockDim.x)
@@ -311,7 +341,8 @@ __global__ __launch_bounds__(kPassThreads) void k_sample_mass(Sample a) {
         uint64_t sum = 0;
         v.each(a, x, s, [&](uint32_t, const f4u &l, int) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += allowed(l[e]) ? r.kept(r.units(l[e])) : 0;
+            for (int e = 0; e < 4; ++e) sum += r.kept(r.units_if_allowed(l[e]));
+            asm volatile("" : "+v"(sum));                              // summed here, not kept apart until the end
         });
         sum = wave_sum_u64(sum);
         if ((threadIdx.x & 63) == 0) a.sums[(size_t)row * a.stretches + s] = sum;
@@ -395,6 +426,7 @@ __global__ __launch_bounds__(kPassThreads) void k_sample_border(Sample a) {
                 fence();
 #pragma unroll
                 for (int e = 0; e < 4; ++e) sum += r.kept(r.units(q[64 * e + lane]));
+                asm volatile("" : "+v"(sum));
                 n -= 256;
                 float tail[4];
 #pragma unroll
@@ -557,7 +589,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
         w[j] = 0;
         if (key_of(j) >= lo) w[j] = r.units(v[j]);
         Z += w[j];
-        __builtin_amdgcn_sched_barrier(0);                             // one at a time: the registers are full
+        if (j % 2) __builtin_amdgcn_sched_barrier(0);                  // two at a time: the registers are full
     }
     if (r.p < 1.0f) {
         Z = sh.sum(Z);
@@ -895,6 +927,8 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
 template <bool CAP>
 static int launch_small(chn_ctx *ctx, const Sample &a, uint32_t n) {
     if (a.V <= 4 * kDrawThreads) k_sample_small<4, CAP><<<n, kDrawThreads, 0, ctx->stream>>>(a);
+    else if (a.V <= 8 * kDrawThreads) k_sample_small<8, CAP><<<n, kDrawThreads, 0, ctx->stream>>>(a);
+    else if (a.V <= 12 * kDrawThreads) k_sample_small<12, CAP><<<n, kDrawThreads, 0, ctx->stream>>>(a);
     else k_sample_small<16, CAP><<<n, kDrawThreads, 0, ctx->stream>>>(a);
     CHN_LAUNCHED(ctx, "k_sample_small");
     return CHN_OK;
