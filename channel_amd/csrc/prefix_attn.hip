@@ -2,25 +2,33 @@
 // blocks all requests share (chn_prefix_decode_attn).
 //
 // The query rows of one KV head - n_req * gqa of them over the prefix, gqa
-// over a request's own tokens - times its keys are matrix products, on
-// v_mfma_f32_16x16x4_f32 (operands and sums in fp32, as the caches are).  A
-// launch holds two kinds of workgroups: prefix items (KV head, RT tiles of 16
-// rows, a range of keys) and own items (KV head, request, a range of its
-// keys); a second launch joins the items' partial results.  In an item the
-// four waves take 16 keys each in turn; a wave multiplies straight from the
-// registers it loaded a key's row into (no key is used by two waves), the
-// query rows come from LDS.
+// over a request's own tokens - times its keys are matrix products, on the
+// fp32 matrix instructions (operands and sums in fp32, as the caches are).
+// One pass over the keys: scores, weights against a running reference, the
+// weighted sum of V, in registers throughout.  A launch holds two kinds of
+// workgroups: prefix items (KV head, some rows, a range of keys; the prefix is
+// read once per 64 or 32 rows) and own items (KV head, request, a range of its
+// keys).  A second launch joins the items' partial results.
 //
-// Lane l = 16 g + c of a wave.  Scores are formed transposed, S^T = K Q^T: as
-// A operand lane l holds key c's dims 16 s + 4 g + j (one 16-byte load per s),
-// as B operand row c's same dims.  The result register i of lane l is key 4 g +
-// i of row c, which is the A operand of step i of P V (row c, key 4 g + i); the
-// B operand of that step is V[key 4 g + i][dim 64 m + 4 c + j], again one
-// 16-byte load.  So nothing is exchanged between lanes but the rare rescaling.
+// Few rows (own items, and prefixes of up to 32 rows) are bound by reading the
+// caches: struct Quads, 4x4x1 instructions straight from the registers the
+// keys are loaded into.  Many rows over a prefix are bound by the matrix
+// instructions (157 TFLOP/s in fp32): struct Rows, 16x16x4 instructions, keys
+// shared through LDS.
 //
-// The running maximum is kept per row and only moved when a score passes it by
-// more than kSlack (in powers of two): weights then lie below 2^kSlack, which
-// fp32 holds as exactly as those below one.
+// The running reference is kept per row and only moved when a score passes it
+// by more than kSlack (in powers of two): weights then lie below 2^kSlack,
+// which fp32 holds as exactly as those below one, and a group of keys seldom
+// pays for rescaling the sums (1 us of 64 with heads of 512; nothing where
+// memory bounds it).
+//
+// Measured (fp32, one decode step, both launches): 8 requests of up to 96
+// tokens behind 512, heads of 256: 16.7 us, most of it the two launches and
+// the block-table, key, weight and join latencies one after another.  64
+// requests of up to 480 tokens behind 3968: 85-95 us; the prefix alone takes
+// 58-67 (27 at the matrix rate), the requests' own keys share the chip with
+// it.  33 requests of up to 333 behind 1488, heads of 512: 62 us.  12 requests
+// of up to 20000 tokens, no prefix: 206 us, 6.2 TB/s.
 #include "chn_internal.h"
 
 #include <cmath>
@@ -32,7 +40,10 @@ typedef float f4a __attribute__((ext_vector_type(4)));
 constexpr uint32_t kBadSlot = 0xFFFFFFFFu;
 constexpr float kSlack = 8.0f;
 constexpr float kNone = -__builtin_inff();
-constexpr uint32_t kOwnMinGroups = 4;       // 16-key groups per own item at least: one per wave
+// 16-key groups per own item at least: one per wave, or two where items of four would not all be resident at once (12
+// groups cost every case below).  Four against eight: one request of up to 4096 tokens 13.0 and 16.2 us, four of 2048
+// 17.1 and 18.9; 64 of up to 500 46.5 and 42.8, 33 of 333 with heads of 512 28.9 and 24.0
+constexpr uint32_t kOwnMinGroups = 4, kOwnMoreGroups = 8;
 
 struct PrefixAttn {
     const float *q, *kc, *vc;
@@ -40,10 +51,10 @@ struct PrefixAttn {
     uint32_t npb, n_req, max_blocks, shift, n_blocks, num_q, num_kv, kv_dim, gqa;
     float exp_hi, exp_lo;      // scale * log2(e) in two parts
     float *out;
-    // prefix items: unit u = (KV head, key range), `tiles` row tiles each; see decode_item
+    // prefix items: unit u = (KV head, key range), `tiles` tiles of rows each
     uint32_t splits, split_keys, tiles, prefix_wgs;
-    // own items: at most own_cap + n_req of them per KV head
-    uint32_t own_cap;
+    // own items: at most own_cap + n_req of them per KV head, of which own_fit run at once
+    uint32_t own_cap, own_fit;
     // partial results, [splits][n_req][num_q] of the prefix and then [own item][num_q]: sums of D values, references
     // and denominators; own_start[n_req + 1]: the first own item of each request
     float *o, *m, *l;
@@ -65,7 +76,8 @@ __device__ __forceinline__ uint32_t own_per(const PrefixAttn &a, int lane) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) sum += (uint64_t)__shfl_xor((unsigned long long)sum, o, 64);
     const uint64_t per = (sum + a.own_cap - 1) / a.own_cap;
-    return (uint32_t)min(max(per, (uint64_t)kOwnMinGroups), (uint64_t)1 << 27);   // 2^31 positions at most
+    const uint32_t least = sum / kOwnMinGroups + a.n_req / 2 > a.own_fit ? kOwnMoreGroups : kOwnMinGroups;
+    return (uint32_t)min(max(per, (uint64_t)least), (uint64_t)1 << 27);           // 2^31 positions at most
 }
 
 __device__ __forceinline__ uint32_t wave_scan_u32(uint32_t v, int lane) {      // inclusive
@@ -99,7 +111,15 @@ __device__ __forceinline__ const float *cache_row(const PrefixAttn &a, const flo
     return slot == kBadSlot ? zero_row : cache + (size_t)slot * a.kv_dim + (size_t)kvh * D;
 }
 
-// 16 query rows of a wave over 256 dims: the weighted sums (lane 16 g + c,
+// 16 query rows of a wave over 256 dims, on v_mfma_f32_16x16x4_f32.  Lane l =
+// 16 g + c.  Scores are formed transposed, S^T = K Q^T: as A operand lane l
+// holds key c's dims 16 s + 4 g + j (one 16-byte read per s), as B operand row
+// c's same dims.  The result register i of lane l is key 4 g + i of row c,
+// which is the A operand of step i of P V (row c, key 4 g + i); the B operand
+// of that step is V[key 4 g + i][dim 64 m + 4 c + j], again one 16-byte read.
+// So nothing is exchanged between lanes but the rare rescaling.
+//
+// Kept here: the weighted sums (lane 16 g + c,
 // element i of o[n][j]: row 4 g + i, dim 64 n + 4 c + j), and row c's reference
 // and this lane's part of its denominator.  lim: how many positions row c may
 // see.
@@ -846,11 +866,15 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
     a.exp_lo = std::isfinite(a.exp_hi) ? (float)(e - a.exp_hi) : 0.0f;
     a.out = out;
     const uint32_t P = n_prefix_blocks << a.shift, M = n_req * gqa_ratio;
+    // Up to 32 rows every workgroup of 16 rows reads the prefix for itself and its waves split the keys; above, 64 (of
+    // heads of 512: 32) rows share what is read.  One way and the other, at 8 KV heads and 3968 keys: 32 rows 35.8 and
+    // 41.5 us, 48 rows 48.0 and 42.9, 128 rows 103 and 94; 512 keys: 16 rows 16.8 and 21.6
     const bool by_rows = P && M > 32;
     if (P) {
         const uint32_t R = !by_rows ? 16 : rows_wg(head_dim);
         a.tiles = (M + R - 1) / R;
-        // about one workgroup per CU, 64 keys (16 per wave) at least
+        // about one workgroup per CU, 64 keys (16 per wave) at least.  128 rows on 3968 keys with own tokens beside them:
+        // 122 us with half as many workgroups, 94 so, 106 with twice as many (and twice the partial results)
         const uint32_t want = std::max(1u, 256 / std::max(1u, a.tiles * a.num_kv));
         a.split_keys = ((P + want - 1) / want + 63) / 64 * 64;
         a.splits = (P + a.split_keys - 1) / a.split_keys;
@@ -860,7 +884,10 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
     }
     uint64_t grid = a.prefix_wgs, items = 0;
     if (max_blocks > n_prefix_blocks) {
+        // at most about eight own items per CU: 12 requests of up to 20000 tokens take 228, 216, 205 and 211 us with
+        // 512, 1024, 2048 and 4096 items; with few tokens the least groups per item decide
         a.own_cap = std::max(1u, 2048 / a.num_kv);
+        a.own_fit = (head_dim == 256 ? 512 : 256) / a.num_kv;      // two workgroups per CU, or one (their registers)
         // no request has more items than its table has room for
         const uint32_t groups = (uint32_t)((((uint64_t)(max_blocks - n_prefix_blocks) << a.shift) + 15) / 16);
         items = std::min<uint64_t>(a.own_cap + n_req, (uint64_t)n_req * ((groups + kOwnMinGroups - 1) / kOwnMinGroups));
