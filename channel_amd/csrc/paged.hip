@@ -50,7 +50,10 @@ __device__ __forceinline__ Grow grow_of(const Tables &a, uint32_t len, uint32_t 
 // one block scan, the lengths from L2), so each knows whether the call holds
 // and where its own share lies, and none waits for another.  A thread then
 // takes a row of the batch (its request by bisection of the starts in LDS);
-// the thread of a block's first token enters the block.
+// the thread of a block's first token enters the block.  Bound by the launch
+// and by three latencies (lengths, table entries, writes): 32 requests of one
+// token 4.8 us, 1024 requests of 131072 tokens in all, with 300 new prefixes,
+// 6.1 us.
 __global__ __launch_bounds__(kTabThreads) void k_block_tables(Tables a) {
     extern __shared__ uint32_t sh[];
     uint32_t *row0 = sh, *blk0 = sh + a.n_req;         // first row, first of the handed-out blocks
@@ -224,14 +227,17 @@ __global__ __launch_bounds__(256) void k_rope_at(RopeAt a) {
 
 // The same for head_dim 256 * N, rows of 16-byte aligned values and rot a
 // multiple of 8: lane l holds dims 4 l + 256 j .. + 3, and the row's partner
-// values come as 16 bytes from the wave's own LDS row.  A workgroup takes 4 *
-// HPW rows of one token, a wave HPW of them with all their loads in flight, so
-// the angles are evaluated once per 4 * HPW rows, while those loads are under
-// way.
+// values come as 16 bytes from the wave's own LDS row.  A workgroup takes 8
+// rows of one token, a wave two of them with all their loads in flight, so
+// the angles are evaluated once per 8 rows, while those loads are under way.
+// Bound by memory: 1500 tokens of 16 query and 4 KV heads of 512 (135 MB)
+// take 27 us, 5.0 TB/s (27 with one row per wave, 31 with four); with 16 and 8
+// heads of 256 18.4 (20.5 and 18.6).  24 tokens of those take 5: the launch,
+// then loads, a sum and writes behind one another.
 typedef float f4p __attribute__((ext_vector_type(4)));
-template <int N, int HPW>
+template <int N>
 __global__ __launch_bounds__(256) void k_rope_at4(RopeAt a) {
-    constexpr uint32_t D = 256 * N;
+    constexpr uint32_t D = 256 * N, HPW = 2;
     __shared__ float2 cs[D / 2];
     __shared__ f4p buf[4][D / 4];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -240,7 +246,7 @@ __global__ __launch_bounds__(256) void k_rope_at4(RopeAt a) {
     const uint32_t slot = a.slots[t], clock = a.clocks[t];
     f4p v[HPW][N], wq[N], wk[N];
 #pragma unroll
-    for (int i = 0; i < HPW; ++i) {
+    for (uint32_t i = 0; i < HPW; ++i) {
         const uint32_t row = min(row0 + i, nrow - 1);                // past the last: it again, left out below
         const float *in = row < a.num_q ? a.q_in + ((size_t)t * a.num_q + row) * D
                           : row < nk    ? a.k_in + ((size_t)t * a.num_kv + row - a.num_q) * D
@@ -256,7 +262,7 @@ __global__ __launch_bounds__(256) void k_rope_at4(RopeAt a) {
     if ((uint32_t)tid < half) cs[tid] = rope_angle(a, clock, tid);
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < HPW; ++i) {
+    for (uint32_t i = 0; i < HPW; ++i) {
         const uint32_t row = row0 + i;
         if (row >= nrow) return;                                     // a whole wave; no barrier follows
         float ss = 0.0f;
@@ -366,15 +372,10 @@ extern "C" int chn_batch_qkv_rope_at(chn_ctx *ctx, const float *q_in, const floa
                           (const void *)k_norm_w, (const void *)q_out, (const void *)k_cache, (const void *)v_cache})
         wide = wide && aligned(p, 16);
     if (wide) {
-        // four rows per wave once they leave a workgroup for every CU
-        const uint32_t rows = num_q_heads + 2 * num_kv_heads;
-        const bool many = (uint64_t)n_tok * rows >= 16 * 512;
         RopeAt b = a;
-        b.groups = many ? (rows + 15) / 16 : groups;
-        if (head_dim == 256 && many) k_rope_at4<1, 4><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
-        else if (head_dim == 256) k_rope_at4<1, 1><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
-        else if (many) k_rope_at4<2, 4><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
-        else k_rope_at4<2, 1><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
+        b.groups = (num_q_heads + 2 * num_kv_heads + 7) / 8;
+        if (head_dim == 256) k_rope_at4<1><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
+        else k_rope_at4<2><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
     } else if (head_dim > 256) k_rope_at<8><<<groups * n_tok, 256, 0, ctx->stream>>>(a);
     else k_rope_at<4><<<groups * n_tok, 256, 0, ctx->stream>>>(a);
     CHN_LAUNCHED(ctx, "k_rope_at");
