@@ -524,6 +524,31 @@ __device__ __forceinline__ float rows4_max(float v) {
     return fmaxf(v, xor32_lane(v));
 }
 
+// 64-bit sums over the lanes in registers (DPP): few instructions,
+// as a workgroup that runs a kernel once waits for its code as well.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint64_t dpp64(uint64_t old, uint64_t v) {
+    const uint32_t lo = __builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp((int)(old >> 32), (int)(v >> 32), CTRL, ROWS, 0xF, false);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {                          // the same lane for all
+    const uint32_t lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
+    return (uint64_t)hi << 32 | lo;
+}
+__device__ __forceinline__ uint64_t row16_scan_u64(uint64_t v) {                            // inclusive, of 16 lanes
+    v += dpp64<0x111, 0xF>(0, v);                                                          // row_shr:1, 2, 4, 8
+    v += dpp64<0x112, 0xF>(0, v);
+    v += dpp64<0x114, 0xF>(0, v);
+    return v + dpp64<0x118, 0xF>(0, v);
+}
+__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {                             // inclusive
+    v = row16_scan_u64(v);
+    v += dpp64<0x142, 0xA>(0, v);                                                          // row_bcast:15, 31
+    return v + dpp64<0x143, 0xC>(0, v);
+}
+__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) { return lane64(wave_scan_u64(v), 63); }
+
 // Transposed pair sums on one lane swap: permlane32_swap(x, y) leaves
 // {x_lo, y_lo} and {x_hi, y_hi}, so lane l of the low half gets
 // x_l + x_{l+32} and lane l of the high half y_{l-32} + y_l (and likewise

@@ -13,21 +13,13 @@ namespace chn {
 // ---------------------------------------------------------------------
 constexpr uint32_t kMaxRequests = 8192;     // two words of LDS each
 constexpr uint32_t kTabThreads = 1024;
+static_assert(kTabThreads / 64 == 16, "the waves' sums are a row of 16 lanes");
 
 struct Tables {
     const uint32_t *lens, *n_new, *prefix, *free_blocks, *taken;
     uint32_t n_req, npb, n_free, n_blocks, shift, max_blocks, max_tokens;
     uint32_t *tables, *lens_out, *row_start, *slots, *clocks, *status;
 };
-
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v, int lane) {      // inclusive
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint64_t w = (uint64_t)__shfl_up((unsigned long long)v, o, 64);
-        if (lane >= o) v += w;
-    }
-    return v;
-}
 
 // What request r does: its first new token's position, and the blocks that
 // hold its tokens before and after.  64-bit: the lengths are the caller's.
@@ -60,7 +52,7 @@ __global__ __launch_bounds__(kTabThreads) void k_block_tables(Tables a) {
     __shared__ uint64_t wsum[2][kTabThreads / 64];
     __shared__ uint32_t bad;
     const uint32_t tid = threadIdx.x, nth = gridDim.x * kTabThreads, gid = blockIdx.x * kTabThreads + tid;
-    const int lane = tid & 63, wave = tid >> 6;
+    const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     if (tid == 0) bad = 0;
     __syncthreads();
     uint64_t rows = 0, blocks = 0;
@@ -71,20 +63,16 @@ __global__ __launch_bounds__(kTabThreads) void k_block_tables(Tables a) {
         const Grow g = grow_of(a, r < a.n_req ? a.lens[r] : 0u, n);
         const uint64_t need = n ? g.last - g.first : 0;
         if (n && g.last > a.max_blocks) flags = CHN_TABLES_TOO_LONG;
-        const uint64_t sn = wave_scan_u64(n, lane), sb = wave_scan_u64(need, lane);
+        const uint64_t sn = wave_scan_u64(n), sb = wave_scan_u64(need);
         if (lane == 63) {
             wsum[0][wave] = sn;
             wsum[1][wave] = sb;
         }
         __syncthreads();
-        uint64_t bn = rows, bb = blocks;
-        for (int w = 0; w < (int)(kTabThreads / 64); ++w) {
-            const uint64_t vn = wsum[0][w], vb = wsum[1][w];
-            bn += w < wave ? vn : 0;
-            bb += w < wave ? vb : 0;
-            rows += vn;
-            blocks += vb;
-        }
+        const uint64_t vn = row16_scan_u64(wsum[0][lane & 15]), vb = row16_scan_u64(wsum[1][lane & 15]);
+        const uint64_t bn = rows + (wave ? lane64(vn, wave - 1) : 0), bb = blocks + (wave ? lane64(vb, wave - 1) : 0);
+        rows += lane64(vn, 15);
+        blocks += lane64(vb, 15);
         if (r < a.n_req) {
             // beyond 32 bits only where the call is refused below
             row0[r] = (uint32_t)(bn + sn - n);

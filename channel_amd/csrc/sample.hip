@@ -206,30 +206,6 @@ struct Row {
     }
 };
 
-// 64-bit sums and minima over the lanes in registers (DPP): few instructions,
-// as a workgroup that runs a kernel once waits for its code as well.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ uint64_t dpp64(uint64_t old, uint64_t v) {
-    const uint32_t lo = __builtin_amdgcn_update_dpp((int)old, (int)v, CTRL, ROWS, 0xF, false);
-    const uint32_t hi = __builtin_amdgcn_update_dpp((int)(old >> 32), (int)(v >> 32), CTRL, ROWS, 0xF, false);
-    return (uint64_t)hi << 32 | lo;
-}
-__device__ __forceinline__ uint64_t lane64(uint64_t v, int lane) {                          // the same lane for all
-    const uint32_t lo = __builtin_amdgcn_readlane((int)v, lane), hi = __builtin_amdgcn_readlane((int)(v >> 32), lane);
-    return (uint64_t)hi << 32 | lo;
-}
-__device__ __forceinline__ uint64_t row16_scan_u64(uint64_t v) {                            // inclusive, of 16 lanes
-    v += dpp64<0x111, 0xF>(0, v);                                                          // row_shr:1, 2, 4, 8
-    v += dpp64<0x112, 0xF>(0, v);
-    v += dpp64<0x114, 0xF>(0, v);
-    return v + dpp64<0x118, 0xF>(0, v);
-}
-__device__ __forceinline__ uint64_t wave_scan_u64(uint64_t v) {                             // inclusive
-    v = row16_scan_u64(v);
-    v += dpp64<0x142, 0xA>(0, v);                                                          // row_bcast:15, 31
-    return v + dpp64<0x143, 0xC>(0, v);
-}
-__device__ __forceinline__ uint64_t wave_sum_u64(uint64_t v) { return lane64(wave_scan_u64(v), 63); }
 __device__ __forceinline__ uint64_t wave_min_u64(uint64_t v) {
     v = min(v, dpp64<0x111, 0xF>(v, v));
     v = min(v, dpp64<0x112, 0xF>(v, v));
