@@ -27,7 +27,7 @@
 // the block-table, key, weight and join latencies one after another.  64
 // requests of up to 480 tokens behind 3968: 85-95 us; the prefix alone takes
 // 58-67 (27 at the matrix rate), the requests' own keys share the chip with
-// it.  33 requests of up to 333 behind 1488, heads of 512: 62 us.  12 requests
+// it.  33 requests of up to 333 behind 1488, heads of 512: 45 us.  12 requests
 // of up to 20000 tokens, no prefix: 206 us, 6.2 TB/s.
 #include "chn_internal.h"
 
@@ -503,21 +503,25 @@ struct Quads {
 
 // --- many rows: a wave takes 16 rows and 256 dims (of heads of 512, two waves
 // the halves, whose scores they exchange) and all waves share the keys, whose K
-// and V rows go through LDS (two buffers of 16 keys: the next group is read
-// while one is multiplied, and stored behind it).  The query rows stay in
-// registers.  A K row's stride of D + 4 floats spreads the 16 rows that a read
+// and V rows go through LDS, 16 at a time: the next group is read into
+// registers while one is multiplied, and stored behind it, into a second buffer
+// where the heads leave room for two.  (With one buffer for heads of 512, two
+// workgroups fit a CU: 33 requests of up to 333 behind 1488, 60 -> 45 us.
+// Another group on its way would need registers: with spills 95 -> 116 us.)  The
+// query rows stay in registers.  A K row's stride of D + 4 floats spreads the 16 rows that a read
 // takes over the banks.
 template <int D>
 struct Shared {
-    f4a k[2][16][D / 4 + 1], v[2][16][D / 4], s[D == 512 ? 4 : 1][64];
-    uint32_t slot[2][16], full;
+    static constexpr int NB = D == 512 ? 1 : 2;    // buffers
+    f4a k[NB][16][D / 4 + 1], v[NB][16][D / 4], s[D == 512 ? 4 : 1][64];
+    uint32_t slot[NB][16], full;
 };
 constexpr uint32_t rows_wg(uint32_t D) { return 64 / (D / 256); }     // rows of a workgroup
 // q: row c of this wave's 16, its 256 dims; n: how many rows the workgroup has
 template <int D, typename F>
 __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a (&q)[16], Shared<D> &sh, const Keys &k,
                                          uint32_t n, F &&where) {
-    constexpr int H = D / 256, RG = 4 / H;
+    constexpr int H = D / 256, RG = 4 / H, NB = Shared<D>::NB;
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rows = wave % RG, half = wave / RG;
     f4a sk[4][H], sv[4][H];                        // keys wave, wave + 4, ..: this lane's dims 4 lane + 256 h
@@ -543,25 +547,26 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
             }
         if (threadIdx.x < 16) sh.slot[b][threadIdx.x] = slot;
     };
-    f4a x[2][4];                                   // four LDS reads ahead of the products, no more: the registers are full
+    constexpr int X = 2;                           // LDS reads ahead of the products, no more: the registers are full
+    f4a x[2][X];
     auto scores = [&](int b) {
         f4a part[4];                               // four chains: shorter sums round less
         auto read = [&](int s) {
 #pragma unroll
-            for (int y = 0; y < 4; ++y) x[s & 1][y] = sh.k[b][c][64 * half + 16 * s + 4 * y + g];
+            for (int y = 0; y < X; ++y) x[s & 1][y] = sh.k[b][c][64 * half + 4 * (X * s + y) + g];
         };
 #pragma unroll
         for (int j = 0; j < 4; ++j) part[j] = f4a{0, 0, 0, 0};
         read(0);
 #pragma unroll
-        for (int s = 0; s < 4; ++s) {
-            if (s + 1 < 4) read(s + 1);
+        for (int s = 0; s < 16 / X; ++s) {
+            if (s + 1 < 16 / X) read(s + 1);
             issue_fence();
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+            for (int y = 0; y < X; ++y)
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
-                    part[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s & 1][y][j], q[4 * s + y][j], part[j], 0, 0, 0);
+                    part[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s & 1][y][j], q[X * s + y][j], part[j], 0, 0, 0);
             issue_fence();
         }
         return (part[0] + part[1]) + (part[2] + part[3]);
@@ -577,20 +582,22 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
         return s;
     };
     auto weigh = [&](const f4a &s, int b) {
-        auto read = [&](int e) {
+        auto read = [&](int i) {                   // the i-th X of a key's four reads, key by key
 #pragma unroll
-            for (int y = 0; y < 4; ++y) x[e & 1][y] = sh.v[b][4 * g + e][64 * half + 16 * y + c];
+            for (int y = 0; y < X; ++y) x[i & 1][y] = sh.v[b][4 * g + i * X / 4][64 * half + 16 * (i * X % 4 + y) + c];
         };
         read(0);
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            if (e + 1 < 4) read(e + 1);
+        for (int i = 0; i < 16 / X; ++i) {
+            if (i + 1 < 16 / X) read(i + 1);
             issue_fence();
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
+            for (int y = 0; y < X; ++y)
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    w.o[y][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(s[e], x[e & 1][y][j], w.o[y][j], 0, 0, 0);
+                for (int j = 0; j < 4; ++j) {
+                    f4a &o = w.o[i * X % 4 + y][j];
+                    o = __builtin_amdgcn_mfma_f32_16x16x4f32(s[i * X / 4], x[i & 1][y][j], o, 0, 0, 0);
+                }
             issue_fence();
         }
     };
@@ -606,7 +613,7 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
     uint32_t kb = k.begin;
     int b = 0;
 #pragma unroll 1
-    for (; kb < full; kb += 16, b ^= 1) {
+    for (; kb < full; kb += 16, b ^= NB - 1) {
         slot = k.slot(a, kb + 16, c, nextb);
         nextb = k.block(a, kb + 32, c);
         load(slot);                                // past the end: the row of zeros, not used
@@ -618,17 +625,19 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
         s = w.softmax(a, s, [&](int i) { return vs[i] != kBadSlot; });
         weigh(s, b);
         issue_fence();
-        store(b ^ 1, slot);                        // last read before the barrier at the end of the round before
+        if constexpr (NB == 1) __syncthreads();
+        store(b ^ (NB - 1), slot);                 // with two buffers last read before the barrier of the round before
         __syncthreads();
     }
 #pragma unroll 1
-    for (; kb < k.end; kb += 16, b ^= 1) {
+    for (; kb < k.end; kb += 16, b ^= NB - 1) {
         slot = k.slot(a, kb + 16, c, k.block(a, kb + 16, c));
         f4a s = whole(scores(b));
         s = w.softmax(a, s, [&](int i) { return sh.slot[b][4 * g + i] != kBadSlot && kb + 4 * g + i < w.lim; });
         w.weigh_part(s, kb, [&](int key) { return (const float *)&sh.v[b][key][64 * half]; });
         load(slot);
-        store(b ^ 1, slot);
+        if constexpr (NB == 1) __syncthreads();
+        store(b ^ (NB - 1), slot);
         __syncthreads();
     }
     w.end(k);
@@ -658,8 +667,9 @@ constexpr size_t lds_bytes() {
 
 // RQ: quads of rows of own items.  ROWS: whether prefix items hold rows_wg
 // rows, 16 a wave, or 16 that the waves share.
+// Two workgroups per CU where the registers can be held to 256.
 template <int D, int RQ, bool ROWS>
-__global__ __launch_bounds__(256, D == 256 ? 2 : 1) void k_prefix_attn(PrefixAttn a) {
+__global__ __launch_bounds__(256, D == 256 || (RQ == 1 && ROWS) ? 2 : 1) void k_prefix_attn(PrefixAttn a) {
     extern __shared__ f4a sh4[];
     float *const sh = (float *)sh4;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -887,7 +897,8 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
         // at most about eight own items per CU: 12 requests of up to 20000 tokens take 228, 216, 205 and 211 us with
         // 512, 1024, 2048 and 4096 items; with few tokens the least groups per item decide
         a.own_cap = std::max(1u, 2048 / a.num_kv);
-        a.own_fit = (head_dim == 256 ? 512 : 256) / a.num_kv;      // two workgroups per CU, or one (their registers)
+        // two workgroups per CU, or one (of heads of 512 the second is the prefix's)
+        a.own_fit = (head_dim == 256 ? 512 : 256) / a.num_kv;
         // no request has more items than its table has room for
         const uint32_t groups = (uint32_t)((((uint64_t)(max_blocks - n_prefix_blocks) << a.shift) + 15) / 16);
         items = std::min<uint64_t>(a.own_cap + n_req, (uint64_t)n_req * ((groups + kOwnMinGroups - 1) / kOwnMinGroups));

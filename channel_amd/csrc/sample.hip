@@ -372,7 +372,7 @@ __global__ __launch_bounds__(kPassThreads) void k_sample_border(Sample a) {
     __shared__ uint32_t nfound, at0;
     const uint32_t row = blockIdx.y, s = blockIdx.x * (kPassThreads / 64) + (threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
-    if (!by_mass(a, row) || !a.top_p || !(a.top_p[row] < 1.0f)) return;
+    if (!by_mass(a, row) || !(a.top_p[row] < 1.0f)) return;
     const float *x = a.logits + (size_t)row * a.ld;
     Stretch v;
     if (s < a.stretches) v.start(a, x, s);
@@ -926,7 +926,7 @@ static void launch_rows(chn_ctx *ctx, const Sample &a, uint32_t n, size_t lds) {
     const dim3 wide((a.stretches + kPassThreads / 64 - 1) / (kPassThreads / 64), n);
     k_sample_max<<<dim3((a.stretches + 3) / 4, n), 256, 0, ctx->stream>>>(a);
     k_sample_mass<CAP><<<wide, kPassThreads, 0, ctx->stream>>>(a);
-    k_sample_border<CAP><<<wide, kPassThreads, 0, ctx->stream>>>(a);
+    if (a.top_p) k_sample_border<CAP><<<wide, kPassThreads, 0, ctx->stream>>>(a);
     k_sample_draw<CAP><<<n, kDrawThreads, lds, ctx->stream>>>(a);
 }
 
