@@ -10,7 +10,7 @@
 // read once per 64 or 32 rows) and own items (KV head, request, a range of its
 // keys).  A second launch joins the items' partial results.
 //
-// Few rows (own items, and prefixes of up to 32 rows) are bound by reading the
+// Few rows (own items, and a prefix's up to 16 or 32 rows) are bound by reading the
 // caches: struct Quads, 4x4x1 instructions straight from the registers the
 // keys are loaded into.  Many rows over a prefix are bound by the matrix
 // instructions (157 TFLOP/s in fp32): struct Rows, 16x16x4 instructions, keys
@@ -25,9 +25,9 @@
 // Measured (fp32, one decode step, both launches): 8 requests of up to 96
 // tokens behind 512, heads of 256: 16.7 us, most of it the two launches and
 // the block-table, key, weight and join latencies one after another.  64
-// requests of up to 480 tokens behind 3968: 85-95 us; the prefix alone takes
-// 58-67 (27 at the matrix rate), the requests' own keys share the chip with
-// it.  33 requests of up to 333 behind 1488, heads of 512: 45 us.  12 requests
+// requests of up to 480 tokens behind 3968: 80 us; the prefix alone takes 59 (27
+// at the matrix rate), the requests' own keys share the chip with it.  33
+// requests of up to 333 behind 1488, heads of 512: 43 us.  12 requests
 // of up to 20000 tokens, no prefix: 206 us, 6.2 TB/s.
 #include "chn_internal.h"
 
@@ -503,10 +503,11 @@ struct Quads {
 
 // --- many rows: a wave takes 16 rows and 256 dims (of heads of 512, two waves
 // the halves, whose scores they exchange) and all waves share the keys, whose K
-// and V rows go through LDS, 16 at a time: the next group is read into
-// registers while one is multiplied, and stored behind it, into a second buffer
-// where the heads leave room for two.  (With one buffer for heads of 512, two
-// workgroups fit a CU: 33 requests of up to 333 behind 1488, 60 -> 45 us.
+// and V rows go through LDS, 16 at a time: the next group's loads are issued
+// between the products of the scores and stored between those of the weighted
+// sum (before and behind them they cost 1300 of 6900 cycles a group, of which the
+// products take 4100), into a second buffer where the heads leave room for two.  (With one buffer for heads of 512, two
+// workgroups fit a CU: 33 requests of up to 333 behind 1488: 60 -> 45 us.
 // Another group on its way would need registers: with spills 95 -> 116 us.)  The
 // query rows stay in registers.  A K row's stride of D + 4 floats spreads the 16 rows that a read
 // takes over the banks.
@@ -525,31 +526,39 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
     const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), rows = wave % RG, half = wave / RG;
     f4a sk[4][H], sv[4][H];                        // keys wave, wave + 4, ..: this lane's dims 4 lane + 256 h
-    auto load = [&](uint32_t slot) {
+    auto load = [&](int x, uint32_t slot) {        // key wave + 4 x of the group
+        const uint32_t s = __builtin_amdgcn_readlane(slot, wave + 4 * x);
+        const float *kr = cache_row<D>(a, a.kc, s, k.kvh) + 4 * lane, *vr = cache_row<D>(a, a.vc, s, k.kvh) + 4 * lane;
 #pragma unroll
-        for (int x = 0; x < 4; ++x) {
-            const uint32_t s = __builtin_amdgcn_readlane(slot, wave + 4 * x);
-            const float *kr = cache_row<D>(a, a.kc, s, k.kvh) + 4 * lane, *vr = cache_row<D>(a, a.vc, s, k.kvh) + 4 * lane;
-#pragma unroll
-            for (int h = 0; h < H; ++h) {
-                sk[x][h] = *(const f4a *)(kr + 256 * h);
-                sv[x][h] = *(const f4a *)(vr + 256 * h);
-            }
+        for (int h = 0; h < H; ++h) {
+            sk[x][h] = *(const f4a *)(kr + 256 * h);
+            sv[x][h] = *(const f4a *)(vr + 256 * h);
         }
     };
-    auto store = [&](int b, uint32_t slot) {
+    auto store_k = [&](int x, int b) {
 #pragma unroll
-        for (int x = 0; x < 4; ++x)
+        for (int h = 0; h < H; ++h) sh.k[b][wave + 4 * x][64 * h + lane] = sk[x][h];
+    };
+    auto store_v = [&](int x, int b) {
 #pragma unroll
-            for (int h = 0; h < H; ++h) {
-                sh.k[b][wave + 4 * x][64 * h + lane] = sk[x][h];
-                sh.v[b][wave + 4 * x][64 * h + lane] = sv[x][h];
-            }
+        for (int h = 0; h < H; ++h) sh.v[b][wave + 4 * x][64 * h + lane] = sv[x][h];
+    };
+    auto load_all = [&](uint32_t slot) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) load(x, slot);
+    };
+    auto store_all = [&](int b, uint32_t slot) {
+#pragma unroll
+        for (int x = 0; x < 4; ++x) {
+            store_k(x, b);
+            store_v(x, b);
+        }
         if (threadIdx.x < 16) sh.slot[b][threadIdx.x] = slot;
     };
     constexpr int X = 2;                           // LDS reads ahead of the products, no more: the registers are full
     f4a x[2][X];
-    auto scores = [&](int b) {
+    // beside(s): what the wave does while its products run, in eight portions
+    auto scores = [&](int b, auto &&beside) {
         f4a part[4];                               // four chains: shorter sums round less
         auto read = [&](int s) {
 #pragma unroll
@@ -567,6 +576,7 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     part[j] = __builtin_amdgcn_mfma_f32_16x16x4f32(x[s & 1][y][j], q[X * s + y][j], part[j], 0, 0, 0);
+            beside(s);
             issue_fence();
         }
         return (part[0] + part[1]) + (part[2] + part[3]);
@@ -581,15 +591,16 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
         }
         return s;
     };
-    auto weigh = [&](const f4a &s, int b) {
-        auto read = [&](int i) {                   // the i-th X of a key's four reads, key by key
+    // the i-th X of the V reads, four a key
+    auto read_v = [&](int i, int b) {
 #pragma unroll
-            for (int y = 0; y < X; ++y) x[i & 1][y] = sh.v[b][4 * g + i * X / 4][64 * half + 16 * (i * X % 4 + y) + c];
-        };
-        read(0);
+        for (int y = 0; y < X; ++y) x[i & 1][y] = sh.v[b][4 * g + i * X / 4][64 * half + 16 * (i * X % 4 + y) + c];
+    };
+    // after read_v(0)
+    auto weigh = [&](const f4a &s, int b, auto &&beside) {
 #pragma unroll
         for (int i = 0; i < 16 / X; ++i) {
-            if (i + 1 < 16 / X) read(i + 1);
+            if (i + 1 < 16 / X) read_v(i + 1, b);
             issue_fence();
 #pragma unroll
             for (int y = 0; y < X; ++y)
@@ -598,6 +609,7 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
                     f4a &o = w.o[i * X % 4 + y][j];
                     o = __builtin_amdgcn_mfma_f32_16x16x4f32(s[i * X / 4], x[i & 1][y][j], o, 0, 0, 0);
                 }
+            beside(i);
             issue_fence();
         }
     };
@@ -606,8 +618,8 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
     __syncthreads();
     if (lane == 0) atomicMin(&sh.full, w.full);
     uint32_t slot = k.slot(a, k.begin, c, k.block(a, k.begin, c)), nextb = k.block(a, k.begin + 16, c);
-    load(slot);
-    store(0, slot);
+    load_all(slot);
+    store_all(0, slot);
     __syncthreads();
     const uint32_t full = __builtin_amdgcn_readfirstlane(sh.full);
     uint32_t kb = k.begin;
@@ -616,28 +628,40 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
     for (; kb < full; kb += 16, b ^= NB - 1) {
         slot = k.slot(a, kb + 16, c, nextb);
         nextb = k.block(a, kb + 32, c);
-        load(slot);                                // past the end: the row of zeros, not used
-        issue_fence();
-        f4a s = whole(scores(b));
+        const int to = b ^ (NB - 1);
+        // past the end: the row of zeros, not used
+        f4a s = whole(scores(b, [&](int i) {
+            if (i < 4) load(i, slot);
+        }));
         uint32_t vs[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) vs[i] = sh.slot[b][4 * g + i];
+        read_v(0, b);
         s = w.softmax(a, s, [&](int i) { return vs[i] != kBadSlot; });
-        weigh(s, b);
-        issue_fence();
-        if constexpr (NB == 1) __syncthreads();
-        store(b ^ (NB - 1), slot);                 // with two buffers last read before the barrier of the round before
+        // The next keys into the other buffer, which was last read before the barrier of the round before; with one, its K
+        // part was last read before the barrier in whole()
+        weigh(s, b, [&](int i) {
+            if (i < 4) return;
+            store_k(i - 4, to);
+            if constexpr (NB == 2) store_v(i - 4, to);
+        });
+        if constexpr (NB == 1) {
+            __syncthreads();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) store_v(i, to);
+        }
+        if (threadIdx.x < 16) sh.slot[to][threadIdx.x] = slot;
         __syncthreads();
     }
 #pragma unroll 1
     for (; kb < k.end; kb += 16, b ^= NB - 1) {
         slot = k.slot(a, kb + 16, c, k.block(a, kb + 16, c));
-        f4a s = whole(scores(b));
+        f4a s = whole(scores(b, [](int) {}));
         s = w.softmax(a, s, [&](int i) { return sh.slot[b][4 * g + i] != kBadSlot && kb + 4 * g + i < w.lim; });
         w.weigh_part(s, kb, [&](int key) { return (const float *)&sh.v[b][key][64 * half]; });
-        load(slot);
+        load_all(slot);
         if constexpr (NB == 1) __syncthreads();
-        store(b ^ (NB - 1), slot);
+        store_all(b ^ (NB - 1), slot);
         __syncthreads();
     }
     w.end(k);
@@ -666,7 +690,7 @@ constexpr size_t lds_bytes() {
 }
 
 // RQ: quads of rows of own items.  ROWS: whether prefix items hold rows_wg
-// rows, 16 a wave, or 16 that the waves share.
+// rows, 16 a wave, or 16 that the waves share (heads of 256).
 // Two workgroups per CU where the registers can be held to 256.
 template <int D, int RQ, bool ROWS>
 __global__ __launch_bounds__(256, D == 256 || (RQ == 1 && ROWS) ? 2 : 1) void k_prefix_attn(PrefixAttn a) {
@@ -709,7 +733,7 @@ __global__ __launch_bounds__(256, D == 256 || (RQ == 1 && ROWS) ? 2 : 1) void k_
 #pragma unroll
             for (int s = 0; s < 16; ++s) q[s] = *(const f4a *)(x + 16 * s);
             run_rows<D>(a, w, q, *(Shared<D> *)sh4, k, n, where);
-        } else {
+        } else if constexpr (D == 256) {               // heads of 512 always share
             Quads<D, 4, false> w;
             w.run(a, sh, k, limit, [&] { load_q(kvh, row0, n, 16); });
             w.join(a, sh, n, where);
@@ -876,10 +900,12 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
     a.exp_lo = std::isfinite(a.exp_hi) ? (float)(e - a.exp_hi) : 0.0f;
     a.out = out;
     const uint32_t P = n_prefix_blocks << a.shift, M = n_req * gqa_ratio;
-    // Up to 32 rows every workgroup of 16 rows reads the prefix for itself and its waves split the keys; above, 64 (of
-    // heads of 512: 32) rows share what is read.  One way and the other, at 8 KV heads and 3968 keys: 32 rows 35.8 and
-    // 41.5 us, 48 rows 48.0 and 42.9, 128 rows 103 and 94; 512 keys: 16 rows 16.8 and 21.6
-    const bool by_rows = P && M > 32;
+    // Few rows of heads of 256: every workgroup of 16 rows reads the prefix for itself and its waves split the keys.
+    // Otherwise 64 (of heads of 512: 32) rows share what is read.  The one way and the other, at 8 KV heads of 256: 8 rows
+    // behind 1024 keys 16.6 and 20.2 us, 16 behind 3968 28.8 and 32.6, 32 behind 512 19.1 and 20.0, behind 1024 22.3 and
+    // 22.5, behind 3968 35.7 and 33.9, 48 47.8 and 35.6, 128 103 and 80; at 4 of 512: 4 rows behind 256 19.7 and 19.4, 32
+    // behind 4000 49 and 34
+    const bool by_rows = P && (head_dim == 512 || M > 32 || (M > 16 && P >= 1024));
     if (P) {
         const uint32_t R = !by_rows ? 16 : rows_wg(head_dim);
         a.tiles = (M + R - 1) / R;
