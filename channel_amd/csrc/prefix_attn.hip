@@ -685,7 +685,7 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
 // keys that they share.
 template <int D, int RQ, bool ROWS>
 constexpr size_t lds_bytes() {
-    const size_t own = (4 * 4 * RQ * (D + 2)) * 4, prefix = ROWS ? sizeof(Shared<D>) : (4 * 16 * (D + 2)) * 4;
+    const size_t own = (4 * 4 * RQ * (D + 2)) * 4, prefix = ROWS ? sizeof(Shared<D>) : D == 256 ? (4 * 16 * (D + 2)) * 4 : 0;
     return own > prefix ? own : prefix;
 }
 
@@ -693,7 +693,7 @@ constexpr size_t lds_bytes() {
 // rows, 16 a wave, or 16 that the waves share (heads of 256).
 // Two workgroups per CU where the registers can be held to 256.
 template <int D, int RQ, bool ROWS>
-__global__ __launch_bounds__(256, D == 256 || (RQ == 1 && ROWS) ? 2 : 1) void k_prefix_attn(PrefixAttn a) {
+__global__ __launch_bounds__(256, D == 256 || RQ == 1 ? 2 : 1) void k_prefix_attn(PrefixAttn a) {
     extern __shared__ f4a sh4[];
     float *const sh = (float *)sh4;
     const int tid = threadIdx.x, lane = tid & 63;
@@ -841,10 +841,11 @@ static void launch_items(hipStream_t st, const PrefixAttn &a, uint32_t grid) {
 template <int D>
 static int launch_prefix(chn_ctx *ctx, const PrefixAttn &a, uint32_t grid, bool rows) {
     if (grid) {
-        if (a.gqa <= 4 && rows) launch_items<D, 1, true>(ctx->stream, a, grid);
-        else if (a.gqa <= 4) launch_items<D, 1, false>(ctx->stream, a, grid);
-        else if (rows) launch_items<D, 4, true>(ctx->stream, a, grid);
-        else launch_items<D, 4, false>(ctx->stream, a, grid);
+        // as few quads as the heads of a group need: 12 requests of up to 20000 tokens with 8 query heads to each of 2 KV
+        // heads take 75 us with two and 94 with four, heads of 512 153 and 180
+        if (a.gqa <= 4) rows ? launch_items<D, 1, true>(ctx->stream, a, grid) : launch_items<D, 1, false>(ctx->stream, a, grid);
+        else if (a.gqa <= 8) rows ? launch_items<D, 2, true>(ctx->stream, a, grid) : launch_items<D, 2, false>(ctx->stream, a, grid);
+        else rows ? launch_items<D, 4, true>(ctx->stream, a, grid) : launch_items<D, 4, false>(ctx->stream, a, grid);
         CHN_LAUNCHED(ctx, "k_prefix_attn");
     }
     k_prefix_join<D><<<a.n_req * a.num_q, 256, 0, ctx->stream>>>(a);
@@ -923,8 +924,8 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
         // at most about eight own items per CU: 12 requests of up to 20000 tokens take 228, 216, 205 and 211 us with
         // 512, 1024, 2048 and 4096 items; with few tokens the least groups per item decide
         a.own_cap = std::max(1u, 2048 / a.num_kv);
-        // two workgroups per CU, or one (of heads of 512 the second is the prefix's)
-        a.own_fit = (head_dim == 256 ? 512 : 256) / a.num_kv;
+        // two workgroups per CU, or one (of heads of 512 another is the prefix's, or fills the registers)
+        a.own_fit = (head_dim == 256 || (!P && gqa_ratio <= 4) ? 512 : 256) / a.num_kv;
         // no request has more items than its table has room for
         const uint32_t groups = (uint32_t)((((uint64_t)(max_blocks - n_prefix_blocks) << a.shift) + 15) / 16);
         items = std::min<uint64_t>(a.own_cap + n_req, (uint64_t)n_req * ((groups + kOwnMinGroups - 1) / kOwnMinGroups));

@@ -193,3 +193,21 @@ def test_one_slot_named_twice(ctx):
     for c in range(2):
         assert np.all((both[c][7] == first[c][7]) | (both[c][7] == second[c][7]))
         assert np.array_equal(both[c][:4], rest[c][:4]) and not both[c][4:7].any()
+
+
+@pytest.mark.parametrize("D", [256, 512])
+@pytest.mark.parametrize("gqa,n,npb", [(4, 3, 0), (5, 3, 0), (8, 3, 0), (9, 3, 0), (5, 9, 64), (8, 2, 64), (9, 5, 70),
+                                       (16, 1, 64), (16, 2, 63), (1, 16, 64), (1, 17, 63), (1, 17, 64), (1, 32, 63),
+                                       (1, 33, 63)])
+def test_rows_on_both_sides_of_the_rules(ctx, D, gqa, n, npb):
+    """Query heads per KV head at the edges of the quads, rows and prefixes at the edges of sharing keys (16 rows, 32
+    rows, 1024 keys)."""
+    attn_case(ctx, n, D, 2 * gqa, gqa, 16, npb, (0, 90))
+
+
+@pytest.mark.parametrize("D", [256, 512])
+def test_lengths_inside_a_shared_prefix(ctx, D):
+    """Rows that see none, a part and all of a prefix whose keys are shared through LDS; the others hold NaN."""
+    lens = [0, 1, 15, 16, 17, 100, 640, 641, 1023, 1024, 1025, 1100, 31, 32, 33, 999, 1024, 2]
+    attn_case(ctx, len(lens), D, 2, 1, 16, 64, None, lens=lens)
+    attn_case(ctx, 6, D, 16, 8, 16, 64, None, lens=lens[2:8], bad=0.2)
