@@ -439,7 +439,7 @@ constexpr uint32_t kDigits = 2 * kDrawThreads;
 struct Group {
     static constexpr int NW = kDrawThreads / 64;
     static_assert(NW == 16, "the waves' parts are a row of 16 lanes");
-    uint64_t hist_w[kDigits], part[NW], found[4];
+    uint64_t hist_w[kDigits], part[NW], part2[NW], found[4];
     uint32_t hist_n[kDigits], n, hit;
 
     __device__ __forceinline__ uint64_t sum(uint64_t v) {
@@ -455,6 +455,19 @@ struct Group {
         if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
         __syncthreads();
         return wave_min_u64(part[threadIdx.x & 15]);
+    }
+    // the largest and the smallest
+    __device__ __forceinline__ void ends(uint64_t &hi, uint64_t &lo) {
+        hi = wave_min_u64(~hi);
+        lo = wave_min_u64(lo);
+        __syncthreads();
+        if ((threadIdx.x & 63) == 0) {
+            part[threadIdx.x >> 6] = hi;
+            part2[threadIdx.x >> 6] = lo;
+        }
+        __syncthreads();
+        hi = ~wave_min_u64(part[threadIdx.x & 15]);
+        lo = wave_min_u64(part2[threadIdx.x & 15]);
     }
     // inclusive running sum over the threads, and the whole sum
     __device__ __forceinline__ uint64_t scan(uint64_t v, uint64_t &total) {
@@ -520,6 +533,47 @@ __device__ __forceinline__ uint64_t target_of(float u, uint64_t Z) {
     return t < Z ? t : Z - 1;
 }
 
+// The draw of a row with top-k from a list of n tokens that holds its k <= kMaxK
+// largest.  sorted: kMaxK words.
+template <bool CAP, typename F>
+__device__ __forceinline__ void draw_listed(const Row<CAP> &r, Group &sh, uint64_t *list, uint64_t *sorted, uint32_t n, float u,
+                                            F &&finish) {
+    const uint32_t tid = threadIdx.x;
+    // the k largest, in order: a thread counts what is larger than its key
+    for (uint32_t i = tid; i < n; i += kDrawThreads) {
+        const uint64_t key = list[i];
+        uint32_t rank = 0;
+#pragma unroll 8
+        for (uint32_t j = 0; j < n; ++j) rank += list[j] > key ? 1u : 0u;
+        if (rank < r.k) sorted[rank] = key;
+    }
+    __syncthreads();
+    const uint32_t k = min(n, r.k);
+    const uint64_t key = tid < k ? sorted[tid] : 0;
+    const uint64_t w = tid < k ? r.units(value_of(key >> 32)) : 0;
+    uint64_t Z, total;
+    const uint64_t incl = sh.scan(w, Z);
+    bool in = tid < k;
+    if (r.p < 1.0f) in = in && incl - w < r.goal(Z);
+    const uint64_t kw = in ? r.kept(w) : 0;
+    (void)sh.scan(kw, total);
+    const uint64_t target = target_of(u, total);
+    // the draw goes by index: a kept token sums the kept ones before it
+    list[tid] = kw;
+    __syncthreads();
+    if (kw) {
+        uint64_t before = 0;
+        const uint32_t mine = (uint32_t)key;                           // ~index: larger for lower indexes
+#pragma unroll 8
+        for (uint32_t j = 0; j < k; ++j) {
+            const uint64_t other = list[j];                          // read either way: no branch, so reads overlap
+            before += (uint32_t)sorted[j] > mine ? other : 0;
+        }
+        if (before <= target && before + kw > target)
+            finish(0xFFFFFFFFu - mine, (float)(r.weight(value_of(key >> 32)) / (double)total));
+    }
+}
+
 // Rows of up to kSmallV: one launch, a workgroup per row, which holds the row in
 // registers (thread t: values t, t + 1024, ..; J of them, as few as V needs:
 // 50 rows of 10007 take 33 us with J = 12 and 38 with 16).  One workgroup's
@@ -528,28 +582,34 @@ __device__ __forceinline__ uint64_t target_of(float u, uint64_t Z) {
 constexpr uint32_t kSmallV = 16 * kDrawThreads;
 template <int J, bool CAP>
 __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
+    constexpr uint32_t kShort = 2048;                                  // a list of the largest
     __shared__ Group sh;
-    __shared__ uint64_t by_wave[J][Group::NW];
-    const uint32_t tid = threadIdx.x, row = blockIdx.x;
-    const int lane = tid & 63, wave = tid >> 6;
+    __shared__ uint64_t list[kShort], sorted[kMaxK];
+    const uint32_t tid = threadIdx.x, row = blockIdx.x, i0 = tid * J;
     const float *x = a.logits + (size_t)row * a.ld;
     float v[J];
 #pragma unroll
-    for (int j = 0; j < J; ++j) {
-        const uint32_t i = tid + j * kDrawThreads;
-        v[j] = i < a.V ? x[i] : __builtin_nanf("");
+    for (int j = 0; j < J; j += 4) {
+        if (i0 + j + 4 <= a.V) {
+            const f4u y = *(const f4u *)(x + i0 + j);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j + e] = y[e];
+        } else
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[j + e] = i0 + j + e < a.V ? x[i0 + j + e] : __builtin_nanf("");
     }
     const float u = a.u[row];
-    uint64_t hi = 0, lo = ~0ull, n = 0;
-    auto key_of = [&](int j) { return allowed(v[j]) ? token_key(v[j], tid + j * kDrawThreads) : 0; };
+    if (tid == 0) sh.n = 0;
+    for (uint32_t i = tid; i < kDigits; i += kDrawThreads) sh.hist_n[i] = 0;
+    uint64_t hi = 0, lo = ~0ull;
+    auto key_of = [&](int j) { return allowed(v[j]) ? token_key(v[j], i0 + j) : 0; };
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const uint64_t key = key_of(j);
         hi = max(hi, key);
         lo = key ? min(lo, key) : lo;
-        n += key ? 1 : 0;
     }
-    hi = ~sh.least(~hi);
+    sh.ends(hi, lo);
     const Row<CAP> r(a, row, (uint32_t)(hi >> 32));
     auto finish = [&](uint32_t token, float prob) {
         a.tokens[row] = token;
@@ -559,16 +619,43 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
         if (tid == 0) finish(r.some ? 0xFFFFFFFFu - (uint32_t)hi : CHN_NO_TOKEN, r.some ? 1.0f : 0.0f);
         return;
     }
-    lo = sh.least(lo);
     if (r.k) {
-        n = sh.sum(n);
-        if (n > r.k)
+        // the logits in up to 2048 parts between the smallest and the largest: where the running count from the top reaches
+        // k, k tokens are that large
+        const uint32_t least = (uint32_t)(lo >> 32), range = (uint32_t)(hi >> 32) - least;
+        const int shift = max(32 - __clz(range) - 11, 0);              // range 0: 0
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+            if (allowed(v[j])) atomicAdd(&sh.hist_n[(orderable(v[j]) - least) >> shift], 1u);
+        __syncthreads();
+        const uint32_t e = kDigits - 1 - 2 * tid, c0 = sh.hist_n[e], c1 = sh.hist_n[e - 1];
+        uint64_t n;
+        const uint64_t before = sh.scan(c0 + c1, n) - c0 - c1;
+        if (n > r.k) {
+            if (before < r.k && before + c0 + c1 >= r.k) sh.found[0] = e - (before + c0 < r.k);
+            __syncthreads();
+            const uint32_t floor_key = least + ((uint32_t)sh.found[0] << shift);
+            if (r.k <= kMaxK) {
+#pragma unroll
+                for (int j = 0; j < J; ++j)
+                    if (allowed(v[j]) && orderable(v[j]) >= floor_key) {
+                        const uint32_t at = atomicAdd(&sh.n, 1u);
+                        if (at < kShort) list[at] = token_key(v[j], i0 + j);
+                    }
+                __syncthreads();
+                if (sh.n <= kShort) {
+                    draw_listed(r, sh, list, sorted, sh.n, u, finish);
+                    return;
+                }
+            }
+            // many equal or near equal ones, or many wanted: key by key
             lo = sh.last_key(
                 [&](auto &&f) {
 #pragma unroll
                     for (int j = 0; j < J; ++j) f(key_of(j), [] { return (uint64_t)1; });   // key 0 is below lo
                 },
                 lo, hi, false, r.k);
+        }
     }
     uint64_t w[J], Z = 0;
 #pragma unroll
@@ -587,31 +674,28 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
             },
             lo, hi, true, r.goal(Z));
     }
-    // sums of 64 consecutive indexes
+    uint64_t own = 0;
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         w[j] = key_of(j) >= lo ? r.kept(w[j]) : 0;
-        const uint64_t s = wave_sum_u64(w[j]);
-        if (lane == 0) by_wave[j][wave] = s;
+        own += w[j];
     }
-    __syncthreads();
-    static_assert(J * Group::NW <= (int)kDrawThreads, "one thread per sum");
-    const uint64_t own = tid < J * Group::NW ? by_wave[tid / Group::NW][tid % Group::NW] : 0;
     const uint64_t incl = sh.scan(own, Z), target = target_of(u, Z);
-    if (own && incl > target && incl - own <= target) {
-        sh.hit = tid;
-        sh.found[0] = target - (incl - own);
-    }
-    __syncthreads();
-    if (wave == (int)(sh.hit % Group::NW)) {
-        const uint64_t rest = sh.found[0];
+    if (own && incl > target && incl - own <= target) {                // one thread
+        uint64_t run = incl - own;
+        uint32_t token = 0;
+        float l = 0.0f;
+        bool hit = false;
 #pragma unroll
-        for (int j = 0; j < J; ++j)
-            if (j == (int)(sh.hit / Group::NW)) {
-                const uint64_t run = wave_scan_u64(w[j]);
-                if (w[j] && run > rest && run - w[j] <= rest)
-                    finish(tid + j * kDrawThreads, (float)(r.weight(v[j]) / (double)Z));
+        for (int j = 0; j < J; ++j) {
+            run += w[j];
+            if (!hit && run > target) {
+                hit = true;
+                token = i0 + j;
+                l = v[j];
             }
+        }
+        finish(token, (float)(r.weight(l) / (double)Z));
     }
 }
 
@@ -874,41 +958,7 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         });
         __syncthreads();
     }
-    const uint32_t n = sh.n;
-    // the k largest, in order: a thread counts what is larger than its key
-    uint64_t *sorted = (uint64_t *)spare;                              // kMaxK
-    for (uint32_t i = tid; i < n; i += kDrawThreads) {
-        const uint64_t key = d.list[i];
-        uint32_t rank = 0;
-#pragma unroll 8
-        for (uint32_t j = 0; j < n; ++j) rank += d.list[j] > key ? 1u : 0u;
-        if (rank < r.k) sorted[rank] = key;
-    }
-    __syncthreads();
-    const uint32_t k = min(n, r.k);
-    const uint64_t key = tid < k ? sorted[tid] : 0;
-    const uint64_t w = tid < k ? r.units(value_of(key >> 32)) : 0;
-    uint64_t Z, total;
-    const uint64_t incl = sh.scan(w, Z);
-    bool in = tid < k;
-    if (r.p < 1.0f) in = in && incl - w < r.goal(Z);
-    const uint64_t kw = in ? r.kept(w) : 0;
-    (void)sh.scan(kw, total);
-    const uint64_t target = target_of(u, total);
-    // the draw goes by index: a kept token sums the kept ones before it
-    d.list[tid] = kw;
-    __syncthreads();
-    if (kw) {
-        uint64_t before = 0;
-        const uint32_t mine = (uint32_t)key;                           // ~index: larger for lower indexes
-#pragma unroll 8
-        for (uint32_t j = 0; j < k; ++j) {
-            const uint64_t other = d.list[j];                          // read either way: no branch, so reads overlap
-            before += (uint32_t)sorted[j] > mine ? other : 0;
-        }
-        if (before <= target && before + kw > target)
-            finish(0xFFFFFFFFu - mine, (float)(r.weight(value_of(key >> 32)) / (double)total));
-    }
+    draw_listed(r, sh, d.list, (uint64_t *)spare, sh.n, u, finish);
 }
 
 template <bool CAP>
