@@ -29,9 +29,10 @@
 //
 // Measured: one row of 262144 with top-k 64 and top-p: 18 us, of which the
 // draw's single workgroup takes 11, step after step.  32 rows of 32 users,
-// softcapped: 51 us.  128 rows (134 MB) by top-p: 138 us; the passes take 28
-// (4.7 TB/s), 52 and 43, the second and third bound by issuing their 64-bit
-// arithmetic (35 without it).  50 rows of 10007 in one launch: 33 us.
+// softcapped: 50 us.  128 rows (134 MB) by top-p: 130 us; the first pass takes
+// 28 (4.7 TB/s), the second and third are bound by issuing their 64-bit
+// arithmetic (the second 53, 38 without it).  50 rows of 10007 in one launch:
+// 25 us.
 #include "chn_internal.h"
 
 #include <cmath>
@@ -47,9 +48,10 @@ constexpr uint32_t kBins = 2048;            // of 2^-6 powers of two each: 32 po
 constexpr uint32_t kList = 4096;            // tokens of a row's list: 32 KB of LDS
 constexpr uint32_t kMaxK = 1024;            // top-k by block maxima: a thread per kept token
 constexpr uint32_t kDrawThreads = 1024;
-// 8 stretches a workgroup, which share a histogram.  256, 512 and 1024 threads take 99, 97 and 112 us for the second and third
-// pass over 128 rows: with 1024 a CU holds one, and nothing is read while it computes
-constexpr uint32_t kPassThreads = 512;
+// Two waves per stretch, as a wave's values are one chain of 64-bit arithmetic (one wave: 57 us instead of 50 at 32 users);
+// 4 stretches a workgroup, which share a histogram: 256, 512 and 1024 threads take 182, 130 and 131 us at 128 rows by
+// top-p (histograms merged more or less often), 51, 50 and 55 at 32 users
+constexpr uint32_t kPassThreads = 512, kPassStretches = kPassThreads / 128;
 constexpr uint32_t kRowsAtOnce = 1024;      // rows that share the workspace (64 KB a row at 262144)
 
 struct Sample {
@@ -232,29 +234,28 @@ struct Stretch {
 #pragma unroll
             for (int e = 0; e < 4; ++e) d[e] = i + e < a.V ? x[i + e] : __builtin_nanf("");
     }
-    __device__ __forceinline__ void start(const Sample &a, const float *x, uint32_t s) {
+    __device__ __forceinline__ void start(const Sample &a, const float *x, uint32_t s, int h) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) load(a, x, s, j, v[j]);
+        for (int j = 0; j < 4; ++j) load(a, x, s, 4 * h + j, v[j]);
     }
-    // f(index of the first, four values, number of the load) for stretch s, which has been started
+    // f(index of the first, four values, number of the load) for the half of stretch s that is here
     template <typename F>
-    __device__ __forceinline__ void each(const Sample &a, const float *x, uint32_t s, F &&f) {
-#pragma unroll 1
-        for (int h = 0; h < 2; ++h) {
+    __device__ __forceinline__ void half(uint32_t s, int h, F &&f) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                f(s * kStretch + 4 * (threadIdx.x & 63) + 256 * (4 * h + j), v[j], 4 * h + j);
-                if (h == 0) load(a, x, s, 4 + j, v[j]);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+        for (int j = 0; j < 4; ++j) {
+            f(s * kStretch + 4 * (threadIdx.x & 63) + 256 * (4 * h + j), v[j], 4 * h + j);
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
 };
+// f over both halves
 template <typename F>
 __device__ __forceinline__ void stretch(const Sample &a, const float *x, uint32_t s, F &&f) {
-    Stretch v;
-    v.start(a, x, s);
-    v.each(a, x, s, f);
+    Stretch v[2];
+    v[0].start(a, x, s, 0);
+    v[1].start(a, x, s, 1);
+    v[0].half(s, 0, f);
+    v[1].half(s, 1, f);
 }
 
 // the row's largest logit, by every wave
@@ -294,23 +295,34 @@ __global__ __launch_bounds__(256) void k_sample_max(Sample a) {
     if (lane == 0) a.smax[(size_t)row * a.stretches + s] = allowed(most) ? orderable(most) : 0u;
 }
 
+// The sums of the stretches from the waves' (two waves take a stretch); all
+// threads, part: a word per wave.
+__device__ __forceinline__ void put_sums(const Sample &a, uint32_t row, uint64_t sum, uint64_t *part) {
+    sum = wave_sum_u64(sum);
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    const uint32_t t = threadIdx.x, s = blockIdx.x * kPassStretches + t;
+    if (t < kPassStretches && s < a.stretches) a.sums[(size_t)row * a.stretches + s] = part[2 * t] + part[2 * t + 1];
+}
+
 // Rows without top-k: the histogram of the weights (with top-p), or the sums of
 // the stretches.
 template <bool CAP>
 __global__ __launch_bounds__(kPassThreads) void k_sample_mass(Sample a) {
     __shared__ uint64_t hist[kBins];
-    const uint32_t row = blockIdx.y, s = blockIdx.x * (kPassThreads / 64) + (threadIdx.x >> 6);
+    const uint32_t row = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t s = blockIdx.x * kPassStretches + wave / 2;
     if (!by_mass(a, row)) return;                                    // the whole workgroup
     const float *x = a.logits + (size_t)row * a.ld;
     Stretch v;
-    if (s < a.stretches) v.start(a, x, s);                            // while the row's settings and bins are prepared
+    if (s < a.stretches) v.start(a, x, s, wave % 2);                            // while the row's settings and bins are prepared
     __builtin_amdgcn_sched_barrier(0);
     const Row<CAP> r(a, row, row_top(a, row));
     if (r.p < 1.0f) {
         for (uint32_t i = threadIdx.x; i < kBins; i += blockDim.x) hist[i] = 0;
         __syncthreads();
         if (s < a.stretches)
-            v.each(a, x, s,
+            v.half(s, wave % 2,
                    [&](uint32_t, const f4u &l, int) {
                        uint64_t w[4];
 #pragma unroll
@@ -322,15 +334,15 @@ __global__ __launch_bounds__(kPassThreads) void k_sample_mass(Sample a) {
         __syncthreads();
         for (uint32_t i = threadIdx.x; i < kBins; i += blockDim.x)
             if (hist[i]) atomicAdd((unsigned long long *)&a.hist[(size_t)row * kBins + i], (unsigned long long)hist[i]);
-    } else if (s < a.stretches) {
+    } else {
         uint64_t sum = 0;
-        v.each(a, x, s, [&](uint32_t, const f4u &l, int) {
+        if (s < a.stretches)
+            v.half(s, wave % 2, [&](uint32_t, const f4u &l, int) {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) sum += r.kept(r.units_if_allowed(l[e]));
-            asm volatile("" : "+v"(sum));                              // summed here, not kept apart until the end
-        });
-        sum = wave_sum_u64(sum);
-        if ((threadIdx.x & 63) == 0) a.sums[(size_t)row * a.stretches + s] = sum;
+                for (int e = 0; e < 4; ++e) sum += r.kept(r.units_if_allowed(l[e]));
+                asm volatile("" : "+v"(sum));                          // summed here, not kept apart until the end
+            });
+        put_sums(a, row, sum, hist);
     }
 }
 
@@ -370,12 +382,13 @@ __global__ __launch_bounds__(kPassThreads) void k_sample_border(Sample a) {
     __shared__ uint64_t sh[20], found[kMine];
     __shared__ float queue[kPassThreads / 64][512];
     __shared__ uint32_t nfound, at0;
-    const uint32_t row = blockIdx.y, s = blockIdx.x * (kPassThreads / 64) + (threadIdx.x >> 6);
+    const uint32_t row = blockIdx.y, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t s = blockIdx.x * kPassStretches + wave / 2;
     const int lane = threadIdx.x & 63;
     if (!by_mass(a, row) || !(a.top_p[row] < 1.0f)) return;
     const float *x = a.logits + (size_t)row * a.ld;
     Stretch v;
-    if (s < a.stretches) v.start(a, x, s);
+    if (s < a.stretches) v.start(a, x, s, wave % 2);
     __builtin_amdgcn_sched_barrier(0);
     const Row<CAP> r(a, row, row_top(a, row));
     if (!r.some) return;
@@ -389,10 +402,10 @@ __global__ __launch_bounds__(kPassThreads) void k_sample_border(Sample a) {
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     };
+    uint64_t sum = 0;
     if (s < a.stretches) {
-        uint32_t n = 0;                                                  // queued, below 64 between steps
-        uint64_t sum = 0;
-        v.each(a, x, s, [&](uint32_t i, const f4u &l, int) {
+        uint32_t n = 0;                                                  // queued, below 256 between steps
+        v.half(s, wave % 2, [&](uint32_t i, const f4u &l, int) {
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
                 const uint32_t b = allowed(l[e]) ? r.bin(l[e]) : kBins;
@@ -423,9 +436,8 @@ __global__ __launch_bounds__(kPassThreads) void k_sample_border(Sample a) {
         });
         fence();
         for (uint32_t e = lane; e < n; e += 64) sum += r.kept(r.units(q[e]));
-        sum = wave_sum_u64(sum);
-        if (lane == 0) a.sums[(size_t)row * a.stretches + s] = sum;
     }
+    put_sums(a, row, sum, sh);
     __syncthreads();
     // more than its share: the row's list counts as full
     if (threadIdx.x == 0 && nfound) at0 = atomicAdd(&a.listed[row], nfound <= kMine ? nfound : kList + 1);
@@ -575,10 +587,10 @@ __device__ __forceinline__ void draw_listed(const Row<CAP> &r, Group &sh, uint64
 }
 
 // Rows of up to kSmallV: one launch, a workgroup per row, which holds the row in
-// registers (thread t: values t, t + 1024, ..; J of them, as few as V needs:
-// 50 rows of 10007 take 33 us with J = 12 and 38 with 16).  One workgroup's
-// steps are latency after latency, but fewer than those of four launches (73
-// us); above 16 values a thread there are no registers left.
+// registers (thread t: values J t .. J t + J - 1; J as few as V needs: 50 rows
+// of 10007 took 33 us with J = 12 and 38 with 16).  One workgroup's steps are
+// latency after latency, but fewer than those of four launches (25 us and 73);
+// above 16 values a thread there are no registers left.
 constexpr uint32_t kSmallV = 16 * kDrawThreads;
 template <int J, bool CAP>
 __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
@@ -973,7 +985,7 @@ static int launch_small(chn_ctx *ctx, const Sample &a, uint32_t n) {
 
 template <bool CAP>
 static void launch_rows(chn_ctx *ctx, const Sample &a, uint32_t n, size_t lds) {
-    const dim3 wide((a.stretches + kPassThreads / 64 - 1) / (kPassThreads / 64), n);
+    const dim3 wide((a.stretches + kPassStretches - 1) / kPassStretches, n);
     k_sample_max<<<dim3((a.stretches + 3) / 4, n), 256, 0, ctx->stream>>>(a);
     k_sample_mass<CAP><<<wide, kPassThreads, 0, ctx->stream>>>(a);
     if (a.top_p) k_sample_border<CAP><<<wide, kPassThreads, 0, ctx->stream>>>(a);
