@@ -44,8 +44,8 @@ __device__ __forceinline__ Grow grow_of(const Tables &a, uint32_t len, uint32_t 
 // takes a row of the batch (its request by bisection of the starts in LDS);
 // the thread of a block's first token enters the block.  Bound by the launch
 // and by three latencies (lengths, table entries, writes): 32 requests of one
-// token 4.8 us, 1024 requests of 131072 tokens in all, with 300 new prefixes,
-// 6.1 us.
+// token 3.9 us, 1024 requests of 131072 tokens in all, with 300 new prefixes,
+// 5.1 us.
 __global__ __launch_bounds__(kTabThreads) void k_block_tables(Tables a) {
     extern __shared__ uint32_t sh[];
     uint32_t *row0 = sh, *blk0 = sh + a.n_req;         // first row, first of the handed-out blocks
@@ -220,7 +220,7 @@ __global__ __launch_bounds__(256) void k_rope_at(RopeAt a) {
 // the angles are evaluated once per 8 rows, while those loads are under way.
 // Bound by memory: 1500 tokens of 16 query and 4 KV heads of 512 (135 MB)
 // take 27 us, 5.0 TB/s (27 with one row per wave, 31 with four); with 16 and 8
-// heads of 256 18.4 (20.5 and 18.6).  24 tokens of those take 5: the launch,
+// heads of 256 18.4 (20.5 and 18.6).  24 tokens of those take 4: the launch,
 // then loads, a sum and writes behind one another.
 typedef float f4p __attribute__((ext_vector_type(4)));
 template <int N>

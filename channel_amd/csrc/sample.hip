@@ -589,8 +589,9 @@ __device__ __forceinline__ void draw_listed(const Row<CAP> &r, Group &sh, uint64
 // Rows of up to kSmallV: one launch, a workgroup per row, which holds the row in
 // registers (thread t: values J t .. J t + J - 1; J as few as V needs: 50 rows
 // of 10007 took 33 us with J = 12 and 38 with 16).  One workgroup's steps are
-// latency after latency, but fewer than those of four launches (25 us and 73);
-// above 16 values a thread there are no registers left.
+// latency after latency, but fewer than those of four launches: 50 rows of
+// 10007 25 us and 49, one of 16000 with top-k 14 and 19; 20 rows of 16000 by
+// top-p 30 and 28, and above that no registers are left.
 constexpr uint32_t kSmallV = 16 * kDrawThreads;
 template <int J, bool CAP>
 __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
