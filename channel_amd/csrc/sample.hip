@@ -551,12 +551,17 @@ template <bool CAP, typename F>
 __device__ __forceinline__ void draw_listed(const Row<CAP> &r, Group &sh, uint64_t *list, uint64_t *sorted, uint32_t n, float u,
                                             F &&finish) {
     const uint32_t tid = threadIdx.x;
+    if (tid == 0 && n % 2) list[n] = 0;                                // below every key
+    __syncthreads();
     // the k largest, in order: a thread counts what is larger than its key
     for (uint32_t i = tid; i < n; i += kDrawThreads) {
         const uint64_t key = list[i];
         uint32_t rank = 0;
 #pragma unroll 8
-        for (uint32_t j = 0; j < n; ++j) rank += list[j] > key ? 1u : 0u;
+        for (uint32_t j = 0; j < n; j += 2) {                          // two a read
+            const ulonglong2 o = *(const ulonglong2 *)(list + j);
+            rank += (o.x > key ? 1u : 0u) + (o.y > key ? 1u : 0u);
+        }
         if (rank < r.k) sorted[rank] = key;
     }
     __syncthreads();
@@ -570,14 +575,14 @@ __device__ __forceinline__ void draw_listed(const Row<CAP> &r, Group &sh, uint64
     const uint64_t kw = in ? r.kept(w) : 0;
     (void)sh.scan(kw, total);
     const uint64_t target = target_of(u, total);
-    // the draw goes by index: a kept token sums the kept ones before it
+    // the draw goes by index: a kept token sums the kept ones before it, which are among the first of the order
     list[tid] = kw;
-    __syncthreads();
+    const uint32_t first = __syncthreads_count(in);
     if (kw) {
         uint64_t before = 0;
         const uint32_t mine = (uint32_t)key;                           // ~index: larger for lower indexes
 #pragma unroll 8
-        for (uint32_t j = 0; j < k; ++j) {
+        for (uint32_t j = 0; j < first; ++j) {
             const uint64_t other = list[j];                          // read either way: no branch, so reads overlap
             before += (uint32_t)sorted[j] > mine ? other : 0;
         }
@@ -597,7 +602,8 @@ template <int J, bool CAP>
 __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
     constexpr uint32_t kShort = 2048;                                  // a list of the largest
     __shared__ Group sh;
-    __shared__ uint64_t list[kShort], sorted[kMaxK];
+    __shared__ __align__(16) uint64_t list[kShort];
+    __shared__ uint64_t sorted[kMaxK];
     const uint32_t tid = threadIdx.x, row = blockIdx.x, i0 = tid * J;
     const float *x = a.logits + (size_t)row * a.ld;
     float v[J];
@@ -714,14 +720,14 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
 
 // LDS of k_sample_draw.
 struct Draw {
-    uint64_t list[kList];
+    __align__(16) uint64_t list[kList];
     Group g;
 };
 
 // A workgroup per row: the kept tokens' last key, then the draw.
 template <bool CAP>
 __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
-    extern __shared__ uint64_t lds[];
+    extern __shared__ __align__(16) uint64_t lds[];
     constexpr int NW = Group::NW;
     Draw &d = *(Draw *)lds;
     Group &sh = d.g;
@@ -940,16 +946,16 @@ __global__ __launch_bounds__(kDrawThreads) void k_sample_draw(Sample a) {
         }
         const uint32_t nb = sh.hit;
         // their tokens at or above the bound
-        for (uint32_t q = wave; q < nb; q += 4 * NW) {
-            float v[4];
-            uint32_t i[4];
+        for (uint32_t q = wave; q < nb; q += 8 * NW) {
+            float v[8];
+            uint32_t i[8];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
+            for (int e = 0; e < 8; ++e) {
                 i[e] = spare[min(q + e * NW, nb - 1)] * 64 + lane;
                 v[e] = x[min(i[e], a.V - 1)];
             }
 #pragma unroll
-            for (int e = 0; e < 4; ++e)
+            for (int e = 0; e < 8; ++e)
                 if (q + e * NW < nb && i[e] < a.V && allowed(v[e]) && orderable(v[e]) >= floor_key) {
                     const uint32_t at = atomicAdd(&sh.n, 1u);
                     if (at < kList) d.list[at] = token_key(v[e], i[e]);
