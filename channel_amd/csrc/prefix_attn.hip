@@ -10,7 +10,7 @@
 // read once per 64 or 32 rows) and own items (KV head, request, a range of its
 // keys).  A second launch joins the items' partial results.
 //
-// Few rows (own items, and a prefix's up to 16 or 32 rows) are bound by reading the
+// Few rows (own items, and prefixes with few rows) are bound by reading the
 // caches: struct Quads, 4x4x1 instructions straight from the registers the
 // keys are loaded into.  Many rows over a prefix are bound by the matrix
 // instructions (157 TFLOP/s in fp32): struct Rows, 16x16x4 instructions, keys
@@ -23,7 +23,7 @@
 // memory bounds it).
 //
 // Measured (fp32, one decode step, both launches): 8 requests of up to 96
-// tokens behind 512, heads of 256: 16.7 us, most of it the two launches and
+// tokens behind 512, heads of 256: 14 us, most of it the two launches and
 // the block-table, key, weight and join latencies one after another.  64
 // requests of up to 480 tokens behind 3968: 80 us; the prefix alone takes 59 (27
 // at the matrix rate), the requests' own keys share the chip with it.  33
@@ -32,6 +32,7 @@
 #include "chn_internal.h"
 
 #include <cmath>
+#include <type_traits>
 
 namespace chn {
 
@@ -52,7 +53,7 @@ struct PrefixAttn {
     float exp_hi, exp_lo;      // scale * log2(e) in two parts
     float *out;
     // prefix items: unit u = (KV head, key range), `tiles` tiles of rows each
-    uint32_t splits, split_keys, tiles, prefix_wgs;
+    uint32_t splits, split_keys, tiles, prefix_wgs, quads;
     // own items: at most own_cap + n_req of them per KV head, of which own_fit run at once
     uint32_t own_cap, own_fit;
     // partial results, [splits][n_req][num_q] of the prefix and then [own item][num_q]: sums of D values, references
@@ -685,12 +686,12 @@ __device__ __forceinline__ void run_rows(const PrefixAttn &a, Rows &w, const f4a
 // keys that they share.
 template <int D, int RQ, bool ROWS>
 constexpr size_t lds_bytes() {
-    const size_t own = (4 * 4 * RQ * (D + 2)) * 4, prefix = ROWS ? sizeof(Shared<D>) : D == 256 ? (4 * 16 * (D + 2)) * 4 : 0;
+    const size_t own = (4 * 4 * RQ * (D + 2)) * 4, prefix = ROWS ? sizeof(Shared<D>) : D == 256 ? (4 * 8 * (D + 2)) * 4 : 0;
     return own > prefix ? own : prefix;
 }
 
 // RQ: quads of rows of own items.  ROWS: whether prefix items hold rows_wg
-// rows, 16 a wave, or 16 that the waves share (heads of 256).
+// rows, 16 a wave, or one or two quads that the waves share (heads of 256).
 // Two workgroups per CU where the registers can be held to 256.
 template <int D, int RQ, bool ROWS>
 __global__ __launch_bounds__(256, D == 256 || RQ == 1 ? 2 : 1) void k_prefix_attn(PrefixAttn a) {
@@ -713,7 +714,7 @@ __global__ __launch_bounds__(256, D == 256 || RQ == 1 ? 2 : 1) void k_prefix_att
     };
     if (blockIdx.x < a.prefix_wgs) {
         // the row tiles of one unit run on one XCD (workgroup i runs on XCD i % 8) and share its keys there
-        constexpr uint32_t R = ROWS ? rows_wg(D) : 16;
+        const uint32_t R = ROWS ? rows_wg(D) : 4 * a.quads;
         const uint32_t b = blockIdx.x, tile = (b >> 3) % a.tiles, u = (b >> 3) / a.tiles * 8 + (b & 7);
         if (u >= a.num_kv * a.splits) return;
         const uint32_t kvh = u % a.num_kv, split = u / a.num_kv, begin = split * a.split_keys;
@@ -734,9 +735,13 @@ __global__ __launch_bounds__(256, D == 256 || RQ == 1 ? 2 : 1) void k_prefix_att
             for (int s = 0; s < 16; ++s) q[s] = *(const f4a *)(x + 16 * s);
             run_rows<D>(a, w, q, *(Shared<D> *)sh4, k, n, where);
         } else if constexpr (D == 256) {               // heads of 512 always share
-            Quads<D, 4, false> w;
-            w.run(a, sh, k, limit, [&] { load_q(kvh, row0, n, 16); });
-            w.join(a, sh, n, where);
+            auto quads = [&](auto Q) {
+                Quads<D, Q, false> w;
+                w.run(a, sh, k, limit, [&] { load_q(kvh, row0, n, 4 * Q); });
+                w.join(a, sh, n, where);
+            };
+            if (a.quads == 1) quads(std::integral_constant<int, 1>{});
+            else quads(std::integral_constant<int, 2>{});
         }
         return;
     }
@@ -901,14 +906,18 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
     a.exp_lo = std::isfinite(a.exp_hi) ? (float)(e - a.exp_hi) : 0.0f;
     a.out = out;
     const uint32_t P = n_prefix_blocks << a.shift, M = n_req * gqa_ratio;
-    // Few rows of heads of 256: every workgroup of 16 rows reads the prefix for itself and its waves split the keys.
-    // Otherwise 64 (of heads of 512: 32) rows share what is read.  The one way and the other, at 8 KV heads of 256: 8 rows
-    // behind 1024 keys 16.6 and 20.2 us, 16 behind 3968 28.8 and 32.6, 32 behind 512 19.1 and 20.0, behind 1024 22.3 and
-    // 22.5, behind 3968 35.7 and 33.9, 48 47.8 and 35.6, 128 103 and 80; at 4 of 512: 4 rows behind 256 19.7 and 19.4, 32
-    // behind 4000 49 and 34
-    const bool by_rows = P && (head_dim == 512 || M > 32 || (M > 16 && P >= 1024));
+    // Few rows or little work with heads of 256: every workgroup of 4 or 8 rows reads the prefix for itself and its waves
+    // split the keys.  Otherwise 64 (of heads of 512: 32) rows share what is read.  The one way and the other, rows x keys
+    // x KV heads of 256: 16 x 512 x 8 13.5 and 18.9 us, 16 x 3968 x 8 25.4 and 32.2, 32 x 1024 x 8 19.4 and 22.5, 48 x
+    // 1024 x 8 25.6 and 24.7, 24 x 2048 x 8 24.5 and 23.5, 64 x 512 x 8 25.7 and 24.0, 128 x 3968 x 8 110 and 58, 64 x
+    // 3968 x 2 25.7 and 25.8; 4 of 512: 4 x 256 19.7 and 19.4, 32 x 4000 49 and 34
+    const uint64_t work = (uint64_t)M * P * (num_q_heads / gqa_ratio);
+    const bool by_rows = P && (head_dim == 512 || (M > 16 && work >= (M >= 64 ? 1u << 18 : 3u << 17)));
     if (P) {
-        const uint32_t R = !by_rows ? 16 : rows_wg(head_dim);
+        // 4 rows behind 512 and 20000 keys take 11.8 and 65 us with one quad, 14.7 and 81 with four; 16 rows 13.6 and 90
+        // with twice two, 16.9 and 85 with four
+        a.quads = M > 4 ? 2 : 1;
+        const uint32_t R = by_rows ? rows_wg(head_dim) : 4 * a.quads;
         a.tiles = (M + R - 1) / R;
         // about one workgroup per CU, 64 keys (16 per wave) at least.  128 rows on 3968 keys with own tokens beside them:
         // 122 us with half as many workgroups, 94 so, 106 with twice as many (and twice the partial results)
