@@ -200,8 +200,7 @@ def test_one_slot_named_twice(ctx):
                                        (16, 1, 64), (16, 2, 63), (1, 16, 64), (1, 17, 63), (1, 17, 64), (1, 32, 63),
                                        (1, 33, 63)])
 def test_rows_on_both_sides_of_the_rules(ctx, D, gqa, n, npb):
-    """Query heads per KV head at the edges of the quads, rows and prefixes at the edges of sharing keys (16 rows, 32
-    rows, 1024 keys)."""
+    """Query heads per KV head at the edges of the quads, rows at the edges of quads and tiles."""
     attn_case(ctx, n, D, 2 * gqa, gqa, 16, npb, (0, 90))
 
 
@@ -211,3 +210,24 @@ def test_lengths_inside_a_shared_prefix(ctx, D):
     lens = [0, 1, 15, 16, 17, 100, 640, 641, 1023, 1024, 1025, 1100, 31, 32, 33, 999, 1024, 2]
     attn_case(ctx, len(lens), D, 2, 1, 16, 64, None, lens=lens)
     attn_case(ctx, 6, D, 16, 8, 16, 64, None, lens=lens[2:8], bad=0.2)
+
+
+@pytest.mark.parametrize("n,nq,gqa,npb,own", [
+    (40, 16, 2, 32, (0, 60)),              # 80 rows, keys shared
+    (63, 8, 1, 33, (0, 40)),               # 63 and 64 rows on the two sides of sharing
+    (64, 8, 1, 32, (0, 40)),
+    (32, 8, 1, 94, (0, 40)),               # 32 and 33 rows behind 1504 keys
+    (33, 8, 1, 94, (0, 40)),
+    (9, 16, 8, 130, (0, 50)),              # a last tile of 8 rows
+    (17, 64, 16, 64, (0, 30)),             # 272 rows
+])
+def test_shared_keys(ctx, n, nq, gqa, npb, own):
+    attn_case(ctx, n, 256, nq, gqa, 16, npb, own)
+
+
+@pytest.mark.parametrize("bad", [0.0, 0.2])
+def test_lengths_inside_a_prefix_of_many_rows(ctx, bad):
+    """72 rows of heads of 256 share keys of which they see none, a part or all; the others hold NaN."""
+    lens = [0, 1, 15, 16, 17, 100, 640, 641, 1023, 1024, 1025, 1100, 31, 32, 33, 999, 1024, 2]
+    attn_case(ctx, len(lens), 256, 16, 4, 16, 64, None, lens=lens, bad=bad)
+    attn_case(ctx, len(lens), 256, 16, 4, 4, 256, None, lens=lens[::-1], bad=bad)
