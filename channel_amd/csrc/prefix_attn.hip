@@ -112,6 +112,14 @@ __device__ __forceinline__ const float *cache_row(const PrefixAttn &a, const flo
     return slot == kBadSlot ? zero_row : cache + (size_t)slot * a.kv_dim + (size_t)kvh * D;
 }
 
+// The weight of a score against a reference: the exponent's rounding is that
+// of its distance to the reference, not of the score.  A score of -inf has the
+// weight zero; exp_lo, of either sign, would make its distance inf - inf.
+__device__ __forceinline__ float weight(const PrefixAttn &a, float s, float ref) {
+    const float e = fmaf(s, a.exp_hi, -ref);
+    return __builtin_amdgcn_exp2f(e == kNone ? e : fmaf(s, a.exp_lo, e));
+}
+
 // 16 query rows of a wave over 256 dims, on v_mfma_f32_16x16x4_f32.  Lane l =
 // 16 g + c.  Scores are formed transposed, S^T = K Q^T: as A operand lane l
 // holds key c's dims 16 s + 4 g + j (one 16-byte read per s), as B operand row
@@ -176,10 +184,9 @@ struct Rows {
             }
         }
         const float ref = m == kNone ? 0.0f : m;
-        // the exponent's rounding is that of its distance to the reference, not of the score
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float w = __builtin_amdgcn_exp2f(fmaf(s[i], a.exp_lo, fmaf(s[i], a.exp_hi, -ref)));
+            const float w = weight(a, s[i], ref);
             s[i] = seen(i) ? w : 0.0f;
         }
         l += (s[0] + s[1]) + (s[2] + s[3]);
@@ -348,8 +355,7 @@ struct Quads {
 #pragma unroll
             for (int x = 0; x < RQ; ++x) {
                 const float ref = m[x] == kNone ? 0.0f : m[x];
-                // the exponent's rounding is that of its distance to the reference, not of the score
-                const float w = __builtin_amdgcn_exp2f(fmaf(s[x], a.exp_lo, fmaf(s[x], a.exp_hi, -ref)));
+                const float w = weight(a, s[x], ref);
                 s[x] = seen(x) ? w : 0.0f;
                 l[x] += s[x];
             }
