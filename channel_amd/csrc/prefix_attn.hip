@@ -114,10 +114,16 @@ __device__ __forceinline__ const float *cache_row(const PrefixAttn &a, const flo
 
 // The weight of a score against a reference: the exponent's rounding is that
 // of its distance to the reference, not of the score.  A score of -inf has the
-// weight zero; exp_lo, of either sign, would make its distance inf - inf.
+// weight zero; exp_lo, of either sign, would make its distance inf - inf.  The
+// reference itself is a rounded product; from 2^24 on its half step passes a
+// power of two (and the exponential's range from 2^32 on), so there the
+// distance is that of the rounded products, zero for the largest.
 __device__ __forceinline__ float weight(const PrefixAttn &a, float s, float ref) {
-    const float e = fmaf(s, a.exp_hi, -ref);
-    return __builtin_amdgcn_exp2f(e == kNone ? e : fmaf(s, a.exp_lo, e));
+#pragma clang fp contract(off)
+    const float d = s * a.exp_hi - ref;
+    float e = fmaf(s, a.exp_hi, -ref);
+    e = e == kNone ? e : fmaf(s, a.exp_lo, e);
+    return __builtin_amdgcn_exp2f(fabsf(ref) < 16777216.0f ? e : d);
 }
 
 // 16 query rows of a wave over 256 dims, on v_mfma_f32_16x16x4_f32.  Lane l =

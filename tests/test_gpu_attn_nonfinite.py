@@ -108,3 +108,24 @@ def test_every_score_minus_infinity(ctx, path):
     a.q[..., 0] = 1.0
     a.k[:, ::a.D] = -np.inf
     assert not a.run(ctx).any()
+
+
+# scores of the j-th key: a (j + 1), exactly apart: rounding cannot change their order, and the next one lies a below
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("a_", [3e6, 1.37e8, 3.3e9, -7.7e9, 1.1e12, 2.9e20, -1.3e30, 1.7e35])
+def test_scores_far_beyond_the_exponential(ctx, path, a_):
+    """Finite scores of any size: the largest one's value, without overflow on the way."""
+    a = Attn(path, short=True)
+    a.q[:] = 0
+    a.q[..., 3] = a_
+    for r in range(a.n):
+        at = a.slots(r)
+        for h in range(a.nkv):
+            a.k[at, h * a.D + 3] = np.arange(1, len(at) + 1)
+    got = a.run(ctx)
+    for r in range(a.n):
+        at = a.slots(r)
+        best = at[-1] if a_ > 0 else at[0]
+        for h in range(a.nq):
+            want = a.v[best, h // a.gqa * a.D:(h // a.gqa + 1) * a.D]
+            assert np.abs(got[r, h] - want).max() <= 2 * (len(at) + 8) * U * np.abs(want).max(), (r, h)
