@@ -464,7 +464,9 @@ struct Quads {
     }
 
     // The four waves' sums of the n first rows joined: a row's sum of D
-    // values, reference and denominator as the partial result where(row).
+    // values, reference and denominator as the partial result where(row).  A
+    // wave without keys for a row is one whose denominator is zero: NaN scores
+    // do not move the reference, but the denominator.
     template <typename F>
     __device__ __forceinline__ void join(const PrefixAttn &a, float *sh, uint32_t n, F &&where) {
         const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, r = lane & 3;
@@ -481,12 +483,12 @@ struct Quads {
         for (int x = 0; x < RQ; ++x) {
             const float *mr = sm + 4 * x + r;
             const float M = fmaxf(fmaxf(mr[0], mr[R]), fmaxf(mr[2 * R], mr[3 * R]));
-            const float f = m[x] == kNone ? 0.0f : __builtin_amdgcn_exp2f(m[x] - M);
+            const float f = l[x] == 0.0f ? 0.0f : __builtin_amdgcn_exp2f(m[x] - M);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
                 if (4 * x + i >= (int)n) continue;
                 const float fr = lane_f(f, i);
-                const bool none = lane_f(m[x], i) == kNone;
+                const bool none = lane_f(l[x], i) == 0.0f;
 #pragma unroll
                 for (int h = 0; h < H; ++h)
                     *(f4a *)(so + (wave * R + 4 * x + i) * D + 256 * h + 4 * lane) =
@@ -499,8 +501,10 @@ struct Quads {
             const float M = fmaxf(fmaxf(mr[0], mr[R]), fmaxf(mr[2 * R], mr[3 * R]));
             float L = 0.0f;
 #pragma unroll
-            for (int y = 0; y < 4; ++y)
-                L += mr[y * R] == kNone ? 0.0f : sl[y * R + tid] * __builtin_amdgcn_exp2f(mr[y * R] - M);
+            for (int y = 0; y < 4; ++y) {
+                const float ly = sl[y * R + tid];
+                L += ly == 0.0f ? 0.0f : ly * __builtin_amdgcn_exp2f(mr[y * R] - M);
+            }
             const size_t at = where(tid);
             a.m[at] = M;
             a.l[at] = L;
@@ -814,10 +818,10 @@ __global__ __launch_bounds__(256) void k_prefix_join(PrefixAttn a) {
         float w = 0.0f, l = 0.0f;
         if ((uint32_t)lane < n) {
             const size_t i = at(p0 + lane);
-            const float m = a.m[i];
-            if (m != kNone) {
+            const float m = a.m[i], part = a.l[i];
+            if (part != 0.0f) {                                  // NaN: whatever its reference is
                 w = __builtin_amdgcn_exp2f(m - M);
-                l = w * a.l[i];
+                l = w * part;
             }
         }
         L += wave_sum64(l);

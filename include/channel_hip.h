@@ -594,7 +594,7 @@ int chn_batch_qkv_rope_at(chn_ctx *ctx, const float *q_in, const float *k_in, co
  * device; its first n_prefix_blocks entries are not read).  Softmax of scale
  * * q.k; a key whose score is -inf has no weight, and a request without tokens
  * (or with no other keys than those) gets zeros; scores beyond 2^127 count as
- * infinite.  A block id that is not below
+ * infinite, and a score of +inf or NaN makes its row NaN.  A block id that is not below
  * n_blocks takes its tokens out of the softmax; slots that no token occupies
  * are never used, whatever they hold.  Query head h reads KV head h /
  * gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; n_prefix_blocks <=

@@ -129,3 +129,44 @@ def test_scores_far_beyond_the_exponential(ctx, path, a_):
         for h in range(a.nq):
             want = a.v[best, h // a.gqa * a.D:(h // a.gqa + 1) * a.D]
             assert np.abs(got[r, h] - want).max() <= 2 * (len(at) + 8) * U * np.abs(want).max(), (r, h)
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_nan_query(ctx, path):
+    """A NaN in a head's query: that head's output is NaN, the others hold to the definition.  (Not bit for bit to a run
+    without it: the references of a wave's rows move together, when one of them must.  Weights
+    against another reference differ by a factor of the row, which the quotient takes out, and one rounding each, so both
+    runs lie within the bound.)"""
+    a = Attn(path, short=True)
+    bad = np.zeros((a.n, a.nq), bool)
+    bad[0, 1] = bad[a.n - 1, 0] = bad[1, a.nq - 1] = True
+    a.q[bad, 7] = np.nan
+    got = a.run(ctx)
+    assert np.isnan(got[bad]).all()
+    a.check(got, 1.0, ~bad)
+
+
+@pytest.mark.parametrize("path", PATHS)
+@pytest.mark.parametrize("first,last", [(0, 1), (0, 16), (16, 32), (0, 64), (64, 128), (5, 90), (0, 100000)])
+def test_nan_keys(ctx, path, first, last):
+    """NaN among the keys at positions first .. last - 1, a group of 16, a part of the work or all: whoever sees one
+    gets NaN, wherever the borders of the parts lie."""
+    a = Attn(path, short=True)
+    seen = np.zeros((a.n, a.nq), bool)
+    for r in (range(a.n) if a.npb else (1,)):                   # the prefix is everybody's
+        at = a.slots(r)[first:last]
+        a.k[at, a.D - 1] = np.nan                               # KV head 0
+        seen[r, :a.gqa] = len(at) > 0
+    got = a.run(ctx)
+    assert np.isnan(got[seen]).all()
+    a.check(got, 1.0, ~seen)
+
+
+@pytest.mark.parametrize("path", PATHS)
+def test_infinite_score(ctx, path):
+    """A score of +inf: inf - inf in the definition's softmax."""
+    a = Attn(path)
+    a.q[..., 0] = np.abs(a.q[..., 0]) + 0.1
+    a.k[a.slots(0)[-1], 0] = np.inf
+    got = a.run(ctx)
+    assert np.isnan(got[0, :a.gqa]).all() and np.isfinite(got[0, a.gqa:]).all()
