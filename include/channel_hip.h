@@ -557,12 +557,23 @@ int chn_model_replay(chn_model *m, int with_logits, uint32_t *topk_ids, float *t
  *    below n_blocks), clocks[row] its position in its sequence;
  *  - lens_out[r] = begin + n_new[r].
  * row_start has n_req + 1 entries, slots and clocks max_tokens.  status (3
- * device words): CHN_TABLES_* flags, taken + the blocks handed out (the next
- * call's `taken` may point at it), the number of rows.  With a flag set
- * nothing else is written; rows behind the last one, and table entries that
- * hold no token yet, are left as they were.  lens, n_new, taken, the prefix
- * and the free list must not overlap what is written (a loop alternates
- * between two sets of lens_out and status). */
+ * device words): CHN_TABLES_* flags, taken + the blocks that the new tokens
+ * open, the number of rows.  With a flag set nothing else is written and no
+ * block is handed out; rows behind the last one, and table entries that hold
+ * no token yet, are left as they were.  lens, n_new, taken, the prefix and the
+ * free list must not overlap what is written (a loop alternates between two
+ * sets of lens_out and status).
+ *
+ * What the rest of a step reads has to hold without a look at status: a
+ * refused call leaves the slots, clocks and lengths of an earlier step, and a
+ * step with a fixed number of rows (a recorded one) reads rows behind the last
+ * one.  So ahead of this call a step fills slots with CHN_NO_SLOT
+ * (chn_fill_u32) and copies lens to lens_out (chn_copy): rows that are not
+ * placed then write no K/V, and a refused step leaves lengths, tables and
+ * caches as they were and can be made again from the same lens and taken.  The
+ * next call's `taken` may point at status[1] of a call without flags only:
+ * read status before the next step, or enqueue no more steps ahead than are
+ * known to fit. */
 #define CHN_TABLES_NO_BLOCKS 1u     /* the free list has too few blocks     */
 #define CHN_TABLES_TOO_LONG 2u      /* a request outgrows max_blocks        */
 #define CHN_TABLES_TOO_MANY 4u      /* more rows than max_tokens            */
