@@ -522,8 +522,8 @@ int chn_model_read_logits(chn_model *m, float *logits_out);
 int chn_model_replay(chn_model *m, int with_logits, uint32_t *topk_ids, float *topk_vals);
 
 /* ======================================================================
- * Several sequences over one paged KV cache: one decode (or admission) step
- * of a batch of requests.  No reference counterpart: the reference decodes
+ * Several sequences over one paged KV cache: one decode step of a batch of
+ * requests.  No reference counterpart: the reference decodes
  * one sequence over its ring (src/ring_buffer.zig).  The caches are the ones
  * the entries above read and write, [slot][kv_dim] fp32, here of n_blocks
  * blocks of block_size consecutive slots (block b holds slots b * block_size
@@ -533,7 +533,14 @@ int chn_model_replay(chn_model *m, int with_logits, uint32_t *topk_ids, float *t
  * with the same prefix, a whole number of blocks that is held once.
  *
  * A step is chn_block_tables, then per layer chn_batch_qkv_rope_at and
- * chn_prefix_decode_attn, then chn_sample on the rows of logits.  All four
+ * chn_prefix_decode_attn, then chn_sample on the rows of logits.  The rows of
+ * the first two are the new tokens, packed by request; those of the other two
+ * are the requests.  They agree as far as every request takes exactly one
+ * token: requests that take none stand behind the others (or are left out of
+ * the batch), or row row_start[r + 1] - 1 of q_out is copied to row r
+ * (chn_copy) for each request that takes any.  The first two also place
+ * several tokens of a request (a prompt's K/V); of those, only the last one's
+ * attention is here.  All four
  * only enqueue on the context's stream, read their lengths, tables and
  * settings from device memory, and can be recorded (chn_record_begin).
  * Argument checks come first: called with ctx == NULL they report through
