@@ -852,6 +852,12 @@ __global__ __launch_bounds__(256) void k_prefix_join(PrefixAttn a) {
         *(f4a *)(a.out + (size_t)row * D + 4 * e) = ((sh[0][e] + sh[1][e]) + (sh[2][e] + sh[3][e])) * inv;
 }
 
+// Own items per KV head at most: no request has more than its table has room for (`slots` of them).
+static uint64_t most_own(uint32_t cap, uint32_t n_req, uint64_t slots) {
+    const uint64_t groups = (slots + 15) / 16;
+    return std::min<uint64_t>((uint64_t)cap + n_req, n_req * ((groups + kOwnMinGroups - 1) / kOwnMinGroups));
+}
+
 template <int D, int RQ, bool ROWS>
 static void launch_items(hipStream_t st, const PrefixAttn &a, uint32_t grid) {
     constexpr size_t lds = lds_bytes<D, RQ, ROWS>();
@@ -951,14 +957,18 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
         a.own_cap = std::max(1u, 2048 / a.num_kv);
         // two workgroups per CU, or one (of heads of 512 another is the prefix's, or fills the registers)
         a.own_fit = (head_dim == 256 || (!P && gqa_ratio <= 4) ? 512 : 256) / a.num_kv;
-        // no request has more items than its table has room for
-        const uint32_t groups = (uint32_t)((((uint64_t)(max_blocks - n_prefix_blocks) << a.shift) + 15) / 16);
-        items = std::min<uint64_t>(a.own_cap + n_req, (uint64_t)n_req * ((groups + kOwnMinGroups - 1) / kOwnMinGroups));
+        items = most_own(a.own_cap, n_req, (uint64_t)(max_blocks - n_prefix_blocks) << a.shift);
         grid += items * a.num_kv;
     }
     if (grid > 0x7FFFFFFF) return set_err(ctx, CHN_E_UNSUPPORTED, "too many requests and heads for one call");
     const size_t rows = ((size_t)a.splits * n_req + (size_t)items) * num_q_heads;
-    rc = ensure_workspace(ctx, rows * (head_dim + 2) * 4 + ((size_t)n_req + 1) * 4);
+    // What any call of these heads with no more requests and no wider tables needs, whatever its prefix, so that one at the
+    // largest size readies the workspace for recordings of all.  splits * n_req falls at every new tile of rows: splits <=
+    // 256 / (tiles * num_kv), tiles >= n_req * gqa / rows of a workgroup
+    const uint64_t prefix_parts = std::max<uint64_t>(
+        n_req, std::min<uint64_t>((uint64_t)n_req * (256 / a.num_kv), 256 * rows_wg(head_dim) / num_q_heads));
+    const uint64_t own_parts = most_own(std::max(1u, 2048 / a.num_kv), n_req, (uint64_t)max_blocks << a.shift);
+    rc = ensure_workspace(ctx, (size_t)(prefix_parts + own_parts) * num_q_heads * (head_dim + 2) * 4 + ((size_t)n_req + 1) * 4);
     if (rc) return rc;
     a.o = (float *)ctx->ws;
     a.m = a.o + rows * head_dim;

@@ -616,8 +616,10 @@ int chn_batch_qkv_rope_at(chn_ctx *ctx, const float *q_in, const float *k_in, co
  * n_blocks takes its tokens out of the softmax; slots that no token occupies
  * are never used, whatever they hold.  Query head h reads KV head h /
  * gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; n_prefix_blocks <=
- * max_blocks, max_blocks * block_size < 2^31.  Workspace: it grows with
- * n_req * num_q_heads * head_dim, not with the lengths. */
+ * max_blocks, max_blocks * block_size < 2^31.  Workspace: for given heads and
+ * block_size a call needs no more than one of as many or more requests and
+ * blocks per table, whatever their prefixes and lengths; it grows with n_req *
+ * num_q_heads * head_dim, not with the lengths. */
 int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
                            const uint32_t *prefix_blocks, uint32_t n_prefix_blocks, const uint32_t *tables,
                            const uint32_t *lens, uint32_t n_req, uint32_t max_blocks, uint32_t block_size,
