@@ -104,7 +104,8 @@ __global__ __launch_bounds__(kTabThreads) void k_block_tables(Tables a) {
         a.row_start[r] = row0[r];
         a.lens_out[r] = (uint32_t)(grow_of(a, a.lens[r], n).begin + n);
     }
-    for (uint32_t t = gid; t < (uint32_t)rows; t += nth) {
+    for (uint64_t t64 = gid; t64 < rows; t64 += nth) {      // up to 2^32 - 1 rows
+        const uint32_t t = (uint32_t)t64;
         uint32_t lo = 0, hi = a.n_req;                  // the last request whose first row is <= t
         while (hi - lo > 1) {
             const uint32_t mid = (lo + hi) / 2;
