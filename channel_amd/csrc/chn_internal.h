@@ -86,6 +86,9 @@ inline bool overlap(const Span &a, const Span &b) {
     return x && y && a.words && b.words && x < y + b.words * 4 && y < x + a.words * 4;
 }
 
+// Workgroups of 256 threads that one launch takes: fewer than 2^32 threads.
+constexpr uint64_t kMaxGrid256 = 0xFFFFFF;
+
 // The geometry of a paged cache: slots and token positions fit 32 bits.
 inline int check_blocks(chn_ctx *ctx, uint32_t block_size, uint32_t n_blocks, uint32_t max_blocks) {
     CHN_REQUIRE(ctx, block_size && block_size <= 1024 && !(block_size & (block_size - 1)),

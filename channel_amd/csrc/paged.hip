@@ -348,25 +348,25 @@ extern "C" int chn_batch_qkv_rope_at(chn_ctx *ctx, const float *q_in, const floa
                 rotary_dim);
     CHN_REQUIRE(ctx, theta > 0.0f && std::isfinite(theta), "theta must be positive and finite");
     CHN_REQUIRE(ctx, num_q_heads <= 65536 && num_kv_heads <= 65536, "too many heads");
-    const uint32_t groups = (num_q_heads + 2 * num_kv_heads + 3) / 4;
-    CHN_REQUIRE(ctx, (uint64_t)groups * n_tok <= 0x7FFFFFFFu, "%u tokens of %u heads are too many for one call", n_tok,
+    if (k_eq_v) v_in = k_in;
+    bool wide = (head_dim == 256 || head_dim == 512) && rotary_dim % 8 == 0;
+    for (const void *p : {(const void *)q_in, (const void *)k_in, (const void *)v_in, (const void *)q_norm_w,
+                          (const void *)k_norm_w, (const void *)q_out, (const void *)k_cache, (const void *)v_cache})
+        wide = wide && aligned(p, 16);
+    const uint32_t per = wide ? 8 : 4, groups = (num_q_heads + 2 * num_kv_heads + per - 1) / per;
+    CHN_REQUIRE(ctx, (uint64_t)groups * n_tok <= kMaxGrid256, "%u tokens of %u heads are too many for one call", n_tok,
                 num_q_heads);
     CHN_REQUIRE(ctx, ctx, "ctx is NULL");
     if (!n_tok || !groups) return CHN_OK;
     DeviceGuard dev(ctx);
-    const RopeAt a{q_in, k_in, k_eq_v ? k_in : v_in, q_norm_w, k_norm_w, q_out, k_cache, v_cache, clocks, slots,
-                   n_slots, num_q_heads, num_kv_heads, head_dim, rotary_dim, groups, std::log2((double)theta), eps};
-    bool wide = (head_dim == 256 || head_dim == 512) && rotary_dim % 8 == 0;
-    for (const void *p : {(const void *)q_in, (const void *)a.k_in, (const void *)a.v_in, (const void *)q_norm_w,
-                          (const void *)k_norm_w, (const void *)q_out, (const void *)k_cache, (const void *)v_cache})
-        wide = wide && aligned(p, 16);
+    const RopeAt a{q_in, k_in, v_in, q_norm_w, k_norm_w, q_out, k_cache, v_cache, clocks, slots, n_slots, num_q_heads,
+                   num_kv_heads, head_dim, rotary_dim, groups, std::log2((double)theta), eps};
+    const uint32_t grid = groups * n_tok;
     if (wide) {
-        RopeAt b = a;
-        b.groups = (num_q_heads + 2 * num_kv_heads + 7) / 8;
-        if (head_dim == 256) k_rope_at4<1><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
-        else k_rope_at4<2><<<b.groups * n_tok, 256, 0, ctx->stream>>>(b);
-    } else if (head_dim > 256) k_rope_at<8><<<groups * n_tok, 256, 0, ctx->stream>>>(a);
-    else k_rope_at<4><<<groups * n_tok, 256, 0, ctx->stream>>>(a);
+        if (head_dim == 256) k_rope_at4<1><<<grid, 256, 0, ctx->stream>>>(a);
+        else k_rope_at4<2><<<grid, 256, 0, ctx->stream>>>(a);
+    } else if (head_dim > 256) k_rope_at<8><<<grid, 256, 0, ctx->stream>>>(a);
+    else k_rope_at<4><<<grid, 256, 0, ctx->stream>>>(a);
     CHN_LAUNCHED(ctx, "k_rope_at");
     return CHN_OK;
 }

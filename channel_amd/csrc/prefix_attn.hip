@@ -904,6 +904,8 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
     if (rc) return rc;
     CHN_REQUIRE(ctx, n_prefix_blocks <= max_blocks, "%u prefix blocks in tables of %u", n_prefix_blocks, max_blocks);
     CHN_REQUIRE(ctx, n_req <= 65536, "n_req %u exceeds 65536", n_req);
+    if ((uint64_t)n_req * num_q_heads > kMaxGrid256)               // the joining launch's workgroups
+        return set_err(ctx, CHN_E_UNSUPPORTED, "%u requests of %u heads are too many for one call", n_req, num_q_heads);
     CHN_REQUIRE(ctx, ctx, "ctx is NULL");
     if (!n_req || !num_q_heads) return CHN_OK;
     DeviceGuard dev(ctx);
@@ -946,9 +948,8 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
         const uint32_t want = std::max(1u, 256 / std::max(1u, a.tiles * a.num_kv));
         a.split_keys = ((P + want - 1) / want + 63) / 64 * 64;
         a.splits = (P + a.split_keys - 1) / a.split_keys;
-        const uint64_t wgs = (uint64_t)(a.num_kv * a.splits + 7) / 8 * 8 * a.tiles;
-        if (wgs > 0x7FFFFFFF) return set_err(ctx, CHN_E_UNSUPPORTED, "too many query rows for one call");
-        a.prefix_wgs = (uint32_t)wgs;
+        // about 256, or below 2^21: 2^24 rows by at least 32 (quads only where rows times keys are few)
+        a.prefix_wgs = (a.num_kv * a.splits + 7) / 8 * 8 * a.tiles;
     }
     uint64_t grid = a.prefix_wgs, items = 0;
     if (max_blocks > n_prefix_blocks) {
@@ -960,7 +961,7 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
         items = most_own(a.own_cap, n_req, (uint64_t)(max_blocks - n_prefix_blocks) << a.shift);
         grid += items * a.num_kv;
     }
-    if (grid > 0x7FFFFFFF) return set_err(ctx, CHN_E_UNSUPPORTED, "too many requests and heads for one call");
+    if (grid > kMaxGrid256) return set_err(ctx, CHN_E_UNSUPPORTED, "too many requests and heads for one call");
     const size_t rows = ((size_t)a.splits * n_req + (size_t)items) * num_q_heads;
     // What any call of these heads with no more requests and no wider tables needs, whatever its prefix, so that one at the
     // largest size readies the workspace for recordings of all.  splits * n_req falls at every new tile of rows: splits <=

@@ -597,7 +597,8 @@ int chn_block_tables(chn_ctx *ctx, const uint32_t *lens, const uint32_t *n_new, 
  * The angle clock * theta^(-2d / rotary_dim) is formed and reduced in 64
  * bits, so far positions keep fp32 accuracy (chn_batch_qkv_rope forms it in
  * fp32 as the reference does).  Two tokens with one slot: either's values,
- * element by element. */
+ * element by element.  A call takes at most (2^24 - 1) / ceil((num_q_heads + 2
+ * * num_kv_heads) / 4) tokens. */
 int chn_batch_qkv_rope_at(chn_ctx *ctx, const float *q_in, const float *k_in, const float *v_in,
                           const float *q_norm_w, const float *k_norm_w, float *q_out, float *k_cache,
                           float *v_cache, const uint32_t *clocks, const uint32_t *slots, uint32_t n_tok,
@@ -615,7 +616,8 @@ int chn_batch_qkv_rope_at(chn_ctx *ctx, const float *q_in, const float *k_in, co
  * infinite, and a score of +inf or NaN makes its row NaN.  A block id that is not below
  * n_blocks takes its tokens out of the softmax; slots that no token occupies
  * are never used, whatever they hold.  Query head h reads KV head h /
- * gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; n_prefix_blocks <=
+ * gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; n_req <= 65536, n_req
+ * * num_q_heads < 2^24 (with gqa_ratio 1 < 2^24 - 2^21); n_prefix_blocks <=
  * max_blocks, max_blocks * block_size < 2^31.  Workspace: for given heads and
  * block_size a call needs no more than one of as many or more requests and
  * blocks per table, whatever their prefixes and lengths; it grows with n_req *
