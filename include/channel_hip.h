@@ -613,10 +613,12 @@ int chn_batch_qkv_rope_at(chn_ctx *ctx, const float *q_in, const float *k_in, co
  * device; its first n_prefix_blocks entries are not read).  Softmax of scale
  * * q.k; a key whose score is -inf has no weight, and a request without tokens
  * (or with no other keys than those) gets zeros; scores beyond 2^127 count as
- * infinite, and a score of +inf or NaN makes its row NaN.  A block id that is not below
- * n_blocks takes its tokens out of the softmax; slots that no token occupies
- * are never used, whatever they hold.  Query head h reads KV head h /
- * gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; n_req <= 65536, n_req
+ * infinite, and a score of +inf or NaN makes its row NaN.  A block id that is
+ * not below n_blocks takes its tokens out of the softmax; slots that no token
+ * occupies are never used, whatever they hold.  There is no window: for a
+ * sliding layer the result is its own only while a request is no longer than
+ * the layer's window (tables and lengths of the window's blocks alone begin it
+ * at a block's first token).  Query head h reads KV head h / gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; n_req <= 65536, n_req
  * * num_q_heads < 2^24 (with gqa_ratio 1 < 2^24 - 2^21); n_prefix_blocks <=
  * max_blocks, max_blocks * block_size < 2^31.  Workspace: for given heads and
  * block_size a call needs no more than one of as many or more requests and
