@@ -147,7 +147,8 @@ struct RopeAt {
 
 // (cos, sin) of clock * theta^(-2d / rot): the turns are formed in 64 bits
 // and only their fraction is rounded to 32, so the angle is off by 2^-25 of a
-// half turn at any clock.
+// half turn (the turns' own roundings, 2^-51 or so of at most clock / 6.28,
+// reach that at clocks of 2^28, and 2^-22 at the last).
 __device__ __forceinline__ float2 rope_angle(const RopeAt &a, uint32_t clock, uint32_t d) {
     const double freq = exp2(-(2.0 * d / a.rot) * a.log2_theta);
     const double turns = (double)clock * freq * 0.15915494309189535;      // 1 / (2 pi)
@@ -161,6 +162,9 @@ __device__ __forceinline__ float2 rope_angle(const RopeAt &a, uint32_t clock, ui
 // unit RMSNorm for V.  Any head_dim up to 64 * DPL, any even rot, any
 // alignment.  A workgroup takes four rows of one token, one per wave; the
 // token's angles are evaluated once, one per thread, and handed round in LDS.
+// 1500 tokens of 16 and 8 heads of 128: 18 us (49 MB, 10 at a copy's rate); of
+// 256 with 100 of them rotated 27 (the form below: 20), of 16 and 4 heads of 512
+// with 500 38 (30): loads of 4 bytes, one row per wave, angles for four rows.
 template <int DPL>
 __global__ __launch_bounds__(256) void k_rope_at(RopeAt a) {
     __shared__ float2 cs[256];

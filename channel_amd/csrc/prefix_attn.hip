@@ -23,12 +23,13 @@
 // memory bounds it).
 //
 // Measured (fp32, one decode step, both launches): 8 requests of up to 96
-// tokens behind 512, heads of 256: 14 us, most of it the two launches and
+// tokens behind 512, heads of 256: 13 us, most of it the two launches and
 // the block-table, key, weight and join latencies one after another.  64
-// requests of up to 480 tokens behind 3968: 80 us; the prefix alone takes 59 (27
+// requests of up to 480 tokens behind 3968: 78 us; the prefix alone takes 57 (28
 // at the matrix rate), the requests' own keys share the chip with it.  33
-// requests of up to 333 behind 1488, heads of 512: 43 us.  12 requests
-// of up to 20000 tokens, no prefix: 206 us, 6.2 TB/s.
+// requests of up to 333 behind 1488, heads of 512: 44 us, the prefix alone 38.
+// 12 requests of up to 20000 tokens, no prefix: 135 us where the lengths drawn
+// come to 0.81 GB, 277 where to 1.77: 6.0 to 6.4 TB/s.
 #include "chn_internal.h"
 
 #include <cmath>
@@ -200,8 +201,7 @@ struct Rows {
     }
     // Weights times V of a group that some row sees a part of, key by key: a
     // weight of zero does not keep an infinity or NaN of an unseen V row out
-    // of a product, so that row is left out.  v(k): key k's V row, or NULL
-    // (the same for the whole wave).
+    // of a product, so that row is left out.  v(k): key k's V row.
     template <typename F>
     __device__ __forceinline__ void weigh_part(const f4a &s, uint32_t kb, F &&v) {
         const int lane = threadIdx.x & 63, g = lane >> 4, c = lane & 15;
@@ -217,7 +217,6 @@ struct Rows {
                 float p[4];
 #pragma unroll
                 for (int i = 0; i < 4; ++i) p[i] = __shfl(s[ki], 16 * kg + 4 * g + i, 64);
-                if (!row) continue;
 #pragma unroll
                 for (int n = 0; n < 4; ++n) {
                     const f4a x = *(const f4a *)(row + 64 * n + 4 * c);
@@ -869,7 +868,8 @@ template <int D>
 static int launch_prefix(chn_ctx *ctx, const PrefixAttn &a, uint32_t grid, bool rows) {
     if (grid) {
         // as few quads as the heads of a group need: 12 requests of up to 20000 tokens with 8 query heads to each of 2 KV
-        // heads take 75 us with two and 94 with four, heads of 512 153 and 180
+        // heads take 72 us with two and 90 with four, heads of 512 148 and 178.  With four the registers do not hold all
+        // (15 to 21 spill): 16 query heads to one KV head of 256 take 61 us for 164 MB, 34 at a copy's rate
         if (a.gqa <= 4) rows ? launch_items<D, 1, true>(ctx->stream, a, grid) : launch_items<D, 1, false>(ctx->stream, a, grid);
         else if (a.gqa <= 8) rows ? launch_items<D, 2, true>(ctx->stream, a, grid) : launch_items<D, 2, false>(ctx->stream, a, grid);
         else rows ? launch_items<D, 4, true>(ctx->stream, a, grid) : launch_items<D, 4, false>(ctx->stream, a, grid);
@@ -944,7 +944,8 @@ extern "C" int chn_prefix_decode_attn(chn_ctx *ctx, const float *q, const float 
         const uint32_t R = by_rows ? rows_wg(head_dim) : 4 * a.quads;
         a.tiles = (M + R - 1) / R;
         // about one workgroup per CU, 64 keys (16 per wave) at least.  128 rows on 3968 keys with own tokens beside them:
-        // 122 us with half as many workgroups, 94 so, 106 with twice as many (and twice the partial results)
+        // 99 us with half as many workgroups, 78 so, 95 with twice as many (and twice the partial results); 132 rows of
+        // heads of 512 on 1488 keys 64, 44 and 62
         const uint32_t want = std::max(1u, 256 / std::max(1u, a.tiles * a.num_kv));
         a.split_keys = ((P + want - 1) / want + 63) / 64 * 64;
         a.splits = (P + a.split_keys - 1) / a.split_keys;

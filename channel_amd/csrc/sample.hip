@@ -29,10 +29,13 @@
 //
 // Measured: one row of 262144 with top-k 64 and top-p: 18 us, of which the
 // draw's single workgroup takes 11, step after step.  32 rows of 32 users,
-// softcapped: 50 us.  128 rows (134 MB) by top-p: 130 us; the first pass takes
+// softcapped: 49 us.  128 rows (134 MB) by top-p: 130 us; the first pass takes
 // 28 (4.7 TB/s), the second and third are bound by issuing their 64-bit
-// arithmetic (the second 53, 38 without it).  50 rows of 10007 in one launch:
-// 25 us.
+// arithmetic (the second 51, 38 without it).  50 rows of 10007 in one launch:
+// 25 us.  The walk costs a pass over the row by one workgroup for every round:
+// a row of 262144 with top-k 1025 takes 213 us (1024: 91), with top-k 5000 and
+// top-p 424, by top-p over equal values or quarters 715 to 720 (distinct ones:
+// 29); 32 such rows 296, 517 and 808 to 835.
 #include "chn_internal.h"
 
 #include <cmath>
@@ -350,7 +353,7 @@ __global__ __launch_bounds__(kPassThreads) void k_sample_mass(Sample a) {
 // there.  All threads; sh: 20 words.
 template <bool CAP>
 __device__ __forceinline__ uint32_t border_bin(const Sample &a, const Row<CAP> &r, uint32_t row, uint64_t *sh, uint64_t &rest) {
-    const uint32_t tid = threadIdx.x, nt = blockDim.x, per = kBins / nt;       // 256 or 1024 threads: 8 or 2 bins
+    const uint32_t tid = threadIdx.x, nt = blockDim.x, per = kBins / nt;       // 512 or 1024 threads: 4 or 2 bins
     const int lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), nw = nt >> 6;
     const uint64_t *h = a.hist + (size_t)row * kBins + tid * per;
     uint64_t own = 0;
@@ -593,10 +596,13 @@ __device__ __forceinline__ void draw_listed(const Row<CAP> &r, Group &sh, uint64
 
 // Rows of up to kSmallV: one launch, a workgroup per row, which holds the row in
 // registers (thread t: values J t .. J t + J - 1; J as few as V needs: 50 rows
-// of 10007 took 33 us with J = 12 and 38 with 16).  One workgroup's steps are
+// of 10007 take 25 us with J = 12 and 35 with 16).  One workgroup's steps are
 // latency after latency, but fewer than those of four launches: 50 rows of
-// 10007 25 us and 49, one of 16000 with top-k 14 and 19; 20 rows of 16000 by
-// top-p 30 and 28, and above that no registers are left.
+// 10007 25 us and 47; one and 128 rows of 16000 with top-k 14 and 17 against 18
+// and 20.  By top-p alone, which only the device knows of a row, it is nearly
+// even there: 1, 20, 50 and 128 rows of 16000 28.5, 30, 30.5 and 32 us against
+// 26, 28.5, 31 and 33.  J = 16 spills already (26 registers, softcapped 54), and
+// with more values the rows would not stay in registers.
 constexpr uint32_t kSmallV = 16 * kDrawThreads;
 template <int J, bool CAP>
 __global__ __launch_bounds__(kDrawThreads) void k_sample_small(Sample a) {
