@@ -104,6 +104,10 @@ PROTOTYPES = {
     "chn_batch_qkv_rope_at": (c_int, [c_void_p] + [c_void_p] * 10 + [c_u32] * 6 + [c_int, c_f32, c_f32]),
     "chn_prefix_decode_attn": (c_int, [c_void_p] * 5 + [c_u32] + [c_void_p] * 2 + [c_u32] * 8 + [c_f32, c_void_p]),
     "chn_sample": (c_int, [c_void_p] * 2 + [c_u32] * 3 + [c_void_p] * 5 + [c_f32] + [c_void_p] * 2),
+    "chn_draft_trees": (c_int, [c_void_p] * 4 + [c_u32] * 3 + [c_void_p] * 2),
+    "chn_paged_causal_attn": (c_int, [c_void_p] * 7 + [c_u32] * 9 + [c_f32, c_u32, c_void_p]),
+    "chn_paged_tree_attn": (c_int, [c_void_p] * 8 + [c_u32] * 10 + [c_f32, c_u32, c_void_p]),
+    "chn_token_logprobs": (c_int, [c_void_p] * 2 + [c_u32] * 3 + [c_void_p] * 2 + [c_f32, c_u32] + [c_void_p] * 5),
     "chn_synth_q4": (c_int, [c_void_p, c_void_p, c_u32, c_u32, c_u64, c_f32, c_f32]),
     "chn_synth_q8": (c_int, [c_void_p, c_void_p, c_u32, c_u32, c_u64, c_f32, c_f32]),
     "chn_synth_normal": (c_int, [c_void_p, c_void_p, c_size, c_u64, c_f32]),

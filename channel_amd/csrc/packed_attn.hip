@@ -1,0 +1,528 @@
+// Attention of several tokens per request over a paged KV cache: packed
+// prompts, causal (chn_paged_causal_attn), and trees of drafted tokens
+// (chn_paged_tree_attn); and the trees' masks and clocks (chn_draft_trees).
+//
+// Work is a list of tiles: (request, KV head, a stretch of the request's new
+// tokens with all query heads of the KV head).  Laid end to end - a tile as
+// long as the keys it walks and a constant for its beginning and end - they
+// are cut into equal shares, one per workgroup, wherever a cut falls: a tile
+// that is cut leaves parts (the sums, their reference and denominator per
+// row), which a second launch joins.  Every workgroup finds its share itself
+// from the lengths, so nothing is planned on the host and no workgroup waits
+// for another.
+#include "chn_internal.h"
+
+#include <cmath>
+
+namespace chn {
+
+typedef float f4q __attribute__((ext_vector_type(4)));
+
+constexpr uint32_t kPackedRequests = 8192;
+constexpr uint32_t kPackedRows = 1u << 24;
+constexpr uint32_t kMaskWords = 8;          // drafted tokens of a request: 256
+constexpr uint32_t kShares = 256;           // workgroups: one per CU
+constexpr int kThreads = 512;
+// Units are keys.  A tile costs kTileCost besides its keys; a share has kLeastShare units or more, and a cut that
+// would fall within kTileCost of a tile's end is moved there.
+constexpr int64_t kTileCost = 64, kLeastShare = 192;
+constexpr float kNoScore = -__builtin_inff();
+
+// Rows of a tile: tokens x query heads of the KV head.
+constexpr uint32_t tile_rows(uint32_t D) { return D == 256 ? 128 : 64; }
+
+// A tile whose last part a workgroup made: the join's work.
+struct Joined {
+    uint32_t first, last;      // the shares that made its parts
+    uint32_t row, rows, kvh;   // the tile's first batch row, its rows (0: no such tile)
+};
+
+struct Packed {
+    const float *q, *kc, *vc;
+    const uint32_t *tables, *row_start, *lens, *masks;
+    uint32_t mask_words;       // 0: causal
+    uint32_t n_req, n_rows, max_blocks, shift, n_blocks, num_q, num_kv, kv_dim, gqa, tokens;   // tokens per tile
+    int window;
+    float c, sign;             // |scale| log2(e), the scale's sign
+    float *out;
+    float *po, *pm, *pl;       // parts: [2 * kShares][rows of a tile](D sums, divided by the denominator; reference; denominator)
+    Joined *joined;
+};
+
+// The new tokens of request r: batch rows row .. row + n - 1, at positions
+// have .. of len.  Row starts that are no sum of counts give other rows, none
+// outside the batch.
+struct Seq {
+    uint32_t row;
+    int n, have, len;
+};
+__device__ __forceinline__ Seq seq_of(const Packed &a, uint32_t r) {
+    const uint32_t s = min(a.row_start[r], a.n_rows), e = min(a.row_start[r + 1], a.n_rows);
+    Seq q;
+    q.row = s;
+    q.n = e > s ? (int)(e - s) : 0;
+    q.len = (int)min(a.lens[r], a.max_blocks << a.shift);
+    q.have = q.len - q.n;
+    return q;
+}
+
+// What the tiles of a request and KV head cost: tile t walks keys lo(t) ..
+// hi(t) - 1, both linear in t (the last tile's end is the work's, not the
+// cost's, matter).
+struct TileKeys {
+    int64_t tiles, T, hi0, lo0;        // hi = hi0 + t T, lo = max(0, lo0 + t T); T is 0 where all tiles see the same keys
+    __device__ __forceinline__ TileKeys(const Packed &a, const Seq &s) {
+        tiles = (s.n + (int64_t)a.tokens - 1) / a.tokens;
+        if (a.mask_words) {
+            T = 0;
+            hi0 = max(0, min(s.len, s.have + (int)(32 * a.mask_words)));
+            lo0 = a.window ? min(max(0, s.have - a.window), (int)hi0) : 0;
+        } else {
+            T = a.tokens;
+            hi0 = max(s.have, 0) + T;
+            lo0 = a.window ? (int64_t)s.have + 1 - a.window : -(tiles + 1) * T;
+        }
+    }
+    __device__ __forceinline__ int64_t hi(int64_t t) const { return hi0 + t * T; }
+    __device__ __forceinline__ int64_t lo(int64_t t) const { return max((int64_t)0, lo0 + t * T); }
+    __device__ __forceinline__ int64_t cost(int64_t t) const { return kTileCost + hi(t) - lo(t); }
+    // of all tiles before t
+    __device__ __forceinline__ int64_t before(int64_t t) const {
+        int64_t sum = t * (kTileCost + hi0) + T * (t * (t - 1) / 2);
+        if (!T) return sum - t * max((int64_t)0, lo0);
+        const int64_t s0 = lo0 > 0 ? 0 : -lo0 / T + 1;      // the first tile whose lo is above 0
+        if (t > s0) sum -= (t - s0) * lo0 + T * ((t - s0) * (s0 + t - 1) / 2);
+        return sum;
+    }
+};
+__device__ __forceinline__ int64_t snapped(int64_t at, int64_t cost) {
+    return at < kTileCost ? 0 : (at + kTileCost > cost ? cost : at);
+}
+
+// One tile's share: rows, and keys key0 .. key1 - 1 (key0 a multiple of 32).
+struct Work {
+    Seq s;
+    const uint32_t *table;
+    uint32_t kvh, tile_row, rows;      // the tile's first batch row; rows (tokens x heads)
+    int token, key0, key1, limit;      // its first token's index; limit: keys from here on are nobody's
+    int part;                          // -1: the whole tile
+};
+
+// What a row sees: cached keys lo .. hi - 1, and by its mask drafted ones.
+struct Seen {
+    int lo, hi;
+    const uint32_t *mask;
+};
+__device__ __forceinline__ Seen seen_by(const Packed &a, const Work &w, int token) {
+    Seen s;
+    s.mask = nullptr;
+    if (a.mask_words) {
+        s.mask = a.masks + (size_t)(w.s.row + token) * a.mask_words;
+        s.hi = max(w.s.have, 0);
+        s.lo = 0;
+        if (a.window) {
+            int ones = 0;
+            for (uint32_t i = 0; i < a.mask_words; ++i) ones += __popc(s.mask[i]);
+            s.lo = max(0, w.s.have + ones - a.window);
+        }
+    } else {
+        s.hi = w.s.have + token + 1;
+        s.lo = a.window ? max(0, s.hi - a.window) : 0;
+    }
+    return s;
+}
+
+__device__ __forceinline__ uint32_t slot_of(const Packed &a, const uint32_t *table, uint32_t pos) {
+    const uint32_t b = table[pos >> a.shift];
+    return b < a.n_blocks ? (b << a.shift) + (pos & ((1u << a.shift) - 1)) : CHN_NO_SLOT;
+}
+
+// A row's result, in lane's dims 4 lane + 256 k .. + 3: to the batch's row, or as a part.
+template <int D>
+__device__ __forceinline__ float *row_out(const Packed &a, const Work &w, uint32_t row) {
+    if (w.part >= 0) return a.po + ((size_t)w.part * tile_rows(D) + row) * D;
+    return a.out + ((size_t)(w.tile_row + row / a.gqa) * a.num_q + w.kvh * a.gqa + row % a.gqa) * D;
+}
+
+// A row per wave, a key at a time, in plain fp32: what any scores and values
+// do, infinities and NaN among them.
+template <int D>
+__device__ __noinline__ void rows_plain(const Packed &a, const Work &w) {
+    constexpr int N = D / 256;
+    const int lane = threadIdx.x & 63;
+    for (uint32_t row = threadIdx.x >> 6; row < w.rows; row += kThreads / 64) {
+        const int token = w.token + (int)(row / a.gqa);
+        const Seen s = seen_by(a, w, token);
+        const float *qr = a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + row % a.gqa) * D;
+        f4q q[N], o[N];
+        for (int k = 0; k < N; ++k) {
+            q[k] = *(const f4q *)(qr + 4 * lane + 256 * k) * a.sign;
+            o[k] = f4q{0, 0, 0, 0};
+        }
+        float m = kNoScore, l = 0.0f;
+        for (int pos = w.key0; pos < w.key1; ++pos) {
+            bool ok = pos >= s.lo && pos < s.hi;
+            const int node = pos - w.s.have;
+            if (s.mask && node >= 0) ok = (s.mask[node >> 5] >> (node & 31)) & 1;      // key1 is below 32 mask_words of them
+            const uint32_t slot = ok ? slot_of(a, w.table, pos) : CHN_NO_SLOT;
+            if (slot == CHN_NO_SLOT) continue;
+            const size_t at = (size_t)slot * a.kv_dim + (size_t)w.kvh * D + 4 * lane;
+            float sum = 0.0f;
+            for (int k = 0; k < N; ++k) {
+                const f4q x = *(const f4q *)(a.kc + at + 256 * k);
+                for (int e = 0; e < 4; ++e) sum = fmaf(x[e], q[k][e], sum);
+            }
+            sum = wave_sum64(sum);
+            const float top = fmaxf(m, sum), ref = top == kNoScore ? 0.0f : top;
+            const float old = __builtin_amdgcn_exp2f((m - ref) * a.c), p = __builtin_amdgcn_exp2f((sum - ref) * a.c);
+            const bool none = sum == kNoScore;                                       // no weight, whatever its V
+            m = top;
+            l = none ? l : l * old + p;
+            for (int k = 0; k < N; ++k) {
+                const f4q x = *(const f4q *)(a.vc + at + 256 * k);
+                if (!none) o[k] = o[k] * old + p * x;
+            }
+        }
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        float *to = row_out<D>(a, w, row);
+        for (int k = 0; k < N; ++k) *(f4q *)(to + 4 * lane + 256 * k) = o[k] * inv;
+        if (w.part >= 0 && lane == 0) {
+            a.pm[(size_t)w.part * tile_rows(D) + row] = m;
+            a.pl[(size_t)w.part * tile_rows(D) + row] = l;
+        }
+    }
+}
+
+// The workgroup's share: f(work) for each of its tiles or parts of tiles.
+template <int D, typename F>
+__device__ __forceinline__ void each_work(const Packed &a, F &&f) {
+    __shared__ int64_t sums[kThreads / 64];
+    __shared__ int64_t found_base;
+    __shared__ uint32_t found;
+    const uint32_t tid = threadIdx.x, per = (a.n_req + kThreads - 1) / kThreads;
+    const int lane = tid & 63, wave = tid >> 6;
+    // every request's units; a thread sums its neighbours
+    const uint32_t r0 = min(tid * per, a.n_req), r1 = min(r0 + per, a.n_req);
+    int64_t mine = 0;
+    for (uint32_t r = r0; r < r1; ++r) {
+        const TileKeys s(a, seq_of(a, r));
+        mine += s.before(s.tiles) * a.num_kv;
+    }
+    const int64_t upto = (int64_t)wave_scan_u64((uint64_t)mine);
+    if (lane == 63) sums[wave] = upto;
+    if (tid == 0) found = 0xFFFFFFFFu;
+    __syncthreads();
+    int64_t total = 0, base = upto - mine;
+    for (int i = 0; i < kThreads / 64; ++i) {
+        base += i < wave ? sums[i] : 0;
+        total += sums[i];
+    }
+    // neighbouring shares, which read the same keys, run on one XCD (workgroup i on XCD i % 8)
+    const uint32_t n = (uint32_t)max((int64_t)1, min((int64_t)kShares, total / kLeastShare)), each = (n + 7) / 8;
+    const uint32_t share = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    const bool some = (blockIdx.x >> 3) < each && share < n;
+    const auto cut = [&](uint32_t w) { return total / n * w + total % n * w / n; };
+    if (tid == 0) a.joined[blockIdx.x].rows = 0;      // of share `share`, or of none
+    if (!some) return;                                // the whole workgroup
+    const int64_t u0 = cut(share), u1 = cut(share + 1);
+    if (u0 >= base && u0 < base + mine) {             // one thread, or none
+        uint32_t r = r0;
+        for (; r + 1 < r1; ++r) {
+            const TileKeys s(a, seq_of(a, r));
+            const int64_t units = s.before(s.tiles) * a.num_kv;
+            if (u0 < base + units) break;
+            base += units;
+        }
+        found = r;
+        found_base = base;
+    }
+    __syncthreads();
+    uint32_t r = __builtin_amdgcn_readfirstlane(found);
+    if (r >= a.n_req) return;
+    Seq s = seq_of(a, r);
+    TileKeys sp(a, s);
+    int64_t rbase = found_base, head = sp.before(sp.tiles);       // of the request; units of one KV head
+    uint32_t kvh = (uint32_t)((u0 - rbase) / head);
+    int64_t t = 0;
+    {
+        const int64_t in = (u0 - rbase) - kvh * head;
+        int64_t lo = 0, hi = sp.tiles;                // before(lo) <= in < before(hi)
+        while (hi - lo > 1) {
+            const int64_t mid = (lo + hi) / 2;
+            if (sp.before(mid) <= in) lo = mid;
+            else hi = mid;
+        }
+        t = lo;
+    }
+    int64_t u = rbase + kvh * head + sp.before(t);
+    while (u < u1) {
+        const int64_t cost = sp.cost(t);
+        const int64_t from = u < u0 ? snapped(u0 - u, cost) : 0, to = u1 - u < cost ? snapped(u1 - u, cost) : cost;
+        if (from < to) {
+            Work w;
+            w.s = s;
+            w.table = a.tables + (size_t)r * a.max_blocks;
+            w.kvh = kvh;
+            w.token = (int)(t * a.tokens);
+            w.tile_row = s.row + w.token;
+            const int tokens = min(s.n - w.token, (int)a.tokens);
+            w.rows = (uint32_t)tokens * a.gqa;
+            const int lo = (int)sp.lo(t);
+            w.limit = a.mask_words ? (int)sp.hi(t) : max(0, s.have + w.token + tokens);
+            // cuts at whole chunks of 32 keys
+            w.key0 = from ? (int)((lo + (from - kTileCost / 2) + 31) / 32 * 32) : lo / 32 * 32;
+            w.key1 = to < cost ? min((int)((lo + (to - kTileCost / 2) + 31) / 32 * 32), w.limit) : w.limit;
+            w.part = from ? 2 * share : (to < cost ? 2 * share + 1 : -1);
+            if (from && to == cost && tid == 0) {
+                // the share that begins this tile: the last whose first cut is at or before it
+                uint32_t first = share;
+                while (first && cut(first) > u && snapped(cut(first) - u, cost)) --first;
+                a.joined[blockIdx.x] = Joined{first, share, w.tile_row, w.rows, kvh};
+            }
+            f(w);
+        }
+        u += cost;
+        if (++t < sp.tiles) continue;
+        t = 0;
+        if (++kvh < a.num_kv) continue;
+        kvh = 0;
+        // the next request that takes tokens: 64 looked at together
+        for (++r; r < a.n_req; r += 64) {
+            const uint64_t takes = __ballot(r + lane < a.n_req && seq_of(a, min(r + lane, a.n_req - 1)).n > 0);
+            if (takes) {
+                r += __builtin_ctzll(takes);
+                break;
+            }
+        }
+        if (r >= a.n_req) break;
+        s = seq_of(a, r);
+        sp = TileKeys(a, s);
+    }
+}
+
+template <int D>
+__global__ __launch_bounds__(kThreads) void k_packed_attn(Packed a) {
+    each_work<D>(a, [&](const Work &w) { rows_plain<D>(a, w); });
+}
+
+// Joins the parts of the tiles that were cut: a wave takes a row at a time, a
+// lane four values per 256 dims.
+constexpr uint32_t kJoinRows = 16;
+template <int D>
+__global__ __launch_bounds__(256) void k_packed_join(Packed a) {
+    constexpr uint32_t R = tile_rows(D);
+    constexpr int N = D / 256;
+    const int lane = threadIdx.x & 63;
+    const Joined j = a.joined[blockIdx.x / (R / kJoinRows)];
+    const uint32_t row0 = blockIdx.x % (R / kJoinRows) * kJoinRows;
+    for (uint32_t row = row0 + (threadIdx.x >> 6); row < min(row0 + kJoinRows, j.rows); row += 4) {
+        // the first part is its share's last tile, the others are their shares' first
+        const auto at = [&](uint32_t p) { return (size_t)(p == j.first ? 2 * p + 1 : 2 * p) * R + row; };
+        float M = kNoScore;
+        for (uint32_t p = j.first + lane; p <= j.last; p += 64) M = fmaxf(M, a.pm[at(p)]);
+        M = wave_max64(M);
+        const float ref = M == kNoScore ? 0.0f : M;
+        float L = 0.0f;
+        f4q o[N];
+        for (int k = 0; k < N; ++k) o[k] = f4q{0, 0, 0, 0};
+        for (uint32_t p0 = j.first; p0 <= j.last; p0 += 64) {
+            const uint32_t n = min(j.last + 1 - p0, 64u);
+            float w = 0.0f;
+            if ((uint32_t)lane < n) {
+                const size_t i = at(p0 + lane);
+                const float part = a.pl[i];
+                if (part != 0.0f) w = __builtin_amdgcn_exp2f((a.pm[i] - ref) * a.c) * part;      // NaN: whatever its reference is
+            }
+            L += wave_sum64(w);
+            for (uint32_t i = 0; i < n; ++i) {
+                const float wi = lane_f(w, i);
+                const float *v = a.po + at(p0 + i) * D + 4 * lane;
+#pragma unroll
+                for (int k = 0; k < N; ++k) {
+                    const f4q x = *(const f4q *)(v + 256 * k);
+                    if (wi != 0.0f) o[k] += wi * x;                // a part without keys holds nothing
+                }
+            }
+        }
+        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+        float *to = a.out + ((size_t)(j.row + row / a.gqa) * a.num_q + j.kvh * a.gqa + row % a.gqa) * D + 4 * lane;
+#pragma unroll
+        for (int k = 0; k < N; ++k) *(f4q *)(to + 256 * k) = o[k] * inv;
+    }
+}
+
+template <int D>
+static int launch_packed(chn_ctx *ctx, const Packed &a) {
+    k_packed_attn<D><<<kShares, kThreads, 0, ctx->stream>>>(a);
+    CHN_LAUNCHED(ctx, "k_packed_attn");
+    k_packed_join<D><<<kShares * (tile_rows(D) / kJoinRows), 256, 0, ctx->stream>>>(a);
+    CHN_LAUNCHED(ctx, "k_packed_join");
+    return CHN_OK;
+}
+
+// Both entries: mask_words 0 is the causal one.
+static int packed_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache, const uint32_t *tables,
+                       const uint32_t *row_start, const uint32_t *lens, const uint32_t *masks, uint32_t mask_words,
+                       uint32_t n_req, uint32_t n_rows, uint32_t max_blocks, uint32_t block_size, uint32_t n_blocks,
+                       uint32_t num_q_heads, uint32_t head_dim, uint32_t kv_dim, uint32_t gqa_ratio, float scale,
+                       uint32_t window, float *out) {
+    CHN_REQUIRE(ctx, q && k_cache && v_cache && tables && row_start && lens && out, "NULL argument");
+    CHN_REQUIRE(ctx, head_dim == 256 || head_dim == 512, "head_dim %u must be 256 or 512", head_dim);
+    CHN_REQUIRE(ctx, gqa_ratio > 0 && gqa_ratio <= 16 && num_q_heads && num_q_heads % gqa_ratio == 0,
+                "num_q_heads %u, gqa ratio %u: a ratio of 1..16 that divides the heads", num_q_heads, gqa_ratio);
+    CHN_REQUIRE(ctx, num_q_heads <= 4096, "num_q_heads %u exceeds 4096", num_q_heads);
+    CHN_REQUIRE(ctx, kv_dim >= (num_q_heads / gqa_ratio) * head_dim && kv_dim % 4 == 0,
+                "kv_dim %u too small for %u kv heads of %u", kv_dim, num_q_heads / gqa_ratio, head_dim);
+    CHN_REQUIRE(ctx, aligned(q, 16) && aligned(k_cache, 16) && aligned(v_cache, 16) && aligned(out, 16),
+                "q, caches and out must be 16-byte aligned");
+    int rc = check_blocks(ctx, block_size, n_blocks, max_blocks);
+    if (rc) return rc;
+    const double c = std::fabs((double)scale) * 1.4426950408889634;
+    CHN_REQUIRE(ctx, c >= 1e-37 && c <= 1e37, "scale %g must be finite and not zero", (double)scale);
+    if (n_req > kPackedRequests) return set_err(ctx, CHN_E_UNSUPPORTED, "n_req %u exceeds %u", n_req, kPackedRequests);
+    if (n_rows > kPackedRows) return set_err(ctx, CHN_E_UNSUPPORTED, "n_rows %u exceeds %u", n_rows, kPackedRows);
+    const size_t words = (size_t)n_rows * num_q_heads * head_dim;
+    CHN_REQUIRE(ctx, !overlap(chn::Span{q, words}, chn::Span{out, words}), "out overlaps q");
+    CHN_REQUIRE(ctx, ctx, "ctx is NULL");
+    if (!n_req || !n_rows) return CHN_OK;
+    DeviceGuard dev(ctx);
+    Packed a{};
+    a.q = q;
+    a.kc = k_cache;
+    a.vc = v_cache;
+    a.tables = tables;
+    a.row_start = row_start;
+    a.lens = lens;
+    a.masks = masks;
+    a.mask_words = mask_words;
+    a.n_req = n_req;
+    a.n_rows = n_rows;
+    a.max_blocks = max_blocks;
+    a.shift = (uint32_t)__builtin_ctz(block_size);
+    a.n_blocks = n_blocks;
+    a.num_q = num_q_heads;
+    a.num_kv = num_q_heads / gqa_ratio;
+    a.kv_dim = kv_dim;
+    a.gqa = gqa_ratio;
+    a.tokens = tile_rows(head_dim) / gqa_ratio;
+    // no list is longer than 2^31 - 1
+    a.window = (int)std::min(window, 0x7FFFFFFFu);
+    a.c = (float)c;
+    a.sign = scale < 0.0f ? -1.0f : 1.0f;
+    a.out = out;
+    // one size for every call of a head_dim, whatever the batch
+    const size_t rows = (size_t)2 * kShares * tile_rows(head_dim);
+    rc = ensure_workspace(ctx, rows * (head_dim + 2) * 4 + kShares * sizeof(Joined));
+    if (rc) return rc;
+    a.po = (float *)ctx->ws;
+    a.pm = a.po + rows * head_dim;
+    a.pl = a.pm + rows;
+    a.joined = (Joined *)(a.pl + rows);
+    return head_dim == 256 ? launch_packed<256>(ctx, a) : launch_packed<512>(ctx, a);
+}
+
+// ---------------------------------------------------------------------
+// Masks and clocks of drafted trees.
+// ---------------------------------------------------------------------
+struct Drafts {
+    const uint32_t *parents, *row_start, *lens;
+    uint32_t n_rows, words;
+    uint32_t *masks, *clocks;
+};
+
+// A workgroup per request, a thread per node: node i's mask is its own bit and
+// its parent's mask, found by doubling - every round takes over what the node
+// that its path has reached has gathered, and that node's reach, so a path of
+// depth d takes log2 d rounds.  A parent that is no earlier node ends a path,
+// so every path ends.
+constexpr uint32_t kNodes = 32 * kMaskWords;
+template <int W>
+__global__ __launch_bounds__(kNodes) void k_draft_trees(Drafts a) {
+    __shared__ uint32_t mask[kNodes][W], reach[kNodes];
+    const uint32_t r = blockIdx.x, i = threadIdx.x;
+    const uint32_t s = min(a.row_start[r], a.n_rows), e = min(a.row_start[r + 1], a.n_rows), len = a.lens[r];
+    const uint32_t n = e > s ? e - s : 0, nodes = min(n, 32 * a.words), have = len > n ? len - n : 0;
+    if (!n) return;
+    uint32_t m[W], to = kNodes;
+    if (i < nodes) {
+        const uint32_t p = a.parents[s + i];
+        if (p < i) to = p;
+    }
+#pragma unroll
+    for (int w = 0; w < W; ++w) m[w] = i < nodes && i / 32 == (uint32_t)w ? 1u << (i % 32) : 0u;
+    while (__syncthreads_or(to < kNodes)) {
+        reach[i] = to;
+#pragma unroll
+        for (int w = 0; w < W; ++w) mask[i][w] = m[w];
+        __syncthreads();
+        if (to < kNodes) {
+#pragma unroll
+            for (int w = 0; w < W; ++w) m[w] |= mask[to][w];
+            to = reach[to];
+        }
+    }
+    if (i < nodes) {
+        uint32_t depth = 0;
+#pragma unroll
+        for (int w = 0; w < W; ++w)
+            if ((uint32_t)w < a.words) {
+                a.masks[(size_t)(s + i) * a.words + w] = m[w];
+                depth += __popc(m[w]);
+            }
+        a.clocks[s + i] = have + depth - 1;
+    }
+    for (uint32_t j = nodes + i; j < n; j += kNodes) {          // more rows than the masks have bits
+        for (uint32_t w = 0; w < a.words; ++w) a.masks[(size_t)(s + j) * a.words + w] = 0;
+        a.clocks[s + j] = have;
+    }
+}
+
+}  // namespace chn
+
+using namespace chn;
+
+extern "C" int chn_paged_causal_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
+                                     const uint32_t *tables, const uint32_t *row_start, const uint32_t *lens,
+                                     uint32_t n_req, uint32_t n_rows, uint32_t max_blocks, uint32_t block_size,
+                                     uint32_t n_blocks, uint32_t num_q_heads, uint32_t head_dim, uint32_t kv_dim,
+                                     uint32_t gqa_ratio, float scale, uint32_t window, float *out) {
+    return packed_attn(ctx, q, k_cache, v_cache, tables, row_start, lens, nullptr, 0, n_req, n_rows, max_blocks, block_size,
+                       n_blocks, num_q_heads, head_dim, kv_dim, gqa_ratio, scale, window, out);
+}
+
+extern "C" int chn_paged_tree_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
+                                   const uint32_t *tables, const uint32_t *row_start, const uint32_t *lens,
+                                   const uint32_t *masks, uint32_t mask_words, uint32_t n_req, uint32_t n_rows,
+                                   uint32_t max_blocks, uint32_t block_size, uint32_t n_blocks, uint32_t num_q_heads,
+                                   uint32_t head_dim, uint32_t kv_dim, uint32_t gqa_ratio, float scale, uint32_t window,
+                                   float *out) {
+    CHN_REQUIRE(ctx, masks, "NULL masks");
+    CHN_REQUIRE(ctx, mask_words && mask_words <= kMaskWords, "mask_words %u must be in 1..%u", mask_words, kMaskWords);
+    CHN_REQUIRE(ctx, !window || window >= 32 * mask_words, "a window of %u is shorter than %u drafted tokens", window,
+                32 * mask_words);
+    return packed_attn(ctx, q, k_cache, v_cache, tables, row_start, lens, masks, mask_words, n_req, n_rows, max_blocks,
+                       block_size, n_blocks, num_q_heads, head_dim, kv_dim, gqa_ratio, scale, window, out);
+}
+
+extern "C" int chn_draft_trees(chn_ctx *ctx, const uint32_t *parents, const uint32_t *row_start, const uint32_t *lens,
+                               uint32_t n_req, uint32_t n_rows, uint32_t mask_words, uint32_t *masks, uint32_t *clocks) {
+    CHN_REQUIRE(ctx, parents && row_start && lens && masks && clocks, "NULL argument");
+    CHN_REQUIRE(ctx, mask_words && mask_words <= kMaskWords, "mask_words %u must be in 1..%u", mask_words, kMaskWords);
+    if (n_req > kPackedRequests) return set_err(ctx, CHN_E_UNSUPPORTED, "n_req %u exceeds %u", n_req, kPackedRequests);
+    if (n_rows > kPackedRows) return set_err(ctx, CHN_E_UNSUPPORTED, "n_rows %u exceeds %u", n_rows, kPackedRows);
+    const Span outs[] = {{masks, (size_t)n_rows * mask_words}, {clocks, n_rows}};
+    const Span ins[] = {{parents, n_rows}, {row_start, (size_t)n_req + 1}, {lens, n_req}};
+    for (const Span &o : outs)
+        for (const Span &i : ins) CHN_REQUIRE(ctx, !overlap(o, i), "an output overlaps an input");
+    CHN_REQUIRE(ctx, !overlap(outs[0], outs[1]), "masks and clocks overlap");
+    CHN_REQUIRE(ctx, ctx, "ctx is NULL");
+    if (!n_req || !n_rows) return CHN_OK;
+    DeviceGuard dev(ctx);
+    const Drafts a{parents, row_start, lens, n_rows, mask_words, masks, clocks};
+    if (mask_words == 1) k_draft_trees<1><<<n_req, kNodes, 0, ctx->stream>>>(a);
+    else if (mask_words == 2) k_draft_trees<2><<<n_req, kNodes, 0, ctx->stream>>>(a);
+    else if (mask_words <= 4) k_draft_trees<4><<<n_req, kNodes, 0, ctx->stream>>>(a);
+    else k_draft_trees<8><<<n_req, kNodes, 0, ctx->stream>>>(a);
+    CHN_LAUNCHED(ctx, "k_draft_trees");
+    return CHN_OK;
+}

@@ -657,6 +657,100 @@ int chn_sample(chn_ctx *ctx, const float *logits, uint32_t n_rows, uint32_t V, u
                const float *u, float softcap, uint32_t *tokens, float *probs);
 
 /* ======================================================================
+ * Steps in which a request takes several tokens, over the same paged cache:
+ * prompts (or chunks of them) of several requests packed behind one another,
+ * trees of drafted tokens, and the scoring of both.  No reference counterpart.
+ * The rows of such a step are those of chn_block_tables and
+ * chn_batch_qkv_rope_at: row_start, lens (its lens_out) and tables are read as
+ * it writes them.  Request r has the n = row_start[r + 1] - row_start[r] rows
+ * from row_start[r] on (none where that is not positive; rows at n_rows and
+ * beyond are nobody's) and holds lens[r] tokens, the last n of which are those
+ * rows.  Every entry of a table up to its request's length is read, a shared
+ * prefix's entries too.
+ *
+ * A prompt's step is chn_block_tables, then per layer chn_batch_qkv_rope_at
+ * and chn_paged_causal_attn, then, where its tokens are scored,
+ * chn_token_logprobs on the rows of logits.  A drafted tree's tokens go behind
+ * their request's as any new tokens do (parents before their children);
+ * chn_draft_trees gives the clocks for chn_batch_qkv_rope_at, in place of
+ * those of chn_block_tables, and the masks for chn_paged_tree_attn.  Of a
+ * tree, the caller keeps the K/V rows of the path that it accepts (chn_copy to
+ * the slots behind the cached tokens, ancestors first) and its length.
+ * All four only enqueue on the context's stream and can be recorded.  Argument
+ * checks come first: called with ctx == NULL they report through
+ * chn_last_error(NULL).
+ * ==================================================================== */
+
+/* Masks and clocks of drafted trees.  The rows of request r are its drafted
+ * tokens; parents[row] is the number of a row's parent among its request's
+ * rows, which has to be an earlier one: any other value, CHN_NO_PARENT for
+ * one, says that the row hangs on the last cached token.  masks (mask_words
+ * words a row, 1..8): bit j (of word j / 32) is set if row j of the request is
+ * the row itself or one of its ancestors.  clocks[row] is the position that
+ * the row's token would have in its sequence: max(lens[r] - n, 0) plus its
+ * number of ancestors.  A request has at most 32 * mask_words drafted tokens:
+ * the rows behind those get a mask of zeros and a root's clock.  n_req <=
+ * 8192, n_rows <= 2^24; outputs must not overlap inputs; rows of no request
+ * are left as they were. */
+#define CHN_NO_PARENT 0xFFFFFFFFu
+int chn_draft_trees(chn_ctx *ctx, const uint32_t *parents, const uint32_t *row_start, const uint32_t *lens,
+                    uint32_t n_req, uint32_t n_rows, uint32_t mask_words, uint32_t *masks, uint32_t *clocks);
+
+/* Causal attention of packed prompts: q and out [n_rows][num_q_heads *
+ * head_dim].  Row i of request r stands at position p = len - n + i, len =
+ * min(lens[r], max_blocks * block_size), and sees the keys at max(0, p + 1 -
+ * window) .. p (window 0: at 0 .. p) through row r of tables ([n_req]
+ * [max_blocks]).  Softmax of scale * q.k; a key whose score is -inf has no
+ * weight, a score of +inf or NaN makes its row NaN; a row without keys gets
+ * zeros.  A block id that is not below n_blocks takes its tokens out of the
+ * softmax.  What lies in slots that a row does not see is not used for it,
+ * whatever it holds.  Rows of no request are left as they were.  Query head h
+ * reads KV head h / gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; scale
+ * finite, not zero; n_req <= 8192, n_rows <= 2^24; max_blocks * block_size <
+ * 2^31.  out must not overlap q.  Products are formed of operands split in two
+ * 11-bit halves (errors as fp32's own) and summed in fp32; rows of a tile that
+ * meets infinities or NaN are recomputed in plain fp32.  Workspace: 65 MB,
+ * whatever the batch. */
+int chn_paged_causal_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
+                          const uint32_t *tables, const uint32_t *row_start, const uint32_t *lens, uint32_t n_req,
+                          uint32_t n_rows, uint32_t max_blocks, uint32_t block_size, uint32_t n_blocks,
+                          uint32_t num_q_heads, uint32_t head_dim, uint32_t kv_dim, uint32_t gqa_ratio, float scale,
+                          uint32_t window, float *out);
+
+/* The same for drafted tokens, of which each sees what its mask says (masks,
+ * mask_words as chn_draft_trees writes them; any bits are allowed): row i of
+ * request r sees the cached tokens, positions 0 .. len - n - 1, and drafted
+ * token j, position len - n + j, if bit j of its mask is set.  With a window
+ * it sees the cached tokens from max(0, len - n + b - window) on, b the number
+ * of bits of its mask: for ancestors' masks the window at its clock.  A window
+ * holds 32 * mask_words tokens at least, so it never cuts off drafted ones. */
+int chn_paged_tree_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
+                        const uint32_t *tables, const uint32_t *row_start, const uint32_t *lens, const uint32_t *masks,
+                        uint32_t mask_words, uint32_t n_req, uint32_t n_rows, uint32_t max_blocks, uint32_t block_size,
+                        uint32_t n_blocks, uint32_t num_q_heads, uint32_t head_dim, uint32_t kv_dim,
+                        uint32_t gqa_ratio, float scale, uint32_t window, float *out);
+
+/* Log probabilities under each of n_rows rows of logits (row r at logits + r *
+ * ld, V of ld values, V <= 2^20).  Barred values, softcap and temperature are
+ * chn_sample's: p = exp((l - l_max) / temperature[r]) over their sum, barred
+ * tokens have none, a temperature <= 0 or NaN gives all to the largest logit
+ * (the lowest such index).  Tokens are ordered by their logit, equal ones by
+ * lower index.
+ *  - logprobs[r] = log p of targets[r], -inf if it is barred; 0 if targets[r]
+ *    is not below V (CHN_NO_TOKEN: nothing to score);
+ *  - entropy[r] = - sum p log p; 0 for a row that bars everything;
+ *  - ranks[r]: how many tokens come before targets[r] (0: the likeliest);
+ *    CHN_NO_TOKEN if it is barred or not below V;
+ *  - top_ids, top_logprobs ([n_rows][n_top], n_top <= 64): the first n_top
+ *    tokens and their log probabilities; CHN_NO_TOKEN and -inf behind the last
+ *    allowed one.
+ * temperature (device, n_rows) NULL: 1; entropy and ranks may be NULL, the top
+ * arrays with n_top 0.  n_rows <= 65535. */
+int chn_token_logprobs(chn_ctx *ctx, const float *logits, uint32_t n_rows, uint32_t V, uint32_t ld,
+                       const uint32_t *targets, const float *temperature, float softcap, uint32_t n_top,
+                       float *logprobs, float *entropy, uint32_t *ranks, uint32_t *top_ids, float *top_logprobs);
+
+/* ======================================================================
  * Seeded synthetic inputs (no reference counterpart: benchmark and test
  * inputs generated in place on the device; the same counter-based hash is
  * restated on the host, so any block can be regenerated for checking)
