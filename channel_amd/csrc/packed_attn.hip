@@ -147,7 +147,7 @@ __device__ __forceinline__ float *row_out(const Packed &a, const Work &w, uint32
 // A row per wave, a key at a time, in plain fp32: what any scores and values
 // do, infinities and NaN among them.
 template <int D>
-__device__ __noinline__ void rows_plain(const Packed &a, const Work &w) {
+__device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
     constexpr int N = D / 256;
     const int lane = threadIdx.x & 63;
     for (uint32_t row = threadIdx.x >> 6; row < w.rows; row += kThreads / 64) {
@@ -192,6 +192,370 @@ __device__ __noinline__ void rows_plain(const Packed &a, const Work &w) {
         }
     }
 }
+
+// ---------------------------------------------------------------------
+// Tiles on matrix instructions.
+// ---------------------------------------------------------------------
+typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+typedef uint32_t u2q __attribute__((ext_vector_type(2)));
+typedef uint32_t u4q __attribute__((ext_vector_type(4)));
+
+// What keys that are nobody's read.
+static __device__ __align__(16) const float no_key[512] = {};
+
+// Two fp32 values as fp16 halves hi + lo of 11 bits each: |x - hi - lo| <=
+// 2^-22 |x|.  The products hi hi, hi lo and lo hi are exact in fp32, where the
+// instructions sum them; lo lo (2^-22 of a product) is dropped.
+__device__ __forceinline__ void halves(float a, float b, uint32_t &hi, uint32_t &lo) {
+    float ra, rb;
+    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(hi) : "v"(a), "v"(b));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(hi), "v"(a));
+    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(hi), "v"(b));
+    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(lo) : "v"(ra), "v"(rb));
+}
+
+// The power of two that brings values of at most |top| below 2^15, and its
+// inverse: fp16 then holds what is 2^-39 of the largest and more.  At most
+// 2^100.
+__device__ __forceinline__ float scale_for(float top, float &inverse) {
+    const uint32_t e = __builtin_bit_cast(uint32_t, top) & 0x7F800000u;
+    const uint32_t f = min(0x86000000u - e, 227u << 23);
+    inverse = __builtin_bit_cast(float, (254u << 23) - f);
+    return __builtin_bit_cast(float, f);
+}
+// of the larger magnitude; NaN if either is
+__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, fabsf(b)); }
+__device__ __forceinline__ bool is_finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
+
+// LDS of a workgroup: 32 keys in the order in which the instructions read
+// them, and their scales' inverses.
+//  K: [tile of 16 keys][step of 32 dims][hi, lo][64 lanes][8 dims]; lane 16 g +
+//     key holds dims 8 g .. + 7 of the step, at place key ^ (4 (step % 4) + g),
+//     so that 16 neighbouring lanes of the store fill 256 bytes
+//  V: [16 dims][hi, lo][64 lanes][8 keys]; lane 16 g + c holds keys 4 g .. + 3
+//     and 16 + 4 g .. + 3, the keys whose weights lane 16 g + row has after the
+//     score's product
+template <int D>
+struct TileLds {
+    static constexpr int kKeyBytes = 32 * D * 4;
+    unsigned char k[kKeyBytes], v[kKeyBytes];
+    float kinv[32], vinv[32];
+    float half[D == 512 ? 8 * 64 * 8 : 4];            // scores of the other half of the dims
+};
+
+// All waves: what was stored in LDS before is visible behind it.  Loads from
+// memory stay in flight.
+__device__ __forceinline__ void lds_barrier() {
+    __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    __asm__ volatile("" ::: "memory");
+}
+
+// Weights are relative to a reference that is moved when a score passes it by
+// more than this, in powers of two.
+constexpr float kLead = 2.0f;
+constexpr float kWeightScale = 8192.0f;               // 2^13: weights of at most 2^kLead stay below 2^15
+
+template <int D>
+struct Tile {
+    static constexpr int H = D / 256, RT = 8 / H;     // waves that share 16 rows (256 dims each), tiles of 16 rows
+    static constexpr int S = D / 32;                  // steps
+    static constexpr int KR = D == 256 ? 2 : 4;       // keys a lane loads dims of, K
+    const Packed &a;
+    const Work &w;
+    TileLds<D> &lds;
+    int lane, wave, rt, half, q, g;
+    f4q kr[KR][2], vr[4][H];
+    uint32_t ids[2], slots, unheld;                   // of 64 keys: the next ones' blocks, these ones' slots
+    bool bad;                                         // an infinity or NaN was met
+
+    __device__ __forceinline__ Tile(const Packed &a_, const Work &w_, TileLds<D> &l) : a(a_), w(w_), lds(l) {
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        rt = wave % RT;
+        half = wave / RT;
+        q = lane & 15;
+        g = lane >> 4;
+        bad = false;
+    }
+
+    // chunks come in pairs, 64 keys, a lane each
+    __device__ __forceinline__ uint32_t block_of(int pair) const {
+        return w.table[min(w.key0 + 64 * pair + lane, w.key1 - 1) >> a.shift];
+    }
+    __device__ __forceinline__ void take_pair(int pair) {
+        const int pos = w.key0 + 64 * pair + lane;
+        const uint32_t b = ids[0];
+        slots = pos < w.key1 && b < a.n_blocks ? (b << a.shift) + (pos & ((1u << a.shift) - 1)) : CHN_NO_SLOT;
+        ids[0] = ids[1];
+        ids[1] = block_of(pair + 2);
+    }
+    __device__ __forceinline__ const float *row_at(const float *cache, uint32_t slot) const {
+        return slot == CHN_NO_SLOT ? no_key : cache + (size_t)slot * a.kv_dim + (size_t)w.kvh * D;
+    }
+
+    __device__ __forceinline__ void load_k(int chunk) {
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+            const int key = 32 * (chunk & 1) + (D == 256 ? 16 * i + 2 * wave : 8 * i + wave);
+            const float *p = row_at(a.kc, __builtin_amdgcn_readlane(slots, key));
+            if (D == 256) {
+                const float *p1 = row_at(a.kc, __builtin_amdgcn_readlane(slots, key + 1));
+                p = lane & 32 ? p1 : p;
+            }
+            const float *x = p + 8 * (lane & (D / 8 - 1));
+            kr[i][0] = *(const f4q *)x;
+            kr[i][1] = *(const f4q *)(x + 4);
+        }
+    }
+    __device__ __forceinline__ void store_k() {
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+            const int key = D == 256 ? 16 * i + 2 * wave + (lane >> 5) : 8 * i + wave, gd = lane & (D / 8 - 1);
+            float top = fabsf(kr[i][0][0]);
+#pragma unroll
+            for (int e = 1; e < 8; ++e) top = larger(top, kr[i][e / 4][e % 4]);
+            bad |= !is_finite(top);
+            top = row16_max(top);
+            top = fmaxf(top, xor16_lane(top));
+            if (D == 512) top = fmaxf(top, xor32_lane(top));
+            float inverse;
+            const float scale = scale_for(top, inverse);
+            u4q hi, lo;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t h, l;
+                halves(kr[i][e / 2][2 * (e % 2)] * scale, kr[i][e / 2][2 * (e % 2) + 1] * scale, h, l);
+                hi[e] = h;
+                lo[e] = l;
+            }
+            unsigned char *to = lds.k + (((key >> 4) * S + (gd >> 2)) * 2) * 1024 + (gd & 3) * 256 + (((key ^ gd) & 15) * 16);
+            *(u4q *)to = hi;
+            *(u4q *)(to + 1024) = lo;
+            if (gd == 0) lds.kinv[key] = inverse;
+        }
+    }
+    // the wave's four keys: 4 (wave / 2) + 16 (wave % 2) .. + 3
+    __device__ __forceinline__ void load_v(int chunk) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float *p = row_at(a.vc, __builtin_amdgcn_readlane(slots, 32 * (chunk & 1) + 4 * (wave >> 1) + 16 * (wave & 1) + i));
+#pragma unroll
+            for (int h = 0; h < H; ++h) vr[i][h] = *(const f4q *)(p + 4 * lane + 256 * h);
+        }
+    }
+    __device__ __forceinline__ void store_v() {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float top = fabsf(vr[i][0][0]);
+#pragma unroll
+            for (int e = 1; e < 4 * H; ++e) top = larger(top, vr[i][e / 4][e % 4]);
+            bad |= !is_finite(top);
+            top = row16_max(top);
+            top = fmaxf(top, xor16_lane(top));
+            top = fmaxf(top, xor32_lane(top));
+            float inverse;
+            const float scale = scale_for(top, inverse);
+#pragma unroll
+            for (int h = 0; h < H; ++h) vr[i][h] *= scale;
+            if (lane == 0) lds.vinv[4 * (wave >> 1) + 16 * (wave & 1) + i] = inverse;
+        }
+#pragma unroll
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                uint32_t h0, h1, l0, l1;
+                halves(vr[0][h][e], vr[1][h][e], h0, l0);
+                halves(vr[2][h][e], vr[3][h][e], h1, l1);
+                // dim 256 h + 4 lane + e is column lane % 16 of 16 dims
+                unsigned char *to = lds.v + ((16 * h + 4 * (lane >> 4) + e) * 2) * 1024 + ((wave >> 1) * 16 + (lane & 15)) * 16 + (wave & 1) * 8;
+                *(u2q *)to = u2q{h0, h1};
+                *(u2q *)(to + 1024) = u2q{l0, l1};
+            }
+    }
+
+    __device__ __forceinline__ void run() {
+        const uint32_t row = rt * 16 + q;
+        const bool valid = row < w.rows, active = (uint32_t)(rt * 16) < w.rows;
+        const int chunks = w.key1 > w.key0 ? (w.key1 - w.key0 + 31) / 32 : 0;
+        // rows of no token see everything, so that they never stand in a chunk's way
+        const int token = w.token + (int)((valid ? row : 0) / a.gqa);
+        Seen s = seen_by(a, w, token);
+        if (!valid) {
+            s.lo = -0x7FFFFFFF;
+            s.hi = 0x7FFFFFFF;
+        }
+        if (chunks) {
+            ids[0] = block_of(0);
+            ids[1] = block_of(1);
+            take_pair(0);
+            load_k(0);
+            load_v(0);
+        }
+        u4q qh[8], ql[8];
+        float qinv = 0.0f;
+        {
+            const float *p = a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + (valid ? row : 0) % a.gqa) * D + 256 * half + 8 * g;
+            f4q x[8][2];
+            float top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 2; ++e) x[i][e] = *(const f4q *)(p + 32 * i + 4 * e);
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 8; ++e) top = larger(top, x[i][e / 4][e % 4]);
+            bad |= !is_finite(top);
+            top = rows4_max(top);
+            const float scale = scale_for(top, qinv) * a.sign;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t h, l;
+                    halves(x[i][e / 2][2 * (e % 2)] * scale, x[i][e / 2][2 * (e % 2) + 1] * scale, h, l);
+                    qh[i][e] = h;
+                    ql[i][e] = l;
+                }
+        }
+        f4q o[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) o[i] = f4q{0, 0, 0, 0};
+        float m = kNoScore, l = 0.0f, vref = 0.0f;
+        const unsigned char *kat[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) kat[i] = lds.k + half * 16384 + g * 256 + ((q ^ (4 * i + g)) * 16);
+        const unsigned char *vat = lds.v + half * 32768 + lane * 16;
+        if (chunks) {
+            unheld = (uint32_t)__ballot(slots == CHN_NO_SLOT);
+            store_k();
+        }
+        for (int c = 0; c < chunks; ++c) {
+            const int k0 = w.key0 + 32 * c;
+            const uint32_t none = unheld;                         // keys of the chunk that are nobody's
+            lds_barrier();
+            if (c + 1 < chunks) {
+                if (c & 1) take_pair((c + 1) >> 1);
+                unheld = (uint32_t)(__ballot(slots == CHN_NO_SLOT) >> (c & 1 ? 0 : 32));
+                load_k(c + 1);
+            }
+            // bit k: the row sees key k0 + k
+            uint32_t ok = 0xFFFFFFFFu;
+            const bool all = !none && __all(s.lo <= k0 && k0 + 32 <= s.hi);
+            if (!all) {
+                const int from = min(max(s.lo - k0, 0), 32), to = min(max(s.hi - k0, 0), 32);
+                if (valid) ok = to > from ? (0xFFFFFFFFu >> (32 - (to - from))) << from : 0u;
+                const int node = k0 - w.s.have;
+                if (valid && s.mask && node > -32 && node < (int)(32 * a.mask_words)) {
+                    const int i = node >> 5;
+                    const uint32_t w0 = i >= 0 ? s.mask[i] : 0u, w1 = i + 1 < (int)a.mask_words ? s.mask[i + 1] : 0u;
+                    ok |= (uint32_t)(((uint64_t)w1 << 32 | w0) >> (node & 31));
+                }
+                ok &= ~none;
+            }
+            const bool some = active && __any(ok != 0 && valid);
+            f4q sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
+            if (some) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const unsigned char *p = kat[i & 3] + (t * S + i) * 2048;
+                        const h8 kh = *(const h8 *)p, kl = *(const h8 *)(p + 1024);
+                        const h8 bh = __builtin_bit_cast(h8, qh[i]), bl = __builtin_bit_cast(h8, ql[i]);
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, bh, sc[t], 0, 0, 0);
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, bl, sc[t], 0, 0, 0);
+                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, bh, sc[t], 0, 0, 0);
+                    }
+#pragma unroll
+                for (int t = 0; t < 2; ++t) sc[t] = (sc[t] * *(const f4q *)(lds.kinv + 16 * t + 4 * g)) * qinv;
+                if (D == 512)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) *(f4q *)(lds.half + ((wave * 2 + t) * 64 + lane) * 4) = sc[t];
+            }
+            store_v();
+            lds_barrier();
+            if (c + 1 < chunks) load_v(c + 1);
+            if (some) {
+                if (D == 512)
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        // the same order of the halves in both waves
+                        const f4q other = *(const f4q *)(lds.half + (((wave ^ RT) * 2 + t) * 64 + lane) * 4);
+                        sc[t] = half ? other + sc[t] : sc[t] + other;
+                    }
+                f4q vi[2];
+#pragma unroll
+                for (int t = 0; t < 2; ++t) vi[t] = *(const f4q *)(lds.vinv + 16 * t + 4 * g);
+                float top = kNoScore, vtop = 0.0f;
+#pragma unroll
+                for (int t = 0; t < 2; ++t)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        if (!all) sc[t][i] = (ok >> (16 * t + 4 * g + i)) & 1 ? sc[t][i] : kNoScore;
+                        top = fmaxf(top, sc[t][i]);
+                        vtop = fmaxf(vtop, vi[t][i]);
+                    }
+                top = rows4_max(top);
+                vtop = lane_f(rows4_max(vtop), 0);
+                const bool up = (top - m) * a.c > kLead;
+                if (__any(up) || vtop > vref) {
+                    const float to = up ? top : m, old = up ? __builtin_amdgcn_exp2f((m - to) * a.c) : 1.0f;
+                    const float vto = fmaxf(vtop, vref), f = old * (vref / vto);
+                    m = to;
+                    vref = vto;
+                    l *= old;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) o[i] *= f;
+                }
+                const float ref = m == kNoScore ? 0.0f : m, unit = kWeightScale / vref;
+                float p[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    p[e] = __builtin_amdgcn_exp2f((sc[e / 4][e % 4] - ref) * a.c);
+                    l += p[e];
+                    p[e] *= vi[e / 4][e % 4] * unit;
+                }
+                u4q ph, pl;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint32_t h, lo;
+                    halves(p[2 * e], p[2 * e + 1], h, lo);
+                    ph[e] = h;
+                    pl[e] = lo;
+                }
+                const h8 bh = __builtin_bit_cast(h8, ph), bl = __builtin_bit_cast(h8, pl);
+#pragma unroll
+                for (int i = 0; i < 16; ++i) {
+                    const h8 vh = *(const h8 *)(vat + i * 2048), vl = *(const h8 *)(vat + i * 2048 + 1024);
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, bh, o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, bl, o[i], 0, 0, 0);
+                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, bh, o[i], 0, 0, 0);
+                }
+            }
+            if (c + 1 < chunks) store_k();
+        }
+        if (__syncthreads_or(bad)) {
+            rows_plain<D>(a, w);
+            return;
+        }
+        l = rows4_sum(l);
+        if (!valid) return;
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f, unit = vref * (1.0f / kWeightScale);
+        float *to = row_out<D>(a, w, row) + 256 * half + 16 * g;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *(f4q *)(to + 64 * j + 4 * i) =
+                    f4q{o[4 * j][i] * inv * unit, o[4 * j + 1][i] * inv * unit, o[4 * j + 2][i] * inv * unit, o[4 * j + 3][i] * inv * unit};
+        if (w.part >= 0 && g == 0 && half == 0) {
+            a.pm[(size_t)w.part * tile_rows(D) + row] = m;
+            a.pl[(size_t)w.part * tile_rows(D) + row] = l;
+        }
+    }
+};
 
 // The workgroup's share: f(work) for each of its tiles or parts of tiles.
 template <int D, typename F>
@@ -302,7 +666,8 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
 
 template <int D>
 __global__ __launch_bounds__(kThreads) void k_packed_attn(Packed a) {
-    each_work<D>(a, [&](const Work &w) { rows_plain<D>(a, w); });
+    extern __shared__ __align__(16) unsigned char sh[];
+    each_work<D>(a, [&](const Work &w) { Tile<D>(a, w, *(TileLds<D> *)sh).run(); });
 }
 
 // Joins the parts of the tiles that were cut: a wave takes a row at a time, a
@@ -353,7 +718,8 @@ __global__ __launch_bounds__(256) void k_packed_join(Packed a) {
 
 template <int D>
 static int launch_packed(chn_ctx *ctx, const Packed &a) {
-    k_packed_attn<D><<<kShares, kThreads, 0, ctx->stream>>>(a);
+    static_assert(sizeof(TileLds<D>) <= 159 * 1024, "LDS per workgroup");
+    k_packed_attn<D><<<kShares, kThreads, sizeof(TileLds<D>), ctx->stream>>>(a);
     CHN_LAUNCHED(ctx, "k_packed_attn");
     k_packed_join<D><<<kShares * (tile_rows(D) / kJoinRows), 256, 0, ctx->stream>>>(a);
     CHN_LAUNCHED(ctx, "k_packed_join");
