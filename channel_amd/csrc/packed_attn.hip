@@ -214,18 +214,73 @@ __device__ __forceinline__ void halves(float a, float b, uint32_t &hi, uint32_t 
     asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(lo) : "v"(ra), "v"(rb));
 }
 
-// The power of two that brings values of at most |top| below 2^15, and its
-// inverse: fp16 then holds what is 2^-39 of the largest and more.  At most
-// 2^100.
-__device__ __forceinline__ float scale_for(float top, float &inverse) {
-    const uint32_t e = __builtin_bit_cast(uint32_t, top) & 0x7F800000u;
-    const uint32_t f = min(0x86000000u - e, 227u << 23);
+// The power of two that brings values of magnitude `top` (its bits) below
+// 2^15, and its inverse: fp16 then holds what is 2^-39 of the largest and
+// more.  At most 2^100.
+__device__ __forceinline__ float scale_for(uint32_t top, float &inverse) {
+    const uint32_t f = min(0x86000000u - (top & 0x7F800000u), 227u << 23);
     inverse = __builtin_bit_cast(float, (254u << 23) - f);
     return __builtin_bit_cast(float, f);
 }
-// of the larger magnitude; NaN if either is
-__device__ __forceinline__ float larger(float a, float b) { return __builtin_elementwise_maximum(a, fabsf(b)); }
-__device__ __forceinline__ bool is_finite(float v) { return (__builtin_bit_cast(uint32_t, v) & 0x7F800000u) != 0x7F800000u; }
+constexpr uint32_t kNotFinite = 0x7F800000u;           // magnitudes from here on are infinities and NaN
+// NaN if either is
+__device__ __forceinline__ float largest(float a, float b) { return __builtin_elementwise_maximum(a, b); }
+// the bits of the largest magnitude of N values, as unsigned words ordered as the values are
+template <int N, typename F>
+__device__ __forceinline__ uint32_t magnitude(F &&at) {
+    float top = largest(fabsf(at(0)), fabsf(at(1)));
+#pragma unroll
+    for (int i = 2; i < N; ++i) top = largest(top, fabsf(at(i)));
+    return __builtin_bit_cast(uint32_t, top);
+}
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
+    return max(v, (uint32_t)__builtin_amdgcn_mov_dpp((int)v, CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t row16_top(uint32_t v) {
+    v = max_dpp<0xB1>(v);                              // quad_perm [1,0,3,2], [2,3,0,1], row_ror:4, row_ror:8
+    v = max_dpp<0x4E>(v);
+    v = max_dpp<0x124>(v);
+    return max_dpp<0x128>(v);
+}
+// The results of a swap pass through an empty asm: this compiler otherwise takes the second for the first.
+__device__ __forceinline__ void swap16(uint32_t &a, uint32_t &b) {           // rows a0 b0 a2 b2, a1 b1 a3 b3
+    const auto r = __builtin_amdgcn_permlane16_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+    __asm__("" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ void swap32(uint32_t &a, uint32_t &b) {           // halves a0 b0, a1 b1
+    const auto r = __builtin_amdgcn_permlane32_swap(a, b, false, false);
+    a = r[0];
+    b = r[1];
+    __asm__("" : "+v"(a), "+v"(b));
+}
+__device__ __forceinline__ uint32_t swap_max16(uint32_t a, uint32_t b) {
+    swap16(a, b);
+    return max(a, b);
+}
+__device__ __forceinline__ uint32_t swap_max32(uint32_t a, uint32_t b) {
+    swap32(a, b);
+    return max(a, b);
+}
+// Four values over the wave, row by row: lanes 16 i of the result hold v[i]'s.
+__device__ __forceinline__ uint32_t wave_top4(const uint32_t (&v)[4]) {
+    return row16_top(swap_max16(swap_max32(v[0], v[2]), swap_max32(v[1], v[3])));
+}
+// over lanes l, l ^ 16, l ^ 32, l ^ 48
+__device__ __forceinline__ float rows4_top(float v) {
+    uint32_t a = __builtin_bit_cast(uint32_t, v), b = a;
+    swap16(a, b);
+    a = b = __builtin_bit_cast(uint32_t, largest(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b)));
+    swap32(a, b);
+    return largest(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+
+// Addresses known to be memory's: flat loads would count as LDS operations,
+// and the barriers below wait for those.
+typedef const __attribute__((address_space(1))) float *mem_t;
+__device__ __forceinline__ f4q load4(mem_t p) { return *(const __attribute__((address_space(1))) f4q *)p; }
 
 // LDS of a workgroup: 32 keys in the order in which the instructions read
 // them, and their scales' inverses.
@@ -254,7 +309,7 @@ __device__ __forceinline__ void lds_barrier() {
 // Weights are relative to a reference that is moved when a score passes it by
 // more than this, in powers of two.
 constexpr float kLead = 2.0f;
-constexpr float kWeightScale = 8192.0f;               // 2^13: weights of at most 2^kLead stay below 2^15
+constexpr float kWeightScale = 8192.0f;               // 2^13: weights of at most 2^kLead stay at or below 2^15
 
 template <int D>
 struct Tile {
@@ -290,37 +345,39 @@ struct Tile {
         ids[0] = ids[1];
         ids[1] = block_of(pair + 2);
     }
-    __device__ __forceinline__ const float *row_at(const float *cache, uint32_t slot) const {
-        return slot == CHN_NO_SLOT ? no_key : cache + (size_t)slot * a.kv_dim + (size_t)w.kvh * D;
+    __device__ __forceinline__ mem_t row_at(const float *cache, uint32_t slot) const {
+        return slot == CHN_NO_SLOT ? (mem_t)no_key : (mem_t)cache + ((size_t)slot * a.kv_dim + (size_t)w.kvh * D);
     }
 
     __device__ __forceinline__ void load_k(int chunk) {
 #pragma unroll
         for (int i = 0; i < KR; ++i) {
             const int key = 32 * (chunk & 1) + (D == 256 ? 16 * i + 2 * wave : 8 * i + wave);
-            const float *p = row_at(a.kc, __builtin_amdgcn_readlane(slots, key));
+            mem_t p = row_at(a.kc, __builtin_amdgcn_readlane(slots, key));
             if (D == 256) {
-                const float *p1 = row_at(a.kc, __builtin_amdgcn_readlane(slots, key + 1));
+                const mem_t p1 = row_at(a.kc, __builtin_amdgcn_readlane(slots, key + 1));
                 p = lane & 32 ? p1 : p;
             }
-            const float *x = p + 8 * (lane & (D / 8 - 1));
-            kr[i][0] = *(const f4q *)x;
-            kr[i][1] = *(const f4q *)(x + 4);
+            const mem_t x = p + 8 * (lane & (D / 8 - 1));
+            kr[i][0] = load4(x);
+            kr[i][1] = load4(x + 4);
         }
     }
     __device__ __forceinline__ void store_k() {
+        uint32_t top[KR], most;
+#pragma unroll
+        for (int i = 0; i < KR; ++i) {
+            top[i] = magnitude<8>([&](int e) { return kr[i][e / 4][e % 4]; });
+            bad |= top[i] >= kNotFinite;
+        }
+        if constexpr (D == 256) most = row16_top(swap_max16(top[0], top[1]));      // rows: keys 0, 16, 1, 17 of the wave's
+        else most = wave_top4(top);
 #pragma unroll
         for (int i = 0; i < KR; ++i) {
             const int key = D == 256 ? 16 * i + 2 * wave + (lane >> 5) : 8 * i + wave, gd = lane & (D / 8 - 1);
-            float top = fabsf(kr[i][0][0]);
-#pragma unroll
-            for (int e = 1; e < 8; ++e) top = larger(top, kr[i][e / 4][e % 4]);
-            bad |= !is_finite(top);
-            top = row16_max(top);
-            top = fmaxf(top, xor16_lane(top));
-            if (D == 512) top = fmaxf(top, xor32_lane(top));
+            const uint32_t t0 = __builtin_amdgcn_readlane(most, 16 * i), t1 = D == 256 ? __builtin_amdgcn_readlane(most, 32 + 16 * i) : t0;
             float inverse;
-            const float scale = scale_for(top, inverse);
+            const float scale = scale_for(lane & 32 ? t1 : t0, inverse);
             u4q hi, lo;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
@@ -339,27 +396,29 @@ struct Tile {
     __device__ __forceinline__ void load_v(int chunk) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const float *p = row_at(a.vc, __builtin_amdgcn_readlane(slots, 32 * (chunk & 1) + 4 * (wave >> 1) + 16 * (wave & 1) + i));
+            const mem_t p = row_at(a.vc, __builtin_amdgcn_readlane(slots, 32 * (chunk & 1) + 4 * (wave >> 1) + 16 * (wave & 1) + i));
 #pragma unroll
-            for (int h = 0; h < H; ++h) vr[i][h] = *(const f4q *)(p + 4 * lane + 256 * h);
+            for (int h = 0; h < H; ++h) vr[i][h] = load4(p + 4 * lane + 256 * h);
         }
     }
     __device__ __forceinline__ void store_v() {
+        uint32_t top[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float top = fabsf(vr[i][0][0]);
+            top[i] = magnitude<4 * H>([&](int e) { return vr[i][e / 4][e % 4]; });
+            bad |= top[i] >= kNotFinite;
+        }
+        const uint32_t most = wave_top4(top);
+        f4q inverse;
 #pragma unroll
-            for (int e = 1; e < 4 * H; ++e) top = larger(top, vr[i][e / 4][e % 4]);
-            bad |= !is_finite(top);
-            top = row16_max(top);
-            top = fmaxf(top, xor16_lane(top));
-            top = fmaxf(top, xor32_lane(top));
-            float inverse;
-            const float scale = scale_for(top, inverse);
+        for (int i = 0; i < 4; ++i) {
+            float inv;
+            const float scale = scale_for(__builtin_amdgcn_readlane(most, 16 * i), inv);
+            inverse[i] = inv;
 #pragma unroll
             for (int h = 0; h < H; ++h) vr[i][h] *= scale;
-            if (lane == 0) lds.vinv[4 * (wave >> 1) + 16 * (wave & 1) + i] = inverse;
         }
+        if (lane == 0) *(f4q *)(lds.vinv + 4 * (wave >> 1) + 16 * (wave & 1)) = inverse;
 #pragma unroll
         for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -397,17 +456,14 @@ struct Tile {
         {
             const float *p = a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + (valid ? row : 0) % a.gqa) * D + 256 * half + 8 * g;
             f4q x[8][2];
-            float top = 0.0f;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) x[i][e] = *(const f4q *)(p + 32 * i + 4 * e);
-#pragma unroll
-            for (int i = 0; i < 8; ++i)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) top = larger(top, x[i][e / 4][e % 4]);
-            bad |= !is_finite(top);
-            top = rows4_max(top);
+                for (int e = 0; e < 2; ++e) x[i][e] = load4((mem_t)p + 32 * i + 4 * e);
+            uint32_t top = magnitude<64>([&](int e) { return x[e / 8][e / 4 % 2][e % 4]; });
+            bad |= top >= kNotFinite;
+            top = swap_max16(top, top);
+            top = swap_max32(top, top);
             const float scale = scale_for(top, qinv) * a.sign;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
@@ -494,11 +550,11 @@ struct Tile {
 #pragma unroll
                     for (int i = 0; i < 4; ++i) {
                         if (!all) sc[t][i] = (ok >> (16 * t + 4 * g + i)) & 1 ? sc[t][i] : kNoScore;
-                        top = fmaxf(top, sc[t][i]);
-                        vtop = fmaxf(vtop, vi[t][i]);
+                        top = largest(top, sc[t][i]);
+                        vtop = largest(vtop, vi[t][i]);
                     }
-                top = rows4_max(top);
-                vtop = lane_f(rows4_max(vtop), 0);
+                top = rows4_top(top);
+                vtop = lane_f(rows4_top(vtop), 0);
                 const bool up = (top - m) * a.c > kLead;
                 if (__any(up) || vtop > vref) {
                     const float to = up ? top : m, old = up ? __builtin_amdgcn_exp2f((m - to) * a.c) : 1.0f;
@@ -509,14 +565,14 @@ struct Tile {
 #pragma unroll
                     for (int i = 0; i < 16; ++i) o[i] *= f;
                 }
-                const float ref = m == kNoScore ? 0.0f : m, unit = kWeightScale / vref;
+                const float ref = m == kNoScore ? 0.0f : m;
+                const float unit = __builtin_bit_cast(float, (267u << 23) - __builtin_bit_cast(uint32_t, vref));      // 2^13 / vref
                 float p[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    p[e] = __builtin_amdgcn_exp2f((sc[e / 4][e % 4] - ref) * a.c);
-                    l += p[e];
-                    p[e] *= vi[e / 4][e % 4] * unit;
-                }
+                for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f((sc[e / 4][e % 4] - ref) * a.c);
+                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) p[e] *= vi[e / 4][e % 4] * unit;
                 u4q ph, pl;
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
