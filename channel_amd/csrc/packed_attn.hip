@@ -21,11 +21,15 @@ typedef float f4q __attribute__((ext_vector_type(4)));
 constexpr uint32_t kPackedRequests = 8192;
 constexpr uint32_t kPackedRows = 1u << 24;
 constexpr uint32_t kMaskWords = 8;          // drafted tokens of a request: 256
-constexpr uint32_t kShares = 256;           // workgroups: one per CU
+constexpr int kShareLog = 8;
+constexpr uint32_t kShares = 1u << kShareLog;   // workgroups: one per CU
 constexpr int kThreads = 512;
-// Units are keys.  A tile costs kTileCost besides its keys; a share has kLeastShare units or more, and a cut that
-// would fall within kTileCost of a tile's end is moved there.
-constexpr int64_t kTileCost = 64, kLeastShare = 192;
+// A key is 2 units, or 3 where both waves of a SIMD have rows (a chunk of 32 keys takes 2.9 and 4.1 us).  A tile costs
+// kTileCost besides its keys, its beginning and end (heads of 256 14 us; heads of 512 16, where a chunk takes 5.4).  A
+// cut that would fall within kNearEnd of a tile's end is moved there; a share has 2^kShareBits units or more, twice
+// that, so that none is empty.
+constexpr int64_t kTileCost = 320, kNearEnd = 128;
+constexpr int kShareBits = 8;
 constexpr float kNoScore = -__builtin_inff();
 
 // Rows of a tile: tokens x query heads of the KV head.
@@ -42,6 +46,7 @@ struct Packed {
     const uint32_t *tables, *row_start, *lens, *masks;
     uint32_t mask_words;       // 0: causal
     uint32_t n_req, n_rows, max_blocks, shift, n_blocks, num_q, num_kv, kv_dim, gqa, tokens;   // tokens per tile
+    uint32_t per_gqa, per_tokens;             // their inverses: 2^16 / gqa, 2^32 / tokens, rounded up
     int window;
     float c, sign;             // |scale| log2(e), the scale's sign
     float *out;
@@ -66,37 +71,59 @@ __device__ __forceinline__ Seq seq_of(const Packed &a, uint32_t r) {
     return q;
 }
 
+// row of a tile -> token
+__device__ __forceinline__ uint32_t token_of(const Packed &a, uint32_t row) { return row * a.per_gqa >> 16; }
+
 // What the tiles of a request and KV head cost: tile t walks keys lo(t) ..
 // hi(t) - 1, both linear in t (the last tile's end is the work's, not the
 // cost's, matter).
 struct TileKeys {
-    int64_t tiles, T, hi0, lo0;        // hi = hi0 + t T, lo = max(0, lo0 + t T); T is 0 where all tiles see the same keys
-    __device__ __forceinline__ TileKeys(const Packed &a, const Seq &s) {
-        tiles = (s.n + (int64_t)a.tokens - 1) / a.tokens;
+    int64_t T, hi0, lo0;               // hi = hi0 + t T, lo = max(0, lo0 + t T); T is 0 where all tiles see the same keys
+    uint32_t tiles, s0;                // the first tile whose lo is above 0
+    bool full, last_full;              // whether a tile's rows, and the last one's, are more than half of a tile's
+    template <int D>
+    static __device__ __forceinline__ TileKeys of(const Packed &a, const Seq &s) {
+        TileKeys k;
+        k.tiles = __umulhi((uint32_t)s.n + a.tokens - 1, a.per_tokens);
+        k.s0 = k.tiles;
+        k.full = a.tokens * a.gqa > tile_rows(D) / 2;
+        k.last_full = (s.n - (k.tiles - 1) * a.tokens) * a.gqa > tile_rows(D) / 2;
         if (a.mask_words) {
-            T = 0;
-            hi0 = max(0, min(s.len, s.have + (int)(32 * a.mask_words)));
-            lo0 = a.window ? min(max(0, s.have - a.window), (int)hi0) : 0;
+            k.T = 0;
+            k.hi0 = max(0, min(s.len, s.have + (int)(32 * a.mask_words)));
+            k.lo0 = a.window ? min(max(0, s.have - a.window), (int)k.hi0) : 0;
         } else {
-            T = a.tokens;
-            hi0 = max(s.have, 0) + T;
-            lo0 = a.window ? (int64_t)s.have + 1 - a.window : -(tiles + 1) * T;
+            k.T = a.tokens;
+            k.hi0 = max(s.have, 0) + k.T;
+            k.lo0 = 0;
+            if (a.window) {
+                k.lo0 = (int64_t)s.have + 1 - a.window;
+                k.s0 = k.lo0 > 0 ? 0 : (uint32_t)-k.lo0 / a.tokens + 1;
+            }
         }
+        return k;
     }
-    __device__ __forceinline__ int64_t hi(int64_t t) const { return hi0 + t * T; }
-    __device__ __forceinline__ int64_t lo(int64_t t) const { return max((int64_t)0, lo0 + t * T); }
-    __device__ __forceinline__ int64_t cost(int64_t t) const { return kTileCost + hi(t) - lo(t); }
-    // of all tiles before t
-    __device__ __forceinline__ int64_t before(int64_t t) const {
-        int64_t sum = t * (kTileCost + hi0) + T * (t * (t - 1) / 2);
-        if (!T) return sum - t * max((int64_t)0, lo0);
-        const int64_t s0 = lo0 > 0 ? 0 : -lo0 / T + 1;      // the first tile whose lo is above 0
-        if (t > s0) sum -= (t - s0) * lo0 + T * ((t - s0) * (s0 + t - 1) / 2);
-        return sum;
+    __device__ __forceinline__ int64_t hi(uint32_t t) const { return hi0 + t * T; }
+    __device__ __forceinline__ int64_t lo(uint32_t t) const { return T && t < s0 ? 0 : lo0 + t * T; }
+    __device__ __forceinline__ bool is_full(uint32_t t) const { return t + 1 < tiles ? full : last_full; }
+    static __device__ __forceinline__ int64_t weighed(int64_t keys, bool full) { return keys * (full ? 3 : 2); }
+    __device__ __forceinline__ int64_t cost(uint32_t t) const { return kTileCost + weighed(hi(t) - lo(t), is_full(t)); }
+    // of the tiles before t, which are not the last
+    __device__ __forceinline__ int64_t before(uint32_t t) const {
+        const int64_t pairs = (int64_t)t * t - t, n = t > s0 ? t - s0 : 0;
+        int64_t keys = t * hi0 + (T * pairs >> 1);
+        keys -= T ? n * lo0 + (T * n * ((int64_t)s0 + t - 1) >> 1) : t * lo0;
+        return t * kTileCost + weighed(keys, full);
+    }
+    __device__ __forceinline__ int64_t all() const { return tiles ? before(tiles - 1) + cost(tiles - 1) : 0; }
+    // units behind a tile's begin -> keys behind its first
+    __device__ __forceinline__ int64_t keys_at(uint32_t t, int64_t units) const {
+        const int64_t u = max(units - kTileCost / 2, (int64_t)0);
+        return is_full(t) ? (int64_t)__umul64hi((uint64_t)u, 0x5555555555555556ull) : u >> 1;
     }
 };
 __device__ __forceinline__ int64_t snapped(int64_t at, int64_t cost) {
-    return at < kTileCost ? 0 : (at + kTileCost > cost ? cost : at);
+    return at < kNearEnd ? 0 : (at + kNearEnd > cost ? cost : at);
 }
 
 // One tile's share: rows, and keys key0 .. key1 - 1 (key0 a multiple of 32).
@@ -104,7 +131,7 @@ struct Work {
     Seq s;
     const uint32_t *table;
     uint32_t kvh, tile_row, rows;      // the tile's first batch row; rows (tokens x heads)
-    int token, key0, key1, limit;      // its first token's index; limit: keys from here on are nobody's
+    int token, key0, key1;             // its first token's index
     int part;                          // -1: the whole tile
 };
 
@@ -141,7 +168,8 @@ __device__ __forceinline__ uint32_t slot_of(const Packed &a, const uint32_t *tab
 template <int D>
 __device__ __forceinline__ float *row_out(const Packed &a, const Work &w, uint32_t row) {
     if (w.part >= 0) return a.po + ((size_t)w.part * tile_rows(D) + row) * D;
-    return a.out + ((size_t)(w.tile_row + row / a.gqa) * a.num_q + w.kvh * a.gqa + row % a.gqa) * D;
+    const uint32_t token = token_of(a, row);
+    return a.out + ((size_t)(w.tile_row + token) * a.num_q + w.kvh * a.gqa + row - token * a.gqa) * D;
 }
 
 // A row per wave, a key at a time, in plain fp32: what any scores and values
@@ -151,9 +179,9 @@ __device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
     constexpr int N = D / 256;
     const int lane = threadIdx.x & 63;
     for (uint32_t row = threadIdx.x >> 6; row < w.rows; row += kThreads / 64) {
-        const int token = w.token + (int)(row / a.gqa);
+        const int token = w.token + (int)token_of(a, row);
         const Seen s = seen_by(a, w, token);
-        const float *qr = a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + row % a.gqa) * D;
+        const float *qr = a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + row - token_of(a, row) * a.gqa) * D;
         f4q q[N], o[N];
         for (int k = 0; k < N; ++k) {
             q[k] = *(const f4q *)(qr + 4 * lane + 256 * k) * a.sign;
@@ -197,21 +225,18 @@ __device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
 // Tiles on matrix instructions.
 // ---------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
-typedef uint32_t u2q __attribute__((ext_vector_type(2)));
-typedef uint32_t u4q __attribute__((ext_vector_type(4)));
+typedef _Float16 h4 __attribute__((ext_vector_type(4)));
 
 // What keys that are nobody's read.
 static __device__ __align__(16) const float no_key[512] = {};
 
-// Two fp32 values as fp16 halves hi + lo of 11 bits each: |x - hi - lo| <=
-// 2^-22 |x|.  The products hi hi, hi lo and lo hi are exact in fp32, where the
-// instructions sum them; lo lo (2^-22 of a product) is dropped.
-__device__ __forceinline__ void halves(float a, float b, uint32_t &hi, uint32_t &lo) {
-    float ra, rb;
-    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(hi) : "v"(a), "v"(b));
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(ra) : "v"(hi), "v"(a));
-    asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(rb) : "v"(hi), "v"(b));
-    asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(lo) : "v"(ra), "v"(rb));
+// x * scale (scale a power of two) as fp16 halves hi + lo of 11 bits each:
+// |x scale - hi - lo| <= 2^-22 |x scale|.  The products hi hi, hi lo and lo hi
+// are exact in fp32, where the instructions sum them; lo lo (2^-22 of a
+// product) is dropped.
+__device__ __forceinline__ void halves(float x, float scale, _Float16 &hi, _Float16 &lo) {
+    hi = (_Float16)fmaf(x, scale, 0.0f);
+    lo = (_Float16)fmaf(x, scale, -(float)hi);
 }
 
 // The power of two that brings values of magnitude `top` (its bits) below
@@ -294,16 +319,37 @@ template <int D>
 struct TileLds {
     static constexpr int kKeyBytes = 32 * D * 4;
     unsigned char k[kKeyBytes], v[kKeyBytes];
-    float kinv[32], vinv[32];
+    float kinv[32], vinv[2][32];
     float half[D == 512 ? 8 * 64 * 8 : 4];            // scores of the other half of the dims
+    uint32_t not_finite;                              // an infinity or NaN was met
 };
 
+// By address: the places of a lane are one register and constants, and the
+// register is made opaque where the compiler would rather keep every sum.
+template <typename T>
+__device__ __forceinline__ T lds_load(uint32_t at) { return *(const __attribute__((address_space(3))) T *)(uintptr_t)at; }
+template <typename T>
+__device__ __forceinline__ void lds_store(uint32_t at, T v) { *(__attribute__((address_space(3))) T *)(uintptr_t)at = v; }
+
 // All waves: what was stored in LDS before is visible behind it.  Loads from
-// memory stay in flight.
+// memory stay in flight, and nothing moves across.
 __device__ __forceinline__ void lds_barrier() {
+    __builtin_amdgcn_sched_barrier(0);
     __asm__ volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     __asm__ volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
+
+// The end of a step of six products: other work stands between them, so that
+// the SIMD issues it while the matrix unit is busy.
+__device__ __forceinline__ void end_step() {
+#pragma unroll
+    for (int i = 0; i < 6; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);        // a product
+        __builtin_amdgcn_sched_group_barrier(0x002, 5, 0);        // vector operations
+    }
+    __builtin_amdgcn_sched_barrier(0);
 }
 
 // Weights are relative to a reference that is moved when a score passes it by
@@ -311,27 +357,46 @@ __device__ __forceinline__ void lds_barrier() {
 constexpr float kLead = 2.0f;
 constexpr float kWeightScale = 8192.0f;               // 2^13: weights of at most 2^kLead stay at or below 2^15
 
+// A tile's walk over its keys, 32 at a time.  Two phases between barriers:
+//   1  the scores of chunk c + 1, beside them the weights of chunk c and its V
+//      into LDS;
+//   2  the sums of chunk c, beside them K of chunk c + 2 into LDS.
+// Each is 48 products of the matrix unit, interleaved in eight steps with the
+// other work, which two waves of a SIMD issue meanwhile.  What a wave loads of
+// K and V (four keys of each) is under way for a phase or two.
 template <int D>
 struct Tile {
     static constexpr int H = D / 256, RT = 8 / H;     // waves that share 16 rows (256 dims each), tiles of 16 rows
     static constexpr int S = D / 32;                  // steps
-    static constexpr int KR = D == 256 ? 2 : 4;       // keys a lane loads dims of, K
+    // heads of 512 have no registers for K and V at once: K is loaded a chunk later, after V has gone to LDS
+    static constexpr bool kBoth = D == 256;
     const Packed &a;
     const Work &w;
     TileLds<D> &lds;
-    int lane, wave, rt, half, q, g;
-    f4q kr[KR][2], vr[4][H];
-    uint32_t ids[2], slots, unheld;                   // of 64 keys: the next ones' blocks, these ones' slots
-    bool bad;                                         // an infinity or NaN was met
+    int lane, wave, rt, half, q, g, keys;             // keys: the first of the four that the wave converts
+    f4q kr[4][H], vr_[kBoth ? 4 : 1][H];              // their dims 4 lane + 256 h .. + 3
+    uint32_t next_block;                              // of 64 keys, a lane each: the next ones' blocks,
+    mem_t ka, va, vnow;                               // these ones' rows (V is loaded later than K)
+    uint64_t unheld;                                  // and which of them are nobody's
+    uint32_t worst;                                   // the largest magnitude met
+    uint32_t k_to, v_to;                              // where the lane's values go in LDS
 
     __device__ __forceinline__ Tile(const Packed &a_, const Work &w_, TileLds<D> &l) : a(a_), w(w_), lds(l) {
         lane = threadIdx.x & 63;
         wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-        rt = wave % RT;
-        half = wave / RT;
+        // the halves of a row's dims on neighbouring SIMDs, so that half of a tile's rows keep all four busy
+        rt = wave / H;
+        half = wave % H;
         q = lane & 15;
         g = lane >> 4;
-        bad = false;
+        keys = 4 * (wave >> 1) + 16 * (wave & 1);
+        worst = 0;
+        k_to = lds_addr(lds.k) + (((wave & 1) * S + (lane >> 3)) * 2) * 1024 + (lane >> 1 & 3) * 256 + (((keys ^ (lane >> 1)) & 15) * 16) + (lane & 1) * 8;
+        v_to = lds_addr(lds.v) + 4 * (lane >> 4) * 2048 + ((wave >> 1) * 16 + (4 * (lane & 3) + (lane >> 2 & 3))) * 16 + (wave & 1) * 8;
+    }
+    __device__ __forceinline__ f4q (&vr())[4][H] {
+        if constexpr (kBoth) return vr_;
+        else return kr;
     }
 
     // chunks come in pairs, 64 keys, a lane each
@@ -340,274 +405,377 @@ struct Tile {
     }
     __device__ __forceinline__ void take_pair(int pair) {
         const int pos = w.key0 + 64 * pair + lane;
-        const uint32_t b = ids[0];
-        slots = pos < w.key1 && b < a.n_blocks ? (b << a.shift) + (pos & ((1u << a.shift) - 1)) : CHN_NO_SLOT;
-        ids[0] = ids[1];
-        ids[1] = block_of(pair + 2);
+        const uint32_t b = next_block;
+        const bool held = pos < w.key1 && b < a.n_blocks;
+        const size_t at = (size_t)((b << a.shift) + (pos & ((1u << a.shift) - 1))) * a.kv_dim + (size_t)w.kvh * D;
+        ka = held ? (mem_t)a.kc + at : (mem_t)no_key;
+        va = held ? (mem_t)a.vc + at : (mem_t)no_key;
+        unheld = ~__ballot(held);
+        next_block = block_of(pair + 1);
     }
-    __device__ __forceinline__ mem_t row_at(const float *cache, uint32_t slot) const {
-        return slot == CHN_NO_SLOT ? (mem_t)no_key : (mem_t)cache + ((size_t)slot * a.kv_dim + (size_t)w.kvh * D);
-    }
-
-    __device__ __forceinline__ void load_k(int chunk) {
-#pragma unroll
-        for (int i = 0; i < KR; ++i) {
-            const int key = 32 * (chunk & 1) + (D == 256 ? 16 * i + 2 * wave : 8 * i + wave);
-            mem_t p = row_at(a.kc, __builtin_amdgcn_readlane(slots, key));
-            if (D == 256) {
-                const mem_t p1 = row_at(a.kc, __builtin_amdgcn_readlane(slots, key + 1));
-                p = lane & 32 ? p1 : p;
-            }
-            const mem_t x = p + 8 * (lane & (D / 8 - 1));
-            kr[i][0] = load4(x);
-            kr[i][1] = load4(x + 4);
-        }
-    }
-    __device__ __forceinline__ void store_k() {
-        uint32_t top[KR], most;
-#pragma unroll
-        for (int i = 0; i < KR; ++i) {
-            top[i] = magnitude<8>([&](int e) { return kr[i][e / 4][e % 4]; });
-            bad |= top[i] >= kNotFinite;
-        }
-        if constexpr (D == 256) most = row16_top(swap_max16(top[0], top[1]));      // rows: keys 0, 16, 1, 17 of the wave's
-        else most = wave_top4(top);
-#pragma unroll
-        for (int i = 0; i < KR; ++i) {
-            const int key = D == 256 ? 16 * i + 2 * wave + (lane >> 5) : 8 * i + wave, gd = lane & (D / 8 - 1);
-            const uint32_t t0 = __builtin_amdgcn_readlane(most, 16 * i), t1 = D == 256 ? __builtin_amdgcn_readlane(most, 32 + 16 * i) : t0;
-            float inverse;
-            const float scale = scale_for(lane & 32 ? t1 : t0, inverse);
-            u4q hi, lo;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                uint32_t h, l;
-                halves(kr[i][e / 2][2 * (e % 2)] * scale, kr[i][e / 2][2 * (e % 2) + 1] * scale, h, l);
-                hi[e] = h;
-                lo[e] = l;
-            }
-            unsigned char *to = lds.k + (((key >> 4) * S + (gd >> 2)) * 2) * 1024 + (gd & 3) * 256 + (((key ^ gd) & 15) * 16);
-            *(u4q *)to = hi;
-            *(u4q *)(to + 1024) = lo;
-            if (gd == 0) lds.kinv[key] = inverse;
-        }
-    }
-    // the wave's four keys: 4 (wave / 2) + 16 (wave % 2) .. + 3
-    __device__ __forceinline__ void load_v(int chunk) {
+    // chunks behind the last are nobody's
+    __device__ __forceinline__ void load(f4q (&to)[4][H], mem_t rows, int chunk) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            const mem_t p = row_at(a.vc, __builtin_amdgcn_readlane(slots, 32 * (chunk & 1) + 4 * (wave >> 1) + 16 * (wave & 1) + i));
+            const mem_t row = (mem_t)lane64((uint64_t)rows, 32 * (chunk & 1) + keys + i);
 #pragma unroll
-            for (int h = 0; h < H; ++h) vr[i][h] = load4(p + 4 * lane + 256 * h);
+            for (int h = 0; h < H; ++h) to[i][h] = load4(row + 4 * lane + 256 * h);
         }
     }
-    __device__ __forceinline__ void store_v() {
+    __device__ __forceinline__ uint32_t load_k(int chunk) {
+        if (!(chunk & 1)) take_pair(chunk >> 1);
+        load(kr, ka, chunk);
+        return (uint32_t)(unheld >> (32 * (chunk & 1)));
+    }
+    // the four keys' scales
+    __device__ __forceinline__ void scales(const f4q (&of)[4][H], float (&scale)[4], float *inverses) {
         uint32_t top[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            top[i] = magnitude<4 * H>([&](int e) { return vr[i][e / 4][e % 4]; });
-            bad |= top[i] >= kNotFinite;
+            top[i] = magnitude<4 * H>([&](int e) { return of[i][e / 4][e % 4]; });
+            worst = max(worst, top[i]);
         }
         const uint32_t most = wave_top4(top);
         f4q inverse;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float inv;
-            const float scale = scale_for(__builtin_amdgcn_readlane(most, 16 * i), inv);
+            scale[i] = scale_for(__builtin_amdgcn_readlane(most, 16 * i), inv);
             inverse[i] = inv;
-#pragma unroll
-            for (int h = 0; h < H; ++h) vr[i][h] *= scale;
         }
-        if (lane == 0) *(f4q *)(lds.vinv + 4 * (wave >> 1) + 16 * (wave & 1)) = inverse;
+        if (lane == 0) *(f4q *)(inverses + keys) = inverse;
+    }
+    // key i of the wave's; a lane's eight dims lie at place key ^ (lane / 2)
+    __device__ __forceinline__ void store_k(int i, float scale) {
+        const uint32_t at = opaque_u32(k_to) ^ (i * 16);
 #pragma unroll
-        for (int h = 0; h < H; ++h)
+        for (int h = 0; h < H; ++h) {
+            h4 hi, lo;
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-                uint32_t h0, h1, l0, l1;
-                halves(vr[0][h][e], vr[1][h][e], h0, l0);
-                halves(vr[2][h][e], vr[3][h][e], h1, l1);
-                // dim 256 h + 4 lane + e is column lane % 16 of 16 dims
-                unsigned char *to = lds.v + ((16 * h + 4 * (lane >> 4) + e) * 2) * 1024 + ((wave >> 1) * 16 + (lane & 15)) * 16 + (wave & 1) * 8;
-                *(u2q *)to = u2q{h0, h1};
-                *(u2q *)(to + 1024) = u2q{l0, l1};
+                _Float16 x, y;
+                halves(kr[i][h][e], scale, x, y);
+                hi[e] = x;
+                lo[e] = y;
             }
+            lds_store(at + 16384 * h, hi);
+            lds_store(at + 16384 * h + 1024, lo);
+        }
+    }
+    // dims 256 h + 4 lane + e: column lane % 16 of 16 dims
+    __device__ __forceinline__ void store_v(int e, const float (&scale)[4]) {
+#pragma unroll
+        for (int h = 0; h < H; ++h) {
+            h4 hi, lo;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                _Float16 x, y;
+                halves(vr()[i][h][e], scale[i], x, y);
+                hi[i] = x;
+                lo[i] = y;
+            }
+            lds_store(v_to + (16 * h + e) * 2048, hi);
+            lds_store(v_to + (16 * h + e) * 2048 + 1024, lo);
+        }
     }
 
     __device__ __forceinline__ void run() {
         const uint32_t row = rt * 16 + q;
         const bool valid = row < w.rows, active = (uint32_t)(rt * 16) < w.rows;
         const int chunks = w.key1 > w.key0 ? (w.key1 - w.key0 + 31) / 32 : 0;
-        // rows of no token see everything, so that they never stand in a chunk's way
-        const int token = w.token + (int)((valid ? row : 0) / a.gqa);
-        Seen s = seen_by(a, w, token);
-        if (!valid) {
-            s.lo = -0x7FFFFFFF;
-            s.hi = 0x7FFFFFFF;
-        }
-        if (chunks) {
-            ids[0] = block_of(0);
-            ids[1] = block_of(1);
-            take_pair(0);
-            load_k(0);
-            load_v(0);
-        }
-        u4q qh[8], ql[8];
+        uint32_t none0 = 0, none1 = 0, none2 = 0, none3 = 0;      // keys that are nobody's, of chunks c ..
+        if (chunks) next_block = block_of(0);
+        const uint32_t of_tile = valid ? token_of(a, row) : 0;
+        const int token = w.token + (int)of_tile;
+        h8 qh[8], ql[8];
         float qinv = 0.0f;
         {
-            const float *p = a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + (valid ? row : 0) % a.gqa) * D + 256 * half + 8 * g;
+            // asked for before K and V, whose addresses wait for the table
+            const mem_t from = (mem_t)a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + (valid ? row : 0) - of_tile * a.gqa) * D + 256 * half + 8 * g;
             f4q x[8][2];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) x[i][e] = load4((mem_t)p + 32 * i + 4 * e);
+                for (int e = 0; e < 2; ++e) x[i][e] = load4(from + 32 * i + 4 * e);
+            __builtin_amdgcn_sched_barrier(0);
+            if (chunks) {
+                none0 = load_k(0);
+                if (kBoth) load(vr(), va, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
             uint32_t top = magnitude<64>([&](int e) { return x[e / 8][e / 4 % 2][e % 4]; });
-            bad |= top >= kNotFinite;
+            worst = max(worst, top);
             top = swap_max16(top, top);
             top = swap_max32(top, top);
             const float scale = scale_for(top, qinv) * a.sign;
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t h, l;
-                    halves(x[i][e / 2][2 * (e % 2)] * scale, x[i][e / 2][2 * (e % 2) + 1] * scale, h, l);
+                for (int e = 0; e < 8; ++e) {
+                    _Float16 h, l;
+                    halves(x[i][e / 4][e % 4], scale, h, l);
                     qh[i][e] = h;
                     ql[i][e] = l;
                 }
         }
+        // rows of no token see everything, so that they never stand in a chunk's way
+        Seen s = seen_by(a, w, token);
+        if (!valid) {
+            s.lo = -0x7FFFFFFF;
+            s.hi = 0x7FFFFFFF;
+        }
         f4q o[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = f4q{0, 0, 0, 0};
+        // Scores stay in units of the row's q scale, whose inverse goes into the exponent's factor; the halves of heads of
+        // 512 have scales of their own
+        const float unit_q = kBoth ? 1.0f : qinv, factor = kBoth ? fminf(a.c * qinv, 3.4028235e38f) : a.c;
         float m = kNoScore, l = 0.0f, vref = 0.0f;
-        const unsigned char *kat[4];
+        const uint32_t k_at = lds_addr(lds.k) + half * 16384 + g * 256 + (q ^ g) * 16, v_at = lds_addr(lds.v) + half * 32768 + lane * 16;
+        f4q sc[2];
+        h8 ph, pl;
+        float p[8], vscale[4];
+        const auto weights = [&](const float *vinv) {             // p relative to the largest V, as halves
+            f4q vi[2];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) kat[i] = lds.k + half * 16384 + g * 256 + ((q ^ (4 * i + g)) * 16);
-        const unsigned char *vat = lds.v + half * 32768 + lane * 16;
+            for (int t = 0; t < 2; ++t) vi[t] = *(const f4q *)(vinv + 16 * t + 4 * g);
+            const float unit = __builtin_bit_cast(float, (267u << 23) - __builtin_bit_cast(uint32_t, vref));      // 2^13 / vref
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                _Float16 x, y;
+                halves(p[e], vi[e / 4][e % 4] * unit, x, y);
+                ph[e] = x;
+                pl[e] = y;
+            }
+        };
+        const auto vtop_of = [&](const float *vinv) {
+            float t = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const f4q v = *(const f4q *)(vinv + 16 * e + 4 * g);
+                t = largest(largest(t, v[0]), largest(largest(v[1], v[2]), v[3]));
+            }
+            return lane_f(rows4_top(t), 0);
+        };
+        h8 fr[4];
+        const auto fetch_k = [&](int i) {                         // both tiles' step i
+            const uint32_t place = i & 3 ? opaque_u32(k_at) ^ ((i & 3) * 64) : k_at;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t at = place + (t * S + i) * 2048;
+                fr[2 * t] = lds_load<h8>(at);
+                fr[2 * t + 1] = lds_load<h8>(at + 1024);
+            }
+        };
+        const auto fetch_v = [&](int i) {                         // dims 32 i .. + 31
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                fr[2 * t] = lds_load<h8>(v_at + (2 * i + t) * 2048);
+                fr[2 * t + 1] = lds_load<h8>(v_at + (2 * i + t) * 2048 + 1024);
+            }
+        };
+        f4q next[2], low[2];
+        // four sums, so that no product waits for the one before
+        const auto score_step = [&](int i) {
+            low[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[1], qh[i], low[0], 0, 0, 0);
+            low[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[3], qh[i], low[1], 0, 0, 0);
+            next[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[0], qh[i], next[0], 0, 0, 0);
+            next[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[2], qh[i], next[1], 0, 0, 0);
+            low[0] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[0], ql[i], low[0], 0, 0, 0);
+            low[1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[2], ql[i], low[1], 0, 0, 0);
+        };
+        const auto begin_scores = [&] {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) next[t] = low[t] = f4q{0, 0, 0, 0};
+        };
+        const auto end_scores = [&] {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                sc[t] = (next[t] + low[t]) * *(const f4q *)(lds.kinv + 16 * t + 4 * g);
+                if (!kBoth) {
+                    sc[t] *= unit_q;
+                    *(f4q *)(lds.half + ((wave * 2 + t) * 64 + lane) * 4) = sc[t];
+                }
+            }
+        };
+        const auto add_half = [&] {
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                // the same order of the halves in both waves
+                const f4q other = *(const f4q *)(lds.half + (((wave ^ 1) * 2 + t) * 64 + lane) * 4);
+                sc[t] = half ? other + sc[t] : sc[t] + other;
+            }
+        };
+        const auto all_k = [&] {
+            float scale[4];
+            scales(kr, scale, lds.kinv);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) store_k(i, scale[i]);
+        };
         if (chunks) {
-            unheld = (uint32_t)__ballot(slots == CHN_NO_SLOT);
-            store_k();
+            all_k();
+            none1 = load_k(1);
+            vnow = va;
+            if (kBoth) scales(vr(), vscale, lds.vinv[0]);
+            lds_barrier();
+            if (threadIdx.x == 0) lds.not_finite = 0;
+            if (active) {
+                begin_scores();
+                static_for<8>([&](auto step) {
+                    fetch_k(decltype(step)::value);
+                    score_step(decltype(step)::value);
+                });
+                end_scores();
+            }
+            lds_barrier();
+            all_k();
+            if (!kBoth) {
+                if (active) add_half();
+                load(vr(), vnow, 0);
+            } else {
+                none2 = load_k(2);
+            }
         }
         for (int c = 0; c < chunks; ++c) {
-            const int k0 = w.key0 + 32 * c;
-            const uint32_t none = unheld;                         // keys of the chunk that are nobody's
+            const float *vinv = lds.vinv[kBoth ? c & 1 : 0];
+            if (c & 1) vnow = va;
             lds_barrier();
-            if (c + 1 < chunks) {
-                if (c & 1) take_pair((c + 1) >> 1);
-                unheld = (uint32_t)(__ballot(slots == CHN_NO_SLOT) >> (c & 1 ? 0 : 32));
-                load_k(c + 1);
-            }
-            // bit k: the row sees key k0 + k
-            uint32_t ok = 0xFFFFFFFFu;
-            const bool all = !none && __all(s.lo <= k0 && k0 + 32 <= s.hi);
-            if (!all) {
-                const int from = min(max(s.lo - k0, 0), 32), to = min(max(s.hi - k0, 0), 32);
-                if (valid) ok = to > from ? (0xFFFFFFFFu >> (32 - (to - from))) << from : 0u;
-                const int node = k0 - w.s.have;
-                if (valid && s.mask && node > -32 && node < (int)(32 * a.mask_words)) {
-                    const int i = node >> 5;
-                    const uint32_t w0 = i >= 0 ? s.mask[i] : 0u, w1 = i + 1 < (int)a.mask_words ? s.mask[i + 1] : 0u;
-                    ok |= (uint32_t)(((uint64_t)w1 << 32 | w0) >> (node & 31));
-                }
-                ok &= ~none;
-            }
-            const bool some = active && __any(ok != 0 && valid);
-            f4q sc[2] = {{0, 0, 0, 0}, {0, 0, 0, 0}};
-            if (some) {
+            // ---- phase 1
+            if (!kBoth) {
+                // the registers hold V of chunk c: to LDS first
+                scales(vr(), vscale, lds.vinv[0]);
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
+                for (int e = 0; e < 4; ++e) store_v(e, vscale);
+                none2 = load_k(c + 2);
+            }
+            if (active) {
+                begin_scores();
+                fetch_k(0);
+                static_for<8>([&](auto step) {
+                    constexpr int i = decltype(step)::value;
+                    score_step(i);
+                    if constexpr (i < 7) fetch_k(i + 1);
+                    if constexpr (i == 0) {
+                        const int k0 = w.key0 + 32 * c;
+                        if (none0 || !__all(s.lo <= k0 && k0 + 32 <= s.hi)) {
+                            // bit k: the row sees key k0 + k
+                            uint32_t ok = 0xFFFFFFFFu;
+                            const int from = min(max(s.lo - k0, 0), 32), to = min(max(s.hi - k0, 0), 32);
+                            if (valid) ok = to > from ? (0xFFFFFFFFu >> (32 - (to - from))) << from : 0u;
+                            const int node = k0 - w.s.have;
+                            if (node > -32 && node < (int)(32 * a.mask_words) && valid) {
+                                const uint32_t *mask = a.masks + (size_t)(w.s.row + opaque_u32(token)) * a.mask_words;
+                                const int n = node >> 5;
+                                const uint32_t w0 = n >= 0 ? mask[n] : 0u, w1 = n + 1 < (int)a.mask_words ? mask[n + 1] : 0u;
+                                ok |= (uint32_t)(((uint64_t)w1 << 32 | w0) >> (node & 31));
+                            }
+                            ok = (ok & ~none0) >> (4 * g);
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        const unsigned char *p = kat[i & 3] + (t * S + i) * 2048;
-                        const h8 kh = *(const h8 *)p, kl = *(const h8 *)(p + 1024);
-                        const h8 bh = __builtin_bit_cast(h8, qh[i]), bl = __builtin_bit_cast(h8, ql[i]);
-                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kl, bh, sc[t], 0, 0, 0);
-                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, bl, sc[t], 0, 0, 0);
-                        sc[t] = __builtin_amdgcn_mfma_f32_16x16x32_f16(kh, bh, sc[t], 0, 0, 0);
+                            for (int e = 0; e < 8; ++e)
+                                sc[e / 4][e % 4] = ok >> (16 * (e / 4) + e % 4) & 1 ? sc[e / 4][e % 4] : kNoScore;
+                        }
                     }
+                    if constexpr (i == 1) {
+                        float top = kNoScore;
 #pragma unroll
-                for (int t = 0; t < 2; ++t) sc[t] = (sc[t] * *(const f4q *)(lds.kinv + 16 * t + 4 * g)) * qinv;
-                if (D == 512)
+                        for (int e = 0; e < 8; ++e) top = largest(top, sc[e / 4][e % 4]);
+                        top = rows4_top(top);
+                        const float vtop = kBoth ? vtop_of(vinv) : 0.0f;
+                        const bool up = (top - m) * factor > kLead;
+                        if (__any(up) || vtop > vref) {
+                            const float to = up ? top : m, old = up ? __builtin_amdgcn_exp2f((m - to) * factor) : 1.0f;
+                            float f = old;
+                            if (kBoth) {
+                                const float vto = vtop > vref ? vtop : vref;
+                                f *= vref / vto;
+                                vref = vto;
+                            }
+                            m = to;
+                            l *= old;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) *(f4q *)(lds.half + ((wave * 2 + t) * 64 + lane) * 4) = sc[t];
+                            for (int e = 0; e < 16; ++e) o[e] *= f;
+                        }
+                    }
+                    if constexpr (i == 2 || i == 3) {
+                        const float ref = m == kNoScore ? 0.0f : m;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) p[4 * (i - 2) + e] = __builtin_amdgcn_exp2f((sc[i - 2][e] - ref) * factor);
+                    }
+                    if constexpr (i == 4) {
+                        l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
+                        if (kBoth) weights(vinv);
+                    }
+                    if constexpr (i >= 4 && kBoth) store_v(i - 4, vscale);
+                    end_step();
+                });
+                end_scores();
+            } else if (kBoth) {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) store_v(e, vscale);
             }
-            store_v();
+            if (kBoth) load(vr(), vnow, c + 1);
             lds_barrier();
-            if (c + 1 < chunks) load_v(c + 1);
-            if (some) {
-                if (D == 512)
+            // ---- phase 2
+            if (active) {
+                if (!kBoth) {
+                    const float vtop = vtop_of(vinv);
+                    if (vtop > vref) {
+                        const float f = vref / vtop;
+                        vref = vtop;
 #pragma unroll
-                    for (int t = 0; t < 2; ++t) {
-                        // the same order of the halves in both waves
-                        const f4q other = *(const f4q *)(lds.half + (((wave ^ RT) * 2 + t) * 64 + lane) * 4);
-                        sc[t] = half ? other + sc[t] : sc[t] + other;
+                        for (int e = 0; e < 16; ++e) o[e] *= f;
                     }
-                f4q vi[2];
-#pragma unroll
-                for (int t = 0; t < 2; ++t) vi[t] = *(const f4q *)(lds.vinv + 16 * t + 4 * g);
-                float top = kNoScore, vtop = 0.0f;
-#pragma unroll
-                for (int t = 0; t < 2; ++t)
-#pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        if (!all) sc[t][i] = (ok >> (16 * t + 4 * g + i)) & 1 ? sc[t][i] : kNoScore;
-                        top = largest(top, sc[t][i]);
-                        vtop = largest(vtop, vi[t][i]);
-                    }
-                top = rows4_top(top);
-                vtop = lane_f(rows4_top(vtop), 0);
-                const bool up = (top - m) * a.c > kLead;
-                if (__any(up) || vtop > vref) {
-                    const float to = up ? top : m, old = up ? __builtin_amdgcn_exp2f((m - to) * a.c) : 1.0f;
-                    const float vto = fmaxf(vtop, vref), f = old * (vref / vto);
-                    m = to;
-                    vref = vto;
-                    l *= old;
-#pragma unroll
-                    for (int i = 0; i < 16; ++i) o[i] *= f;
+                    weights(vinv);
                 }
-                const float ref = m == kNoScore ? 0.0f : m;
-                const float unit = __builtin_bit_cast(float, (267u << 23) - __builtin_bit_cast(uint32_t, vref));      // 2^13 / vref
-                float p[8];
-#pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] = __builtin_amdgcn_exp2f((sc[e / 4][e % 4] - ref) * a.c);
-                l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
-#pragma unroll
-                for (int e = 0; e < 8; ++e) p[e] *= vi[e / 4][e % 4] * unit;
-                u4q ph, pl;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    uint32_t h, lo;
-                    halves(p[2 * e], p[2 * e + 1], h, lo);
-                    ph[e] = h;
-                    pl[e] = lo;
-                }
-                const h8 bh = __builtin_bit_cast(h8, ph), bl = __builtin_bit_cast(h8, pl);
-#pragma unroll
-                for (int i = 0; i < 16; ++i) {
-                    const h8 vh = *(const h8 *)(vat + i * 2048), vl = *(const h8 *)(vat + i * 2048 + 1024);
-                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vl, bh, o[i], 0, 0, 0);
-                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, bl, o[i], 0, 0, 0);
-                    o[i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(vh, bh, o[i], 0, 0, 0);
-                }
+                float scale[4];
+                fetch_v(0);
+                static_for<8>([&](auto step) {
+                    constexpr int i = decltype(step)::value;
+                    o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[1], ph, o[2 * i], 0, 0, 0);
+                    o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[3], ph, o[2 * i + 1], 0, 0, 0);
+                    o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[0], pl, o[2 * i], 0, 0, 0);
+                    o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[2], pl, o[2 * i + 1], 0, 0, 0);
+                    o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[0], ph, o[2 * i], 0, 0, 0);
+                    o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[2], ph, o[2 * i + 1], 0, 0, 0);
+                    if constexpr (i < 7) fetch_v(i + 1);
+                    if constexpr (i == 2) scales(kr, scale, lds.kinv);
+                    if constexpr (i >= 3 && i < 7) store_k(i - 3, scale[i - 3]);
+                    end_step();
+                });
+                if (!kBoth) add_half();
+            } else {
+                all_k();
             }
-            if (c + 1 < chunks) store_k();
+            if (!kBoth) {
+                load(vr(), vnow, c + 1);
+            } else {
+                scales(vr(), vscale, lds.vinv[(c + 1) & 1]);
+                none3 = load_k(c + 3);
+            }
+            none0 = none1;
+            none1 = none2;
+            none2 = none3;
         }
-        if (__syncthreads_or(bad)) {
-            rows_plain<D>(a, w);
-            return;
+        if (chunks) {
+            if (__any(worst >= kNotFinite) && lane == 0) lds.not_finite = 1;
+            lds_barrier();
+            if (lds.not_finite) {
+                rows_plain<D>(a, w);
+                return;
+            }
         }
         l = rows4_sum(l);
         if (!valid) return;
         const float inv = l != 0.0f ? 1.0f / l : 0.0f, unit = vref * (1.0f / kWeightScale);
-        float *to = row_out<D>(a, w, row) + 256 * half + 16 * g;
+        float *to = row_out<D>(a, w, row) + 256 * half + 4 * g;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                *(f4q *)(to + 64 * j + 4 * i) =
+                *(f4q *)(to + 64 * j + 16 * i) =
                     f4q{o[4 * j][i] * inv * unit, o[4 * j + 1][i] * inv * unit, o[4 * j + 2][i] * inv * unit, o[4 * j + 3][i] * inv * unit};
         if (w.part >= 0 && g == 0 && half == 0) {
-            a.pm[(size_t)w.part * tile_rows(D) + row] = m;
+            a.pm[(size_t)w.part * tile_rows(D) + row] = kBoth ? m * qinv : m;
             a.pl[(size_t)w.part * tile_rows(D) + row] = l;
         }
     }
@@ -616,40 +784,41 @@ struct Tile {
 // The workgroup's share: f(work) for each of its tiles or parts of tiles.
 template <int D, typename F>
 __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
-    __shared__ int64_t sums[kThreads / 64];
-    __shared__ int64_t found_base;
+    __shared__ int64_t sums[kThreads / 64], found_base;
     __shared__ uint32_t found;
     const uint32_t tid = threadIdx.x, per = (a.n_req + kThreads - 1) / kThreads;
     const int lane = tid & 63, wave = tid >> 6;
     // every request's units; a thread sums its neighbours
     const uint32_t r0 = min(tid * per, a.n_req), r1 = min(r0 + per, a.n_req);
+    const auto units_of = [&](uint32_t r) {
+        return TileKeys::of<D>(a, seq_of(a, r)).all() * a.num_kv;
+    };
     int64_t mine = 0;
-    for (uint32_t r = r0; r < r1; ++r) {
-        const TileKeys s(a, seq_of(a, r));
-        mine += s.before(s.tiles) * a.num_kv;
-    }
+    for (uint32_t r = r0; r < r1; ++r) mine += units_of(r);
     const int64_t upto = (int64_t)wave_scan_u64((uint64_t)mine);
     if (lane == 63) sums[wave] = upto;
-    if (tid == 0) found = 0xFFFFFFFFu;
+    if (tid == 0) {
+        found = 0xFFFFFFFFu;
+        a.joined[blockIdx.x].rows = 0;
+    }
     __syncthreads();
     int64_t total = 0, base = upto - mine;
+#pragma unroll
     for (int i = 0; i < kThreads / 64; ++i) {
         base += i < wave ? sums[i] : 0;
         total += sums[i];
     }
-    // neighbouring shares, which read the same keys, run on one XCD (workgroup i on XCD i % 8)
-    const uint32_t n = (uint32_t)max((int64_t)1, min((int64_t)kShares, total / kLeastShare)), each = (n + 7) / 8;
-    const uint32_t share = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
-    const bool some = (blockIdx.x >> 3) < each && share < n;
-    const auto cut = [&](uint32_t w) { return total / n * w + total % n * w / n; };
-    if (tid == 0) a.joined[blockIdx.x].rows = 0;      // of share `share`, or of none
-    if (!some) return;                                // the whole workgroup
+    total = (int64_t)lane64((uint64_t)total, 0);
+    // a power of two of shares; neighbours, which read the same keys, run on one XCD (workgroup i on XCD i % 8)
+    const int bits = total >> kShareBits ? min(63 - __builtin_clzll((uint64_t)total >> kShareBits), kShareLog) : 0;
+    const uint32_t n = 1u << bits, each = (n + 7) / 8, share = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    if ((blockIdx.x >> 3) >= each || share >= n) return;      // the whole workgroup
+    const auto cut = [&](uint32_t w) { return total * w >> bits; };
     const int64_t u0 = cut(share), u1 = cut(share + 1);
-    if (u0 >= base && u0 < base + mine) {             // one thread, or none
+    if (u0 >= base && u0 < base + mine) {                     // one thread, or none
         uint32_t r = r0;
         for (; r + 1 < r1; ++r) {
-            const TileKeys s(a, seq_of(a, r));
-            const int64_t units = s.before(s.tiles) * a.num_kv;
+            const int64_t units = units_of(r);
             if (u0 < base + units) break;
             base += units;
         }
@@ -657,42 +826,47 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
         found_base = base;
     }
     __syncthreads();
-    uint32_t r = __builtin_amdgcn_readfirstlane(found);
+    uint32_t r = __builtin_amdgcn_readfirstlane(found), kvh = 0, t = 0;
     if (r >= a.n_req) return;
-    Seq s = seq_of(a, r);
-    TileKeys sp(a, s);
-    int64_t rbase = found_base, head = sp.before(sp.tiles);       // of the request; units of one KV head
-    uint32_t kvh = (uint32_t)((u0 - rbase) / head);
-    int64_t t = 0;
+    int64_t u = (int64_t)lane64((uint64_t)found_base, 0);
     {
-        const int64_t in = (u0 - rbase) - kvh * head;
-        int64_t lo = 0, hi = sp.tiles;                // before(lo) <= in < before(hi)
-        while (hi - lo > 1) {
-            const int64_t mid = (lo + hi) / 2;
-            if (sp.before(mid) <= in) lo = mid;
+        // the KV head, then the tile, that u0 falls into
+        const TileKeys k = TileKeys::of<D>(a, seq_of(a, r));
+        const int64_t head = k.all();
+        uint32_t hi = a.num_kv;
+        while (hi - kvh > 1) {
+            const uint32_t mid = (kvh + hi) / 2;
+            if (u + mid * head <= u0) kvh = mid;
             else hi = mid;
         }
-        t = lo;
+        u += kvh * head;
+        hi = k.tiles;
+        while (hi - t > 1) {
+            const uint32_t mid = (t + hi) / 2;
+            if (u + k.before(mid) <= u0) t = mid;
+            else hi = mid;
+        }
+        u += k.before(t);
     }
-    int64_t u = rbase + kvh * head + sp.before(t);
     while (u < u1) {
-        const int64_t cost = sp.cost(t);
+        // made again for every tile, so that little is held in registers meanwhile
+        Work w;
+        w.s = seq_of(a, r);
+        const TileKeys k = TileKeys::of<D>(a, w.s);
+        const int64_t cost = k.cost(t);
         const int64_t from = u < u0 ? snapped(u0 - u, cost) : 0, to = u1 - u < cost ? snapped(u1 - u, cost) : cost;
         if (from < to) {
-            Work w;
-            w.s = s;
             w.table = a.tables + (size_t)r * a.max_blocks;
             w.kvh = kvh;
             w.token = (int)(t * a.tokens);
-            w.tile_row = s.row + w.token;
-            const int tokens = min(s.n - w.token, (int)a.tokens);
+            w.tile_row = w.s.row + w.token;
+            const int tokens = min(w.s.n - w.token, (int)a.tokens), lo = (int)k.lo(t);
             w.rows = (uint32_t)tokens * a.gqa;
-            const int lo = (int)sp.lo(t);
-            w.limit = a.mask_words ? (int)sp.hi(t) : max(0, s.have + w.token + tokens);
+            const int limit = a.mask_words ? (int)k.hi(t) : max(0, w.s.have + w.token + tokens);
             // cuts at whole chunks of 32 keys
-            w.key0 = from ? (int)((lo + (from - kTileCost / 2) + 31) / 32 * 32) : lo / 32 * 32;
-            w.key1 = to < cost ? min((int)((lo + (to - kTileCost / 2) + 31) / 32 * 32), w.limit) : w.limit;
-            w.part = from ? 2 * share : (to < cost ? 2 * share + 1 : -1);
+            w.key0 = from ? (int)((lo + k.keys_at(t, from) + 31) >> 5 << 5) : lo >> 5 << 5;
+            w.key1 = to < cost ? min((int)((lo + k.keys_at(t, to) + 31) >> 5 << 5), limit) : limit;
+            w.part = from ? (int)(2 * share) : (to < cost ? (int)(2 * share + 1) : -1);
             if (from && to == cost && tid == 0) {
                 // the share that begins this tile: the last whose first cut is at or before it
                 uint32_t first = share;
@@ -702,7 +876,7 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
             f(w);
         }
         u += cost;
-        if (++t < sp.tiles) continue;
+        if (++t < k.tiles) continue;
         t = 0;
         if (++kvh < a.num_kv) continue;
         kvh = 0;
@@ -715,14 +889,12 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
             }
         }
         if (r >= a.n_req) break;
-        s = seq_of(a, r);
-        sp = TileKeys(a, s);
     }
 }
 
 template <int D>
 __global__ __launch_bounds__(kThreads) void k_packed_attn(Packed a) {
-    extern __shared__ __align__(16) unsigned char sh[];
+    extern __shared__ __align__(1024) unsigned char sh[];
     each_work<D>(a, [&](const Work &w) { Tile<D>(a, w, *(TileLds<D> *)sh).run(); });
 }
 
@@ -766,7 +938,8 @@ __global__ __launch_bounds__(256) void k_packed_join(Packed a) {
             }
         }
         const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        float *to = a.out + ((size_t)(j.row + row / a.gqa) * a.num_q + j.kvh * a.gqa + row % a.gqa) * D + 4 * lane;
+        const uint32_t token = token_of(a, row);
+        float *to = a.out + ((size_t)(j.row + token) * a.num_q + j.kvh * a.gqa + row - token * a.gqa) * D + 4 * lane;
 #pragma unroll
         for (int k = 0; k < N; ++k) *(f4q *)(to + 256 * k) = o[k] * inv;
     }
@@ -827,6 +1000,8 @@ static int packed_attn(chn_ctx *ctx, const float *q, const float *k_cache, const
     a.kv_dim = kv_dim;
     a.gqa = gqa_ratio;
     a.tokens = tile_rows(head_dim) / gqa_ratio;
+    a.per_gqa = 65536 / gqa_ratio + 1;
+    a.per_tokens = (uint32_t)((1ull << 32) / a.tokens) + 1;      // exact for the up to 2^24 rows
     // no list is longer than 2^31 - 1
     a.window = (int)std::min(window, 0x7FFFFFFFu);
     a.c = (float)c;
