@@ -87,7 +87,9 @@ struct TileKeys {
         k.tiles = __umulhi((uint32_t)s.n + a.tokens - 1, a.per_tokens);
         k.s0 = k.tiles;
         k.full = a.tokens * a.gqa > tile_rows(D) / 2;
-        k.last_full = (s.n - (k.tiles - 1) * a.tokens) * a.gqa > tile_rows(D) / 2;
+        // of many tiles the last counts as the others: where shares are whole tiles, the workgroups of an XCD then walk the
+        // same keys together (2000 tokens behind 30000: 3.52 ms, 3.85 with the last of 32 tiles a third shorter)
+        k.last_full = k.tiles > 8 ? k.full : (s.n - (k.tiles - 1) * a.tokens) * a.gqa > tile_rows(D) / 2;
         if (a.mask_words) {
             k.T = 0;
             k.hi0 = max(0, min(s.len, s.have + (int)(32 * a.mask_words)));
@@ -310,11 +312,13 @@ __device__ __forceinline__ f4q load4(mem_t p) { return *(const __attribute__((ad
 // LDS of a workgroup: 32 keys in the order in which the instructions read
 // them, and their scales' inverses.
 //  K: [tile of 16 keys][step of 32 dims][hi, lo][64 lanes][8 dims]; lane 16 g +
-//     key holds dims 8 g .. + 7 of the step, at place key ^ (4 (step % 4) + g),
-//     so that 16 neighbouring lanes of the store fill 256 bytes
+//     key holds dims 4 g .. + 3 and 16 + 4 g .. + 3 of the step (the query's
+//     lanes then load 64 bytes of a row together), at place key ^ (4 (step % 4)
+//     + g), so that neighbouring lanes of a store fill 256 bytes
 //  V: [16 dims][hi, lo][64 lanes][8 keys]; lane 16 g + c holds keys 4 g .. + 3
 //     and 16 + 4 g .. + 3, the keys whose weights lane 16 g + row has after the
-//     score's product
+//     score's product; of 64 dims, tile e holds dims e, 4 + e, 8 + e .. in the
+//     order in which a result's lanes store 64 bytes of a row together
 template <int D>
 struct TileLds {
     static constexpr int kKeyBytes = 32 * D * 4;
@@ -391,7 +395,8 @@ struct Tile {
         g = lane >> 4;
         keys = 4 * (wave >> 1) + 16 * (wave & 1);
         worst = 0;
-        k_to = lds_addr(lds.k) + (((wave & 1) * S + (lane >> 3)) * 2) * 1024 + (lane >> 1 & 3) * 256 + (((keys ^ (lane >> 1)) & 15) * 16) + (lane & 1) * 8;
+        const int quad = 4 * (lane >> 3) + (lane & 3);
+        k_to = lds_addr(lds.k) + (((wave & 1) * S + (lane >> 3)) * 2) * 1024 + (lane & 3) * 256 + (((keys ^ quad) & 15) * 16) + (lane >> 2 & 1) * 8;
         v_to = lds_addr(lds.v) + 4 * (lane >> 4) * 2048 + ((wave >> 1) * 16 + (4 * (lane & 3) + (lane >> 2 & 3))) * 16 + (wave & 1) * 8;
     }
     __device__ __forceinline__ f4q (&vr())[4][H] {
@@ -445,7 +450,7 @@ struct Tile {
         }
         if (lane == 0) *(f4q *)(inverses + keys) = inverse;
     }
-    // key i of the wave's; a lane's eight dims lie at place key ^ (lane / 2)
+    // key i of the wave's
     __device__ __forceinline__ void store_k(int i, float scale) {
         const uint32_t at = opaque_u32(k_to) ^ (i * 16);
 #pragma unroll
@@ -491,12 +496,12 @@ struct Tile {
         float qinv = 0.0f;
         {
             // asked for before K and V, whose addresses wait for the table
-            const mem_t from = (mem_t)a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + (valid ? row : 0) - of_tile * a.gqa) * D + 256 * half + 8 * g;
+            const mem_t from = (mem_t)a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + (valid ? row : 0) - of_tile * a.gqa) * D + 256 * half + 4 * g;
             f4q x[8][2];
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int e = 0; e < 2; ++e) x[i][e] = load4(from + 32 * i + 4 * e);
+                for (int e = 0; e < 2; ++e) x[i][e] = load4(from + 32 * i + 16 * e);
             __builtin_amdgcn_sched_barrier(0);
             if (chunks) {
                 none0 = load_k(0);
@@ -898,8 +903,9 @@ __global__ __launch_bounds__(kThreads) void k_packed_attn(Packed a) {
     each_work<D>(a, [&](const Work &w) { Tile<D>(a, w, *(TileLds<D> *)sh).run(); });
 }
 
-// Joins the parts of the tiles that were cut: a wave takes a row at a time, a
-// lane four values per 256 dims.
+// Joins the parts of the tiles that were cut: a wave takes four rows
+// together, 16 lanes the parts of one (of up to 16 at a time), a lane four
+// values of each per 256 dims.
 constexpr uint32_t kJoinRows = 16;
 template <int D>
 __global__ __launch_bounds__(256) void k_packed_join(Packed a) {
@@ -907,41 +913,50 @@ __global__ __launch_bounds__(256) void k_packed_join(Packed a) {
     constexpr int N = D / 256;
     const int lane = threadIdx.x & 63;
     const Joined j = a.joined[blockIdx.x / (R / kJoinRows)];
-    const uint32_t row0 = blockIdx.x % (R / kJoinRows) * kJoinRows;
-    for (uint32_t row = row0 + (threadIdx.x >> 6); row < min(row0 + kJoinRows, j.rows); row += 4) {
-        // the first part is its share's last tile, the others are their shares' first
-        const auto at = [&](uint32_t p) { return (size_t)(p == j.first ? 2 * p + 1 : 2 * p) * R + row; };
-        float M = kNoScore;
-        for (uint32_t p = j.first + lane; p <= j.last; p += 64) M = fmaxf(M, a.pm[at(p)]);
-        M = wave_max64(M);
-        const float ref = M == kNoScore ? 0.0f : M;
-        float L = 0.0f;
-        f4q o[N];
-        for (int k = 0; k < N; ++k) o[k] = f4q{0, 0, 0, 0};
-        for (uint32_t p0 = j.first; p0 <= j.last; p0 += 64) {
-            const uint32_t n = min(j.last + 1 - p0, 64u);
-            float w = 0.0f;
-            if ((uint32_t)lane < n) {
-                const size_t i = at(p0 + lane);
-                const float part = a.pl[i];
-                if (part != 0.0f) w = __builtin_amdgcn_exp2f((a.pm[i] - ref) * a.c) * part;      // NaN: whatever its reference is
-            }
-            L += wave_sum64(w);
-            for (uint32_t i = 0; i < n; ++i) {
-                const float wi = lane_f(w, i);
-                const float *v = a.po + at(p0 + i) * D + 4 * lane;
+    const uint32_t row0 = blockIdx.x % (R / kJoinRows) * kJoinRows + 4 * (threadIdx.x >> 6);
+    if (row0 >= j.rows) return;                                  // a whole wave
+    const uint32_t rows = min(j.rows - row0, 4u), mine = row0 + min((uint32_t)lane >> 4, rows - 1);
+    // the first part is its share's last tile, the others are their shares' first
+    const auto at = [&](uint32_t p, uint32_t row) { return (size_t)(p == j.first ? 2 * p + 1 : 2 * p) * R + row; };
+    float M = kNoScore;
+    for (uint32_t p = j.first + (lane & 15); p <= j.last; p += 16) M = fmaxf(M, a.pm[at(p, mine)]);
+    M = row16_max(M);
+    const float ref = M == kNoScore ? 0.0f : M;
+    float L = 0.0f;
+    f4q o[4][N];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int k = 0; k < N; ++k) o[i][k] = f4q{0, 0, 0, 0};
+    for (uint32_t p0 = j.first; p0 <= j.last; p0 += 16) {
+        const uint32_t n = min(j.last + 1 - p0, 16u);
+        float w = 0.0f;
+        if ((uint32_t)(lane & 15) < n) {
+            const size_t i = at(p0 + (lane & 15), mine);
+            const float part = a.pl[i];
+            if (part != 0.0f) w = __builtin_amdgcn_exp2f((a.pm[i] - ref) * a.c) * part;      // NaN: whatever its reference is
+        }
+        L += row16_sum(w);
+        for (uint32_t p = 0; p < n; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float wi = lane_f(w, 16 * i + p);
+                const float *v = a.po + at(p0 + p, row0 + min((uint32_t)i, rows - 1)) * D + 4 * lane;
 #pragma unroll
                 for (int k = 0; k < N; ++k) {
                     const f4q x = *(const f4q *)(v + 256 * k);
-                    if (wi != 0.0f) o[k] += wi * x;                // a part without keys holds nothing
+                    o[i][k] += wi != 0.0f ? wi * x : f4q{0, 0, 0, 0};      // a part without keys holds nothing
                 }
             }
-        }
-        const float inv = L != 0.0f ? 1.0f / L : 0.0f;
-        const uint32_t token = token_of(a, row);
+    }
+    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 4; ++i) {
+        if (i >= rows) break;
+        const uint32_t row = row0 + i, token = token_of(a, row);
         float *to = a.out + ((size_t)(j.row + token) * a.num_q + j.kvh * a.gqa + row - token * a.gqa) * D + 4 * lane;
 #pragma unroll
-        for (int k = 0; k < N; ++k) *(f4q *)(to + 256 * k) = o[k] * inv;
+        for (int k = 0; k < N; ++k) *(f4q *)(to + 256 * k) = o[i][k] * lane_f(inv, 16 * i);
     }
 }
 
