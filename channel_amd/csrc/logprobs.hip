@@ -21,11 +21,10 @@ typedef float f4l __attribute__((ext_vector_type(4), aligned(4)));
 constexpr uint32_t kScoreMaxV = 1u << 20;
 constexpr uint32_t kScoreStretch = 2048, kScoreBlock = 256;
 constexpr uint32_t kScoreTop = 64;
-constexpr uint32_t kScoreThreads = 1024;
+constexpr uint32_t kScoreThreads = 256;
 constexpr uint32_t kScoreRows = 1024;        // rows that share the workspace
 constexpr uint32_t kBlockBits = 12;
 static_assert(kScoreMaxV / kScoreBlock == 1u << kBlockBits, "a block's number");
-constexpr uint32_t kScoreKeys = (1u << kBlockBits) / kScoreThreads;      // of a thread
 
 struct LogProbs {
     const float *logits;
@@ -59,7 +58,7 @@ template <bool CAP>
 __device__ __forceinline__ float capped(float l, float cap, float inv_cap) {
     if (!CAP) return l;
     const float t = __builtin_amdgcn_exp2f(-2.8853900817779268f * fabsf(l * inv_cap));
-    return copysignf(cap * ((1.0f - t) / (1.0f + t)), l);
+    return copysignf(cap * ((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t)), l);
 }
 template <bool CAP>
 __device__ __forceinline__ double capped64(float l, float cap) {
@@ -75,7 +74,43 @@ __device__ __forceinline__ float powers_of(const LogProbs &a, uint32_t row, bool
 __device__ __forceinline__ float distance(float v, float top, float powers) {
     return v == top ? 0.0f : fmaxf((v - top) * powers, -200.0f);
 }
+// the larger; m if v is NaN
+__device__ __forceinline__ float larger_of(float v, float m) { return __builtin_amdgcn_fmed3f(v, m, __builtin_inff()); }
+template <int CTRL>
+__device__ __forceinline__ float max_row(float v) {
+    return larger_of(__builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true)), v);
+}
+// Exchanges halves (rows) of two registers; an empty asm keeps this compiler from taking the second result for the first.
+__device__ __forceinline__ float max_of_halves(float x, float y) {       // low half: x's, high half: y's
+    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), false, false);
+    uint32_t a = r[0], b = r[1];
+    __asm__("" : "+v"(a), "+v"(b));
+    return larger_of(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+__device__ __forceinline__ float max_of_rows(float x, float y) {         // even rows: x's, odd rows: y's
+    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(uint32_t, x), __builtin_bit_cast(uint32_t, y), false, false);
+    uint32_t a = r[0], b = r[1];
+    __asm__("" : "+v"(a), "+v"(b));
+    return larger_of(__builtin_bit_cast(float, a), __builtin_bit_cast(float, b));
+}
+// The largest of each of eight values over the wave: lanes 8 i .. 8 i + 7 get that of v[order(i)].
+__device__ __forceinline__ float wave_max8(const float (&v)[8], int lane) {
+    float h[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) h[i] = max_of_halves(v[i], v[i + 4]);                    // halves: i, i + 4
+    const float a = max_of_rows(h[0], h[1]), b = max_of_rows(h[2], h[3]);              // rows: 0 1 4 5, 2 3 6 7
+    const float keep = lane & 8 ? b : a, give = lane & 8 ? a : b;
+    float m = larger_of(__builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, give), 0x128, 0xF, 0xF, true)), keep);
+    m = max_row<0xB1>(m);                                                              // quad_perm [1,0,3,2], [2,3,0,1]
+    m = max_row<0x4E>(m);
+    return max_row<0x141>(m);                                                          // row_half_mirror
+}
+__device__ __forceinline__ int max8_order(int i) {                       // the value whose maximum lanes 8 i hold
+    return (i >> 2) * 4 + (i & 1) * 2 + (i >> 1 & 1);
+}
 
+// A wave's 2048 values: 256 a load, four of them a lane.  Bound by memory where
+// there are many rows.
 template <bool CAP>
 __global__ __launch_bounds__(256) void k_logprob_sums(LogProbs a) {
     const uint32_t row = blockIdx.y, s = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -84,55 +119,75 @@ __global__ __launch_bounds__(256) void k_logprob_sums(LogProbs a) {
     const float *x = a.logits + (size_t)row * a.ld;
     const uint32_t i0 = s * kScoreStretch + 4 * lane;
     f4l v[8];
+    if ((s + 1) * kScoreStretch <= a.V) {
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        const uint32_t i = i0 + 256 * j;
-        if (i + 4 <= a.V) v[j] = *(const f4l *)(x + i);
-        else
+        for (int j = 0; j < 8; ++j) v[j] = *(const f4l *)(x + i0 + 256 * j);
+    } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[j][e] = i + e < a.V ? x[i + e] : __builtin_nanf("");
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t i = i0 + 256 * j + e;
+                const float l = x[min(i, a.V - 1)];
+                v[j][e] = i < a.V ? l : __builtin_nanf("");
+            }
     }
     const uint32_t target = a.targets[row];
     const float mine = target < a.V ? x[target] : __builtin_nanf("");
     bool greedy;
     const float powers = powers_of(a, row, greedy), cap = a.cap, inv_cap = 1.0f / cap;
-    float top = -__builtin_inff();
-    uint32_t before = 0;
+    float m[8];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        float m = -__builtin_inff();
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t i = i0 + 256 * j + e;
-            before += scored(v[j][e]) && (v[j][e] > mine || (v[j][e] == mine && i < target));
-            m = fmaxf(m, scored(v[j][e]) ? v[j][e] : -__builtin_inff());
-        }
-        if (a.n_top) {
-            const float b = wave_max64(m);
-            const uint32_t block = s * (kScoreStretch / kScoreBlock) + j;
-            if (lane == 0 && block < a.blocks) a.bmax[(size_t)row * a.blocks + block] = scored(b) ? ordered(b) : 0u;
-        }
-        top = fmaxf(top, m);
+    for (int j = 0; j < 8; ++j) m[j] = larger_of(v[j][3], larger_of(v[j][2], larger_of(v[j][1], larger_of(v[j][0], -__builtin_inff()))));
+    const float most = wave_max8(m, lane);
+    const size_t at = (size_t)row * a.stretches + s;
+    if (a.n_top && (lane & 7) == 0) {
+        const uint32_t block = s * (kScoreStretch / kScoreBlock) + max8_order(lane >> 3);
+        if (block < a.blocks) a.bmax[(size_t)row * a.blocks + block] = scored(most) ? ordered(most) : 0u;
     }
-    top = wave_max64(top);
-    before = (uint32_t)wave_sum_u64(before);
-    float S = 0.0f, X = 0.0f;
-    if (scored(top) && !greedy) {
-        const float ref = capped<CAP>(top, cap, inv_cap);
+    const float top = wave_max64(most);
+    // NaN compares false, and what is barred lies below a given token that is not
+    uint32_t before = 0;
+    if (scored(mine)) {
 #pragma unroll
         for (int j = 0; j < 8; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const float d = distance(capped<CAP>(v[j][e], cap, inv_cap), ref, powers);
-                const float p = scored(v[j][e]) ? __builtin_amdgcn_exp2f(d) : 0.0f;
-                S += p;
-                X = scored(v[j][e]) ? fmaf(p, d, X) : X;
-            }
+            for (int e = 0; e < 4; ++e) before += (uint32_t)__popcll(__ballot(v[j][e] > mine));
+        uint32_t same = 0;
+#pragma unroll
+        for (int j = 0; j < 8; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) same += v[j][e] == mine && i0 + 256 * j + e < target;
+        if (__any(same)) before += (uint32_t)wave_sum_u64(same);
+    }
+    float S = 0.0f, X = 0.0f;
+    if (scored(top) && !greedy) {
+        const float ref = capped<CAP>(top, cap, inv_cap);
+        if (fabsf(ref) <= 1e30f && powers >= 1e-6f && powers <= 1e30f) {
+            // barred values lie 200 powers below and more, NaN is taken for that
+#pragma unroll
+            for (int j = 0; j < 8; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    const float d = larger_of((capped<CAP>(v[j][e], cap, inv_cap) - ref) * powers, -200.0f);
+                    float p = __builtin_amdgcn_exp2f(d);
+                    if (CAP) p = scored(v[j][e]) ? p : 0.0f;              // -inf is capped too
+                    S += p;
+                    X = fmaf(p, d, X);
+                }
+        } else {
+            for (int j = 0; j < 8; ++j)
+                for (int e = 0; e < 4; ++e) {
+                    const float d = distance(capped<CAP>(v[j][e], cap, inv_cap), ref, powers);
+                    const float p = scored(v[j][e]) ? __builtin_amdgcn_exp2f(d) : 0.0f;
+                    S += p;
+                    X += scored(v[j][e]) ? p * d : 0.0f;
+                }
+        }
         S = wave_sum64(S);
         X = wave_sum64(X);
     }
     if (lane == 0) {
-        const size_t at = (size_t)row * a.stretches + s;
         a.smax[at] = scored(top) ? ordered(top) : 0u;
         a.ahead[at] = before;
         a.sum[at] = S;
@@ -140,67 +195,49 @@ __global__ __launch_bounds__(256) void k_logprob_sums(LogProbs a) {
     }
 }
 
-// Sums and maxima over the workgroup, the same bits for every thread.
+// What a row's workgroup exchanges.
+constexpr int kScoreWaves = kScoreThreads / 64;
 struct RowSums {
-    float part[kScoreThreads / 64];
-    uint32_t count[kScoreThreads / 64];
-    uint64_t counts[2][kScoreThreads / 64];
+    float sum[kScoreWaves], xsum[kScoreWaves];
+    uint32_t most[kScoreWaves], before[kScoreWaves];
+    uint32_t counts[2][kScoreWaves][4];
 };
-__device__ __forceinline__ float group_sum(RowSums &sh, float v) {
-    v = wave_sum64(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.part[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return row16_sum(sh.part[threadIdx.x & 15]);
-}
-__device__ __forceinline__ uint32_t group_sum(RowSums &sh, uint32_t v) {
-    v = (uint32_t)wave_sum_u64(v);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.count[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint32_t t = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kScoreThreads / 64; ++i) t += sh.count[i];
-    return t;
-}
-__device__ __forceinline__ uint32_t group_max(RowSums &sh, uint32_t v) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = max(v, (uint32_t)__shfl_xor(v, o, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) sh.count[threadIdx.x >> 6] = v;
-    __syncthreads();
-    uint32_t t = 0;
-#pragma unroll
-    for (uint32_t i = 0; i < kScoreThreads / 64; ++i) t = max(t, sh.count[i]);
-    return t;
-}
 
-// The n-th largest of unique keys below 2^BITS (0: none), from the top bits
-// down, two at a time: each(f) calls f(key) for the thread's keys.  0 where
-// there are fewer than n.
+// The n-th largest of unique keys below 2^BITS (0: none), or any bound that n
+// of them reach, from the top bits down, two at a time: each(f) calls f(key)
+// for the thread's keys, the same number of times in every lane.  0 where there
+// are fewer than n.
 template <int BITS, typename F>
 __device__ __forceinline__ uint64_t nth_largest(RowSums &sh, uint32_t n, F &&each) {
     uint64_t least = 0;
     for (int bit = BITS - 2, turn = 0; bit >= 0; bit -= 2, turn ^= 1) {
         const uint64_t step = 1ull << bit;
-        uint64_t mine = 0;                                     // three counts of 20 bits
+        uint32_t c[3] = {0, 0, 0};
         each([&](uint64_t key) {
-            mine += (uint64_t)(key >= least + step) + ((uint64_t)(key >= least + 2 * step) << 20) +
-                    ((uint64_t)(key >= least + 3 * step) << 40);
+#pragma unroll
+            for (int i = 0; i < 3; ++i) c[i] += (uint32_t)__popcll(__ballot(key >= least + (i + 1) * step));
         });
-        mine = wave_sum_u64(mine);
-        if ((threadIdx.x & 63) == 0) sh.counts[turn][threadIdx.x >> 6] = mine;
+        if ((threadIdx.x & 63) == 0)
+#pragma unroll
+            for (int i = 0; i < 3; ++i) sh.counts[turn][threadIdx.x >> 6][i] = c[i];
         __syncthreads();
-        const uint64_t all = lane64(row16_scan_u64(sh.counts[turn][threadIdx.x & 15]), 15);
-        const uint32_t c1 = (uint32_t)all & 0xFFFFF, c2 = (uint32_t)(all >> 20) & 0xFFFFF, c3 = (uint32_t)(all >> 40);
-        least += (c3 >= n ? 3 : c2 >= n ? 2 : c1 >= n ? 1 : 0) * step;
+#pragma unroll
+        for (int i = 0; i < 3; ++i) {
+            c[i] = 0;
+#pragma unroll
+            for (int w = 0; w < kScoreWaves; ++w) c[i] += sh.counts[turn][w][i];
+        }
+        const int take = c[2] >= n ? 3 : c[1] >= n ? 2 : c[0] >= n ? 1 : 0;
+        least += take * step;
+        if (take && c[take - 1] == n) break;
     }
     return least;
 }
 
-constexpr uint32_t kScoreFew = 512;          // keys that are ranked by counting
+constexpr uint32_t kScoreFew = 256;          // keys that are ranked by counting
 
-template <bool CAP>
+// KEYS: block maxima of a thread.
+template <bool CAP, int KEYS>
 __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
     extern __shared__ uint64_t list[];                          // n_top * kScoreBlock keys
     __shared__ RowSums sh;
@@ -215,75 +252,113 @@ __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
     const float powers = powers_of(a, row, greedy), inv_cap = 1.0f / a.cap;
     if (tid == 0) n_chosen = n_list = n_few = 0;
 
-    // the stretches: at most 512, a thread each
-    uint32_t m = 0, before = 0;
-    float S = 0.0f, X = 0.0f;
-    if (tid < a.stretches) {
-        const size_t at = (size_t)row * a.stretches + tid;
-        m = a.smax[at];
-        before = a.ahead[at];
-        S = a.sum[at];
-        X = a.xsum[at];
+    // the stretches: at most 512, two a thread; the blocks' maxima
+    uint32_t m[2], before = 0;
+    float S[2], X[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+        const uint32_t s = tid + kScoreThreads * i;
+        const size_t at = (size_t)row * a.stretches + min(s, a.stretches - 1);
+        const bool there = s < a.stretches;
+        m[i] = there ? a.smax[at] : 0u;
+        before += there ? a.ahead[at] : 0u;
+        S[i] = a.sum[at];
+        X[i] = a.xsum[at];
     }
-    const uint32_t most = group_max(sh, m);
+    uint64_t key[KEYS];
+    if (a.n_top) {
+        const uint32_t *bmax = a.bmax + (size_t)row * a.blocks;
+#pragma unroll
+        for (uint32_t k = 0; k < KEYS; ++k) {
+            const uint32_t b = tid + kScoreThreads * k, o = b < a.blocks ? bmax[b] : 0u;
+            key[k] = o ? (uint64_t)o << kBlockBits | ((1u << kBlockBits) - 1 - b) : 0;
+        }
+    }
+    uint32_t most = max(m[0], m[1]);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) most = max(most, (uint32_t)__shfl_xor(most, o, 64));
+    if (lane == 0) sh.most[wave] = most;
+    __syncthreads();
+#pragma unroll
+    for (int w = 0; w < kScoreWaves; ++w) most = max(most, sh.most[w]);
     const float top = unordered(most);
-    if (most && m) {
-        const float d = distance(capped<CAP>(unordered(m), a.cap, inv_cap), capped<CAP>(top, a.cap, inv_cap), powers);
-        const float f = __builtin_amdgcn_exp2f(d);
-        X = f * (X + d * S);
-        S *= f;
+    float sum = 0.0f, xsum = 0.0f;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+        if (m[i]) {
+            const float d = distance(capped<CAP>(unordered(m[i]), a.cap, inv_cap), capped<CAP>(top, a.cap, inv_cap), powers);
+            const float f = __builtin_amdgcn_exp2f(d);
+            xsum += f * (X[i] + d * S[i]);
+            sum += f * S[i];
+        }
+    sum = wave_sum64(sum);
+    xsum = wave_sum64(xsum);
+    before = (uint32_t)wave_sum_u64(before);
+    if (lane == 0) {
+        sh.sum[wave] = sum;
+        sh.xsum[wave] = xsum;
+        sh.before[wave] = before;
     }
-    S = group_sum(sh, S);
-    X = group_sum(sh, X);
-    before = group_sum(sh, before);
-    const double log_sum = greedy ? 0.0 : log((double)S);
-    // of an allowed logit that `first` tokens come before
+    __syncthreads();
+    sum = xsum = 0.0f;
+    before = 0;
+#pragma unroll
+    for (int w = 0; w < kScoreWaves; ++w) {
+        sum += sh.sum[w];
+        xsum += sh.xsum[w];
+        before += sh.before[w];
+    }
+    const double log_sum = greedy ? 0.0 : log((double)sum);
+    // of an allowed logit; `first`: no token comes before it
     const auto logp = [&](float l, bool first) {
         if (greedy) return first ? 0.0f : -__builtin_inff();
         const double T = a.temperature ? (double)a.temperature[row] : 1.0;
         return (float)((l == top ? 0.0 : (capped64<CAP>(l, a.cap) - capped64<CAP>(top, a.cap)) / T) - log_sum);
     };
-    if (tid == 0) {
+    if (wave == kScoreWaves - 1 && lane == 0) {
         const bool given = target < a.V, ok = most && scored(mine);
         a.logp[row] = !given ? 0.0f : ok ? logp(mine, before == 0) : -__builtin_inff();
-        if (a.entropy) a.entropy[row] = most && !greedy ? (float)(log_sum - 0.69314718055994531 * (double)X / (double)S) : 0.0f;
+        if (a.entropy) a.entropy[row] = most && !greedy ? (float)(log_sum - 0.69314718055994531 * (double)xsum / (double)sum) : 0.0f;
         if (a.ranks) a.ranks[row] = ok ? before : CHN_NO_TOKEN;
     }
     if (!a.n_top) return;
 
     // the blocks with the largest maxima, equal ones by lower number
-    const uint32_t *bmax = a.bmax + (size_t)row * a.blocks;
-    uint64_t key[kScoreKeys];
-#pragma unroll
-    for (uint32_t k = 0; k < kScoreKeys; ++k) {
-        const uint32_t b = tid + kScoreThreads * k, o = b < a.blocks ? bmax[b] : 0u;
-        key[k] = o ? (uint64_t)o << kBlockBits | ((1u << kBlockBits) - 1 - b) : 0;
-    }
     const uint64_t least = nth_largest<32 + kBlockBits>(sh, a.n_top, [&](auto &&f) {
 #pragma unroll
-        for (uint32_t k = 0; k < kScoreKeys; ++k) f(key[k]);
+        for (int k = 0; k < KEYS; ++k) f(key[k]);
     });
 #pragma unroll
-    for (uint32_t k = 0; k < kScoreKeys; ++k)
+    for (int k = 0; k < KEYS; ++k)
         if (key[k] && key[k] >= least) chosen[atomicAdd(&n_chosen, 1u)] = tid + kScoreThreads * k;
     __syncthreads();
+    // the bound's bits above the block's number: of the n_top values that reach it, none is below
     const uint32_t floor_key = (uint32_t)(least >> kBlockBits);
-    for (uint32_t c = wave; c < n_chosen; c += kScoreThreads / 64) {
-        const uint32_t i0 = chosen[c] * kScoreBlock + 4 * lane;
+    for (uint32_t c = wave; c < n_chosen; c += 2 * kScoreWaves) {
+        // two blocks in flight
+        float v[2][4];
+        uint32_t i0[2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            const uint32_t i = i0 + e;
-            const float v = x[min(i, a.V - 1)];
-            if (i < a.V && scored(v) && ordered(v) >= floor_key)
-                list[atomicAdd(&n_list, 1u)] = (uint64_t)ordered(v) << 32 | (0xFFFFFFFFu - i);
+        for (int h = 0; h < 2; ++h) {
+            i0[h] = chosen[min(c + kScoreWaves * h, n_chosen - 1)] * kScoreBlock + 4 * lane;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[h][e] = x[min(i0[h] + e, a.V - 1)];
         }
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t i = i0[h] + e;
+                if (c + kScoreWaves * h < n_chosen && i < a.V && scored(v[h][e]) && ordered(v[h][e]) >= floor_key)
+                    list[atomicAdd(&n_list, 1u)] = (uint64_t)ordered(v[h][e]) << 32 | (0xFFFFFFFFu - i);
+            }
     }
     __syncthreads();
     const uint64_t *keys = list;
     uint32_t n = n_list;
     if (n > kScoreFew) {
         const uint64_t last = nth_largest<64>(sh, a.n_top, [&](auto &&f) {
-            for (uint32_t i = tid; i < n; i += kScoreThreads) f(list[i]);
+            for (uint32_t i = tid; i < (n + kScoreThreads - 1) / kScoreThreads * kScoreThreads; i += kScoreThreads) f(i < n ? list[i] : 0);
         });
         for (uint32_t i = tid; i < n; i += kScoreThreads)
             if (list[i] >= last) few[atomicAdd(&n_few, 1u)] = list[i];       // n_top of them
@@ -311,7 +386,9 @@ __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
 template <bool CAP>
 static void launch_scores(chn_ctx *ctx, const LogProbs &a, uint32_t n) {
     k_logprob_sums<CAP><<<dim3((a.stretches + 3) / 4, n), 256, 0, ctx->stream>>>(a);
-    k_logprob_rows<CAP><<<n, kScoreThreads, (size_t)a.n_top * kScoreBlock * 8, ctx->stream>>>(a);
+    const size_t lds = (size_t)a.n_top * kScoreBlock * 8;
+    if (a.blocks <= 4 * kScoreThreads) k_logprob_rows<CAP, 4><<<n, kScoreThreads, lds, ctx->stream>>>(a);
+    else k_logprob_rows<CAP, (1 << kBlockBits) / kScoreThreads><<<n, kScoreThreads, lds, ctx->stream>>>(a);
 }
 
 }  // namespace chn
