@@ -619,7 +619,7 @@ struct Tile {
         };
         if (chunks) {
             all_k();
-            none1 = load_k(1);
+            if (chunks > 1) none1 = load_k(1);
             vnow = va;
             if (kBoth) scales(vr(), vscale, lds.vinv[0]);
             lds_barrier();
@@ -633,15 +633,17 @@ struct Tile {
                 end_scores();
             }
             lds_barrier();
-            all_k();
+            if (chunks > 1) all_k();
             if (!kBoth) {
                 if (active) add_half();
                 load(vr(), vnow, 0);
-            } else {
+            } else if (chunks > 1) {
                 none2 = load_k(2);
             }
         }
-        for (int c = 0; c < chunks; ++c) {
+        // the last chunk has no next one
+        const auto walk = [&](int c, auto more) {
+            constexpr bool kMore = decltype(more)::value;
             const float *vinv = lds.vinv[kBoth ? c & 1 : 0];
             if (c & 1) vnow = va;
             lds_barrier();
@@ -651,15 +653,19 @@ struct Tile {
                 scales(vr(), vscale, lds.vinv[0]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) store_v(e, vscale);
-                none2 = load_k(c + 2);
+                if (kMore) none2 = load_k(c + 2);
             }
             if (active) {
-                begin_scores();
-                fetch_k(0);
+                if constexpr (kMore) {
+                    begin_scores();
+                    fetch_k(0);
+                }
                 static_for<8>([&](auto step) {
                     constexpr int i = decltype(step)::value;
-                    score_step(i);
-                    if constexpr (i < 7) fetch_k(i + 1);
+                    if constexpr (kMore) {
+                        score_step(i);
+                        if constexpr (i < 7) fetch_k(i + 1);
+                    }
                     if constexpr (i == 0) {
                         const int k0 = w.key0 + 32 * c;
                         if (none0 || !__all(s.lo <= k0 && k0 + 32 <= s.hi)) {
@@ -711,14 +717,14 @@ struct Tile {
                         if (kBoth) weights(vinv);
                     }
                     if constexpr (i >= 4 && kBoth) store_v(i - 4, vscale);
-                    end_step();
+                    if constexpr (kMore) end_step();
                 });
-                end_scores();
+                if constexpr (kMore) end_scores();
             } else if (kBoth) {
 #pragma unroll
                 for (int e = 0; e < 4; ++e) store_v(e, vscale);
             }
-            if (kBoth) load(vr(), vnow, c + 1);
+            if (kBoth && kMore) load(vr(), vnow, c + 1);
             lds_barrier();
             // ---- phase 2
             if (active) {
@@ -743,24 +749,30 @@ struct Tile {
                     o[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[0], ph, o[2 * i], 0, 0, 0);
                     o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[2], ph, o[2 * i + 1], 0, 0, 0);
                     if constexpr (i < 7) fetch_v(i + 1);
-                    if constexpr (i == 2) scales(kr, scale, lds.kinv);
-                    if constexpr (i >= 3 && i < 7) store_k(i - 3, scale[i - 3]);
+                    if constexpr (kMore) {
+                        if constexpr (i == 2) scales(kr, scale, lds.kinv);
+                        if constexpr (i >= 3 && i < 7) store_k(i - 3, scale[i - 3]);
+                    }
                     end_step();
                 });
-                if (!kBoth) add_half();
-            } else {
+                if (!kBoth && kMore) add_half();
+            } else if (kMore) {
                 all_k();
             }
-            if (!kBoth) {
-                load(vr(), vnow, c + 1);
-            } else {
-                scales(vr(), vscale, lds.vinv[(c + 1) & 1]);
-                none3 = load_k(c + 3);
+            if constexpr (kMore) {
+                if (!kBoth) {
+                    load(vr(), vnow, c + 1);
+                } else {
+                    scales(vr(), vscale, lds.vinv[(c + 1) & 1]);
+                    none3 = load_k(c + 3);
+                }
+                none0 = none1;
+                none1 = none2;
+                none2 = none3;
             }
-            none0 = none1;
-            none1 = none2;
-            none2 = none3;
-        }
+        };
+        for (int c = 0; c + 1 < chunks; ++c) walk(c, std::true_type());
+        if (chunks) walk(chunks - 1, std::false_type());
         if (chunks) {
             if (__any(worst >= kNotFinite) && lane == 0) lds.not_finite = 1;
             lds_barrier();
