@@ -190,28 +190,42 @@ __device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
             o[k] = f4q{0, 0, 0, 0};
         }
         float m = kNoScore, l = 0.0f;
-        for (int pos = w.key0; pos < w.key1; ++pos) {
-            bool ok = pos >= s.lo && pos < s.hi;
-            const int node = pos - w.s.have;
-            if (s.mask && node >= 0) ok = (s.mask[node >> 5] >> (node & 31)) & 1;      // key1 is below 32 mask_words of them
-            const uint32_t slot = ok ? slot_of(a, w.table, pos) : CHN_NO_SLOT;
-            if (slot == CHN_NO_SLOT) continue;
-            const size_t at = (size_t)slot * a.kv_dim + (size_t)w.kvh * D + 4 * lane;
-            float sum = 0.0f;
-            for (int k = 0; k < N; ++k) {
-                const f4q x = *(const f4q *)(a.kc + at + 256 * k);
-                for (int e = 0; e < 4; ++e) sum = fmaf(x[e], q[k][e], sum);
+        for (int k0 = w.key0; k0 < w.key1; k0 += 32) {
+            // 32 keys from zero, then added, so that long lists keep fp32's digits
+            f4q some[N];
+            float part = 0.0f;
+            for (int k = 0; k < N; ++k) some[k] = f4q{0, 0, 0, 0};
+            for (int pos = k0; pos < min(k0 + 32, w.key1); ++pos) {
+                bool ok = pos >= s.lo && pos < s.hi;
+                const int node = pos - w.s.have;
+                if (s.mask && node >= 0) ok = (s.mask[node >> 5] >> (node & 31)) & 1;      // key1 is below 32 mask_words of them
+                const uint32_t slot = ok ? slot_of(a, w.table, pos) : CHN_NO_SLOT;
+                if (slot == CHN_NO_SLOT) continue;
+                const size_t at = (size_t)slot * a.kv_dim + (size_t)w.kvh * D + 4 * lane;
+                float sum = 0.0f;
+                for (int k = 0; k < N; ++k) {
+                    const f4q x = *(const f4q *)(a.kc + at + 256 * k);
+                    for (int e = 0; e < 4; ++e) sum = fmaf(x[e], q[k][e], sum);
+                }
+                sum = wave_sum64(sum);
+                if (sum == kNoScore) continue;                                            // no weight, whatever its V
+                if (sum > m) {
+                    const float old = m == kNoScore ? 0.0f : __builtin_amdgcn_exp2f((m - sum) * a.c);
+                    m = sum;
+                    l *= old;
+                    part *= old;
+                    for (int k = 0; k < N; ++k) {
+                        o[k] *= old;
+                        some[k] *= old;
+                    }
+                }
+                // of a NaN score, or of two infinite ones, NaN
+                const float p = __builtin_amdgcn_exp2f((sum - (m == kNoScore ? 0.0f : m)) * a.c);
+                part += p;
+                for (int k = 0; k < N; ++k) some[k] += p * *(const f4q *)(a.vc + at + 256 * k);
             }
-            sum = wave_sum64(sum);
-            const float top = fmaxf(m, sum), ref = top == kNoScore ? 0.0f : top;
-            const float old = __builtin_amdgcn_exp2f((m - ref) * a.c), p = __builtin_amdgcn_exp2f((sum - ref) * a.c);
-            const bool none = sum == kNoScore;                                       // no weight, whatever its V
-            m = top;
-            l = none ? l : l * old + p;
-            for (int k = 0; k < N; ++k) {
-                const f4q x = *(const f4q *)(a.vc + at + 256 * k);
-                if (!none) o[k] = o[k] * old + p * x;
-            }
+            l += part;
+            for (int k = 0; k < N; ++k) o[k] += some[k];
         }
         const float inv = l != 0.0f ? 1.0f / l : 0.0f;
         float *to = row_out<D>(a, w, row);
@@ -406,12 +420,11 @@ struct Tile {
 
     // chunks come in pairs, 64 keys, a lane each
     __device__ __forceinline__ uint32_t block_of(int pair) const {
-        return w.table[min(w.key0 + 64 * pair + lane, w.key1 - 1) >> a.shift];
+        return w.table[min((uint32_t)w.key0 + 64 * pair + lane, (uint32_t)w.key1 - 1) >> a.shift];
     }
     __device__ __forceinline__ void take_pair(int pair) {
-        const int pos = w.key0 + 64 * pair + lane;
-        const uint32_t b = next_block;
-        const bool held = pos < w.key1 && b < a.n_blocks;
+        const uint32_t pos = (uint32_t)w.key0 + 64 * pair + lane, b = next_block;      // unsigned: up to 2^31 and a pair
+        const bool held = pos < (uint32_t)w.key1 && b < a.n_blocks;
         const size_t at = (size_t)((b << a.shift) + (pos & ((1u << a.shift) - 1))) * a.kv_dim + (size_t)w.kvh * D;
         ka = held ? (mem_t)a.kc + at : (mem_t)no_key;
         va = held ? (mem_t)a.vc + at : (mem_t)no_key;
@@ -526,7 +539,7 @@ struct Tile {
         // rows of no token see everything, so that they never stand in a chunk's way
         Seen s = seen_by(a, w, token);
         if (!valid) {
-            s.lo = -0x7FFFFFFF;
+            s.lo = 0;
             s.hi = 0x7FFFFFFF;
         }
         f4q o[16];
@@ -668,7 +681,7 @@ struct Tile {
                     }
                     if constexpr (i == 0) {
                         const int k0 = w.key0 + 32 * c;
-                        if (none0 || !__all(s.lo <= k0 && k0 + 32 <= s.hi)) {
+                        if (none0 || !__all(s.lo <= k0 && s.hi - k0 >= 32)) {
                             // bit k: the row sees key k0 + k
                             uint32_t ok = 0xFFFFFFFFu;
                             const int from = min(max(s.lo - k0, 0), 32), to = min(max(s.hi - k0, 0), 32);
@@ -915,51 +928,70 @@ __global__ __launch_bounds__(kThreads) void k_packed_attn(Packed a) {
     each_work<D>(a, [&](const Work &w) { Tile<D>(a, w, *(TileLds<D> *)sh).run(); });
 }
 
-// Joins the parts of the tiles that were cut: a wave takes four rows
-// together, 16 lanes the parts of one (of up to 16 at a time), a lane four
-// values of each per 256 dims.
+// Joins the parts of the tiles that were cut.  A wave takes four rows
+// together: 16 lanes hold the references and denominators of one row's parts,
+// up to 16 of them at a time, and the sums (a lane four values per 256 dims) of
+// four parts are under way while those become weights.  Bound by three
+// latencies one after another (the tile, its references, nothing else where
+// there are up to four parts).
 constexpr uint32_t kJoinRows = 16;
 template <int D>
 __global__ __launch_bounds__(256) void k_packed_join(Packed a) {
     constexpr uint32_t R = tile_rows(D);
-    constexpr int N = D / 256;
+    constexpr int N = D / 256, P = 4;
     const int lane = threadIdx.x & 63;
     const Joined j = a.joined[blockIdx.x / (R / kJoinRows)];
-    const uint32_t row0 = blockIdx.x % (R / kJoinRows) * kJoinRows + 4 * (threadIdx.x >> 6);
+    const uint32_t row0 = blockIdx.x % (R / kJoinRows) * kJoinRows + 4 * __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     if (row0 >= j.rows) return;                                  // a whole wave
     const uint32_t rows = min(j.rows - row0, 4u), mine = row0 + min((uint32_t)lane >> 4, rows - 1);
     // the first part is its share's last tile, the others are their shares' first
     const auto at = [&](uint32_t p, uint32_t row) { return (size_t)(p == j.first ? 2 * p + 1 : 2 * p) * R + row; };
-    float M = kNoScore;
-    for (uint32_t p = j.first + (lane & 15); p <= j.last; p += 16) M = fmaxf(M, a.pm[at(p, mine)]);
-    M = row16_max(M);
-    const float ref = M == kNoScore ? 0.0f : M;
-    float L = 0.0f;
-    f4q o[4][N];
+    f4q o[4][N], v[P][4][N];
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
         for (int k = 0; k < N; ++k) o[i][k] = f4q{0, 0, 0, 0};
+    const auto fetch = [&](uint32_t p0) {
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int k = 0; k < N; ++k)
+                    v[p][i][k] = *(const f4q *)(a.po + at(min(p0 + p, j.last), row0 + min((uint32_t)i, rows - 1)) * D + 4 * lane + 256 * k);
+    };
+    float M = kNoScore, L = 0.0f;
     for (uint32_t p0 = j.first; p0 <= j.last; p0 += 16) {
-        const uint32_t n = min(j.last + 1 - p0, 16u);
-        float w = 0.0f;
-        if ((uint32_t)(lane & 15) < n) {
-            const size_t i = at(p0 + (lane & 15), mine);
-            const float part = a.pl[i];
-            if (part != 0.0f) w = __builtin_amdgcn_exp2f((a.pm[i] - ref) * a.c) * part;      // NaN: whatever its reference is
-        }
-        L += row16_sum(w);
-        for (uint32_t p = 0; p < n; ++p)
+        const uint32_t n = min(j.last + 1 - p0, 16u), p = min((uint32_t)lane & 15, n - 1);
+        const size_t where = at(p0 + p, mine);
+        float m = a.pm[where], part = a.pl[where];
+        __builtin_amdgcn_sched_barrier(0);
+        fetch(p0);
+        __builtin_amdgcn_sched_barrier(0);
+        if (p != ((uint32_t)lane & 15)) part = 0.0f;
+        if (part == 0.0f) m = kNoScore;                          // a part without keys has none
+        const float top = fmaxf(M, row16_max(m)), ref = top == kNoScore ? 0.0f : top;
+        // NaN: whatever its reference is
+        const float old = M == kNoScore ? 0.0f : __builtin_amdgcn_exp2f((M - ref) * a.c);
+        const float w = part != 0.0f ? __builtin_amdgcn_exp2f((m - ref) * a.c) * part : 0.0f;
+        M = top;
+        L = L * old + row16_sum(w);
+        if (p0 != j.first)
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const float wi = lane_f(w, 16 * i + p);
-                const float *v = a.po + at(p0 + p, row0 + min((uint32_t)i, rows - 1)) * D + 4 * lane;
+            for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int k = 0; k < N; ++k) {
-                    const f4q x = *(const f4q *)(v + 256 * k);
-                    o[i][k] += wi != 0.0f ? wi * x : f4q{0, 0, 0, 0};      // a part without keys holds nothing
+                for (int k = 0; k < N; ++k) o[i][k] *= lane_f(old, 16 * i);
+        for (uint32_t q = 0; q < n; q += P) {
+            if (q) fetch(p0 + q);
+#pragma unroll
+            for (int e = 0; e < P; ++e)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float wi = q + e < n ? lane_f(w, 16 * i + min(q + e, 15u)) : 0.0f;
+#pragma unroll
+                    for (int k = 0; k < N; ++k) o[i][k] += wi != 0.0f ? wi * v[e][i][k] : f4q{0, 0, 0, 0};
                 }
-            }
+        }
     }
     const float inv = L != 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll

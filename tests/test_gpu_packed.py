@@ -294,6 +294,33 @@ def test_small_values_beside_large_ones(ctx):
     assert small.max() <= 2.0 ** -17 * np.abs(b.vc[:, 1::2]).max()
 
 
+def test_long_rows_beside_a_nan_keep_their_digits(ctx):
+    """Rows of a tile that meets a NaN are recomputed key by key: they stay as exact as the others."""
+    say("long rows, NaN")
+    b = Batch(ctx, 19, [2], [20000], nq=2, bs=64)
+    b.q[1, 3] = np.nan                                                   # the second row alone
+    out, (want, _, _, _) = b.run(), b.want()
+    assert np.isnan(out[1, :256]).all() and np.isfinite(out[0]).all()
+    assert np.linalg.norm(out[0] - want[0]) <= 4e-6 * np.linalg.norm(want[0])
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_random_batches(ctx, seed):
+    """Batches of any shape: heads, groups, block sizes, windows, masks, empty and new requests, bad blocks."""
+    rng = np.random.default_rng(1000 + seed)
+    D, gqa, words = int(rng.choice([256, 512])), int(rng.integers(1, 17)), int(rng.choice([0, 0, 1, 2, 4]))
+    n = int(np.exp(rng.uniform(0, np.log(20))))
+    new = rng.integers(0, min(32 * words if words else 150, 900 // n) + 1, n)
+    have = np.where(rng.random(n) < 0.3, 0, rng.integers(0, 900 // n + 2, n))
+    window = int(rng.choice([0, 0, 128, int(rng.integers(128, 400))])) if words else int(rng.choice([0, 0, 1, 40, int(rng.integers(1, 400))]))
+    shape = dict(D=D, gqa=gqa, nq=gqa * int(rng.integers(1, 3)), bs=int(2 ** rng.integers(0, 8)), words=words, window=window)
+    say("random", seed, shape, new.tolist(), have.tolist())
+    b = Batch(ctx, 2000 + seed, new, have, **shape)
+    if seed % 4 == 3:
+        b.tables[rng.random(b.tables.shape) < 0.1] = BAD
+    b.check()
+
+
 DRAFTS = [([1], 1), ([32, 0, 5], 1), ([33, 40], 1), ([64, 1, 2, 3], 2), ([100, 70, 65], 3), ([128], 4), ([256, 255, 31], 8),
           ([300, 600], 8), ([5] * 600, 1), ([0, 0], 2)]
 
