@@ -242,6 +242,7 @@ __device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
 // ---------------------------------------------------------------------
 typedef _Float16 h8 __attribute__((ext_vector_type(8)));
 typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+typedef _Float16 h2 __attribute__((ext_vector_type(2)));
 
 // What keys that are nobody's read.
 static __device__ __align__(16) const float no_key[512] = {};
@@ -250,9 +251,18 @@ static __device__ __align__(16) const float no_key[512] = {};
 // |x scale - hi - lo| <= 2^-22 |x scale|.  The products hi hi, hi lo and lo hi
 // are exact in fp32, where the instructions sum them; lo lo (2^-22 of a
 // product) is dropped.
-__device__ __forceinline__ void halves(float x, float scale, _Float16 &hi, _Float16 &lo) {
-    hi = (_Float16)fmaf(x, scale, 0.0f);
-    lo = (_Float16)fmaf(x, scale, -(float)hi);
+// Two values together.  ONCE: an empty asm keeps the compiler from making the
+// second one's hi twice, once to be packed and once to be subtracted (prompts of
+// 256-wide heads 1195 -> 1140 us for 48, one of 24 16.1 -> 14.7).  512-wide heads
+// have no register for it but at V: 131 -> 137 us with all, in 13 trees' step.
+template <bool ONCE, typename V>
+__device__ __forceinline__ void halves(float x0, float scale0, float x1, float scale1, V &hi, V &lo, int at) {
+    h2 h = {(_Float16)fmaf(x0, scale0, 0.0f), (_Float16)fmaf(x1, scale1, 0.0f)};
+    if (ONCE) __asm__("" : "+v"(h));
+    hi[at] = h[0];
+    hi[at + 1] = h[1];
+    lo[at] = (_Float16)fmaf(x0, scale0, -(float)h[0]);
+    lo[at + 1] = (_Float16)fmaf(x1, scale1, -(float)h[1]);
 }
 
 // The power of two that brings values of magnitude `top` (its bits) below
@@ -470,11 +480,8 @@ struct Tile {
         for (int h = 0; h < H; ++h) {
             h4 hi, lo;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                _Float16 x, y;
-                halves(kr[i][h][e], scale, x, y);
-                hi[e] = x;
-                lo[e] = y;
+            for (int e = 0; e < 4; e += 2) {
+                halves<D == 256>(kr[i][h][e], scale, kr[i][h][e + 1], scale, hi, lo, e);
             }
             lds_store(at + 16384 * h, hi);
             lds_store(at + 16384 * h + 1024, lo);
@@ -486,11 +493,8 @@ struct Tile {
         for (int h = 0; h < H; ++h) {
             h4 hi, lo;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                _Float16 x, y;
-                halves(vr()[i][h][e], scale[i], x, y);
-                hi[i] = x;
-                lo[i] = y;
+            for (int i = 0; i < 4; i += 2) {
+                halves<true>(vr()[i][h][e], scale[i], vr()[i + 1][h][e], scale[i + 1], hi, lo, i);
             }
             lds_store(v_to + (16 * h + e) * 2048, hi);
             lds_store(v_to + (16 * h + e) * 2048 + 1024, lo);
@@ -529,11 +533,8 @@ struct Tile {
 #pragma unroll
             for (int i = 0; i < 8; ++i)
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    _Float16 h, l;
-                    halves(x[i][e / 4][e % 4], scale, h, l);
-                    qh[i][e] = h;
-                    ql[i][e] = l;
+                for (int e = 0; e < 8; e += 2) {
+                    halves<D == 256>(x[i][e / 4][e % 4], scale, x[i][e / 4][e % 4 + 1], scale, qh[i], ql[i], e);
                 }
         }
         // rows of no token see everything, so that they never stand in a chunk's way
@@ -559,11 +560,8 @@ struct Tile {
             for (int t = 0; t < 2; ++t) vi[t] = *(const f4q *)(vinv + 16 * t + 4 * g);
             const float unit = __builtin_bit_cast(float, (267u << 23) - __builtin_bit_cast(uint32_t, vref));      // 2^13 / vref
 #pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                _Float16 x, y;
-                halves(p[e], vi[e / 4][e % 4] * unit, x, y);
-                ph[e] = x;
-                pl[e] = y;
+            for (int e = 0; e < 8; e += 2) {
+                halves<D == 256>(p[e], vi[e / 4][e % 4] * unit, p[e + 1], vi[e / 4][e % 4 + 1] * unit, ph, pl, e);
             }
         };
         const auto vtop_of = [&](const float *vinv) {
