@@ -406,6 +406,13 @@ extern "C" int chn_token_logprobs(chn_ctx *ctx, const float *logits, uint32_t n_
     CHN_REQUIRE(ctx, ld >= V, "ld=%u is below V=%u", ld, V);
     CHN_REQUIRE(ctx, softcap >= 0.0f && std::isfinite(softcap), "softcap must be finite and not negative");
     CHN_REQUIRE(ctx, n_rows <= 65535, "n_rows=%u exceeds 65535", n_rows);
+    const size_t n_all = n_rows, n_tops = n_all * n_top;
+    const Span outs[] = {{logprobs, n_all}, {entropy, n_all}, {ranks, n_all}, {top_ids, n_tops}, {top_logprobs, n_tops}};
+    const Span ins[] = {{logits, n_all ? (n_all - 1) * ld + V : 0}, {targets, n_all}, {temperature, n_all}};
+    for (const Span &o : outs) {
+        for (const Span &i : ins) CHN_REQUIRE(ctx, !overlap(i, o), "an output overlaps an input");
+        for (const Span &p : outs) CHN_REQUIRE(ctx, &p == &o || !overlap(p, o), "two outputs overlap");
+    }
     CHN_REQUIRE(ctx, ctx, "ctx is NULL");
     if (!n_rows) return CHN_OK;
     DeviceGuard dev(ctx);

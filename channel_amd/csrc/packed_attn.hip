@@ -1033,8 +1033,10 @@ static int packed_attn(chn_ctx *ctx, const float *q, const float *k_cache, const
     CHN_REQUIRE(ctx, c >= 1e-37 && c <= 1e37, "scale %g must be finite and not zero", (double)scale);
     if (n_req > kPackedRequests) return set_err(ctx, CHN_E_UNSUPPORTED, "n_req %u exceeds %u", n_req, kPackedRequests);
     if (n_rows > kPackedRows) return set_err(ctx, CHN_E_UNSUPPORTED, "n_rows %u exceeds %u", n_rows, kPackedRows);
-    const size_t words = (size_t)n_rows * num_q_heads * head_dim;
-    CHN_REQUIRE(ctx, !overlap(chn::Span{q, words}, chn::Span{out, words}), "out overlaps q");
+    const size_t words = (size_t)n_rows * num_q_heads * head_dim, cache = (size_t)n_blocks * block_size * kv_dim;
+    const Span ins[] = {{q, words}, {k_cache, cache}, {v_cache, cache}, {tables, (size_t)n_req * max_blocks},
+                        {row_start, (size_t)n_req + 1}, {lens, n_req}, {masks, (size_t)n_rows * mask_words}};
+    for (const Span &i : ins) CHN_REQUIRE(ctx, !overlap(i, Span{out, words}), "out overlaps an input");
     CHN_REQUIRE(ctx, ctx, "ctx is NULL");
     if (!n_req || !n_rows) return CHN_OK;
     DeviceGuard dev(ctx);

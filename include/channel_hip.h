@@ -675,7 +675,9 @@ int chn_sample(chn_ctx *ctx, const float *logits, uint32_t n_rows, uint32_t V, u
  * chn_draft_trees gives the clocks for chn_batch_qkv_rope_at, in place of
  * those of chn_block_tables, and the masks for chn_paged_tree_attn.  Of a
  * tree, the caller keeps the K/V rows of the path that it accepts (chn_copy to
- * the slots behind the cached tokens, ancestors first) and its length.
+ * the slots behind the cached tokens, ancestors first) and its length.  Blocks
+ * that only rejected tokens had opened stay taken; a step that comes to them
+ * again opens others, so the caller gives those back.
  * All four only enqueue on the context's stream and can be recorded.  Argument
  * checks come first: called with ctx == NULL they report through
  * chn_last_error(NULL).
@@ -707,10 +709,11 @@ int chn_draft_trees(chn_ctx *ctx, const uint32_t *parents, const uint32_t *row_s
  * whatever it holds.  Rows of no request are left as they were.  Query head h
  * reads KV head h / gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; scale
  * finite, not zero; n_req <= 8192, n_rows <= 2^24; max_blocks * block_size <
- * 2^31.  out must not overlap q.  Products are formed of operands split in two
- * 11-bit halves (errors as fp32's own) and summed in fp32; rows of a tile that
- * meets infinities or NaN are recomputed in plain fp32.  Workspace: 65 MB,
- * whatever the batch. */
+ * 2^31.  out must not overlap an input.  Products are formed of operands split
+ * in two 11-bit halves (errors as fp32's own) and summed in fp32; the rows of a
+ * tile (up to 128, with the keys that any of them sees) that meets an infinity
+ * or a NaN in q, K or V are computed again in plain fp32, several times slower.
+ * Workspace: 68 MB, whatever the batch. */
 int chn_paged_causal_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
                           const uint32_t *tables, const uint32_t *row_start, const uint32_t *lens, uint32_t n_req,
                           uint32_t n_rows, uint32_t max_blocks, uint32_t block_size, uint32_t n_blocks,
@@ -745,7 +748,8 @@ int chn_paged_tree_attn(chn_ctx *ctx, const float *q, const float *k_cache, cons
  *    tokens and their log probabilities; CHN_NO_TOKEN and -inf behind the last
  *    allowed one.
  * temperature (device, n_rows) NULL: 1; entropy and ranks may be NULL, the top
- * arrays with n_top 0.  n_rows <= 65535. */
+ * arrays with n_top 0.  Outputs must not overlap inputs or one another.  n_rows
+ * <= 65535.  Workspace: at most 26 MB, for the largest V. */
 int chn_token_logprobs(chn_ctx *ctx, const float *logits, uint32_t n_rows, uint32_t V, uint32_t ld,
                        const uint32_t *targets, const float *temperature, float softcap, uint32_t n_top,
                        float *logprobs, float *entropy, uint32_t *ranks, uint32_t *top_ids, float *top_logprobs);

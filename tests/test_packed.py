@@ -83,6 +83,27 @@ def test_token_logprobs_optional_arguments(change):
     assert refused("chn_token_logprobs", with_(SCORES, **change)) == "ctx is NULL"
 
 
+@pytest.mark.parametrize("at", [A[1], A[2], A[3], A[4], A[5], A[1] + 100 * 16 * 512 * 4 - 16, A[3] + 4 * (4 * 32 - 4), A[4] + 16])
+def test_attention_into_an_input_is_refused(at):
+    assert "overlaps" in refused("chn_paged_causal_attn", with_(CAUSAL, _17=at))
+    assert "overlaps" in refused("chn_paged_tree_attn", with_(TREE, _19=at))
+
+
+def test_attention_into_its_masks_is_refused():
+    assert "overlaps" in refused("chn_paged_tree_attn", with_(TREE, _19=A[7] + 4 * (64 * 2 - 4)))
+
+
+@pytest.mark.parametrize("change", [dict(_8=A[0] + 4 * 3999), dict(_9=A[1] + 12), dict(_10=A[2]), dict(_11=A[0]), dict(_12=A[1]),
+                                    dict(_8=A[4]), dict(_10=A[6] + 4 * 79), dict(_12=A[6] + 16)])
+def test_scores_into_an_input_or_each_other_are_refused(change):
+    assert "overlap" in refused("chn_token_logprobs", with_(SCORES, **change))
+
+
+def test_scores_behind_the_logits_are_taken():
+    # ld counts between rows: behind the last one lies nothing that is read
+    assert refused("chn_token_logprobs", with_(SCORES, _3=2000, _8=A[0] + 4 * 7000)) == "ctx is NULL"
+
+
 def test_oracle_trees():
     none = packed.NO_TOKEN
     #       0 1 2 3     4 (two requests, then one without rows; 0 <- 1 <- 3, 0 <- 2; 5 names itself, 6 a later one)
