@@ -10,6 +10,22 @@
 // row), which a second launch joins.  Every workgroup finds its share itself
 // from the lengths, so nothing is planned on the host and no workgroup waits
 // for another.
+//
+// A row's result is sum_k 2^(c (s_k - m)) v_k / sum_k 2^(c (s_k - m)), s = q.k,
+// c = |scale| log2 e, for any reference m: one pass over the keys, the
+// reference moved when a score passes it.  Both products run on the fp16 matrix
+// instructions with every fp32 operand split in two halves (three products of
+// the four): 409 TFLOP/s at the rate that a large fp16 product reaches (1227
+// TFLOP/s), against 154 of the fp32 instructions.
+//
+// Measured (us, first launch + second) and what bounds it: 8 trees of up to 16
+// tokens behind up to 700: 25 + 7, a chain of latencies; 64 trees on a sliding
+// layer 165-185 + 11, and 5 trees of up to 64 behind up to 60000 310-360 + 9, K
+// and V from memory (0.77 and 1.65 GB); 13 trees of 512-wide heads 117 + 12, a
+// chunk's latencies, the share of a tile per CU; a prompt of 24 tokens 12 + 2, a
+// tile's beginning and end; 48 prompts on a sliding layer 1150 + 17, issue and
+// 12 tiles' beginnings and ends per CU; 2000 tokens behind 30000 3350 + 18,
+// issue (905 TFLOP/s of fp16 products); 9 prompts of 512-wide heads 190 + 17.
 #include "chn_internal.h"
 
 #include <cmath>
@@ -345,9 +361,9 @@ __device__ __forceinline__ f4q load4(mem_t p) { return *(const __attribute__((ad
 //     order in which a result's lanes store 64 bytes of a row together
 template <int D>
 struct TileLds {
-    static constexpr int kKeyBytes = 32 * D * 4;
-    unsigned char k[kKeyBytes], v[kKeyBytes];
-    float kinv[32], vinv[2][32];
+    static constexpr int kKeyBytes = 32 * D * 4, kBuffers = D == 256 ? 2 : 1;      // of chunks in turn
+    unsigned char k[kBuffers][kKeyBytes], v[kBuffers][kKeyBytes];
+    float kinv[kBuffers][32], vinv[kBuffers][32];
     float half[D == 512 ? 8 * 64 * 8 : 4];            // scores of the other half of the dims
     uint32_t not_finite;                              // an infinity or NaN was met
 };
@@ -385,19 +401,32 @@ __device__ __forceinline__ void end_step() {
 constexpr float kLead = 2.0f;
 constexpr float kWeightScale = 8192.0f;               // 2^13: weights of at most 2^kLead stay at or below 2^15
 
-// A tile's walk over its keys, 32 at a time.  Two phases between barriers:
-//   1  the scores of chunk c + 1, beside them the weights of chunk c and its V
-//      into LDS;
+// A tile's walk over its keys, 32 at a time.  A chunk has two phases:
+//   1  the scores of chunk c + 1, beside them the weights of chunk c and a V
+//      into LDS: that of chunk c + 1, with heads of 512 chunk c's;
 //   2  the sums of chunk c, beside them K of chunk c + 2 into LDS.
 // Each is 48 products of the matrix unit, interleaved in eight steps with the
 // other work, which two waves of a SIMD issue meanwhile.  What a wave loads of
-// K and V (four keys of each) is under way for a phase or two.
+// K and V (four keys of each) is under way for a phase or two.  Heads of 256
+// have two LDS buffers of each in turn, and one barrier a chunk; heads of 512
+// have room for one, and a barrier ahead of each phase (with heads of 256 that
+// is 3.46 against 3.37 ms for 2000 tokens behind 30000).
+//
+// The sums and the query's halves of 16 rows stay in a wave's registers, 128 of
+// its 256 with heads of 256, so every wave reads every key's halves from LDS:
+// 448 KB a chunk and CU, 3600 cycles of its 8000, beside 3072 of products and
+// about 4000 of vector instructions.  Measured and not taken: products' operands
+// asked for a step ahead (spills, 48 prompts 1470 us), four waves a workgroup
+// and two workgroups a CU (1575), keys shared by no waves, each with chunks of
+// its own (64 trees 280 us, 191 shared).
 template <int D>
 struct Tile {
     static constexpr int H = D / 256, RT = 8 / H;     // waves that share 16 rows (256 dims each), tiles of 16 rows
     static constexpr int S = D / 32;                  // steps
     // heads of 512 have no registers for K and V at once: K is loaded a chunk later, after V has gone to LDS
     static constexpr bool kBoth = D == 256;
+    static constexpr int kBuffers = TileLds<D>::kBuffers;
+    static constexpr uint32_t kBuffer = TileLds<D>::kKeyBytes;
     const Packed &a;
     const Work &w;
     TileLds<D> &lds;
@@ -408,6 +437,7 @@ struct Tile {
     uint64_t unheld;                                  // and which of them are nobody's
     uint32_t worst;                                   // the largest magnitude met
     uint32_t k_to, v_to;                              // where the lane's values go in LDS
+    uint32_t k_at, v_at;                              // and where it takes its operands
 
     __device__ __forceinline__ Tile(const Packed &a_, const Work &w_, TileLds<D> &l) : a(a_), w(w_), lds(l) {
         lane = threadIdx.x & 63;
@@ -421,6 +451,8 @@ struct Tile {
         worst = 0;
         const int quad = 4 * (lane >> 3) + (lane & 3);
         k_to = lds_addr(lds.k) + (((wave & 1) * S + (lane >> 3)) * 2) * 1024 + (lane & 3) * 256 + (((keys ^ quad) & 15) * 16) + (lane >> 2 & 1) * 8;
+        k_at = lds_addr(lds.k) + half * 16384 + g * 256 + (q ^ g) * 16;
+        v_at = lds_addr(lds.v) + half * 32768 + lane * 16;
         v_to = lds_addr(lds.v) + 4 * (lane >> 4) * 2048 + ((wave >> 1) * 16 + (4 * (lane & 3) + (lane >> 2 & 3))) * 16 + (wave & 1) * 8;
     }
     __device__ __forceinline__ f4q (&vr())[4][H] {
@@ -550,7 +582,6 @@ struct Tile {
         // 512 have scales of their own
         const float unit_q = kBoth ? 1.0f : qinv, factor = kBoth ? fminf(a.c * qinv, 3.4028235e38f) : a.c;
         float m = kNoScore, l = 0.0f, vref = 0.0f;
-        const uint32_t k_at = lds_addr(lds.k) + half * 16384 + g * 256 + (q ^ g) * 16, v_at = lds_addr(lds.v) + half * 32768 + lane * 16;
         f4q sc[2];
         h8 ph, pl;
         float p[8], vscale[4];
@@ -604,10 +635,11 @@ struct Tile {
 #pragma unroll
             for (int t = 0; t < 2; ++t) next[t] = low[t] = f4q{0, 0, 0, 0};
         };
-        const auto end_scores = [&] {
+        const auto end_scores = [&](int c) {                      // of chunk c
+            const float *kinv = lds.kinv[kBoth ? c & 1 : 0];
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                sc[t] = (next[t] + low[t]) * *(const f4q *)(lds.kinv + 16 * t + 4 * g);
+                sc[t] = (next[t] + low[t]) * *(const f4q *)(kinv + 16 * t + 4 * g);
                 if (!kBoth) {
                     sc[t] *= unit_q;
                     *(f4q *)(lds.half + ((wave * 2 + t) * 64 + lane) * 4) = sc[t];
@@ -622,17 +654,24 @@ struct Tile {
                 sc[t] = half ? other + sc[t] : sc[t] + other;
             }
         };
-        const auto all_k = [&] {
+        const auto all_k = [&](int c) {                           // chunk c
             float scale[4];
-            scales(kr, scale, lds.kinv);
+            scales(kr, scale, lds.kinv[kBoth ? c & 1 : 0]);
 #pragma unroll
             for (int i = 0; i < 4; ++i) store_k(i, scale[i]);
         };
         if (chunks) {
-            all_k();
-            if (chunks > 1) none1 = load_k(1);
+            all_k(0);
+            if (kBoth) {
+                scales(vr(), vscale, lds.vinv[0]);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) store_v(e, vscale);
+            }
+            if (chunks > 1) {
+                none1 = load_k(1);
+                if (kBoth) load(vr(), va, 1);
+            }
             vnow = va;
-            if (kBoth) scales(vr(), vscale, lds.vinv[0]);
             lds_barrier();
             if (threadIdx.x == 0) lds.not_finite = 0;
             if (active) {
@@ -641,24 +680,32 @@ struct Tile {
                     fetch_k(decltype(step)::value);
                     score_step(decltype(step)::value);
                 });
-                end_scores();
+                end_scores(0);
             }
-            lds_barrier();
-            if (chunks > 1) all_k();
-            if (!kBoth) {
+            if (kBoth) {
+                k_to += kBuffer;
+                if (chunks > 1) {
+                    all_k(1);
+                    none2 = load_k(2);
+                }
+                k_to -= kBuffer;
+                k_at += kBuffer;
+                v_to += kBuffer;
+            } else {
+                lds_barrier();
+                if (chunks > 1) all_k(1);
                 if (active) add_half();
                 load(vr(), vnow, 0);
-            } else if (chunks > 1) {
-                none2 = load_k(2);
             }
         }
         // the last chunk has no next one
         const auto walk = [&](int c, auto more) {
             constexpr bool kMore = decltype(more)::value;
             const float *vinv = lds.vinv[kBoth ? c & 1 : 0];
-            if (c & 1) vnow = va;
+            if (!kBoth && (c & 1)) vnow = va;
             lds_barrier();
             // ---- phase 1
+
             if (!kBoth) {
                 // the registers hold V of chunk c: to LDS first
                 scales(vr(), vscale, lds.vinv[0]);
@@ -727,16 +774,21 @@ struct Tile {
                         l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
                         if (kBoth) weights(vinv);
                     }
-                    if constexpr (i >= 4 && kBoth) store_v(i - 4, vscale);
+                    if constexpr (i == 3 && kBoth && kMore) scales(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
+                    if constexpr (i >= 4 && kBoth && kMore) store_v(i - 4, vscale);
                     if constexpr (kMore) end_step();
                 });
-                if constexpr (kMore) end_scores();
-            } else if (kBoth) {
+                if constexpr (kMore) end_scores(c + 1);
+            } else if (kBoth && kMore) {
+                scales(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) store_v(e, vscale);
             }
-            if (kBoth && kMore) load(vr(), vnow, c + 1);
-            lds_barrier();
+            if (kBoth) {
+                if (kMore) load(vr(), va, c + 2);
+            } else {
+                lds_barrier();
+            }
             // ---- phase 2
             if (active) {
                 if (!kBoth) {
@@ -761,21 +813,25 @@ struct Tile {
                     o[2 * i + 1] = __builtin_amdgcn_mfma_f32_16x16x32_f16(fr[2], ph, o[2 * i + 1], 0, 0, 0);
                     if constexpr (i < 7) fetch_v(i + 1);
                     if constexpr (kMore) {
-                        if constexpr (i == 2) scales(kr, scale, lds.kinv);
+                        if constexpr (i == 2) scales(kr, scale, lds.kinv[kBoth ? c & 1 : 0]);
                         if constexpr (i >= 3 && i < 7) store_k(i - 3, scale[i - 3]);
                     }
                     end_step();
                 });
                 if (!kBoth && kMore) add_half();
             } else if (kMore) {
-                all_k();
+                all_k(c);
             }
             if constexpr (kMore) {
                 if (!kBoth) {
                     load(vr(), vnow, c + 1);
                 } else {
-                    scales(vr(), vscale, lds.vinv[(c + 1) & 1]);
                     none3 = load_k(c + 3);
+                    const uint32_t turn = c & 1 ? kBuffer : -kBuffer;
+                    k_at += turn;
+                    v_to += turn;
+                    k_to -= turn;
+                    v_at -= turn;
                 }
                 none0 = none1;
                 none1 = none2;
@@ -1090,7 +1146,8 @@ struct Drafts {
 // its parent's mask, found by doubling - every round takes over what the node
 // that its path has reached has gathered, and that node's reach, so a path of
 // depth d takes log2 d rounds.  A parent that is no earlier node ends a path,
-// so every path ends.
+// so every path ends.  A launch's latency: 3.5 us for 8 requests, 7 for 500 of up
+// to 256 nodes (a walk up the path, node by node, would be 256 dependent reads).
 constexpr uint32_t kNodes = 32 * kMaskWords;
 template <int W>
 __global__ __launch_bounds__(kNodes) void k_draft_trees(Drafts a) {
