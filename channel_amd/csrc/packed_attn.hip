@@ -815,17 +815,17 @@ struct Tile {
                     if constexpr (kMore) {
                         if constexpr (i == 2) scales(kr, scale, lds.kinv[kBoth ? c & 1 : 0]);
                         if constexpr (i >= 3 && i < 7) store_k(i - 3, scale[i - 3]);
+                        if constexpr (!kBoth && i == 7) load(vr(), vnow, c + 1);
                     }
                     end_step();
                 });
                 if (!kBoth && kMore) add_half();
             } else if (kMore) {
                 all_k(c);
+                if (!kBoth) load(vr(), vnow, c + 1);
             }
             if constexpr (kMore) {
-                if (!kBoth) {
-                    load(vr(), vnow, c + 1);
-                } else {
+                if (kBoth) {
                     none3 = load_k(c + 3);
                     const uint32_t turn = c & 1 ? kBuffer : -kBuffer;
                     k_at += turn;
