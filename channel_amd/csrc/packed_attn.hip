@@ -20,12 +20,13 @@
 //
 // Measured (us, first launch + second) and what bounds it: 8 trees of up to 16
 // tokens behind up to 700: 25 + 7, a chain of latencies; 64 trees on a sliding
-// layer 165-185 + 11, and 5 trees of up to 64 behind up to 60000 310-360 + 9, K
+// layer 166-183 + 11, and 5 trees of up to 64 behind up to 60000 305-365 + 10, K
 // and V from memory (0.77 and 1.65 GB); 13 trees of 512-wide heads 117 + 12, a
 // chunk's latencies, the share of a tile per CU; a prompt of 24 tokens 12 + 2, a
-// tile's beginning and end; 48 prompts on a sliding layer 1150 + 17, issue and
-// 12 tiles' beginnings and ends per CU; 2000 tokens behind 30000 3350 + 18,
-// issue (905 TFLOP/s of fp16 products); 9 prompts of 512-wide heads 190 + 17.
+// tile's beginning and end; 48 prompts on a sliding layer 1070-1210 + 18, LDS
+// reads, products and issue, and 12 tiles' beginnings and ends per CU; 2000 tokens
+// behind 30000 3180-3350 + 18, the same (905 TFLOP/s of fp16 products); 9 prompts of
+// 512-wide heads 205-220 + 17, V's latency in every chunk.
 #include "chn_internal.h"
 
 #include <cmath>
@@ -414,8 +415,8 @@ constexpr float kWeightScale = 8192.0f;               // 2^13: weights of at mos
 //
 // The sums and the query's halves of 16 rows stay in a wave's registers, 128 of
 // its 256 with heads of 256, so every wave reads every key's halves from LDS:
-// 448 KB a chunk and CU, 3600 cycles of its 8000, beside 3072 of products and
-// about 4000 of vector instructions.  Measured and not taken: products' operands
+// 512 KB a chunk and CU, 4100 of its 8000 cycles at 128 B a cycle, beside 3072
+// of products and 2400 of vector instructions.  Measured and not taken: products' operands
 // asked for a step ahead (spills, 48 prompts 1470 us), four waves a workgroup
 // and two workgroups a CU (1575), keys shared by no waves, each with chunks of
 // its own (64 trees 280 us, 191 shared).
