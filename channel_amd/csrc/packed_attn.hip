@@ -26,7 +26,8 @@
 // tile's beginning and end; 48 prompts on a sliding layer 1070-1210 + 18, LDS
 // reads, products and issue, and 12 tiles' beginnings and ends per CU; 2000 tokens
 // behind 30000 3180-3350 + 18, the same (905 TFLOP/s of fp16 products); 9 prompts of
-// 512-wide heads 205-220 + 17, V's latency in every chunk.
+// 512-wide heads 205-220 + 17, two latencies a chunk: K and V take turns in the
+// same registers.
 #include "chn_internal.h"
 
 #include <cmath>
