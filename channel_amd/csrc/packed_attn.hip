@@ -19,7 +19,7 @@
 // TFLOP/s), against 154 of the fp32 instructions.
 //
 // Measured (us, first launch + second) and what bounds it: 8 trees of up to 16
-// tokens behind up to 700: 25 + 7, a chain of latencies; 64 trees on a sliding
+// tokens behind up to 700: 18.5 + 7, a chain of latencies; 64 trees on a sliding
 // layer 166-183 + 11, and 5 trees of up to 64 behind up to 60000 305-365 + 10, K
 // and V from memory (0.77 and 1.65 GB); 13 trees of 512-wide heads 117 + 12, a
 // chunk's latencies, the share of a tile per CU; a prompt of 24 tokens 12 + 2, a
@@ -44,10 +44,9 @@ constexpr uint32_t kShares = 1u << kShareLog;   // workgroups: one per CU
 constexpr int kThreads = 512;
 // A key is 2 units, or 3 where both waves of a SIMD have rows (a chunk of 32 keys takes 2.9 and 4.1 us).  A tile costs
 // kTileCost besides its keys, its beginning and end (heads of 256 14 us; heads of 512 16, where a chunk takes 5.4).  A
-// cut that would fall within kNearEnd of a tile's end is moved there; a share has 2^kShareBits units or more, twice
-// that, so that none is empty.
-constexpr int64_t kTileCost = 320, kNearEnd = 128;
-constexpr int kShareBits = 8;
+// cut that would fall within kNearEnd of a tile's end is moved there; a share has kShareUnits or more, twice that, so
+// that none is empty.
+constexpr int64_t kTileCost = 320, kNearEnd = 96, kShareUnits = 2 * kNearEnd;
 constexpr float kNoScore = -__builtin_inff();
 
 // Rows of a tile: tokens x query heads of the KV head.
@@ -416,7 +415,7 @@ constexpr float kWeightScale = 8192.0f;               // 2^13: weights of at mos
 //
 // The sums and the query's halves of 16 rows stay in a wave's registers, 128 of
 // its 256 with heads of 256, so every wave reads every key's halves from LDS:
-// 512 KB a chunk and CU, 4100 of its 8000 cycles at 128 B a cycle, beside 3072
+// 512 KB a chunk and CU, 4100 of its 8000 cycles at 128 B a cycle, beside 3070
 // of products and 2400 of vector instructions.  Measured and not taken: products' operands
 // asked for a step ahead (spills, 48 prompts 1470 us), four waves a workgroup
 // and two workgroups a CU (1575), keys shared by no waves, each with chunks of
@@ -895,12 +894,27 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
         total += sums[i];
     }
     total = (int64_t)lane64((uint64_t)total, 0);
-    // a power of two of shares; neighbours, which read the same keys, run on one XCD (workgroup i on XCD i % 8)
-    const int bits = total >> kShareBits ? min(63 - __builtin_clzll((uint64_t)total >> kShareBits), kShareLog) : 0;
-    const uint32_t n = 1u << bits, each = (n + 7) / 8, share = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
+    // As many shares as there are CUs, a power of two.  Where there is less work and the tiles are long, shares of the
+    // least size (8 trees 27.3 us, 32.4 by powers of two; 3 behind up to 1500 24.4, 33.6); where they are short, by powers of two
+    // again, as equal tiles then stay whole (one prompt of 24 tokens 14.7, cut 16.7).
+    int64_t size = total;                                      // of 2^bits shares
+    int bits = kShareLog;
+    uint32_t n = kShares;
+    if (total < (kShareUnits << kShareLog)) {
+        bits = 0;
+        n = max((uint32_t)total / (uint32_t)kShareUnits, 1u);
+        if (total >= 512 * (int64_t)a.n_req * a.num_kv) {
+            size = kShareUnits;
+        } else {
+            bits = total >> 8 ? 31 - __builtin_clz((uint32_t)total >> 8) : 0;
+            n = 1u << bits;
+        }
+    }
+    // neighbours, which read the same keys, run on one XCD (workgroup i on XCD i % 8)
+    const uint32_t each = (n + 7) / 8, share = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
     if ((blockIdx.x >> 3) >= each || share >= n) return;      // the whole workgroup
-    const auto cut = [&](uint32_t w) { return total * w >> bits; };
-    const int64_t u0 = cut(share), u1 = cut(share + 1);
+    const auto cut = [&](uint32_t w) { return size * w >> bits; };
+    const int64_t u0 = cut(share), u1 = share + 1 == n ? total : cut(share + 1);
     if (u0 >= base && u0 < base + mine) {                     // one thread, or none
         uint32_t r = r0;
         for (; r + 1 < r1; ++r) {
