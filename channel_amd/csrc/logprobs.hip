@@ -312,12 +312,18 @@ __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
         xsum += sh.xsum[w];
         before += sh.before[w];
     }
-    const double log_sum = greedy ? 0.0 : log((double)sum);
+    const double T = a.temperature ? (double)a.temperature[row] : 1.0, log_sum = greedy ? 0.0 : log((double)sum);
+    // The sums are relative to the largest capped in fp32.  Its rounding is taken out of what the other tokens add to
+    // the largest's one; theirs go both ways.  (In the entropy it cancels.)
+    double log_all = log_sum;
+    if (CAP && !greedy) {
+        const double off = ((double)capped<CAP>(top, a.cap, inv_cap) - capped64<CAP>(top, a.cap)) / T;
+        log_all = log(1.0 + ((double)sum - 1.0) * exp(fmin(fmax(off, -50.0), 50.0)));
+    }
     // of an allowed logit; `first`: no token comes before it
     const auto logp = [&](float l, bool first) {
         if (greedy) return first ? 0.0f : -__builtin_inff();
-        const double T = a.temperature ? (double)a.temperature[row] : 1.0;
-        return (float)((l == top ? 0.0 : (capped64<CAP>(l, a.cap) - capped64<CAP>(top, a.cap)) / T) - log_sum);
+        return (float)((l == top ? 0.0 : (capped64<CAP>(l, a.cap) - capped64<CAP>(top, a.cap)) / T) - log_all);
     };
     if (wave == kScoreWaves - 1 && lane == 0) {
         const bool given = target < a.V, ok = most && scored(mine);
