@@ -312,23 +312,26 @@ __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
         xsum += sh.xsum[w];
         before += sh.before[w];
     }
-    const double T = a.temperature ? (double)a.temperature[row] : 1.0, log_sum = greedy ? 0.0 : log((double)sum);
-    // The sums are relative to the largest capped in fp32.  Its rounding is taken out of what the other tokens add to
-    // the largest's one; theirs go both ways.  (In the entropy it cancels.)
-    double log_all = log_sum;
+    const double T = a.temperature ? (double)a.temperature[row] : 1.0;
+    // The sums are relative to the largest capped in fp32: its rounding is taken out of what the other tokens add to the
+    // largest's one.  Theirs go both ways.
+    double all = (double)sum, mean = 0.69314718055994531 * (double)xsum;
     if (CAP && !greedy) {
-        const double off = ((double)capped<CAP>(top, a.cap, inv_cap) - capped64<CAP>(top, a.cap)) / T;
-        log_all = log(1.0 + ((double)sum - 1.0) * exp(fmin(fmax(off, -50.0), 50.0)));
+        const double off = fmin(fmax(((double)capped<CAP>(top, a.cap, inv_cap) - capped64<CAP>(top, a.cap)) / T, -50.0), 50.0);
+        const double f = exp(off), others = all - 1.0;
+        mean = f * (mean + others * off);
+        all = 1.0 + others * f;
     }
+    const double log_sum = greedy ? 0.0 : log(all);
     // of an allowed logit; `first`: no token comes before it
     const auto logp = [&](float l, bool first) {
         if (greedy) return first ? 0.0f : -__builtin_inff();
-        return (float)((l == top ? 0.0 : (capped64<CAP>(l, a.cap) - capped64<CAP>(top, a.cap)) / T) - log_all);
+        return (float)((l == top ? 0.0 : (capped64<CAP>(l, a.cap) - capped64<CAP>(top, a.cap)) / T) - log_sum);
     };
     if (wave == kScoreWaves - 1 && lane == 0) {
         const bool given = target < a.V, ok = most && scored(mine);
         a.logp[row] = !given ? 0.0f : ok ? logp(mine, before == 0) : -__builtin_inff();
-        if (a.entropy) a.entropy[row] = most && !greedy ? (float)(log_sum - 0.69314718055994531 * (double)xsum / (double)sum) : 0.0f;
+        if (a.entropy) a.entropy[row] = most && !greedy ? (float)(log_sum - mean / all) : 0.0f;
         if (a.ranks) a.ranks[row] = ok ? before : CHN_NO_TOKEN;
     }
     if (!a.n_top) return;
