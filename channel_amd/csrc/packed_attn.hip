@@ -45,8 +45,8 @@ constexpr int kThreads = 512;
 // A key is 2 units, or 3 where both waves of a SIMD have rows (a chunk of 32 keys takes 2.9 and 4.1 us).  A tile costs
 // kTileCost besides its keys, its beginning and end (heads of 256 14 us; heads of 512 16, where a chunk takes 5.4).  A
 // cut that would fall within kNearEnd of a tile's end is moved there; a share has kShareUnits or more, twice that, so
-// that none is empty.
-constexpr int64_t kTileCost = 320, kNearEnd = 96, kShareUnits = 2 * kNearEnd;
+// that no share of a tile that is cut is empty.  A tile below kShortTile, three chunks, is not worth the join.
+constexpr int64_t kTileCost = 320, kNearEnd = 96, kShareUnits = 2 * kNearEnd, kShortTile = 512;
 constexpr float kNoScore = -__builtin_inff();
 
 // Rows of a tile: tokens x query heads of the KV head.
@@ -141,7 +141,8 @@ struct TileKeys {
         return is_full(t) ? (int64_t)__umul64hi((uint64_t)u, 0x5555555555555556ull) : u >> 1;
     }
 };
-__device__ __forceinline__ int64_t snapped(int64_t at, int64_t cost) {
+__device__ __forceinline__ int64_t snapped(int64_t at, int64_t cost, bool whole) {
+    if (whole && cost < kShortTile) return 2 * at < cost ? 0 : cost;
     return at < kNearEnd ? 0 : (at + kNearEnd > cost ? cost : at);
 }
 
@@ -870,46 +871,46 @@ struct Tile {
 template <int D, typename F>
 __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
     __shared__ int64_t sums[kThreads / 64], found_base;
-    __shared__ uint32_t found;
+    __shared__ uint32_t found, tile_sums[kThreads / 64];
     const uint32_t tid = threadIdx.x, per = (a.n_req + kThreads - 1) / kThreads;
     const int lane = tid & 63, wave = tid >> 6;
     // every request's units; a thread sums its neighbours
     const uint32_t r0 = min(tid * per, a.n_req), r1 = min(r0 + per, a.n_req);
-    const auto units_of = [&](uint32_t r) {
-        return TileKeys::of<D>(a, seq_of(a, r)).all() * a.num_kv;
-    };
     int64_t mine = 0;
-    for (uint32_t r = r0; r < r1; ++r) mine += units_of(r);
+    uint32_t tiles = 0;                                        // of a request at most one more than there are shares
+    for (uint32_t r = r0; r < r1; ++r) {
+        const TileKeys k = TileKeys::of<D>(a, seq_of(a, r));
+        mine += k.all() * a.num_kv;
+        tiles += min(min(k.tiles, kShares + 1) * a.num_kv, kShares + 1);
+    }
     const int64_t upto = (int64_t)wave_scan_u64((uint64_t)mine);
-    if (lane == 63) sums[wave] = upto;
+    tiles = (uint32_t)wave_sum_u64(tiles);
+    if (lane == 63) {
+        sums[wave] = upto;
+        tile_sums[wave] = tiles;
+    }
     if (tid == 0) {
         found = 0xFFFFFFFFu;
         a.joined[blockIdx.x].rows = 0;
     }
     __syncthreads();
     int64_t total = 0, base = upto - mine;
+    tiles = 0;
 #pragma unroll
     for (int i = 0; i < kThreads / 64; ++i) {
         base += i < wave ? sums[i] : 0;
         total += sums[i];
+        tiles += tile_sums[i];
     }
     total = (int64_t)lane64((uint64_t)total, 0);
-    // As many shares as there are CUs, a power of two.  Where there is less work and the tiles are long, shares of the
-    // least size (8 trees 27.3 us, 32.4 by powers of two; 3 behind up to 1500 24.4, 33.6); where they are short, by powers of two
-    // again, as equal tiles then stay whole (one prompt of 24 tokens 14.7, cut 16.7).
-    int64_t size = total;                                      // of 2^bits shares
-    int bits = kShareLog;
-    uint32_t n = kShares;
-    if (total < (kShareUnits << kShareLog)) {
-        bits = 0;
-        n = max((uint32_t)total / (uint32_t)kShareUnits, 1u);
-        if (total >= 512 * (int64_t)a.n_req * a.num_kv) {
-            size = kShareUnits;
-        } else {
-            bits = total >> 8 ? 31 - __builtin_clz((uint32_t)total >> 8) : 0;
-            n = 1u << bits;
-        }
-    }
+    // As many shares as there are CUs; of the least size where there is less work (8 trees 27 us, 32 with a power of two of
+    // larger ones).  Where there are no more tiles than CUs, short ones stay whole and need no join (a prompt of 24 tokens
+    // 14.7 us, cut 16.7; 20 of up to 30 21.4, cut 26.7).
+    const bool much = total >= kShareUnits << kShareLog;
+    const int bits = much ? kShareLog : 0;
+    const int64_t size = much ? total : kShareUnits;           // of 2^bits shares
+    const uint32_t n = much ? kShares : max((uint32_t)total / (uint32_t)kShareUnits, 1u);
+    const bool whole = __builtin_amdgcn_readfirstlane(tiles) <= kShares;
     // neighbours, which read the same keys, run on one XCD (workgroup i on XCD i % 8)
     const uint32_t each = (n + 7) / 8, share = (blockIdx.x & 7) * each + (blockIdx.x >> 3);
     if ((blockIdx.x >> 3) >= each || share >= n) return;      // the whole workgroup
@@ -918,7 +919,7 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
     if (u0 >= base && u0 < base + mine) {                     // one thread, or none
         uint32_t r = r0;
         for (; r + 1 < r1; ++r) {
-            const int64_t units = units_of(r);
+            const int64_t units = TileKeys::of<D>(a, seq_of(a, r)).all() * a.num_kv;
             if (u0 < base + units) break;
             base += units;
         }
@@ -954,7 +955,7 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
         w.s = seq_of(a, r);
         const TileKeys k = TileKeys::of<D>(a, w.s);
         const int64_t cost = k.cost(t);
-        const int64_t from = u < u0 ? snapped(u0 - u, cost) : 0, to = u1 - u < cost ? snapped(u1 - u, cost) : cost;
+        const int64_t from = u < u0 ? snapped(u0 - u, cost, whole) : 0, to = u1 - u < cost ? snapped(u1 - u, cost, whole) : cost;
         if (from < to) {
             w.table = a.tables + (size_t)r * a.max_blocks;
             w.kvh = kvh;
@@ -970,7 +971,7 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
             if (from && to == cost && tid == 0) {
                 // the share that begins this tile: the last whose first cut is at or before it
                 uint32_t first = share;
-                while (first && cut(first) > u && snapped(cut(first) - u, cost)) --first;
+                while (first && cut(first) > u && snapped(cut(first) - u, cost, whole)) --first;
                 a.joined[blockIdx.x] = Joined{first, share, w.tile_row, w.rows, kvh};
             }
             f(w);

@@ -52,6 +52,18 @@ def test_the_same_call_gives_the_same_bits(ctx, words):
     b.check(first)
 
 
+@pytest.mark.parametrize("new,have", [
+    ([3] * 32, [5] * 32), ([3] * 33, [5] * 33), ([3] * 31 + [60], [5] * 31 + [1500]), ([60] + [3] * 31, [1500] + [5] * 31),
+    ([2, 60, 2, 64, 1], [0, 700, 3, 100, 90]), ([1] * 20, [95, 96, 97, 98] * 5), ([64] * 8, [0, 31, 32, 33, 63, 64, 65, 95]),
+    ([65] * 6, [40] * 6), ([1], [192 * 128]), ([5] * 40, [150] * 40),
+])
+@pytest.mark.parametrize("words", [0, 2])
+def test_shares_of_short_and_long_tiles(ctx, new, have, words):
+    """As many tiles as CUs and one more, tiles on both sides of those that are cut, short ones beside long ones."""
+    say("shares", new, have, words)
+    Batch(ctx, 50, [min(n, 64) for n in new] if words else new, have, nq=16, words=words).check()
+
+
 def test_rows_behind_4_gib(ctx):
     """A request whose rows of q and out lie behind 4 GiB."""
     say("rows behind 4 GiB")
