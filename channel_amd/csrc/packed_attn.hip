@@ -442,8 +442,10 @@ struct Tile {
     uint32_t k_at, v_at;                              // and where it takes its operands
 
     __device__ __forceinline__ Tile(const Packed &a_, const Work &w_, TileLds<D> &l) : a(a_), w(w_), lds(l) {
-        lane = threadIdx.x & 63;
-        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        // made again for every tile: held over the tiles, what follows from them would be spilled
+        const uint32_t thread = opaque_u32(threadIdx.x);
+        lane = thread & 63;
+        wave = __builtin_amdgcn_readfirstlane(thread >> 6);
         // the halves of a row's dims on neighbouring SIMDs, so that half of a tile's rows keep all four busy
         rt = wave / H;
         half = wave % H;
@@ -871,6 +873,7 @@ struct Tile {
 template <int D, typename F>
 __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
     __shared__ int64_t sums[kThreads / 64], found_base;
+    __shared__ Seq found_seq, seqs[kThreads / 64];             // every wave's request: a load from there, not from memory, for each tile
     __shared__ uint32_t found, tile_sums[kThreads / 64];
     const uint32_t tid = threadIdx.x, per = (a.n_req + kThreads - 1) / kThreads;
     const int lane = tid & 63, wave = tid >> 6;
@@ -925,14 +928,24 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
         }
         found = r;
         found_base = base;
+        found_seq = seq_of(a, r);
     }
     __syncthreads();
     uint32_t r = __builtin_amdgcn_readfirstlane(found), kvh = 0, t = 0;
     if (r >= a.n_req) return;
     int64_t u = (int64_t)lane64((uint64_t)found_base, 0);
+    const auto uniform = [](const Seq &of) {
+        Seq s;
+        s.row = __builtin_amdgcn_readfirstlane(of.row);
+        s.n = __builtin_amdgcn_readfirstlane(of.n);
+        s.have = __builtin_amdgcn_readfirstlane(of.have);
+        s.len = __builtin_amdgcn_readfirstlane(of.len);
+        return s;
+    };
+    seqs[wave] = found_seq;
     {
         // the KV head, then the tile, that u0 falls into
-        const TileKeys k = TileKeys::of<D>(a, seq_of(a, r));
+        const TileKeys k = TileKeys::of<D>(a, uniform(found_seq));
         const int64_t head = k.all();
         uint32_t hi = a.num_kv;
         while (hi - kvh > 1) {
@@ -952,7 +965,7 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
     while (u < u1) {
         // made again for every tile, so that little is held in registers meanwhile
         Work w;
-        w.s = seq_of(a, r);
+        w.s = uniform(seqs[wave]);
         const TileKeys k = TileKeys::of<D>(a, w.s);
         const int64_t cost = k.cost(t);
         const int64_t from = u < u0 ? snapped(u0 - u, cost, whole) : 0, to = u1 - u < cost ? snapped(u1 - u, cost, whole) : cost;
@@ -990,6 +1003,7 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
             }
         }
         if (r >= a.n_req) break;
+        seqs[wave] = seq_of(a, r);
     }
 }
 
