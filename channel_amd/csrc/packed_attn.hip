@@ -20,13 +20,13 @@
 //
 // Measured (us, first launch + second) and what bounds it: 8 trees of up to 16
 // tokens behind up to 700: 18.5 + 7, a chain of latencies; 64 trees on a sliding
-// layer 166-183 + 11, and 5 trees of up to 64 behind up to 60000 305-365 + 10, K
+// layer 161-180 + 11, and 5 trees of up to 64 behind up to 60000 302-370 + 10, K
 // and V from memory (0.77 and 1.65 GB); 13 trees of 512-wide heads 117 + 12, a
 // chunk's latencies, the share of a tile per CU; a prompt of 24 tokens 12 + 2, a
 // tile's beginning and end; 48 prompts on a sliding layer 1070-1210 + 18, LDS
 // reads, products and issue, and 12 tiles' beginnings and ends per CU; 2000 tokens
 // behind 30000 3180-3350 + 18, the same (905 TFLOP/s of fp16 products); 9 prompts of
-// 512-wide heads 205-220 + 17, two latencies a chunk: K and V take turns in the
+// 512-wide heads 201-215 + 17, two latencies a chunk: K and V take turns in the
 // same registers.
 #include "chn_internal.h"
 
