@@ -401,7 +401,12 @@ __device__ __forceinline__ void end_step() {
 // Weights are relative to a reference that is moved when a score passes it by
 // more than this, in powers of two.
 constexpr float kLead = 2.0f;
-constexpr float kWeightScale = 8192.0f;               // 2^13: weights of at most 2^kLead stay at or below 2^15
+// A row's sums are kept relative to the largest weight times V scale of the keys that it sees (a power of two, vref):
+// whatever its other keys' slots hold, and whatever lies under weights of nothing, takes no digits from them.  The
+// halves of those products are relative to it, 2^kWeightLog for one, so what is below 2^-36 of it is rounded to that;
+// it is raised when a product passes it by more than kRoom, which keeps them at or below 2^15.
+constexpr int kWeightLog = 12;
+constexpr float kRoom = 8.0f, kLeastRef = 0x1p-100f;
 
 // A tile's walk over its keys, 32 at a time.  A chunk has two phases:
 //   1  the scores of chunk c + 1, beside them the weights of chunk c and a V
@@ -585,28 +590,33 @@ struct Tile {
         // Scores stay in units of the row's q scale, whose inverse goes into the exponent's factor; the halves of heads of
         // 512 have scales of their own
         const float unit_q = kBoth ? 1.0f : qinv, factor = kBoth ? fminf(a.c * qinv, 3.4028235e38f) : a.c;
-        float m = kNoScore, l = 0.0f, vref = 0.0f;
+        float m = kNoScore, l = 0.0f, vref = kLeastRef;
+        bool moved = false;                                       // a row's m, and with it vref, which is no power of two then
         f4q sc[2];
         h8 ph, pl;
         float p[8], vscale[4];
-        const auto weights = [&](const float *vinv) {             // p relative to the largest V, as halves
-            f4q vi[2];
+        const auto weights = [&](const float *vinv) {             // p times the keys' V scales, as halves
+            float top = 0.0f;
 #pragma unroll
-            for (int t = 0; t < 2; ++t) vi[t] = *(const f4q *)(vinv + 16 * t + 4 * g);
-            const float unit = __builtin_bit_cast(float, (267u << 23) - __builtin_bit_cast(uint32_t, vref));      // 2^13 / vref
+            for (int t = 0; t < 2; ++t) {
+                const f4q vi = *(const f4q *)(vinv + 16 * t + 4 * g);
 #pragma unroll
-            for (int e = 0; e < 8; e += 2) {
-                halves<D == 256>(p[e], vi[e / 4][e % 4] * unit, p[e + 1], vi[e / 4][e % 4 + 1] * unit, ph, pl, e);
+                for (int e = 0; e < 4; ++e) {
+                    p[4 * t + e] *= vi[e];
+                    top = largest(top, p[4 * t + e]);
+                }
             }
-        };
-        const auto vtop_of = [&](const float *vinv) {
-            float t = 0.0f;
+            top = rows4_top(top);
+            if (moved || __any(top > kRoom * vref)) {
+                const float to = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, fmaxf(fmaxf(vref, top), kLeastRef)) & 0x7F800000u);
+                const float f = vref * __builtin_bit_cast(float, (254u << 23) - __builtin_bit_cast(uint32_t, to));
+                vref = to;
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-                const f4q v = *(const f4q *)(vinv + 16 * e + 4 * g);
-                t = largest(largest(t, v[0]), largest(largest(v[1], v[2]), v[3]));
+                for (int e = 0; e < 16; ++e) o[e] *= f;
             }
-            return lane_f(rows4_top(t), 0);
+            const float unit = __builtin_bit_cast(float, ((254u + kWeightLog) << 23) - __builtin_bit_cast(uint32_t, vref));
+#pragma unroll
+            for (int e = 0; e < 8; e += 2) halves<D == 256>(p[e], unit, p[e + 1], unit, ph, pl, e);
         };
         h8 fr[4];
         const auto fetch_k = [&](int i) {                         // both tiles' step i
@@ -753,21 +763,12 @@ struct Tile {
 #pragma unroll
                         for (int e = 0; e < 8; ++e) top = largest(top, sc[e / 4][e % 4]);
                         top = rows4_top(top);
-                        const float vtop = kBoth ? vtop_of(vinv) : 0.0f;
                         const bool up = (top - m) * factor > kLead;
-                        if (__any(up) || vtop > vref) {
-                            const float to = up ? top : m, old = up ? __builtin_amdgcn_exp2f((m - to) * factor) : 1.0f;
-                            float f = old;
-                            if (kBoth) {
-                                const float vto = vtop > vref ? vtop : vref;
-                                f *= vref / vto;
-                                vref = vto;
-                            }
-                            m = to;
-                            l *= old;
-#pragma unroll
-                            for (int e = 0; e < 16; ++e) o[e] *= f;
-                        }
+                        moved = __any(up);
+                        const float old = up ? __builtin_amdgcn_exp2f((m - top) * factor) : 1.0f;
+                        m = up ? top : m;
+                        l *= old;
+                        vref *= old;                              // and the sums are in its units
                     }
                     if constexpr (i == 2 || i == 3) {
                         const float ref = m == kNoScore ? 0.0f : m;
@@ -795,16 +796,7 @@ struct Tile {
             }
             // ---- phase 2
             if (active) {
-                if (!kBoth) {
-                    const float vtop = vtop_of(vinv);
-                    if (vtop > vref) {
-                        const float f = vref / vtop;
-                        vref = vtop;
-#pragma unroll
-                        for (int e = 0; e < 16; ++e) o[e] *= f;
-                    }
-                    weights(vinv);
-                }
+                if (!kBoth) weights(vinv);
                 float scale[4];
                 fetch_v(0);
                 static_for<8>([&](auto step) {
@@ -854,7 +846,7 @@ struct Tile {
         }
         l = rows4_sum(l);
         if (!valid) return;
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f, unit = vref * (1.0f / kWeightScale);
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f, unit = vref * (1.0f / (1 << kWeightLog));
         float *to = row_out<D>(a, w, row) + 256 * half + 4 * g;
 #pragma unroll
         for (int j = 0; j < 4; ++j)
@@ -863,7 +855,7 @@ struct Tile {
                 *(f4q *)(to + 64 * j + 16 * i) =
                     f4q{o[4 * j][i] * inv * unit, o[4 * j + 1][i] * inv * unit, o[4 * j + 2][i] * inv * unit, o[4 * j + 3][i] * inv * unit};
         if (w.part >= 0 && g == 0 && half == 0) {
-            a.pm[(size_t)w.part * tile_rows(D) + row] = kBoth ? m * qinv : m;
+            a.pm[(size_t)w.part * tile_rows(D) + row] = kBoth ? m * (factor / a.c) : m;       // qinv again, not held over the walk
             a.pl[(size_t)w.part * tile_rows(D) + row] = l;
         }
     }

@@ -46,9 +46,11 @@ def seen_by(i, n, length, window, mask=None):
     return np.array(list(range(first, max(0, have))) + drafted, np.int64)
 
 
-def packed_attn(q, kc, vc, tables, row_start, lens, bs, n_blocks, num_q, D, gqa, scale, window, masks=None, out=None):
+def packed_attn(q, kc, vc, tables, row_start, lens, bs, n_blocks, num_q, D, gqa, scale, window, masks=None, out=None,
+                sizes=None):
     """q [n_rows][num_q * D], caches [slots][kv_dim]: (out, the largest |score|, the largest sum of |q k|
-    products, the most keys of a row)."""
+    products, the most keys of a row).  sizes ([n_rows][num_q][3], or None) receives for each row and head the sum of
+    weight times largest |v| over the keys that it sees, its largest sum of |q k| products, and its keys."""
     n_rows = len(q)
     out = np.zeros((n_rows, num_q * D)) if out is None else np.array(out, np.float64)
     big = absum = 0.0
@@ -80,7 +82,10 @@ def packed_attn(q, kc, vc, tables, row_start, lens, bs, n_blocks, num_q, D, gqa,
                         o[:] = np.nan
                 if np.isfinite(score).all():
                     big = max(big, float(np.abs(score).max()))
-                    absum = max(absum, float((np.abs(k[keep]) @ np.abs(qv)).max() * abs(scale)))
+                    mine = float((np.abs(k[keep]) @ np.abs(qv)).max() * abs(scale))
+                    absum = max(absum, mine)
+                    if sizes is not None:
+                        sizes[s + i, h] = p @ np.abs(v).max(1) / p.sum(), mine, len(at)
     return out, big, absum, most
 
 

@@ -1,0 +1,123 @@
+"""Attention of packed prompts and of drafted trees where operands differ widely
+in size: what a row does not see, and what lies under weights of nothing, takes
+no digits from what it sees.
+
+Tolerance, for each row and head by the keys that IT sees (u = 2^-24): a score
+is off by (D + 14) u S at most, S its largest sum of |q k| (see
+test_gpu_packed.py), which moves a weight by twice that of its own; the
+exponential, the sums of L keys and the split operands move it by 2 (L + 20) u.
+With w_k the exact weights and v_k the keys' values, no value is off by more
+than (2 (D + 14) u S + 2 (L + 20) u) sum_k w_k max|v_k|.  The halves of a
+weight times V scale leave 2^-36 of the largest such product, and V's own 2^-39
+of the key's largest value: L times both is below what the second term has
+for the L keys."""
+import numpy as np
+import pytest
+
+from gpu_util import say
+from oracle import packed
+from test_gpu_packed import U, Batch
+
+pytestmark = pytest.mark.gpu
+
+
+def check_rows(b, out=None):
+    out = b.run() if out is None else out
+    sizes = np.zeros((b.rows, b.nq, 3))
+    want, _, _, _ = packed.packed_attn(b.q, b.kc, b.vc, b.tables, b.row_start, b.lens, b.bs, b.nb, b.nq, b.D, b.gqa, b.scale,
+                                       b.window, b.masks, b.old, sizes)
+    A, S, L = sizes[..., 0], sizes[..., 1], sizes[..., 2]
+    bound = (2 * (b.D + 14) * U * S + 2 * (L + 20) * U) * A
+    assert np.isfinite(out).all()
+    off = np.abs(out - want).reshape(b.rows, b.nq, b.D).max(2)
+    taken = int(min(b.row_start[-1], b.rows))
+    worst = (off[:taken] / np.maximum(bound[:taken], 1e-300)).max()
+    say(f"  {worst:.3g} of the bound; relative {(off[:taken] / np.maximum(A[:taken], 1e-300)).max():.3g}")
+    assert (off <= bound).all(), np.argwhere(off > bound)[:4]
+    assert np.array_equal(out[taken:], b.old[taken:])
+
+
+def slots_of(b, r, positions):
+    positions = np.asarray(positions)
+    return b.tables[r, positions // b.bs] * b.bs + positions % b.bs
+
+
+@pytest.mark.parametrize("what", [1e6, 1e12, 1e16])
+@pytest.mark.parametrize("D", [256, 512])
+def test_finite_values_in_unseen_slots(ctx, D, what):
+    """Slots of no token, of tokens outside the window, of other requests' blocks."""
+    say("finite unseen", D, what)
+    b = Batch(ctx, 12, [30, 70, 4], [41, 0, 200], D=D, window=48)
+    seen = np.zeros(len(b.kc), bool)
+    for r in range(b.n):
+        n, length = int(b.row_start[r + 1] - b.row_start[r]), int(b.lens[r])
+        seen[slots_of(b, r, np.arange(max(0, length - n + 1 - 48), length))] = True
+    b.kc[~seen] *= np.float32(what)
+    b.vc[~seen] *= np.float32(what)
+    check_rows(b)
+
+
+@pytest.mark.parametrize("log", [16, 24, 40, 52])
+@pytest.mark.parametrize("D", [256, 512])
+def test_large_values_of_later_tokens(ctx, D, log):
+    """The prompts' last tokens' V is larger by a power of two: the rows before them do not see it."""
+    say("later tokens", D, log)
+    b = Batch(ctx, 60, [7, 90, 33], [0, 31, 300], D=D)
+    for r in range(b.n):
+        b.vc[slots_of(b, r, [b.lens[r] - 1])] *= np.float32(2.0 ** log)
+    check_rows(b)
+
+
+@pytest.mark.parametrize("log", [24, 45])
+@pytest.mark.parametrize("D", [256, 512])
+def test_large_values_of_other_branches(ctx, D, log):
+    """Every third drafted token's V is large: its descendants see it, the other branches do not."""
+    say("branches", D, log)
+    b = Batch(ctx, 61, [40, 64, 9], [70, 3, 0], D=D, words=2)
+    for r in range(b.n):
+        b.vc[slots_of(b, r, np.arange(b.lens[r] - 1, b.lens[r] - (b.row_start[r + 1] - b.row_start[r]), -3))] *= np.float32(2.0 ** log)
+    check_rows(b)
+
+
+@pytest.mark.parametrize("at", [0, 31, 64, 150, 199])
+@pytest.mark.parametrize("words", [0, 1])
+@pytest.mark.parametrize("D", [256, 512])
+def test_large_values_under_weights_of_nothing(ctx, D, words, at):
+    """A cached token 85 powers of two below the others' scores has a V 2^45 times theirs: 2^-40 of the result."""
+    say("weights of nothing", D, words, at)
+    b = Batch(ctx, 62, [20], [200], D=D, words=words, nq=2, sigma=0.25)
+    common = np.random.default_rng(1).standard_normal(D).astype(np.float32) / np.float32(np.sqrt(D))
+    b.q += np.tile(common, 2)                                             # every query's product with it: about one
+    slot = slots_of(b, 0, [at])
+    b.kc[slot] = -59.0 * common
+    b.vc[slot] *= np.float32(2.0 ** 45)
+    check_rows(b)
+
+
+@pytest.mark.parametrize("order", [1, -1])
+@pytest.mark.parametrize("D", [256, 512])
+def test_scores_that_rise_as_values_fall(ctx, D, order):
+    """Along 300 keys scores rise (or fall) by 60 powers of two and V's sizes fall (or rise) by as many, so that every
+    key adds alike; and V's alone by 50, so that the last (or first) keys' results remain."""
+    say("rise and fall", D, order)
+    for fall in (60, 50):
+        b = Batch(ctx, 63, [30], [300], D=D, nq=2, sigma=0.25)
+        common = np.random.default_rng(2).standard_normal(D).astype(np.float32)
+        common /= np.linalg.norm(common)
+        b.q = np.float32(0.01) * b.q + np.tile(common, 2)
+        pos = np.arange(330)
+        part = pos / 330.0 * order
+        slot = slots_of(b, 0, pos)
+        b.kc[slot] = np.float32(0.1) * b.kc[slot] + ((60 * np.log(2) * part)[:, None] * common).astype(np.float32)
+        b.vc[slot] *= (2.0 ** (-fall * part))[:, None].astype(np.float32)
+        check_rows(b)
+
+
+@pytest.mark.parametrize("words", [0, 2])
+@pytest.mark.parametrize("D", [256, 512])
+def test_values_of_any_size_by_what_a_row_sees(ctx, D, words):
+    """V's rows from 2^-50 to 2^50, cut tiles among them."""
+    say("any size by row", D, words)
+    b = Batch(ctx, 64, [40, 9, 60], [60, 200, 2500], D=D, words=words)
+    b.vc *= (2.0 ** np.random.default_rng(3).integers(-50, 50, (len(b.vc), 1))).astype(np.float32)
+    check_rows(b)
