@@ -588,8 +588,9 @@ struct Tile {
 #pragma unroll
         for (int i = 0; i < 16; ++i) o[i] = f4q{0, 0, 0, 0};
         // Scores stay in units of the row's q scale, whose inverse goes into the exponent's factor; the halves of heads of
-        // 512 have scales of their own
-        const float unit_q = kBoth ? 1.0f : qinv, factor = kBoth ? fminf(a.c * qinv, 3.4028235e38f) : a.c;
+        // 512 have scales of their own.  A factor of zero would make NaN of hidden keys' -inf; the least normal one keeps
+        // all weights at one as well.
+        const float unit_q = kBoth ? 1.0f : qinv, factor = kBoth ? fminf(fmaxf(a.c * qinv, 0x1p-126f), 3.4028235e38f) : a.c;
         float m = kNoScore, l = 0.0f, vref = kLeastRef;
         bool moved = false;                                       // a row's m, and with it vref, which is no power of two then
         f4q sc[2];

@@ -121,3 +121,16 @@ def test_values_of_any_size_by_what_a_row_sees(ctx, D, words):
     b = Batch(ctx, 64, [40, 9, 60], [60, 200, 2500], D=D, words=words)
     b.vc *= (2.0 ** np.random.default_rng(3).integers(-50, 50, (len(b.vc), 1))).astype(np.float32)
     check_rows(b)
+
+
+@pytest.mark.parametrize("words", [0, 1])
+@pytest.mark.parametrize("D", [256, 512])
+def test_rows_of_zeros_under_any_scale(ctx, D, words):
+    """Queries of zeros and of tiny values under scales from 1e-36 up: every key that a row sees weighs alike, no other
+    does."""
+    say("zeros", D, words)
+    for scale in (1e-36, 1e-20, 1e-6, 1.0, 1e20):
+        b = Batch(ctx, 65, [30, 9], [40, 900], D=D, words=words, scale=scale, sigma=4.0 * min(1.0, 1.0 / scale))
+        b.q[::3] = 0
+        b.q[1::3] *= np.float32(1e-18)
+        check_rows(b)
