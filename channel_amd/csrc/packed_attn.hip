@@ -285,9 +285,10 @@ __device__ __forceinline__ void halves(float x0, float scale0, float x1, float s
 
 // The power of two that brings values of magnitude `top` (its bits) below
 // 2^15, and its inverse: fp16 then holds what is 2^-39 of the largest and
-// more.  At most 2^100.
+// more.  At most 2^126, so that the inverse is no denormal; what is rounded
+// then lies below the type's least value.
 __device__ __forceinline__ float scale_for(uint32_t top, float &inverse) {
-    const uint32_t f = min(0x86000000u - (top & 0x7F800000u), 227u << 23);
+    const uint32_t f = min(0x86000000u - (top & 0x7F800000u), 253u << 23);
     inverse = __builtin_bit_cast(float, (254u << 23) - f);
     return __builtin_bit_cast(float, f);
 }
@@ -405,7 +406,9 @@ constexpr float kLead = 2.0f;
 // whatever its other keys' slots hold, and whatever lies under weights of nothing, takes no digits from them.  The
 // halves of those products are relative to it, 2^kWeightLog for one, so what is below 2^-36 of it is rounded to that;
 // it is raised when a product passes it by more than kRoom, which keeps them at or below 2^15.
-constexpr int kWeightLog = 12;
+// The inverses of V's scales are held times 2^kValueLog, so that weights times those of the least values, 2^-126, keep
+// their digits.
+constexpr int kWeightLog = 12, kValueLog = 40;
 constexpr float kRoom = 8.0f, kLeastRef = 0x1p-100f;
 
 // A tile's walk over its keys, 32 at a time.  A chunk has two phases:
@@ -496,7 +499,8 @@ struct Tile {
         load(kr, ka, chunk);
         return (uint32_t)(unheld >> (32 * (chunk & 1)));
     }
-    // the four keys' scales
+    // the four keys' scales, and their inverses times 2^LOG
+    template <int LOG = 0>
     __device__ __forceinline__ void scales(const f4q (&of)[4][H], float (&scale)[4], float *inverses) {
         uint32_t top[4];
 #pragma unroll
@@ -510,7 +514,7 @@ struct Tile {
         for (int i = 0; i < 4; ++i) {
             float inv;
             scale[i] = scale_for(__builtin_amdgcn_readlane(most, 16 * i), inv);
-            inverse[i] = inv;
+            inverse[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, inv) + (LOG << 23));
         }
         if (lane == 0) *(f4q *)(inverses + keys) = inverse;
     }
@@ -678,7 +682,7 @@ struct Tile {
         if (chunks) {
             all_k(0);
             if (kBoth) {
-                scales(vr(), vscale, lds.vinv[0]);
+                scales<kValueLog>(vr(), vscale, lds.vinv[0]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) store_v(e, vscale);
             }
@@ -723,7 +727,7 @@ struct Tile {
 
             if (!kBoth) {
                 // the registers hold V of chunk c: to LDS first
-                scales(vr(), vscale, lds.vinv[0]);
+                scales<kValueLog>(vr(), vscale, lds.vinv[0]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) store_v(e, vscale);
                 if (kMore) none2 = load_k(c + 2);
@@ -780,13 +784,13 @@ struct Tile {
                         l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
                         if (kBoth) weights(vinv);
                     }
-                    if constexpr (i == 3 && kBoth && kMore) scales(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
+                    if constexpr (i == 3 && kBoth && kMore) scales<kValueLog>(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
                     if constexpr (i >= 4 && kBoth && kMore) store_v(i - 4, vscale);
                     if constexpr (kMore) end_step();
                 });
                 if constexpr (kMore) end_scores(c + 1);
             } else if (kBoth && kMore) {
-                scales(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
+                scales<kValueLog>(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) store_v(e, vscale);
             }
@@ -847,7 +851,7 @@ struct Tile {
         }
         l = rows4_sum(l);
         if (!valid) return;
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f, unit = vref * (1.0f / (1 << kWeightLog));
+        const float inv = l != 0.0f ? 1.0f / l : 0.0f, unit = vref * (1.0f / (1ull << (kWeightLog + kValueLog)));
         float *to = row_out<D>(a, w, row) + 256 * half + 4 * g;
 #pragma unroll
         for (int j = 0; j < 4; ++j)

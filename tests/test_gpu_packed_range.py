@@ -134,3 +134,23 @@ def test_rows_of_zeros_under_any_scale(ctx, D, words):
         b.q[::3] = 0
         b.q[1::3] *= np.float32(1e-18)
         check_rows(b)
+
+
+@pytest.mark.parametrize("what,log", [("q", -115), ("q", -100), ("k", -115), ("k", -104), ("v", -100), ("v", -108), ("v", -118)])
+@pytest.mark.parametrize("D", [256, 512])
+def test_tiny_operands(ctx, D, what, log):
+    """Queries, K or V far below one, the scale making the scores ordinary ones; a row of V of zeros."""
+    say("tiny", D, what, log)
+    b = Batch(ctx, 67, [30, 9], [40, 900], D=D, scale=2.0 ** -log if what != "v" else 1.0)
+    {"q": b.q, "k": b.kc, "v": b.vc}[what][:] *= np.float32(2.0 ** log)
+    b.vc[slots_of(b, 0, [3])] = 0
+    check_rows(b)
+
+
+@pytest.mark.parametrize("D", [256, 512])
+def test_tiny_values_beside_ordinary_ones(ctx, D):
+    """Cached V near 2^-110, a new token's near one: rows before it keep their digits, those behind see both."""
+    say("tiny beside", D)
+    b = Batch(ctx, 68, [30], [40], D=D)
+    b.vc[slots_of(b, 0, np.arange(60))] *= np.float32(2.0 ** -110)
+    check_rows(b)
