@@ -292,7 +292,9 @@ __device__ __forceinline__ float scale_for(uint32_t top, float &inverse) {
     inverse = __builtin_bit_cast(float, (254u << 23) - f);
     return __builtin_bit_cast(float, f);
 }
-constexpr uint32_t kNotFinite = 0x7F800000u;           // magnitudes from here on are infinities and NaN
+// Magnitudes from here on, 2^56 (infinities and NaN among them), are left to fp32: below it no product of q and K, in units
+// of either's scale or of both, passes the type's range.
+constexpr uint32_t kPlain = (127u + 56) << 23;
 // NaN if either is
 __device__ __forceinline__ float largest(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 // the bits of the largest magnitude of N values, as unsigned words ordered as the values are
@@ -368,7 +370,7 @@ struct TileLds {
     unsigned char k[kBuffers][kKeyBytes], v[kBuffers][kKeyBytes];
     float kinv[kBuffers][32], vinv[kBuffers][32];
     float half[D == 512 ? 8 * 64 * 8 : 4];            // scores of the other half of the dims
-    uint32_t not_finite;                              // an infinity or NaN was met
+    uint32_t plain;                                   // what is left to fp32 was met
 };
 
 // By address: the places of a lane are one register and constants, and the
@@ -593,8 +595,9 @@ struct Tile {
         for (int i = 0; i < 16; ++i) o[i] = f4q{0, 0, 0, 0};
         // Scores stay in units of the row's q scale, whose inverse goes into the exponent's factor; the halves of heads of
         // 512 have scales of their own.  A factor of zero would make NaN of hidden keys' -inf; the least normal one keeps
-        // all weights at one as well.
-        const float unit_q = kBoth ? 1.0f : qinv, factor = kBoth ? fminf(fmaxf(a.c * qinv, 0x1p-126f), 3.4028235e38f) : a.c;
+        // all weights at one as well.  One that is too large is no number: fp32 computes the tile.
+        const float unit_q = kBoth ? 1.0f : qinv, factor = kBoth ? fmaxf(a.c * qinv, 0x1p-126f) : a.c;
+        if (factor > 3.4028235e38f) worst = kPlain;
         float m = kNoScore, l = 0.0f, vref = kLeastRef;
         bool moved = false;                                       // a row's m, and with it vref, which is no power of two then
         f4q sc[2];
@@ -692,7 +695,7 @@ struct Tile {
             }
             vnow = va;
             lds_barrier();
-            if (threadIdx.x == 0) lds.not_finite = 0;
+            if (threadIdx.x == 0) lds.plain = 0;
             if (active) {
                 begin_scores();
                 static_for<8>([&](auto step) {
@@ -842,9 +845,9 @@ struct Tile {
         for (int c = 0; c + 1 < chunks; ++c) walk(c, std::true_type());
         if (chunks) walk(chunks - 1, std::false_type());
         if (chunks) {
-            if (__any(worst >= kNotFinite) && lane == 0) lds.not_finite = 1;
+            if (__any(worst >= kPlain) && lane == 0) lds.plain = 1;
             lds_barrier();
-            if (lds.not_finite) {
+            if (lds.plain) {
                 rows_plain<D>(a, w);
                 return;
             }

@@ -711,8 +711,10 @@ int chn_draft_trees(chn_ctx *ctx, const uint32_t *parents, const uint32_t *row_s
  * finite, not zero; n_req <= 8192, n_rows <= 2^24; max_blocks * block_size <
  * 2^31.  out must not overlap an input.  Products are formed of operands split
  * in two 11-bit halves (errors as fp32's own) and summed in fp32; the rows of a
- * tile (up to 128, with the keys that any of them sees) that meets an infinity
- * or a NaN in q, K or V are computed again in plain fp32, several times slower.
+ * tile (up to 128, with the keys that any of them sees) that meets an infinity,
+ * a NaN or a magnitude of 2^56 and more in q, K or V, or a query whose largest
+ * component times the scale passes 2^141, are computed again in plain fp32, much
+ * slower.
  * Workspace: 68 MB, whatever the batch. */
 int chn_paged_causal_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
                           const uint32_t *tables, const uint32_t *row_start, const uint32_t *lens, uint32_t n_req,

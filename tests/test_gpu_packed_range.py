@@ -154,3 +154,52 @@ def test_tiny_values_beside_ordinary_ones(ctx, D):
     b = Batch(ctx, 68, [30], [40], D=D)
     b.vc[slots_of(b, 0, np.arange(60))] *= np.float32(2.0 ** -110)
     check_rows(b)
+
+
+@pytest.mark.parametrize("D", [256, 512])
+def test_factors_beyond_the_type(ctx, D):
+    """Scale times the queries' largest component passes 2^128, their products with K are of ordinary size: no key has
+    anything where the query is large."""
+    say("factors", D)
+    b = Batch(ctx, 66, [30, 9], [40, 900], D=D, scale=2.0 ** 122)
+    b.q[:, ::D] = 2.0 ** 24
+    b.kc *= np.float32(2.0 ** -122)
+    b.kc[:, ::D] = 0
+    check_rows(b)
+
+
+@pytest.mark.parametrize("k,q", [(60, -60), (104, -104), (112, -112), (124, -124), (-60, 60), (-104, 104), (-112, 112)])
+@pytest.mark.parametrize("D", [256, 512])
+def test_large_keys_and_queries(ctx, D, k, q):
+    """K or queries up to 2^124, the other as small: ordinary scores."""
+    say("large", D, k, q)
+    b = Batch(ctx, 69, [30, 9], [40, 900], D=D)
+    b.kc *= np.float32(2.0 ** k)
+    b.q *= np.float32(2.0 ** q)
+    check_rows(b)
+
+
+@pytest.mark.parametrize("words", [0, 1])
+@pytest.mark.parametrize("log", [55, 57, 100, 120])
+@pytest.mark.parametrize("D", [256, 512])
+def test_large_values(ctx, D, log, words):
+    """All of V large; one cached token's, which all rows see; one drafted or later token's."""
+    say("large V", D, log, words)
+    for at in (slice(None), 5, 950):
+        b = Batch(ctx, 70, [30, 20], [40, 940], D=D, words=words)
+        b.vc[at if isinstance(at, slice) else slots_of(b, 1, [at])] *= np.float32(2.0 ** log)
+        check_rows(b)
+
+
+@pytest.mark.parametrize("what", [1e18, 1e30])
+@pytest.mark.parametrize("D", [256, 512])
+def test_huge_values_in_unseen_slots(ctx, D, what):
+    say("huge unseen", D, what)
+    b = Batch(ctx, 71, [30, 70], [41, 0], D=D, window=48)
+    seen = np.zeros(len(b.kc), bool)
+    for r in range(b.n):
+        n, length = int(b.row_start[r + 1] - b.row_start[r]), int(b.lens[r])
+        seen[slots_of(b, r, np.arange(max(0, length - n + 1 - 48), length))] = True
+    b.kc[~seen] *= np.float32(what)
+    b.vc[~seen] *= np.float32(what)
+    check_rows(b)
