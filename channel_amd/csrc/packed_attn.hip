@@ -109,7 +109,7 @@ struct TileKeys {
         k.last_full = k.tiles > 8 ? k.full : (s.n - (k.tiles - 1) * a.tokens) * a.gqa > tile_rows(D) / 2;
         if (a.mask_words) {
             k.T = 0;
-            k.hi0 = max(0, min(s.len, s.have + (int)(32 * a.mask_words)));
+            k.hi0 = max(0, s.have + min(s.n, (int)(32 * a.mask_words)));      // no sum passes the length
             k.lo0 = a.window ? min(max(0, s.have - a.window), (int)k.hi0) : 0;
         } else {
             k.T = a.tokens;
@@ -146,7 +146,7 @@ __device__ __forceinline__ int64_t snapped(int64_t at, int64_t cost, bool whole)
     return at < kNearEnd ? 0 : (at + kNearEnd > cost ? cost : at);
 }
 
-// One tile's share: rows, and keys key0 .. key1 - 1 (key0 a multiple of 32).
+// One tile's share: rows, and keys key0 .. key1 - 1 (key0 a multiple of 32, or no keys).
 struct Work {
     Seq s;
     const uint32_t *table;
@@ -208,12 +208,12 @@ __device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
             o[k] = f4q{0, 0, 0, 0};
         }
         float m = kNoScore, l = 0.0f;
-        for (int k0 = w.key0; k0 < w.key1; k0 += 32) {
+        for (uint32_t k0 = w.key0; k0 < (uint32_t)w.key1; k0 += 32) {                         // up to 2^31 and 32
             // 32 keys from zero, then added, so that long lists keep fp32's digits
             f4q some[N];
             float part = 0.0f;
             for (int k = 0; k < N; ++k) some[k] = f4q{0, 0, 0, 0};
-            for (int pos = k0; pos < min(k0 + 32, w.key1); ++pos) {
+            for (int pos = (int)k0; pos < (int)min(k0 + 32, (uint32_t)w.key1); ++pos) {
                 bool ok = pos >= s.lo && pos < s.hi;
                 const int node = pos - w.s.have;
                 if (s.mask && node >= 0) ok = (s.mask[node >> 5] >> (node & 31)) & 1;      // key1 is below 32 mask_words of them
@@ -476,10 +476,10 @@ struct Tile {
 
     // chunks come in pairs, 64 keys, a lane each
     __device__ __forceinline__ uint32_t block_of(int pair) const {
-        return w.table[min((uint32_t)w.key0 + 64 * pair + lane, (uint32_t)w.key1 - 1) >> a.shift];
+        return w.table[min((uint32_t)w.key0 + 64u * pair + lane, (uint32_t)w.key1 - 1) >> a.shift];
     }
     __device__ __forceinline__ void take_pair(int pair) {
-        const uint32_t pos = (uint32_t)w.key0 + 64 * pair + lane, b = next_block;      // unsigned: up to 2^31 and a pair
+        const uint32_t pos = (uint32_t)w.key0 + 64u * pair + lane, b = next_block;      // unsigned: up to 2^31 and a pair
         const bool held = pos < (uint32_t)w.key1 && b < a.n_blocks;
         const size_t at = (size_t)((b << a.shift) + (pos & ((1u << a.shift) - 1))) * a.kv_dim + (size_t)w.kvh * D;
         ka = held ? (mem_t)a.kc + at : (mem_t)no_key;
@@ -551,7 +551,7 @@ struct Tile {
     __device__ __forceinline__ void run() {
         const uint32_t row = rt * 16 + q;
         const bool valid = row < w.rows, active = (uint32_t)(rt * 16) < w.rows;
-        const int chunks = w.key1 > w.key0 ? (w.key1 - w.key0 + 31) / 32 : 0;
+        const int chunks = w.key1 > w.key0 ? (int)(((uint32_t)(w.key1 - w.key0) + 31) / 32) : 0;
         uint32_t none0 = 0, none1 = 0, none2 = 0, none3 = 0;      // keys that are nobody's, of chunks c ..
         if (chunks) next_block = block_of(0);
         const uint32_t of_tile = valid ? token_of(a, row) : 0;
@@ -977,9 +977,10 @@ __device__ __forceinline__ void each_work(const Packed &a, F &&f) {
             const int tokens = min(w.s.n - w.token, (int)a.tokens), lo = (int)k.lo(t);
             w.rows = (uint32_t)tokens * a.gqa;
             const int limit = a.mask_words ? (int)k.hi(t) : max(0, w.s.have + w.token + tokens);
-            // cuts at whole chunks of 32 keys
-            w.key0 = from ? (int)((lo + k.keys_at(t, from) + 31) >> 5 << 5) : lo >> 5 << 5;
-            w.key1 = to < cost ? min((int)((lo + k.keys_at(t, to) + 31) >> 5 << 5), limit) : limit;
+            // cuts at whole chunks of 32 keys, none behind the last
+            const auto chunk_at = [&](int64_t units) { return (int)min((lo + k.keys_at(t, units) + 31) >> 5 << 5, (int64_t)limit); };
+            w.key0 = from ? chunk_at(from) : lo >> 5 << 5;
+            w.key1 = to < cost ? chunk_at(to) : limit;
             w.part = from ? (int)(2 * share) : (to < cost ? (int)(2 * share + 1) : -1);
             if (from && to == cost && tid == 0) {
                 // the share that begins this tile: the last whose first cut is at or before it

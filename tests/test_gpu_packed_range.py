@@ -14,20 +14,25 @@ for the L keys."""
 import numpy as np
 import pytest
 
+import channel_amd as ca
 from gpu_util import say
 from oracle import packed
 from test_gpu_packed import U, Batch
+from test_gpu_paged import up32
 
 pytestmark = pytest.mark.gpu
 
 
-def check_rows(b, out=None):
+def check_rows(b, out=None, but=()):
+    """All rows but the ones named."""
     out = b.run() if out is None else out
     sizes = np.zeros((b.rows, b.nq, 3))
     want, _, _, _ = packed.packed_attn(b.q, b.kc, b.vc, b.tables, b.row_start, b.lens, b.bs, b.nb, b.nq, b.D, b.gqa, b.scale,
                                        b.window, b.masks, b.old, sizes)
     A, S, L = sizes[..., 0], sizes[..., 1], sizes[..., 2]
     bound = (2 * (b.D + 14) * U * S + 2 * (L + 20) * U) * A
+    out, want = out.copy(), want.copy()
+    out[list(but)] = want[list(but)] = 0
     assert np.isfinite(out).all()
     off = np.abs(out - want).reshape(b.rows, b.nq, b.D).max(2)
     taken = int(min(b.row_start[-1], b.rows))
@@ -203,3 +208,29 @@ def test_huge_values_in_unseen_slots(ctx, D, what):
     b.kc[~seen] *= np.float32(what)
     b.vc[~seen] *= np.float32(what)
     check_rows(b)
+
+
+@pytest.mark.parametrize("plain", [False, True])
+@pytest.mark.parametrize("words", [0, 1])
+@pytest.mark.parametrize("D", [256, 512])
+def test_lengths_at_the_end_of_their_range(ctx, D, words, plain):
+    """A request of 2^31 - 16 tokens on a sliding layer, the last block of its table full: the same as one of 128 tokens
+    whose table is that table's end.  plain: a row's query is NaN, so that its tile is computed in plain fp32."""
+    say("long end", D, words, plain)
+    width, small = (1 << 27) - 1, 8
+    b = Batch(ctx, 72, [5], [small * 16 - 5], D=D, words=words, window=64, width=small, spare=0)
+    if plain:
+        b.q[3, 7] = np.nan
+    b.up()
+    table = ctx.zeros(width * 4)
+    end = np.ascontiguousarray(b.tables, np.uint32)
+    ctx._check("chn_upload", ca.lib.chn_upload(ctx.handle, table.offset((width - small) * 4), end.ctypes.data, end.nbytes))
+    b.dev.update(tables=table, lens=up32(ctx, [width * 16]))
+    b.width = width
+    b.call()
+    out = b.got()
+    table.free()
+    b.width = small
+    if plain:
+        assert np.isnan(out[3, :D]).all()
+    check_rows(b, out, [3] if plain else [])
