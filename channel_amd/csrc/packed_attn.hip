@@ -110,7 +110,7 @@ struct TileKeys {
         if (a.mask_words) {
             k.T = 0;
             k.hi0 = max(0, s.have + min(s.n, (int)(32 * a.mask_words)));      // no sum passes the length
-            k.lo0 = a.window ? min(max(0, s.have - a.window), (int)k.hi0) : 0;
+            k.lo0 = a.window && s.have > a.window ? s.have - a.window : 0;
         } else {
             k.T = a.tokens;
             k.hi0 = max(s.have, 0) + k.T;
@@ -170,11 +170,11 @@ __device__ __forceinline__ Seen seen_by(const Packed &a, const Work &w, int toke
         if (a.window) {
             int ones = 0;
             for (uint32_t i = 0; i < a.mask_words; ++i) ones += __popc(s.mask[i]);
-            s.lo = max(0, w.s.have + ones - a.window);
+            s.lo = w.s.have > a.window - ones ? w.s.have - (a.window - ones) : 0;      // a window is no shorter than a mask
         }
     } else {
         s.hi = w.s.have + token + 1;
-        s.lo = a.window ? max(0, s.hi - a.window) : 0;
+        s.lo = a.window && s.hi > a.window ? s.hi - a.window : 0;
     }
     return s;
 }

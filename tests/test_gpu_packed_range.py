@@ -234,3 +234,13 @@ def test_lengths_at_the_end_of_their_range(ctx, D, words, plain):
     if plain:
         assert np.isnan(out[3, :D]).all()
     check_rows(b, out, [3] if plain else [])
+
+
+@pytest.mark.parametrize("window", [0, 128, (1 << 31) - 2, (1 << 31) - 1, (1 << 32) - 1])
+@pytest.mark.parametrize("words", [0, 1, 2])
+def test_windows_longer_than_any_request(ctx, words, window):
+    """Windows up to 2^32 - 1 where requests hold fewer tokens than they have rows, as many, and more."""
+    say("long windows", words, window)
+    b = Batch(ctx, 73, [30, 9, 20, 8], [0, 0, 100, 3], words=words, window=window)
+    b.lens = np.array([12, 9, 120, 5])
+    check_rows(b)
