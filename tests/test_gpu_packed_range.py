@@ -241,6 +241,6 @@ def test_lengths_at_the_end_of_their_range(ctx, D, words, plain):
 def test_windows_longer_than_any_request(ctx, words, window):
     """Windows up to 2^32 - 1 where requests hold fewer tokens than they have rows, as many, and more."""
     say("long windows", words, window)
-    b = Batch(ctx, 73, [30, 9, 20, 8], [0, 0, 100, 3], words=words, window=window)
-    b.lens = np.array([12, 9, 120, 5])
+    b = Batch(ctx, 73, [30, 9, 60, 20, 8, 64], [0, 0, 0, 100, 3, 0], words=words, window=window)
+    b.lens = np.array([12, 9, 50, 120, 5, 63])
     check_rows(b)
