@@ -37,6 +37,7 @@ struct LogProbs {
     uint32_t *ranks, *ids;
     float *tops;
     // workspace, per row: block maxima and, per stretch, maxima (orderable, 0: nothing allowed), the two sums, the count
+    // (16 bits) and, with a softcap, how many equal the maximum (above them; the sums are then without those)
     uint32_t blocks, stretches;
     uint32_t *bmax, *smax, *ahead;
     float *sum, *xsum;
@@ -162,6 +163,7 @@ __global__ __launch_bounds__(256) void k_logprob_sums(LogProbs a) {
         if (__any(same)) before += (uint32_t)wave_sum_u64(same);
     }
     float S = 0.0f, X = 0.0f;
+    uint32_t ties = 0;
     if (scored(top) && !greedy) {
         const float ref = capped<CAP>(top, cap, inv_cap);
         if (fabsf(ref) <= 1e30f && powers >= 1e-6f && powers <= 1e30f) {
@@ -172,7 +174,11 @@ __global__ __launch_bounds__(256) void k_logprob_sums(LogProbs a) {
                 for (int e = 0; e < 4; ++e) {
                     const float d = larger_of((capped<CAP>(v[j][e], cap, inv_cap) - ref) * powers, -200.0f);
                     float p = __builtin_amdgcn_exp2f(d);
-                    if (CAP) p = scored(v[j][e]) ? p : 0.0f;              // -inf is capped too
+                    if (CAP) {
+                        const bool tie = v[j][e] == top;
+                        ties += tie;
+                        p = scored(v[j][e]) && !tie ? p : 0.0f;           // -inf is capped too
+                    }
                     S += p;
                     X = fmaf(p, d, X);
                 }
@@ -180,17 +186,20 @@ __global__ __launch_bounds__(256) void k_logprob_sums(LogProbs a) {
             for (int j = 0; j < 8; ++j)
                 for (int e = 0; e < 4; ++e) {
                     const float d = distance(capped<CAP>(v[j][e], cap, inv_cap), ref, powers);
-                    const float p = scored(v[j][e]) ? __builtin_amdgcn_exp2f(d) : 0.0f;
+                    const bool tie = CAP && v[j][e] == top;
+                    ties += tie;
+                    const float p = scored(v[j][e]) && !tie ? __builtin_amdgcn_exp2f(d) : 0.0f;
                     S += p;
-                    X += scored(v[j][e]) ? p * d : 0.0f;
+                    X += scored(v[j][e]) && !tie ? p * d : 0.0f;
                 }
         }
         S = wave_sum64(S);
         X = wave_sum64(X);
+        if (CAP) ties = __any(ties > 1) ? (uint32_t)wave_sum_u64(ties) : (uint32_t)__popcll(__ballot(ties));
     }
     if (lane == 0) {
         a.smax[at] = scored(top) ? ordered(top) : 0u;
-        a.ahead[at] = before;
+        a.ahead[at] = before | ties << 16;
         a.sum[at] = S;
         a.xsum[at] = X;
     }
@@ -201,6 +210,7 @@ constexpr int kScoreWaves = kScoreThreads / 64;
 struct RowSums {
     float sum[kScoreWaves], xsum[kScoreWaves];
     uint32_t most[kScoreWaves], before[kScoreWaves];
+    float ties[kScoreWaves];
     uint32_t counts[2][kScoreWaves][4];
 };
 
@@ -257,7 +267,7 @@ __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
     if (tid == 0) n_chosen = n_list = n_few = 0;
 
     // the stretches: at most 512, two a thread; the blocks' maxima
-    uint32_t m[2], before = 0;
+    uint32_t m[2], ahead[2];
     float S[2], X[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -265,7 +275,7 @@ __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
         const size_t at = (size_t)row * a.stretches + min(s, a.stretches - 1);
         const bool there = s < a.stretches;
         m[i] = there ? a.smax[at] : 0u;
-        before += there ? a.ahead[at] : 0u;
+        ahead[i] = there ? a.ahead[at] : 0u;
         S[i] = a.sum[at];
         X[i] = a.xsum[at];
     }
@@ -287,40 +297,52 @@ __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
     for (int w = 0; w < kScoreWaves; ++w) most = max(most, sh.most[w]);
     const float top = unordered(most);
     float sum = 0.0f, xsum = 0.0f;
+    uint32_t before = 0;
+    float ties = 0.0f;                                          // of the row's largest: at most 2^20
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i) {
+        const float same = (float)(ahead[i] >> 16);
+        before += ahead[i] & 0xFFFFu;
+        if (CAP && m[i] == most) ties += same;
+        else if (CAP) S[i] += same;
         if (m[i]) {
             const float d = distance(capped<CAP>(unordered(m[i]), a.cap, inv_cap), capped<CAP>(top, a.cap, inv_cap), powers);
             const float f = __builtin_amdgcn_exp2f(d);
             xsum += f * (X[i] + d * S[i]);
             sum += f * S[i];
         }
+    }
     sum = wave_sum64(sum);
     xsum = wave_sum64(xsum);
     before = (uint32_t)wave_sum_u64(before);
+    if (CAP) ties = wave_sum64(ties);
     if (lane == 0) {
         sh.sum[wave] = sum;
         sh.xsum[wave] = xsum;
         sh.before[wave] = before;
+        if (CAP) sh.ties[wave] = ties;
     }
     __syncthreads();
-    sum = xsum = 0.0f;
+    sum = xsum = ties = 0.0f;
     before = 0;
 #pragma unroll
     for (int w = 0; w < kScoreWaves; ++w) {
         sum += sh.sum[w];
         xsum += sh.xsum[w];
         before += sh.before[w];
+        if (CAP) ties += sh.ties[w];
     }
     const double T = a.temperature ? (double)a.temperature[row] : 1.0;
-    // The sums are relative to the largest capped in fp32: its rounding is taken out of what the other tokens add to the
-    // largest's one.  Theirs go both ways.
+    // With a softcap the sums are those of the other tokens, relative to the largest capped in fp32: its rounding is taken
+    // out of them again, theirs go both ways.  Where that is much of an exponent (T near a step of fp32's of the cap, and
+    // below) it is left in: a token's weight is then one at most.
     double all = (double)sum, mean = 0.69314718055994531 * (double)xsum;
     if (CAP && !greedy) {
-        const double off = fmin(fmax(((double)capped<CAP>(top, a.cap, inv_cap) - capped64<CAP>(top, a.cap)) / T, -50.0), 50.0);
-        const double f = exp(off), others = all - 1.0;
+        double off = ((double)capped<CAP>(top, a.cap, inv_cap) - capped64<CAP>(top, a.cap)) / T;
+        if (!(fabs(off) <= 0.5)) off = 0.0;
+        const double f = exp(off), others = all;
         mean = f * (mean + others * off);
-        all = 1.0 + others * f;
+        all = (double)ties + others * f;
     }
     const double log_sum = greedy ? 0.0 : log(all);
     // of an allowed logit; `first`: no token comes before it
