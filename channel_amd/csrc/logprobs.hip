@@ -52,16 +52,23 @@ __device__ __forceinline__ float unordered(uint32_t o) {
     return __builtin_bit_cast(float, (o & 0x80000000u) ? (o & 0x7FFFFFFFu) : ~o);
 }
 
-// cap tanh(l / cap) from exp(-2 |l / cap|), off by about two steps of fp32:
-// the sums average it out, and what is returned of single tokens is formed in
-// 64 bits.
-template <bool CAP>
+// CAP: 0 no softcap, 1 and 2 cap tanh(l / cap) from exp(-2 |l / cap|), off by
+// about two steps of fp32 of the cap: the sums average it out, and what is
+// returned of single tokens is formed in 64 bits.  A cap that is large beside
+// the logits would take their digits, so 2 has the series of tanh below a quarter
+// of the cap, off by steps of the logit (its next term is 2^-27 of it).  Caps
+// up to kStepCap take 1: 500 rows of 262144 in 124 us, with 2 143.
+constexpr float kStepCap = 64.0f;
+template <int CAP>
 __device__ __forceinline__ float capped(float l, float cap, float inv_cap) {
     if (!CAP) return l;
-    const float t = __builtin_amdgcn_exp2f(-2.8853900817779268f * fabsf(l * inv_cap));
-    return copysignf(cap * ((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t)), l);
+    const float x = l * inv_cap, t = __builtin_amdgcn_exp2f(-2.8853900817779268f * fabsf(x));
+    const float y = copysignf(cap * ((1.0f - t) * __builtin_amdgcn_rcpf(1.0f + t)), l);
+    if (CAP == 1) return y;
+    const float z = x * x, series = fmaf(fmaf(fmaf(62.0f / 2835, z, -17.0f / 315), z, 2.0f / 15), z, -1.0f / 3);
+    return fabsf(x) < 0.25f ? fmaf(l * z, series, l) : y;
 }
-template <bool CAP>
+template <int CAP>
 __device__ __forceinline__ double capped64(float l, float cap) {
     return CAP ? (double)cap * tanh((double)l / (double)cap) : (double)l;
 }
@@ -113,7 +120,7 @@ __device__ __forceinline__ int max8_order(int i) {                       // the 
 // A wave's 2048 values: 256 a load, four of them a lane, all eight loads under
 // way at once.  Bound by memory where there are many rows: 500 rows of 262144,
 // 524 MB, in 84-90 us (5.8-6.3 TB/s); one row is a latency, 4.0 us.
-template <bool CAP>
+template <int CAP>
 __global__ __launch_bounds__(256) void k_logprob_sums(LogProbs a) {
     const uint32_t row = blockIdx.y, s = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int lane = threadIdx.x & 63;
@@ -251,7 +258,7 @@ constexpr uint32_t kScoreFew = 256;          // keys that are ranked by counting
 // sums, the bound on the block maxima two bits at a time, the chosen blocks,
 // their ranks.  500 rows with 5 alternatives 10.4 us; one with 20, softcapped,
 // 11.7.  KEYS: block maxima of a thread (4 up to 262144 values, else 16).
-template <bool CAP, int KEYS>
+template <int CAP, int KEYS>
 __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
     extern __shared__ uint64_t list[];                          // n_top * kScoreBlock keys
     __shared__ RowSums sh;
@@ -418,7 +425,7 @@ __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
     }
 }
 
-template <bool CAP>
+template <int CAP>
 static void launch_scores(chn_ctx *ctx, const LogProbs &a, uint32_t n) {
     k_logprob_sums<CAP><<<dim3((a.stretches + 3) / 4, n), 256, 0, ctx->stream>>>(a);
     const size_t lds = (size_t)a.n_top * kScoreBlock * 8;
@@ -476,7 +483,9 @@ extern "C" int chn_token_logprobs(chn_ctx *ctx, const float *logits, uint32_t n_
         a.ids = n_top ? top_ids + (size_t)r0 * n_top : nullptr;
         a.tops = n_top ? top_logprobs + (size_t)r0 * n_top : nullptr;
         const uint32_t n = std::min(n_rows - r0, kScoreRows);
-        softcap > 0.0f ? launch_scores<true>(ctx, a, n) : launch_scores<false>(ctx, a, n);
+        if (softcap > kStepCap) launch_scores<2>(ctx, a, n);
+        else if (softcap > 0.0f) launch_scores<1>(ctx, a, n);
+        else launch_scores<0>(ctx, a, n);
         CHN_LAUNCHED(ctx, "k_logprob");
     }
     return CHN_OK;

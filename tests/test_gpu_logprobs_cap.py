@@ -79,3 +79,25 @@ def test_a_dominant_token(ctx):
     at = rng.integers(0, 30000, 8)
     x[np.arange(8), at] = rng.uniform(27, 60, 8).astype(np.float32)
     check_capped(ctx, x, at, [1.0] * 8, 50.0)
+
+
+@pytest.mark.parametrize("cap", [65.0, 100.0, 1e3, 1e4, 1e6, 1e15, 3e38])
+def test_softcaps_far_above_the_logits(ctx, cap):
+    """Softcaps that hardly bend the logits: with the capped logit off by 8 u of its own size, and not of the cap's, log S
+    is off by 8 u max|l| / T and the rest of it as without a softcap."""
+    say("large softcaps", cap)
+    x, rng = model_rows(23, 6, 9000)
+    x[3] *= 4
+    x[4, ::7] = -np.inf
+    x[5, ::5] = np.float32(-1e30)                                          # at the cap's other end
+    T = [1, 0.5, 2, 1, 1, 1]
+    targets = rng.integers(0, 9000, 6) // 7 * 7 + 1
+    lp, ent, ranks, ids, tops = run(ctx, x, targets, T, cap, 5)
+    for r in range(6):
+        w = packed.logprob_row(x[r], int(targets[r]), T[r], cap, 5)
+        size = np.abs(x[r][np.abs(x[r]) < 1e20]).max()
+        bound = 4 * U * w[1] + U * (4 + 2 * np.log2(9000)) + 8 * U * size / T[r]
+        say(f"  {abs(lp[r] - w[0]):.2g} {abs(ent[r] - w[1]):.2g} of {bound:.2g}")
+        assert near(lp[r], w[0], bound) and near(ent[r], w[1], 2 * bound), (r, lp[r], w[:2], ent[r])
+        assert ranks[r] == w[2] and ids[r].tolist() == w[3]
+        assert all(near(g, v, bound) for g, v in zip(tops[r], w[4]))
