@@ -68,6 +68,8 @@ __device__ __forceinline__ float capped(float l, float cap, float inv_cap) {
     const float z = x * x, series = fmaf(fmaf(fmaf(62.0f / 2835, z, -17.0f / 315), z, 2.0f / 15), z, -1.0f / 3);
     return fabsf(x) < 0.25f ? fmaf(l * z, series, l) : y;
 }
+// of denormal caps no infinity, whose product with zero is none
+__device__ __forceinline__ float inverse_of(float cap) { return fminf(1.0f / cap, 3.4028235e38f); }
 template <int CAP>
 __device__ __forceinline__ double capped64(float l, float cap) {
     return CAP ? (double)cap * tanh((double)l / (double)cap) : (double)l;
@@ -144,7 +146,7 @@ __global__ __launch_bounds__(256) void k_logprob_sums(LogProbs a) {
     const uint32_t target = a.targets[row];
     const float mine = target < a.V ? x[target] : __builtin_nanf("");
     bool greedy;
-    const float powers = powers_of(a, row, greedy), cap = a.cap, inv_cap = 1.0f / cap;
+    const float powers = powers_of(a, row, greedy), cap = a.cap, inv_cap = inverse_of(cap);
     float m[8];
 #pragma unroll
     for (int j = 0; j < 8; ++j) m[j] = larger_of(v[j][3], larger_of(v[j][2], larger_of(v[j][1], larger_of(v[j][0], -__builtin_inff()))));
@@ -270,7 +272,7 @@ __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
     const uint32_t target = a.targets[row];
     const float mine = target < a.V ? x[target] : __builtin_nanf("");
     bool greedy;
-    const float powers = powers_of(a, row, greedy), inv_cap = 1.0f / a.cap;
+    const float powers = powers_of(a, row, greedy), inv_cap = inverse_of(a.cap);
     if (tid == 0) n_chosen = n_list = n_few = 0;
 
     // the stretches: at most 512, two a thread; the blocks' maxima

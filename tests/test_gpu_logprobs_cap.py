@@ -101,3 +101,20 @@ def test_softcaps_far_above_the_logits(ctx, cap):
         assert near(lp[r], w[0], bound) and near(ent[r], w[1], 2 * bound), (r, lp[r], w[:2], ent[r])
         assert ranks[r] == w[2] and ids[r].tolist() == w[3]
         assert all(near(g, v, bound) for g, v in zip(tops[r], w[4]))
+
+
+@pytest.mark.parametrize("cap", [1e-45, 1e-40, 1e-30, 1e-3])
+def test_softcaps_of_nothing(ctx, cap):
+    """All logits capped to nothing beside the temperature, zeros among them: every token alike."""
+    say("small softcaps", cap)
+    x, rng = model_rows(24, 3, 5000)
+    x[1, ::3] = 0
+    x[2] = 0
+    targets = rng.integers(0, 5000, 3)
+    T = 1e3
+    lp, ent, ranks, ids, _ = run(ctx, x, targets, [T] * 3, cap, 5)
+    for r in range(3):
+        w = packed.logprob_row(x[r], int(targets[r]), T, cap, 5)
+        bound = 4 * U * w[1] + U * (4 + 2 * np.log2(5000)) + 8 * U * cap / T
+        assert near(lp[r], w[0], bound) and near(ent[r], w[1], 2 * bound), (r, lp[r], w[:2])
+        assert ranks[r] == w[2] and ids[r].tolist() == w[3]
