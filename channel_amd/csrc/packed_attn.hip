@@ -292,9 +292,9 @@ __device__ __forceinline__ float scale_for(uint32_t top, float &inverse) {
     inverse = __builtin_bit_cast(float, (254u << 23) - f);
     return __builtin_bit_cast(float, f);
 }
-// Magnitudes from here on, 2^56 (infinities and NaN among them), are left to fp32: below it no product of q and K, in units
-// of either's scale or of both, passes the type's range.
-constexpr uint32_t kPlain = (127u + 56) << 23;
+// Magnitudes of q and K from here on, 2^56 (infinities and NaN among them), are left to fp32: below it none of their
+// products, in units of either's scale or of both, passes the type's range.  Of V's only infinities and NaN are.
+constexpr uint32_t kPlain = (127u + 56) << 23, kNotFinite = 0x7F800000u;
 // NaN if either is
 __device__ __forceinline__ float largest(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 // the bits of the largest magnitude of N values, as unsigned words ordered as the values are
@@ -408,10 +408,10 @@ constexpr float kLead = 2.0f;
 // whatever its other keys' slots hold, and whatever lies under weights of nothing, takes no digits from them.  The
 // halves of those products are relative to it, 2^kWeightLog for one, so what is below 2^-36 of it is rounded to that;
 // it is raised when a product passes it by more than kRoom, which keeps them at or below 2^15.
-// The inverses of V's scales are held times 2^kValueLog, so that weights times those of the least values, 2^-126, keep
-// their digits.
-constexpr int kWeightLog = 12, kValueLog = 40;
-constexpr float kRoom = 8.0f, kLeastRef = 0x1p-100f;
+// The inverses of V's scales, 2^-126 to 2^113, are held times 2^kValueLog, so that weights times the least of them keep
+// their digits and times the greatest stay below 2^127.
+constexpr int kWeightLog = 12, kValueLog = 11;
+constexpr float kRoom = 8.0f, kLeastRef = 0x1p-115f;
 
 // A tile's walk over its keys, 32 at a time.  A chunk has two phases:
 //   1  the scores of chunk c + 1, beside them the weights of chunk c and a V
@@ -501,22 +501,23 @@ struct Tile {
         load(kr, ka, chunk);
         return (uint32_t)(unheld >> (32 * (chunk & 1)));
     }
-    // the four keys' scales, and their inverses times 2^LOG
-    template <int LOG = 0>
+    // the four keys' scales, and their inverses: K's, or V's times 2^kValueLog
+    template <bool VALUES = false>
     __device__ __forceinline__ void scales(const f4q (&of)[4][H], float (&scale)[4], float *inverses) {
         uint32_t top[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             top[i] = magnitude<4 * H>([&](int e) { return of[i][e / 4][e % 4]; });
-            worst = max(worst, top[i]);
         }
+        const uint32_t here = max(max(top[0], top[1]), max(top[2], top[3]));
+        worst = max(worst, VALUES ? __builtin_elementwise_sub_sat(here, kNotFinite - kPlain) : here);
         const uint32_t most = wave_top4(top);
         f4q inverse;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float inv;
             scale[i] = scale_for(__builtin_amdgcn_readlane(most, 16 * i), inv);
-            inverse[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, inv) + (LOG << 23));
+            inverse[i] = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, inv) + (VALUES ? kValueLog << 23 : 0));
         }
         if (lane == 0) *(f4q *)(inverses + keys) = inverse;
     }
@@ -685,7 +686,7 @@ struct Tile {
         if (chunks) {
             all_k(0);
             if (kBoth) {
-                scales<kValueLog>(vr(), vscale, lds.vinv[0]);
+                scales<true>(vr(), vscale, lds.vinv[0]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) store_v(e, vscale);
             }
@@ -730,7 +731,7 @@ struct Tile {
 
             if (!kBoth) {
                 // the registers hold V of chunk c: to LDS first
-                scales<kValueLog>(vr(), vscale, lds.vinv[0]);
+                scales<true>(vr(), vscale, lds.vinv[0]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) store_v(e, vscale);
                 if (kMore) none2 = load_k(c + 2);
@@ -787,13 +788,13 @@ struct Tile {
                         l += ((p[0] + p[1]) + (p[2] + p[3])) + ((p[4] + p[5]) + (p[6] + p[7]));
                         if (kBoth) weights(vinv);
                     }
-                    if constexpr (i == 3 && kBoth && kMore) scales<kValueLog>(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
+                    if constexpr (i == 3 && kBoth && kMore) scales<true>(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
                     if constexpr (i >= 4 && kBoth && kMore) store_v(i - 4, vscale);
                     if constexpr (kMore) end_step();
                 });
                 if constexpr (kMore) end_scores(c + 1);
             } else if (kBoth && kMore) {
-                scales<kValueLog>(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
+                scales<true>(vr(), vscale, lds.vinv[(c + 1) & (kBuffers - 1)]);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) store_v(e, vscale);
             }

@@ -712,9 +712,9 @@ int chn_draft_trees(chn_ctx *ctx, const uint32_t *parents, const uint32_t *row_s
  * 2^31.  out must not overlap an input.  Products are formed of operands split
  * in two 11-bit halves (errors as fp32's own) and summed in fp32; the rows of a
  * tile (up to 128, with the keys that any of them sees) that meets an infinity,
- * a NaN or a magnitude of 2^56 and more in q, K or V, or a query whose largest
- * component times the scale passes 2^141, are computed again in plain fp32, much
- * slower.
+ * a NaN, or a magnitude of 2^56 and more in q or K, or (head_dim 256) a query
+ * whose largest component times |scale| passes 2^141, are computed again in plain
+ * fp32, much slower.
  * Workspace: 68 MB, whatever the batch. */
 int chn_paged_causal_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
                           const uint32_t *tables, const uint32_t *row_start, const uint32_t *lens, uint32_t n_req,

@@ -244,3 +244,20 @@ def test_windows_longer_than_any_request(ctx, words, window):
     b = Batch(ctx, 73, [30, 9, 60, 20, 8, 64], [0, 0, 0, 100, 3, 0], words=words, window=window)
     b.lens = np.array([12, 9, 50, 120, 5, 63])
     check_rows(b)
+
+
+def largest_values(b, log):
+    """V's rows as large as the type allows, or 2^log times what they were: many of one sign in every column."""
+    b.vc = np.float32(2.0 ** log) * (np.float32(1.0) + np.float32(0.9) * np.abs(np.tanh(b.vc)))
+    b.vc[:, 1::2] *= -1
+    b.q[::2] = 0                                                          # every key alike: hundreds of them sum up
+    return b
+
+
+@pytest.mark.parametrize("words", [0, 1])
+@pytest.mark.parametrize("log", [60, 112, 127])
+@pytest.mark.parametrize("D", [256, 512])
+def test_values_whose_sums_pass_the_type(ctx, D, words, log):
+    """Up to 50 keys of equal weight whose V is near the type's largest: their mean is no larger."""
+    say("largest V", D, words, log)
+    check_rows(largest_values(Batch(ctx, 75, [30], [20], D=D, words=words), log))
