@@ -1062,32 +1062,33 @@ __global__ __launch_bounds__(256) void k_packed_join(Packed a) {
         const float old = M == kNoScore ? 0.0f : __builtin_amdgcn_exp2f((M - ref) * a.c);
         const float w = part != 0.0f ? __builtin_amdgcn_exp2f((m - ref) * a.c) * part : 0.0f;
         M = top;
-        L = L * old + row16_sum(w);
+        // divided as they are added: a denominator times values near the type's largest would pass it
+        const float sum = L * old + row16_sum(w), inv = sum != 0.0f ? 1.0f / sum : 0.0f, share = w * inv;
         if (p0 != j.first)
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int k = 0; k < N; ++k) o[i][k] *= lane_f(old, 16 * i);
+                for (int k = 0; k < N; ++k) o[i][k] *= lane_f(L * old * inv, 16 * i);
+        L = sum;
         for (uint32_t q = 0; q < n; q += P) {
             if (q) fetch(p0 + q);
 #pragma unroll
             for (int e = 0; e < P; ++e)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float wi = q + e < n ? lane_f(w, 16 * i + min(q + e, 15u)) : 0.0f;
+                    const float wi = q + e < n ? lane_f(share, 16 * i + min(q + e, 15u)) : 0.0f;
 #pragma unroll
                     for (int k = 0; k < N; ++k) o[i][k] += wi != 0.0f ? wi * v[e][i][k] : f4q{0, 0, 0, 0};
                 }
         }
     }
-    const float inv = L != 0.0f ? 1.0f / L : 0.0f;
 #pragma unroll
     for (uint32_t i = 0; i < 4; ++i) {
         if (i >= rows) break;
         const uint32_t row = row0 + i, token = token_of(a, row);
         float *to = a.out + ((size_t)(j.row + token) * a.num_q + j.kvh * a.gqa + row - token * a.gqa) * D + 4 * lane;
 #pragma unroll
-        for (int k = 0; k < N; ++k) *(f4q *)(to + 256 * k) = o[i][k] * lane_f(inv, 16 * i);
+        for (int k = 0; k < N; ++k) *(f4q *)(to + 256 * k) = o[i][k];
     }
 }
 

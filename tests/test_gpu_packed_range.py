@@ -261,3 +261,12 @@ def test_values_whose_sums_pass_the_type(ctx, D, words, log):
     """Up to 50 keys of equal weight whose V is near the type's largest: their mean is no larger."""
     say("largest V", D, words, log)
     check_rows(largest_values(Batch(ctx, 75, [30], [20], D=D, words=words), log))
+
+
+@pytest.mark.parametrize("words", [0, 1])
+@pytest.mark.parametrize("have", [60, 700, 2500, 9000])
+@pytest.mark.parametrize("D", [256, 512])
+def test_parts_whose_sums_pass_the_type(ctx, D, words, have):
+    """The same in tiles that are cut, into a few parts and into more than the join takes at a time."""
+    say("largest V in parts", D, words, have)
+    check_rows(largest_values(Batch(ctx, 74, [5, 30], [have, 60], D=D, words=words), 127))
