@@ -192,8 +192,9 @@ __device__ __forceinline__ float *row_out(const Packed &a, const Work &w, uint32
     return a.out + ((size_t)(w.tile_row + token) * a.num_q + w.kvh * a.gqa + row - token * a.gqa) * D;
 }
 
-// A row per wave, a key at a time, in plain fp32: what any scores and values
-// do, infinities and NaN among them.
+// A row per wave, a key at a time: scores in plain fp32, what any of them do,
+// infinities and NaN among them; sums in 64 bits, which no values pass and
+// which keep the digits of long lists.
 template <int D>
 __device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
     constexpr int N = D / 256;
@@ -202,55 +203,50 @@ __device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
         const int token = w.token + (int)token_of(a, row);
         const Seen s = seen_by(a, w, token);
         const float *qr = a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + row - token_of(a, row) * a.gqa) * D;
-        f4q q[N], o[N];
+        f4q q[N];
+        double o[N][4];
         for (int k = 0; k < N; ++k) {
             q[k] = *(const f4q *)(qr + 4 * lane + 256 * k) * a.sign;
-            o[k] = f4q{0, 0, 0, 0};
+            for (int e = 0; e < 4; ++e) o[k][e] = 0.0;
         }
-        float m = kNoScore, l = 0.0f;
-        for (uint32_t k0 = w.key0; k0 < (uint32_t)w.key1; k0 += 32) {                         // up to 2^31 and 32
-            // 32 keys from zero, then added, so that long lists keep fp32's digits
-            f4q some[N];
-            float part = 0.0f;
-            for (int k = 0; k < N; ++k) some[k] = f4q{0, 0, 0, 0};
-            for (int pos = (int)k0; pos < (int)min(k0 + 32, (uint32_t)w.key1); ++pos) {
-                bool ok = pos >= s.lo && pos < s.hi;
-                const int node = pos - w.s.have;
-                if (s.mask && node >= 0) ok = (s.mask[node >> 5] >> (node & 31)) & 1;      // key1 is below 32 mask_words of them
-                const uint32_t slot = ok ? slot_of(a, w.table, pos) : CHN_NO_SLOT;
-                if (slot == CHN_NO_SLOT) continue;
-                const size_t at = (size_t)slot * a.kv_dim + (size_t)w.kvh * D + 4 * lane;
-                float sum = 0.0f;
-                for (int k = 0; k < N; ++k) {
-                    const f4q x = *(const f4q *)(a.kc + at + 256 * k);
-                    for (int e = 0; e < 4; ++e) sum = fmaf(x[e], q[k][e], sum);
-                }
-                sum = wave_sum64(sum);
-                if (sum == kNoScore) continue;                                            // no weight, whatever its V
-                if (sum > m) {
-                    const float old = m == kNoScore ? 0.0f : __builtin_amdgcn_exp2f((m - sum) * a.c);
-                    m = sum;
-                    l *= old;
-                    part *= old;
-                    for (int k = 0; k < N; ++k) {
-                        o[k] *= old;
-                        some[k] *= old;
-                    }
-                }
-                // of a NaN score, or of two infinite ones, NaN
-                const float p = __builtin_amdgcn_exp2f((sum - (m == kNoScore ? 0.0f : m)) * a.c);
-                part += p;
-                for (int k = 0; k < N; ++k) some[k] += p * *(const f4q *)(a.vc + at + 256 * k);
+        float m = kNoScore;
+        double l = 0.0;
+        for (int pos = w.key0; pos < w.key1; ++pos) {
+            bool ok = pos >= s.lo && pos < s.hi;
+            const int node = pos - w.s.have;
+            if (s.mask && node >= 0) ok = (s.mask[node >> 5] >> (node & 31)) & 1;          // key1 is below 32 mask_words of them
+            const uint32_t slot = ok ? slot_of(a, w.table, pos) : CHN_NO_SLOT;
+            if (slot == CHN_NO_SLOT) continue;
+            const size_t at = (size_t)slot * a.kv_dim + (size_t)w.kvh * D + 4 * lane;
+            float sum = 0.0f;
+            for (int k = 0; k < N; ++k) {
+                const f4q x = *(const f4q *)(a.kc + at + 256 * k);
+                for (int e = 0; e < 4; ++e) sum = fmaf(x[e], q[k][e], sum);
             }
-            l += part;
-            for (int k = 0; k < N; ++k) o[k] += some[k];
+            sum = wave_sum64(sum);
+            if (sum == kNoScore) continue;                                                // no weight, whatever its V
+            if (sum > m) {
+                const double old = m == kNoScore ? 0.0 : (double)__builtin_amdgcn_exp2f((m - sum) * a.c);
+                m = sum;
+                l *= old;
+                for (int k = 0; k < N; ++k)
+                    for (int e = 0; e < 4; ++e) o[k][e] *= old;
+            }
+            // of a NaN score, or of two infinite ones, NaN
+            const double p = __builtin_amdgcn_exp2f((sum - (m == kNoScore ? 0.0f : m)) * a.c);
+            l += p;
+            for (int k = 0; k < N; ++k) {
+                const f4q x = *(const f4q *)(a.vc + at + 256 * k);
+                for (int e = 0; e < 4; ++e) o[k][e] = fma(p, (double)x[e], o[k][e]);
+            }
         }
-        const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+        const double inv = l != 0.0 ? 1.0 / l : 0.0;
         float *to = row_out<D>(a, w, row);
-        for (int k = 0; k < N; ++k) *(f4q *)(to + 4 * lane + 256 * k) = o[k] * inv;
+        for (int k = 0; k < N; ++k)
+            *(f4q *)(to + 4 * lane + 256 * k) = f4q{(float)(o[k][0] * inv), (float)(o[k][1] * inv), (float)(o[k][2] * inv), (float)(o[k][3] * inv)};
         if (w.part >= 0 && lane == 0) {
             a.pm[(size_t)w.part * tile_rows(D) + row] = m;
-            a.pl[(size_t)w.part * tile_rows(D) + row] = l;
+            a.pl[(size_t)w.part * tile_rows(D) + row] = (float)l;
         }
     }
 }

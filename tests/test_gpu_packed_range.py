@@ -270,3 +270,13 @@ def test_parts_whose_sums_pass_the_type(ctx, D, words, have):
     """The same in tiles that are cut, into a few parts and into more than the join takes at a time."""
     say("largest V in parts", D, words, have)
     check_rows(largest_values(Batch(ctx, 74, [5, 30], [have, 60], D=D, words=words), 127))
+
+
+@pytest.mark.parametrize("have", [60, 2500])
+@pytest.mark.parametrize("D", [256, 512])
+def test_plain_sums_pass_the_type(ctx, D, have):
+    """The same where a NaN in one row's query leaves its tile to plain fp32."""
+    say("largest V, plain", D, have)
+    b = largest_values(Batch(ctx, 76, [5, 30], [have, 60], D=D), 127)
+    b.q[[3, 9], ::D] = np.nan
+    check_rows(b, but=[3, 9])
