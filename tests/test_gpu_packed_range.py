@@ -280,3 +280,22 @@ def test_plain_sums_pass_the_type(ctx, D, have):
     b = largest_values(Batch(ctx, 76, [5, 30], [have, 60], D=D), 127)
     b.q[[3, 9], ::D] = np.nan
     check_rows(b, but=[3, 9])
+
+
+@pytest.mark.parametrize("seed", range(16))
+def test_random_batches_of_any_size(ctx, seed):
+    """Batches of any shape whose rows of q, K and V have sizes of their own, V's up to 2^120 apart."""
+    rng = np.random.default_rng(3000 + seed)
+    D, gqa, words = int(rng.choice([256, 512])), int(rng.integers(1, 17)), int(rng.choice([0, 0, 1, 2, 4]))
+    n = int(np.exp(rng.uniform(0, np.log(12))))
+    new = rng.integers(0, min(32 * words if words else 100, 400 // n) + 1, n)
+    have = np.where(rng.random(n) < 0.3, 0, rng.integers(0, 1500 // n + 2, n))
+    window = int(rng.choice([0, 0, 128, int(rng.integers(128, 400))]))
+    shape = dict(D=D, gqa=gqa, nq=gqa * int(rng.integers(1, 3)), bs=int(2 ** rng.integers(0, 8)), words=words, window=window)
+    say("random sizes", seed, shape, new.tolist(), have.tolist())
+    b = Batch(ctx, 4000 + seed, new, have, **shape)
+    size = lambda x, lo, hi: (2.0 ** rng.integers(lo, hi, (len(x), 1))).astype(np.float32)  # noqa: E731
+    b.vc *= size(b.vc, -60, 61)
+    b.kc *= size(b.kc, -8, 3)
+    b.q *= size(b.q, -8, 2)
+    check_rows(b)
