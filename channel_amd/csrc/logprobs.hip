@@ -121,7 +121,8 @@ __device__ __forceinline__ int max8_order(int i) {                       // the 
 
 // A wave's 2048 values: 256 a load, four of them a lane, all eight loads under
 // way at once.  Bound by memory where there are many rows: 500 rows of 262144,
-// 524 MB, in 84-90 us (5.8-6.3 TB/s); one row is a latency, 4.0 us.
+// 524 MB, in 85-90 us (5.8-6.2 TB/s); softcapped 98-109, memory and issue; one
+// row is a latency, 4.6 us.
 template <int CAP>
 __global__ __launch_bounds__(256) void k_logprob_sums(LogProbs a) {
     const uint32_t row = blockIdx.y, s = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -258,8 +259,8 @@ constexpr uint32_t kScoreFew = 256;          // keys that are ranked by counting
 
 // Bound by its chain of latencies, the same for one row and for hundreds: the
 // sums, the bound on the block maxima two bits at a time, the chosen blocks,
-// their ranks.  500 rows with 5 alternatives 10.4 us; one with 20, softcapped,
-// 11.7.  KEYS: block maxima of a thread (4 up to 262144 values, else 16).
+// their ranks.  500 rows with 5 alternatives 10.5 us, softcapped 15.8; one with
+// 20, softcapped, 11.8.  KEYS: block maxima of a thread (4 up to 262144 values, else 16).
 template <int CAP, int KEYS>
 __global__ __launch_bounds__(kScoreThreads) void k_logprob_rows(LogProbs a) {
     extern __shared__ uint64_t list[];                          // n_top * kScoreBlock keys

@@ -18,16 +18,18 @@
 // the four): 409 TFLOP/s at the rate that a large fp16 product reaches (1227
 // TFLOP/s), against 154 of the fp32 instructions.
 //
-// Measured (us, first launch + second) and what bounds it: 8 trees of up to 16
-// tokens behind up to 700: 18.5 + 7, a chain of latencies; 64 trees on a sliding
-// layer 161-180 + 11, and 5 trees of up to 64 behind up to 60000 302-370 + 10, K
-// and V from memory (0.77 and 1.65 GB); 13 trees of 512-wide heads 117 + 12, a
-// chunk's latencies, the share of a tile per CU; a prompt of 24 tokens 12 + 2, a
-// tile's beginning and end; 48 prompts on a sliding layer 1070-1210 + 18, LDS
-// reads, products and issue, and 12 tiles' beginnings and ends per CU; 2000 tokens
-// behind 30000 3180-3350 + 18, the same (905 TFLOP/s of fp16 products); 9 prompts of
-// 512-wide heads 201-215 + 17, two latencies a chunk: K and V take turns in the
-// same registers.
+// Measured (us, first launch + second, least and mean of 30 calls under a
+// profiler) and what bounds it: 8 trees of up to 16 tokens behind up to 700 17-18 +
+// 7-8, a chain of latencies, the second launch's among them; 64 trees on a sliding
+// layer 164-183 + 11-12, and 5 trees of up to 64 behind up to 60000 300-362 + 9-11,
+// K and V from memory (0.77 and 1.65 GB); 64 requests of one token on a sliding
+// layer 178-201 + 6, the same (0.92 GB); 13 trees of 512-wide heads 115-120 + 12, a
+// chunk's latencies, the share of a tile per CU; a prompt of 24 tokens 12-13 + 1-4,
+// a tile's beginning and end, and a launch with nothing to do; 48 prompts on a
+// sliding layer 1090-1213 + 18, LDS reads, products and issue, and 12 tiles'
+// beginnings and ends per CU; 2000 tokens behind 30000 3172-3373 + 18, the same (905
+// TFLOP/s of fp16 products at the latter); 9 prompts of 512-wide heads 199-216 + 17,
+// two latencies a chunk: K and V take turns in the same registers.
 #include "chn_internal.h"
 
 #include <cmath>
@@ -104,8 +106,11 @@ struct TileKeys {
         k.tiles = __umulhi((uint32_t)s.n + a.tokens - 1, a.per_tokens);
         k.s0 = k.tiles;
         k.full = a.tokens * a.gqa > tile_rows(D) / 2;
-        // of many tiles the last counts as the others: where shares are whole tiles, the workgroups of an XCD then walk the
-        // same keys together (2000 tokens behind 30000: 3.52 ms, 3.85 with the last of 32 tiles a third shorter)
+        // of many tiles the last counts as the others: shares then begin at the same keys of neighbouring tiles, which the
+        // workgroups of an XCD walk together (as itself / as the others: 2000 tokens behind 30000, whose tiles are as many as
+        // the shares, 3560-3815 us / 3390; 2500 behind 20000, 40 tiles per head, 3350 / 3170; 1500 behind 12000 1110 / 1080;
+        // 600 of 512-wide heads 840 / 748; 600 behind 8000, 4100 behind 10000 and 7000 alone within 2 %; two to eight tiles
+        // within 4 % either way)
         k.last_full = k.tiles > 8 ? k.full : (s.n - (k.tiles - 1) * a.tokens) * a.gqa > tile_rows(D) / 2;
         if (a.mask_words) {
             k.T = 0;
@@ -194,7 +199,10 @@ __device__ __forceinline__ float *row_out(const Packed &a, const Work &w, uint32
 
 // A row per wave, a key at a time: scores in plain fp32, what any of them do,
 // infinities and NaN among them; sums in 64 bits, which no values pass and
-// which keep the digits of long lists.
+// which keep the digits of long lists.  Every row reads its keys for itself: a
+// prompt of 24 tokens 59 us instead of 15, 64 requests of one token on a sliding
+// layer 2.2 ms instead of 0.2, 16 prompts of 200 14.5 instead of 0.18, 2000 tokens
+// behind 30000 479 instead of 3.4, and 379 with one NaN in one head's first keys.
 template <int D>
 __device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
     constexpr int N = D / 256;
@@ -403,7 +411,8 @@ constexpr float kLead = 2.0f;
 // A row's sums are kept relative to the largest weight times V scale of the keys that it sees (a power of two, vref):
 // whatever its other keys' slots hold, and whatever lies under weights of nothing, takes no digits from them.  The
 // halves of those products are relative to it, 2^kWeightLog for one, so what is below 2^-36 of it is rounded to that;
-// it is raised when a product passes it by more than kRoom, which keeps them at or below 2^15.
+// it is raised when a product passes it by more than kRoom, which keeps them at or below 2^15.  A reference of all keys
+// walked, known before the scores, is 5 us less for 64 trees (176) and 0.6 for a prompt of 24 (14.1), and wrong.
 // The inverses of V's scales, 2^-126 to 2^113, are held times 2^kValueLog, so that weights times the least of them keep
 // their digits and times the greatest stay below 2^127.
 constexpr int kWeightLog = 12, kValueLog = 11;
@@ -423,7 +432,7 @@ constexpr float kRoom = 8.0f, kLeastRef = 0x1p-115f;
 // The sums and the query's halves of 16 rows stay in a wave's registers, 128 of
 // its 256 with heads of 256, so every wave reads every key's halves from LDS:
 // 512 KB a chunk and CU, 4100 of its 8000 cycles at 128 B a cycle, beside 3070
-// of products and 2400 of vector instructions.  Measured and not taken: products' operands
+// of products and 2550 of vector instructions.  Measured and not taken: products' operands
 // asked for a step ahead (spills, 48 prompts 1470 us), four waves a workgroup
 // and two workgroups a CU (1575), keys shared by no waves, each with chunks of
 // its own (64 trees 280 us, 191 shared).

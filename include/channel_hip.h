@@ -710,11 +710,16 @@ int chn_draft_trees(chn_ctx *ctx, const uint32_t *parents, const uint32_t *row_s
  * reads KV head h / gqa_ratio.  head_dim 256 or 512, any gqa_ratio <= 16; scale
  * finite, not zero; n_req <= 8192, n_rows <= 2^24; max_blocks * block_size <
  * 2^31.  out must not overlap an input.  Products are formed of operands split
- * in two 11-bit halves (errors as fp32's own) and summed in fp32; the rows of a
- * tile (up to 128, with the keys that any of them sees) that meets an infinity,
- * a NaN, or a magnitude of 2^56 and more in q or K, or (head_dim 256) a query
- * whose largest component times |scale| passes 2^141, are computed again in plain
- * fp32, much slower.
+ * in two 11-bit halves and summed in fp32: a value of q, K or V keeps 2^-22 of its
+ * own size, or 2^-39 of the largest of its row's and head's where that is more,
+ * and a key's weight times its largest |v| 2^-22, or 2^-36 of the row's largest
+ * such product.  For values of like sizes that is fp32's own error; components
+ * 2^-17 and less of their row's largest keep fewer digits than fp32's.  The rows
+ * of a tile (up to 128, with the keys that any of them sees) that meets an
+ * infinity, a NaN, or a magnitude of 2^56 and more in q or K, or (head_dim 256) a
+ * query whose largest component times |scale| passes 2^141, are computed again
+ * with scores in plain fp32, 4 to 140 times slower: one NaN in a cached prefix
+ * puts all tiles that walk it there.
  * Workspace: 68 MB, whatever the batch. */
 int chn_paged_causal_attn(chn_ctx *ctx, const float *q, const float *k_cache, const float *v_cache,
                           const uint32_t *tables, const uint32_t *row_start, const uint32_t *lens, uint32_t n_req,
@@ -749,6 +754,8 @@ int chn_paged_tree_attn(chn_ctx *ctx, const float *q, const float *k_cache, cons
  *  - top_ids, top_logprobs ([n_rows][n_top], n_top <= 64): the first n_top
  *    tokens and their log probabilities; CHN_NO_TOKEN and -inf behind the last
  *    allowed one.
+ * The sums over a row are fp32's, of weights whose exponents are off by up to
+ * 2^-21 softcap / temperature (softcaps above 64: of the logit in its place).
  * temperature (device, n_rows) NULL: 1; entropy and ranks may be NULL, the top
  * arrays with n_top 0.  Outputs must not overlap inputs or one another.  n_rows
  * <= 65535.  Workspace: at most 26 MB, for the largest V. */
