@@ -200,14 +200,16 @@ __device__ __forceinline__ float *row_out(const Packed &a, const Work &w, uint32
 // A row per wave, a key at a time: scores in plain fp32, what any of them do,
 // infinities and NaN among them; sums in 64 bits, which no values pass and
 // which keep the digits of long lists.  Every row reads its keys for itself: a
-// prompt of 24 tokens 59 us instead of 15, 64 requests of one token on a sliding
-// layer 2.2 ms instead of 0.2, 16 prompts of 200 14.5 instead of 0.18, 2000 tokens
-// behind 30000 479 instead of 3.4, and 379 with one NaN in one head's first keys.
+// prompt of 24 tokens 58 us instead of 15, 64 requests of one token on a sliding
+// layer 2.2 ms instead of 0.2, 16 prompts of 200 14.0 instead of 0.18, 2000 tokens
+// behind 30000 471 instead of 3.4, and 372 with one NaN in one head's first keys.
 template <int D>
 __device__ __forceinline__ void rows_plain(const Packed &a, const Work &w) {
     constexpr int N = D / 256;
-    const int lane = threadIdx.x & 63;
-    for (uint32_t row = threadIdx.x >> 6; row < w.rows; row += kThreads / 64) {
+    // made again here: what follows from it would be held over the tiles, all the others' time (a prompt of 24 14.7 us, 14.5)
+    const uint32_t thread = opaque_u32(threadIdx.x);
+    const int lane = thread & 63;
+    for (uint32_t row = __builtin_amdgcn_readfirstlane(thread >> 6); row < w.rows; row += kThreads / 64) {
         const int token = w.token + (int)token_of(a, row);
         const Seen s = seen_by(a, w, token);
         const float *qr = a.q + ((size_t)(w.s.row + token) * a.num_q + w.kvh * a.gqa + row - token_of(a, row) * a.gqa) * D;
@@ -412,7 +414,7 @@ constexpr float kLead = 2.0f;
 // whatever its other keys' slots hold, and whatever lies under weights of nothing, takes no digits from them.  The
 // halves of those products are relative to it, 2^kWeightLog for one, so what is below 2^-36 of it is rounded to that;
 // it is raised when a product passes it by more than kRoom, which keeps them at or below 2^15.  A reference of all keys
-// walked, known before the scores, is 5 us less for 64 trees (176) and 0.6 for a prompt of 24 (14.1), and wrong.
+// walked, known before the scores, is 3 us less for 64 trees (174) and 0.5 for a prompt of 24 (14.0), and wrong.
 // The inverses of V's scales, 2^-126 to 2^113, are held times 2^kValueLog, so that weights times the least of them keep
 // their digits and times the greatest stay below 2^127.
 constexpr int kWeightLog = 12, kValueLog = 11;
